@@ -139,6 +139,110 @@ int mfx_layer_norm_bwd(const mfx_norm_bwd_args* args, void* stream);
 size_t mfx_layer_norm_bwd_workspace_size(const mfx_norm_bwd_args* args);
 
 /*
+ * RMSNorm of each query and key head and the rotation by the token's position,
+ * in one pass: what an attention layer does between its projection and its
+ * attention.  No counterpart in the reference, whose models have learned or no
+ * positions; it stands beside mfx_rms_norm and q_rms_eps of mfx_sdpa_fwd.
+ *
+ * Logical shapes q [B, Hq, T, D], k [B, Hkv, T, D] and outputs of the same;
+ * element strides in (batch, head, seq, feature) order, feature stride 1, so
+ * BHTD and BTNH buffers, packed tokens (B = 1) and slices of one projection's
+ * output are all passed without a copy.  Hkv = 0 (or Hq = 0): only the other.
+ *   y = x / sqrt(mean(x^2) + eps) * weight        (eps < 0: y = x, no weights)
+ *   out = y with pair i of its first `rot` features (a, b) turned to
+ *         (a cos t - b sin t, b cos t + a sin t),  t = positions[axis(i)] * f_i
+ * Pair i holds features i and i + rot / 2, or with `interleaved` 2 i and
+ * 2 i + 1; features from rot on are only normalised; rot = 0 turns none.
+ * freqs[rot / 2] are the frequencies as mfx_rope_freqs makes them, in device
+ * memory.  positions are int32 (any value, negative ones turn back), read at
+ * axis * ps[0] + b * ps[1] + t * ps[2]; with axes > 1 (time, height, width)
+ * the first sections[0] pairs take axis 0, the next sections[1] axis 1, ...;
+ * sections of the axes add up to rot / 2.
+ * weights are [D] vectors of `param_dtype` (`dtype` or f32), each may be NULL
+ * (ones).  Arithmetic in fp32, one rounding at the store.  D up to 256.
+ * q_out may be q, and k_out k, when their strides are equal; outputs must not
+ * overlap otherwise.
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const void* q_weight;
+  const void* k_weight;
+  const int32_t* positions;
+  const uint64_t* freqs;
+  int64_t B, T, Hq, Hkv, D, rot;
+  int64_t q_strides[4];
+  int64_t k_strides[4];
+  int64_t qo_strides[4];
+  int64_t ko_strides[4];
+  int64_t pos_strides[3];
+  int32_t sections[4];
+  int32_t axes;
+  int32_t interleaved;
+  int32_t dtype;
+  int32_t param_dtype;
+  float eps;
+  int32_t reserved;
+} mfx_qk_norm_rope_args;
+
+int mfx_qk_norm_rope(const mfx_qk_norm_rope_args* args, void* stream);
+
+/* Fills out[rot / 2] (host memory) with the frequencies of a rotation as
+ * fractions of a turn per position in units of 2^-64, modulo whole turns:
+ * theta^(-2 i / rot) radians per position, or inv_freq[i] (scaled frequencies
+ * of a long-context model) when that is non-null.  position * out[i] modulo
+ * 2^64 is then the angle at any distance.  Host only; no device needed. */
+int mfx_rope_freqs(double theta, int64_t rot, const double* inv_freq, uint64_t* out);
+
+/*
+ * Backward of mfx_qk_norm_rope: dq, dk (and with non-null pointers the weight
+ * gradients dq_weight, dk_weight of `param_dtype`) from the forward's inputs
+ * and the gradients dq_out, dk_out of its outputs.  dq may be q or dq_out
+ * where the strides are equal, dk likewise.  The weights' row sums go through
+ * a workspace of mfx_qk_norm_rope_bwd_workspace_size() bytes (NULL: library
+ * scratch) in a fixed order: deterministic.
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* dq_out;
+  const void* dk_out;
+  void* dq;
+  void* dk;
+  const void* q_weight;
+  const void* k_weight;
+  void* dq_weight;
+  void* dk_weight;
+  const int32_t* positions;
+  const uint64_t* freqs;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t B, T, Hq, Hkv, D, rot;
+  int64_t q_strides[4];
+  int64_t k_strides[4];
+  int64_t dqo_strides[4];
+  int64_t dko_strides[4];
+  int64_t dq_strides[4];
+  int64_t dk_strides[4];
+  int64_t pos_strides[3];
+  int32_t sections[4];
+  int32_t axes;
+  int32_t interleaved;
+  int32_t dtype;
+  int32_t param_dtype;
+  float eps;
+  int32_t reserved;
+} mfx_qk_norm_rope_bwd_args;
+
+int mfx_qk_norm_rope_bwd(const mfx_qk_norm_rope_bwd_args* args, void* stream);
+
+/* Bytes of workspace mfx_qk_norm_rope_bwd needs for these arguments, at any
+ * alignment of the tensors (0 if none). */
+size_t mfx_qk_norm_rope_bwd_workspace_size(const mfx_qk_norm_rope_bwd_args* args);
+
+/*
  * Scaled dot-product attention, out = softmax(scale * Q K^T + M) V.
  *
  * Logical shapes q [B, Hq, Tq, D], k [B, Hkv, Tk, D], v [B, Hkv, Tk, Dv],

@@ -6,6 +6,7 @@ GPU is missing, calls raise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import struct
@@ -136,6 +137,32 @@ class SdpaBwdArgs(ctypes.Structure):
     ]
 
 
+class QkNormRopeArgs(ctypes.Structure):
+    """mfx_qk_norm_rope_args (include/mfx_kernels.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_weight", "k_weight", "positions",
+                                                "freqs")]
+                + [(n, ctypes.c_int64) for n in ("B", "T", "Hq", "Hkv", "D", "rot")]
+                + [(n, I64x4) for n in ("q_strides", "k_strides", "qo_strides", "ko_strides")]
+                + [("pos_strides", ctypes.c_int64 * 3), ("sections", ctypes.c_int32 * 4)]
+                + [(n, ctypes.c_int32) for n in ("axes", "interleaved", "dtype", "param_dtype")]
+                + [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)])
+
+
+class QkNormRopeBwdArgs(ctypes.Structure):
+    """mfx_qk_norm_rope_bwd_args (include/mfx_kernels.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "dq_out", "dk_out", "dq", "dk", "q_weight", "k_weight",
+                                                "dq_weight", "dk_weight", "positions", "freqs", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int64) for n in ("B", "T", "Hq", "Hkv", "D", "rot")]
+                + [(n, I64x4) for n in ("q_strides", "k_strides", "dqo_strides", "dko_strides", "dq_strides",
+                                        "dk_strides")]
+                + [("pos_strides", ctypes.c_int64 * 3), ("sections", ctypes.c_int32 * 4)]
+                + [(n, ctypes.c_int32) for n in ("axes", "interleaved", "dtype", "param_dtype")]
+                + [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)])
+
+
 class GemmArgs(ctypes.Structure):
     """mfx_gemm_args (include/mfx_kernels.h)."""
 
@@ -262,6 +289,14 @@ def load(path: str | os.PathLike | None = None, make_default: bool = False) -> c
     lib.mfx_sdpa_workspace_size.restype = ctypes.c_size_t
     lib.mfx_sdpa_kernel_name.argtypes = [ctypes.POINTER(SdpaArgs)]
     lib.mfx_sdpa_kernel_name.restype = ctypes.c_char_p
+    lib.mfx_rope_freqs.argtypes = [ctypes.c_double, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]
+    lib.mfx_rope_freqs.restype = ctypes.c_int
+    lib.mfx_qk_norm_rope.argtypes = [ctypes.POINTER(QkNormRopeArgs), ctypes.c_void_p]
+    lib.mfx_qk_norm_rope.restype = ctypes.c_int
+    lib.mfx_qk_norm_rope_bwd.argtypes = [ctypes.POINTER(QkNormRopeBwdArgs), ctypes.c_void_p]
+    lib.mfx_qk_norm_rope_bwd.restype = ctypes.c_int
+    lib.mfx_qk_norm_rope_bwd_workspace_size.argtypes = [ctypes.POINTER(QkNormRopeBwdArgs)]
+    lib.mfx_qk_norm_rope_bwd_workspace_size.restype = ctypes.c_size_t
     lib.mfx_gemm.argtypes = [ctypes.POINTER(GemmArgs), ctypes.c_void_p]
     lib.mfx_gemm.restype = ctypes.c_int
     lib.mfx_gemm_kernel_name.argtypes = [ctypes.POINTER(GemmArgs)]
@@ -578,6 +613,182 @@ def sdpa_bwd_kernel_name(q, k, v, **kw) -> str:
 def sdpa_bwd_workspace_size(q, k, v, **kw) -> int:
     a = sdpa_bwd_args(q, k, v, q, q, k, v, **kw)
     return int(load().mfx_sdpa_bwd_workspace_size(ctypes.byref(a)))
+
+
+# ---- query / key norm with rotation ----------------------------------------------
+
+def _on(t, *others):
+    """Context in which work for t's device is launched: t's device made the
+    current one if it is not.  The other tensors must live there too."""
+    torch = _torch()
+    _require_gpu(t, *others)
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise ValueError(f"tensors on {t.device} and {o.device}")
+    if torch.cuda.current_device() == t.device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else 0
+
+
+def rope_table(rot: int, theta: float = 10000.0, *, inv_freq=None, device="cuda"):
+    """The frequencies of a rotation of `rot` features, as qk_norm_rope takes
+    them: theta^(-2 i / rot) radians per position, or the given inv_freq
+    [rot / 2] (scaled frequencies), as 64-bit fractions of a turn
+    (mfx_rope_freqs).  Made once and kept, like a weight."""
+    torch = _torch()
+    out = torch.empty(rot // 2, dtype=torch.int64)
+    f = None
+    if inv_freq is not None:
+        f = torch.as_tensor(inv_freq, dtype=torch.float64).cpu().contiguous()
+        if f.shape != (rot // 2,):
+            raise ValueError(f"inv_freq must have rot / 2 = {rot // 2} entries")
+    check(load().mfx_rope_freqs(float(theta), rot, _ptr(f), out.data_ptr()))
+    return out.to(device)
+
+
+_QK_PACK = struct.Struct("8P6q16q3q4i4ifi").pack
+_QK_BWD_PACK = struct.Struct("13PN6q24q3q4i4ifi").pack
+
+
+def _head_rows(t, layout):
+    """((B, H, T, D), strides) of [T, H, D] tokens or a 4-D tensor."""
+    if t.dim() == 3:
+        s = t.stride()
+        return (1, t.shape[1], t.shape[0], t.shape[2]), (t.shape[0] * s[0], s[1], s[0], s[2])
+    if t.dim() != 4:
+        raise ValueError("queries and keys are [T, H, D] or 4-D")
+    return _dims(t, layout), _strides4(t, layout)
+
+
+def _qk_fields(q, k, positions, table, q_weight, k_weight, eps, sections, interleaved, layout, more):
+    """Checked (pointers of positions and table, dims, strides of q, k and of
+    the (q-shaped, k-shaped) pairs in `more`, the rest) for the packed structs."""
+    torch = _torch()
+    if q is None and k is None:
+        raise ValueError("q or k is needed")
+    first = q if q is not None else k
+    (B, _, T, D), _ = _head_rows(first, layout)
+    heads, strides = [0, 0], []
+    for pair in ((q, k), *more):
+        for i, t in enumerate(pair):
+            like = (q, k)[i]
+            if (t is None) != (like is None):
+                raise ValueError("q and k each need their outputs (and gradients)")
+            if t is None:
+                strides.append((0, 0, 0, 1))
+                continue
+            if t.shape != like.shape or t.dtype != first.dtype or t.dim() != first.dim():
+                raise ValueError("q and k (and their outputs and gradients) must agree in shape and dtype")
+            (b, h, n, d), st = _head_rows(t, layout)
+            if (b, n, d) != (B, T, D):
+                raise ValueError("q and k must agree in batch, tokens and head size")
+            heads[i] = h
+            strides.append(st)
+    rot = 2 * table.numel() if table is not None else 0
+    ps, axes, secs = (0, 0, 0), 1, (rot // 2, 0, 0, 0)
+    if rot:
+        if table.dtype != torch.int64 or table.dim() != 1 or not table.is_contiguous():
+            raise ValueError("table must come from rope_table")
+        if positions is None or positions.dtype != torch.int32:
+            raise TypeError("positions must be an int32 tensor")
+        p = positions
+        if sections is not None:
+            secs = tuple(int(x) for x in sections)
+            axes = len(secs)
+            if not 1 <= axes <= 4:
+                raise ValueError("sections of 1 to 4 axes")
+            if p.dim() < 2 or p.shape[0] != axes:
+                raise ValueError("positions must be [axes, T] or [axes, B, T]")
+            secs = secs + (0,) * (4 - axes)
+            tail, ts, a0 = p.shape[1:], p.stride()[1:], p.stride(0)
+        else:
+            tail, ts, a0 = p.shape, p.stride(), 0
+        if tuple(tail) == (T,):
+            ps = (a0, 0, ts[0])
+        elif tuple(tail) == (B, T):
+            ps = (a0, ts[0], ts[1])
+        else:
+            raise ValueError(f"positions {tuple(p.shape)} do not fit {B} x {T} tokens")
+    pd = None
+    for w in (q_weight, k_weight):
+        if w is None:
+            continue
+        if w.shape != (D,) or not w.is_contiguous() or (pd is not None and w.dtype != pd):
+            raise ValueError("weights must be contiguous [head size] vectors of one dtype")
+        pd = w.dtype
+    code = dtype_code(first.dtype)
+    return ((_ptr(positions) if rot else 0, _ptr(table) if rot else 0), (B, T, heads[0], heads[1], D, rot),
+            tuple([x for st in strides for x in st]) + tuple(ps) + secs
+            + (axes, 1 if interleaved else 0, code, dtype_code(pd) if pd is not None else code,
+               -1.0 if eps is None else _f32(eps), 0))
+
+
+def qk_norm_rope(q, k, positions, table, *, q_weight=None, k_weight=None, eps=1e-6, sections=None, interleaved=False,
+                 layout="bhtd", q_out=None, k_out=None):
+    """(q_out, k_out): each head row of q and k normalised by its root mean
+    square (times its weight) and turned by its token's position
+    (mfx_qk_norm_rope).
+
+    q [T, Hq, D] and k [T, Hkv, D], or 4-D in `layout` ("bhtd" / "bthd"); k (or
+    q) may be None.  positions: int32 [T] or [B, T]; with `sections` (pairs per
+    position axis) [axes, T] or [axes, B, T].  table: rope_table(rot, ...)
+    (None: no rotation, positions unused).  eps None: no norm.  interleaved:
+    pairs side by side instead of half the rotated features apart.  The
+    outputs are contiguous unless given (q_out may be q, k_out k)."""
+    torch = _torch()
+    first = q if q is not None else k
+    if q is not None and q_out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k is not None and k_out is None:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    ptrs, dims, rest = _qk_fields(q, k, positions, table, q_weight, k_weight, eps, sections, interleaved, layout,
+                                  ((q_out, k_out),))
+    a = QkNormRopeArgs.from_buffer_copy(_QK_PACK(_ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), _ptr(q_weight),
+                                                 _ptr(k_weight), *ptrs, *dims, *rest))
+    with _on(first, q, k, q_out, k_out, q_weight, k_weight, positions, table):
+        check(load().mfx_qk_norm_rope(ctypes.byref(a), _stream_handle(first)))
+    return q_out, k_out
+
+
+def qk_norm_rope_bwd(q, k, dq_out, dk_out, positions, table, *, q_weight=None, k_weight=None, eps=1e-6, sections=None,
+                     interleaved=False, layout="bhtd", dq=None, dk=None, workspace=None):
+    """(dq, dk, dq_weight, dk_weight) of qk_norm_rope for the gradients dq_out,
+    dk_out of its outputs (mfx_qk_norm_rope_bwd); q, k are the forward's inputs.
+    A weight's gradient has its dtype; None for an absent weight."""
+    torch = _torch()
+    first = q if q is not None else k
+    if q is not None and dq is None:
+        dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k is not None and dk is None:
+        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+    ptrs, dims, rest = _qk_fields(q, k, positions, table, q_weight, k_weight, eps, sections, interleaved, layout,
+                                  ((dq_out, dk_out), (dq, dk)))
+    dqw = torch.empty_like(q_weight) if q_weight is not None else None
+    dkw = torch.empty_like(k_weight) if k_weight is not None else None
+    a = QkNormRopeBwdArgs.from_buffer_copy(_QK_BWD_PACK(
+        _ptr(q), _ptr(k), _ptr(dq_out), _ptr(dk_out), _ptr(dq), _ptr(dk), _ptr(q_weight), _ptr(k_weight), _ptr(dqw),
+        _ptr(dkw), *ptrs, 0, 0, *dims, *rest))
+    with _on(first, q, k, dq_out, dk_out, dq, dk, q_weight, k_weight, positions, table, workspace):
+        keep = _workspace(a, "mfx_qk_norm_rope_bwd_workspace_size", workspace, first)  # noqa: F841 (until the launch)
+        check(load().mfx_qk_norm_rope_bwd(ctypes.byref(a), _stream_handle(first)))
+    return dq, dk, dqw, dkw
+
+
+def _workspace(a, query, workspace, like):
+    """Sets a.workspace: the caller's, or one from torch's allocator for this
+    call (also inside a captured graph, whose pool then owns it)."""
+    if workspace is None:
+        need = int(getattr(load(), query)(ctypes.byref(a)))
+        if not need:
+            return None
+        workspace = _torch().empty(need, dtype=_torch().uint8, device=like.device)
+    a.workspace = workspace.data_ptr()
+    a.workspace_bytes = workspace.numel() * workspace.element_size()
+    return workspace
 
 
 # ---- GEMM ----------------------------------------------------------------------
