@@ -425,6 +425,98 @@ size_t mfx_sdpa_bwd_workspace_size(const mfx_sdpa_bwd_args* args);
  * take every other call.  NULL if the arguments are invalid. */
 const char* mfx_sdpa_bwd_kernel_name(const mfx_sdpa_bwd_args* args);
 
+/*
+ * Attention over packed sequences: T tokens, sequence s of them
+ * seq_offsets[s] <= t < seq_offsets[s + 1], each token attending within its
+ * sequence (with `causal`, to the tokens at or before it).  What
+ * mfx_sdpa_fwd computes for each sequence alone, in one launch for any mix of
+ * lengths, one token to the whole batch.  The reference has no counterpart
+ * (jax.nn.dot_product_attention's segment-free form pads).
+ *
+ * Logical shapes q, out [Hq, T, D], k, v [Hkv, T, D]; element strides in
+ * (head, token, feature) order, feature stride 1.  Grouped heads, types, head
+ * sizes and scale as in mfx_sdpa_args; D is also the values' size.
+ * seq_offsets: num_seqs + 1 non-decreasing int32 values within 0 .. T, in
+ * device memory (the host never reads them: a captured call may be replayed
+ * with others).  Sequences may be empty.  Rows of out and lse in no sequence
+ * (before the first, behind the last) are left as they were.  Offsets out of
+ * order or range lead to no access outside the tensors; which rows are
+ * computed then is unspecified.
+ *
+ * No sequence sees another's rows, whatever they hold; within a sequence rows
+ * that causality hides behave as in mfx_sdpa_fwd.
+ * lse (optional): [Hq][T] fp32, as in mfx_sdpa_args.  No workspace.
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const int32_t* seq_offsets;
+  float* lse;
+  int64_t T, num_seqs, Hq, Hkv, D;
+  int64_t q_strides[3];
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int64_t o_strides[3];
+  float scale;
+  int32_t causal;
+  int32_t dtype;
+  int32_t reserved;
+} mfx_sdpa_packed_args;
+
+int mfx_sdpa_packed(const mfx_sdpa_packed_args* args, void* stream);
+
+/* Which kernel mfx_sdpa_packed would launch ("packed_bf16_d128", ...; bf16 /
+ * f16 of head size 32, 64, 96, 128 and f32 of those and 256 on the matrix
+ * cores, under mfx_sdpa_fwd's rules of alignment and extent, here for all T
+ * tokens; "packed_generic", a wavefront a row, otherwise; "none" without
+ * tokens or sequences), or NULL if invalid. */
+const char* mfx_sdpa_packed_kernel_name(const mfx_sdpa_packed_args* args);
+
+/*
+ * Backward of mfx_sdpa_packed from the forward's out and lse: dq, dk, dv, dk
+ * and dv of a kv head summed over its query heads.  Rows in no sequence are
+ * left as they were.  dq, dk and dv must not share memory with the inputs or
+ * each other.  Workspace: mfx_sdpa_packed_bwd_workspace_size() bytes, 256-byte
+ * aligned, or NULL for library scratch.  Deterministic: no atomics.
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* dout;
+  const void* out;
+  const float* lse;
+  void* dq;
+  void* dk;
+  void* dv;
+  const int32_t* seq_offsets;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t T, num_seqs, Hq, Hkv, D;
+  int64_t q_strides[3];
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int64_t do_strides[3];
+  int64_t o_strides[3];
+  int64_t dq_strides[3];
+  int64_t dk_strides[3];
+  int64_t dv_strides[3];
+  float scale;
+  int32_t causal;
+  int32_t dtype;
+  int32_t reserved;
+} mfx_sdpa_packed_bwd_args;
+
+int mfx_sdpa_packed_bwd(const mfx_sdpa_packed_bwd_args* args, void* stream);
+
+size_t mfx_sdpa_packed_bwd_workspace_size(const mfx_sdpa_packed_bwd_args* args);
+
+/* As mfx_sdpa_packed_kernel_name (head sizes 32 and 96 in 16 bits run through
+ * padded copies, as in mfx_sdpa_bwd; f32 of 256 on "packed_generic"). */
+const char* mfx_sdpa_packed_bwd_kernel_name(const mfx_sdpa_packed_bwd_args* args);
+
 /* ==========================================================================
  * Generic ops: the graph regions the pattern matcher does not fuse.
  * The reference evaluates these op by op with MLX (reference

@@ -27,6 +27,7 @@
 #include <cmath>
 
 #include "sdpa_common.h"
+#include "sdpa_packed.h"
 
 namespace mfx {
 namespace {
@@ -34,7 +35,9 @@ namespace {
 constexpr int kMaxD = 256;
 constexpr int kFeat = kMaxD / 64;
 
-template <typename T>
+// PACKED, here and below: rows of a packed batch (sdpa_packed.h); a row in no
+// sequence is left alone.
+template <typename T, bool PACKED = false>
 __global__ __launch_bounds__(256) void bwd_delta_kernel(SdpaBwdParams p, float* delta) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -43,6 +46,10 @@ __global__ __launch_bounds__(256) void bwd_delta_kernel(SdpaBwdParams p, float* 
   const int t = (int)(row % p.Tq);
   const int bh = (int)(row / p.Tq);
   const int b = bh / p.Hq, h = bh % p.Hq;
+  if constexpr (PACKED) {
+    int start, len;
+    if (!packed_seq(p.seq_off, p.num_seqs, p.total, t, start, len)) return;
+  }
   const T* orow = static_cast<const T*>(p.o) + b * p.os[0] + h * p.os[1] + t * p.os[2];
   const T* grow = static_cast<const T*>(p.dout) + b * p.dos[0] + h * p.dos[1] + t * p.dos[2];
   float s = 0.f;
@@ -59,22 +66,28 @@ __device__ __forceinline__ float bwd_score(const SdpaBwdParams& p, float dot, in
 }
 
 // dQ: one wavefront per query row (b, h, i).
-template <typename T>
+template <typename T, bool PACKED = false>
 __global__ __launch_bounds__(64) void bwd_dq_generic(SdpaBwdParams p) {
   __shared__ float q_lds[kMaxD];
   __shared__ float g_lds[kMaxD];
   __shared__ float ds_lds[64];
   const int lane = threadIdx.x;
   const int64_t row = blockIdx.x;
-  const int i = (int)(row % p.Tq);
+  int i = (int)(row % p.Tq);
   const int bh = (int)(row / p.Tq);
   const int b = bh / p.Hq, h = bh % p.Hq, hk = h / p.group;
+  const float lse = p.lse[row], dl = p.delta[row];
+  if constexpr (PACKED) {
+    int start, len;
+    if (!packed_seq(p.seq_off, p.num_seqs, p.total, i, start, len)) return;
+    packed_shift<(int)sizeof(T)>(p, start, len);
+    i -= start;
+  }
   const T* qrow = static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1] + i * p.qs[2];
   const T* grow = static_cast<const T*>(p.dout) + b * p.dos[0] + h * p.dos[1] + i * p.dos[2];
   for (int d = lane; d < p.D; d += 64) q_lds[d] = to_f32(qrow[d]);
   for (int d = lane; d < p.Dv; d += 64) g_lds[d] = to_f32(grow[d]);
   __syncthreads();
-  const float lse = p.lse[row], dl = p.delta[row];
   const T* kbase = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[1];
   const T* vbase = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[1];
   float acc[kFeat];
@@ -117,7 +130,7 @@ __global__ __launch_bounds__(64) void bwd_dq_generic(SdpaBwdParams p) {
 
 // dK and dV: one wavefront per key row (b, hk, j), over every query row of
 // the group's heads that sees key j.
-template <typename T>
+template <typename T, bool PACKED = false>
 __global__ __launch_bounds__(64) void bwd_dkdv_generic(SdpaBwdParams p) {
   __shared__ float k_lds[kMaxD];
   __shared__ float v_lds[kMaxD];
@@ -125,9 +138,15 @@ __global__ __launch_bounds__(64) void bwd_dkdv_generic(SdpaBwdParams p) {
   __shared__ float ds_lds[64];
   const int lane = threadIdx.x;
   const int64_t row = blockIdx.x;
-  const int j = (int)(row % p.Tk);
+  int j = (int)(row % p.Tk);
   const int bhk = (int)(row / p.Tk);
   const int b = bhk / p.Hkv, hk = bhk % p.Hkv;
+  if constexpr (PACKED) {
+    int start, len;
+    if (!packed_seq(p.seq_off, p.num_seqs, p.total, j, start, len)) return;
+    packed_shift<(int)sizeof(T)>(p, start, len);
+    j -= start;
+  }
   const T* krow = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[1] + j * p.ks[2];
   const T* vrow = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[1] + j * p.vs[2];
   for (int d = lane; d < p.D; d += 64) k_lds[d] = to_f32(krow[d]);
@@ -141,7 +160,7 @@ __global__ __launch_bounds__(64) void bwd_dkdv_generic(SdpaBwdParams p) {
     const int h = hk * p.group + g;
     const T* qbase = static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1];
     const T* gbase = static_cast<const T*>(p.dout) + b * p.dos[0] + h * p.dos[1];
-    const int64_t rbase = ((int64_t)b * p.Hq + h) * p.Tq;
+    const int64_t rbase = ((int64_t)b * p.Hq + h) * row_pitch<PACKED>(p);
     for (int qb = qstart; qb < p.Tq; qb += 64) {
       const int i = qb + lane;
       float pr = 0.f, ds = 0.f;
@@ -187,17 +206,21 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 // Copies rows [rows][D] (element strides s0..s2 over (b, h, t), feature
 // stride 1) into contiguous rows of Dp >= D features, the rest zero; or back
 // (unpad: the first D features of each contiguous row to the strided rows).
-// One thread per 16-byte chunk (D and Dp multiples of 8 elements).
+// One thread per 16-byte chunk (D and Dp multiples of 8 elements).  off, when
+// given: the offsets of n packed sequences; rows in none of them stay out of
+// the rows written back.
 template <bool UNPAD>
 __global__ __launch_bounds__(256) void pad_rows_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst,
                                                        int64_t rows, int D, int Dp, int H, int T, int64_t s0,
-                                                       int64_t s1, int64_t s2) {
+                                                       int64_t s1, int64_t s2, const int32_t* off = nullptr,
+                                                       int seqs = 0) {
   const int cpr = Dp / 8;  // chunks per padded row
   const int64_t n = rows * cpr;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / cpr;
     const int c = (int)(i % cpr) * 8;
     const int t = (int)(r % T);
+    if (UNPAD && off && (t < off[0] || t >= off[seqs])) continue;
     const int64_t bh = r / T;
     const int64_t strided = (bh / H) * s0 + (bh % H) * s1 + t * s2 + c;
     if constexpr (UNPAD) {
@@ -404,14 +427,45 @@ int pad_rows(const void* src, void* dst, const BwdPlan& pl, int H, int T, const 
   const unsigned blocks = (unsigned)std::min<int64_t>((chunks + 255) / 256, 4096);
   if (unpad)
     hipLaunchKernelGGL((pad_rows_kernel<true>), dim3(blocks), dim3(256), 0, s, static_cast<const uint16_t*>(src),
-                       static_cast<uint16_t*>(dst), rows, pl.p.D, pl.dp, H, T, st[0], st[1], st[2]);
+                       static_cast<uint16_t*>(dst), rows, pl.p.D, pl.dp, H, T, st[0], st[1], st[2], nullptr, 0);
   else
     hipLaunchKernelGGL((pad_rows_kernel<false>), dim3(blocks), dim3(256), 0, s, static_cast<const uint16_t*>(src),
-                       static_cast<uint16_t*>(dst), rows, pl.p.D, pl.dp, H, T, st[0], st[1], st[2]);
+                       static_cast<uint16_t*>(dst), rows, pl.p.D, pl.dp, H, T, st[0], st[1], st[2], nullptr, 0);
   return launch_status("pad_rows_kernel");
 }
 
+template <typename T>
+void launch_generic_t(const SdpaBwdParams& p, hipStream_t s) {
+  const int64_t rows = (int64_t)p.Hq * p.Tq;
+  hipLaunchKernelGGL((bwd_delta_kernel<T, true>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p, p.delta);
+  hipLaunchKernelGGL((bwd_dkdv_generic<T, true>), dim3((unsigned)((int64_t)p.Hkv * p.Tk)), dim3(64), 0, s, p);
+  hipLaunchKernelGGL((bwd_dq_generic<T, true>), dim3((unsigned)rows), dim3(64), 0, s, p);
+}
+
 }  // namespace
+
+int launch_packed_bwd_generic(const SdpaBwdParams& p, hipStream_t s) {
+  if (p.dtype == MFX_BF16) launch_generic_t<bf16>(p, s);
+  else if (p.dtype == MFX_F16) launch_generic_t<_Float16>(p, s);
+  else launch_generic_t<float>(p, s);
+  return launch_status("bwd generic kernels (packed)");
+}
+
+int packed_pad_rows(const void* src, void* dst, const SdpaBwdParams& p, int H, int dp, const int64_t* st, bool unpad,
+                    hipStream_t s) {
+  const int64_t rows = (int64_t)H * p.total;
+  const unsigned blocks = (unsigned)std::min<int64_t>((rows * (dp / 8) + 255) / 256, 4096);
+  auto* in = static_cast<const uint16_t*>(src);
+  auto* out = static_cast<uint16_t*>(dst);
+  if (unpad)
+    hipLaunchKernelGGL((pad_rows_kernel<true>), dim3(blocks), dim3(256), 0, s, in, out, rows, p.D, dp, H, p.total,
+                       st[0], st[1], st[2], p.seq_off, p.num_seqs);
+  else
+    hipLaunchKernelGGL((pad_rows_kernel<false>), dim3(blocks), dim3(256), 0, s, in, out, rows, p.D, dp, H, p.total,
+                       st[0], st[1], st[2], p.seq_off, p.num_seqs);
+  return launch_status("pad_rows_kernel (packed)");
+}
+
 }  // namespace mfx
 
 extern "C" {

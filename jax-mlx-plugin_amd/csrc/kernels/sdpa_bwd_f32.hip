@@ -35,6 +35,7 @@
 // 914 and 1575; 64 heads of one query and one key 14 and 17; at D = 32 to 128
 // over 96 such shapes 0.03 to 0.87 of their time).
 #include "sdpa_f32.h"
+#include "sdpa_packed.h"
 
 namespace mfx {
 namespace {
@@ -241,7 +242,7 @@ __device__ __forceinline__ void dq_row(const SdpaBwdParams& p, int b, int h, int
 }
 
 // dK and dV of key j, which queries j .. Tq - 1 of every head of the group see.
-template <int D, int MT>
+template <int D, int MT, bool PACKED>
 __device__ __forceinline__ void dkdv_row(const SdpaBwdParams& p, int b, int hk, int j, int lane) {
   const float* k = static_cast<const float*>(p.k) + b * p.ks[0] + hk * p.ks[1] + (int64_t)j * p.ks[2];
   const float* v = static_cast<const float*>(p.v) + b * p.vs[0] + hk * p.vs[1] + (int64_t)j * p.vs[2];
@@ -249,7 +250,8 @@ __device__ __forceinline__ void dkdv_row(const SdpaBwdParams& p, int b, int hk, 
   for (int h = hk * p.group; h < (hk + 1) * p.group; ++h) {
     const float* q = static_cast<const float*>(p.q) + b * p.qs[0] + h * p.qs[1];
     const float* g = static_cast<const float*>(p.dout) + b * p.dos[0] + h * p.dos[1];
-    const int64_t mcol = MT ? b * p.ms[0] + h * p.ms[1] + j * p.ms[3] : 0, rows = ((int64_t)b * p.Hq + h) * p.Tq;
+    const int64_t mcol = MT ? b * p.ms[0] + h * p.ms[1] + j * p.ms[3] : 0;
+    const int64_t rows = ((int64_t)b * p.Hq + h) * row_pitch<PACKED>(p);
     for (int qb = j; qb < p.Tq; qb += 64) {
       const int i = min(qb + lane, p.Tq - 1);
       const float x = row_score<D, MT>(p, q + (int64_t)i * p.qs[2], k, mcol + (MT ? i * p.ms[2] : 0));
@@ -281,7 +283,8 @@ __device__ __forceinline__ void map_block(int id, int heads, int blocks, int& he
 
 // Two wavefronts per SIMD (256 registers) up to D = 64; D = 96 and 128 hold
 // 2 D/2 operand and D/2 or D accumulator registers and take one.
-template <int D, int NW, int MT>
+// PACKED: one sequence of a packed batch (sdpa_packed.h).
+template <int D, int NW, int MT, bool PACKED = false>
 __global__ __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) void bwd_f32_dq_kernel(SdpaBwdParams p) {
   __shared__ __attribute__((aligned(16))) float k_lds[2][kTile * kRow<D>];
   __shared__ __attribute__((aligned(16))) float v_lds[2][kTile * kRow<D>];
@@ -289,8 +292,17 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) void bwd_f32_dq_kernel(Sd
   const int half = lane >> 5, l32 = lane & 31;
   const int nb = (p.Tq + 32 * NW - 1) / (32 * NW);
   int bh, blk;
-  map_block(blockIdx.x, p.B * p.Hq, nb, bh, blk);
-  blk = nb - 1 - blk;  // longest causal blocks first
+  if constexpr (PACKED) {
+    int slot;
+    PackedBlock pb;
+    packed_head(blockIdx.x, p.Hq, gridDim.x / p.Hq, bh, slot);
+    if (!packed_block<32 * NW>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
+    blk = pb.work;
+    packed_shift<4>(p, pb.start, pb.len);
+  } else {
+    map_block(blockIdx.x, p.B * p.Hq, nb, bh, blk);
+    blk = nb - 1 - blk;  // longest causal blocks first
+  }
   const int b = bh / p.Hq, h = bh % p.Hq, hk = h / p.group;
   const int Tq = p.Tq, Tk = p.Tk;
   const bool causal = p.causal;  // (uniform: not worth a second kernel)
@@ -313,7 +325,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) void bwd_f32_dq_kernel(Sd
   float qf[D / 2], gf[D / 2];
   load_row<D>(static_cast<const float*>(p.q) + b * p.qs[0] + h * p.qs[1] + (int64_t)qc * p.qs[2], qv, half, qf);
   load_row<D>(static_cast<const float*>(p.dout) + b * p.dos[0] + h * p.dos[1] + (int64_t)qc * p.dos[2], qv, half, gf);
-  const int64_t row = (int64_t)bh * Tq + qc;
+  const int64_t row = (int64_t)bh * row_pitch<PACKED>(p) + qc;
   const float lse = p.lse[row];
   float delta = 0.f;
   {
@@ -378,7 +390,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) void bwd_f32_dq_kernel(Sd
   }
 }
 
-template <int D, int NW, int MT>
+template <int D, int NW, int MT, bool PACKED = false>
 __global__ __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) void bwd_f32_dkdv_kernel(SdpaBwdParams p) {
   __shared__ __attribute__((aligned(16))) float q_lds[2][kTile * kRow<D>];
   __shared__ __attribute__((aligned(16))) float g_lds[2][kTile * kRow<D>];
@@ -387,7 +399,16 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) void bwd_f32_dkdv_kernel(
   const int half = lane >> 5, l32 = lane & 31;
   const int nb = (p.Tk + 32 * NW - 1) / (32 * NW);
   int bhk, blk;
-  map_block(blockIdx.x, p.B * p.Hkv, nb, bhk, blk);
+  if constexpr (PACKED) {
+    int slot;
+    PackedBlock pb;
+    packed_head(blockIdx.x, p.Hkv, gridDim.x / p.Hkv, bhk, slot);
+    if (!packed_block<32 * NW>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
+    blk = pb.nb - 1 - pb.work;
+    packed_shift<4>(p, pb.start, pb.len);
+  } else {
+    map_block(blockIdx.x, p.B * p.Hkv, nb, bhk, blk);
+  }
   const int b = bhk / p.Hkv, hk = bhk % p.Hkv;
   const int Tq = p.Tq, Tk = p.Tk, G = p.group;
   const bool causal = p.causal;
@@ -408,7 +429,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) void bwd_f32_dkdv_kernel(
             static_cast<const float*>(p.dout) + b * p.dos[0] + h * p.dos[1] + (int64_t)i0 * gs2, gs2, Tq - i0);
     if (tid < 2 * kTile) {
       const int i = min(i0 + (tid & (kTile - 1)), Tq - 1);
-      rr = (tid < kTile ? p.lse : p.delta)[((int64_t)b * p.Hq + h) * Tq + i];
+      rr = (tid < kTile ? p.lse : p.delta)[((int64_t)b * p.Hq + h) * row_pitch<PACKED>(p) + i];
     }
   };
   auto store = [&](int buf) {
@@ -478,7 +499,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) void bwd_f32_dkdv_kernel(
       const int m = min(32, Tq - k0);
       odd |= odd_rows<D, false>(q, qs2, m, l32, half) | odd_rows<D, false>(g, gs2, m, l32, half);
       blank |= odd_rows<D, true>(g, gs2, m, l32, half);
-      const int64_t rows = ((int64_t)b * p.Hq + h) * Tq;
+      const int64_t rows = ((int64_t)b * p.Hq + h) * row_pitch<PACKED>(p);
       for (int i = k0 + lane; i < Tq; i += 64) {
         if (p.lse[rows + i] != p.lse[rows + i]) nan_lse = max(nan_lse, i);
         if (p.delta[rows + i] != p.delta[rows + i]) nan_delta = max(nan_delta, i);
@@ -498,7 +519,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) void bwd_f32_dkdv_kernel(
     store_row<D>(static_cast<float*>(p.dk) + b * p.dks[0] + hk * p.dks[1] + (int64_t)key * p.dks[2], dk, half, p.scale);
     store_row<D>(static_cast<float*>(p.dv) + b * p.dvs[0] + hk * p.dvs[1] + (int64_t)key * p.dvs[2], dv, half, 1.f);
   }
-  for (; again; again &= again - 1) dkdv_row<D, MT>(p, b, hk, k0 + __builtin_ctz(again), lane);
+  for (; again; again &= again - 1) dkdv_row<D, MT, PACKED>(p, b, hk, k0 + __builtin_ctz(again), lane);
 }
 
 // Wavefronts per workgroup of a kernel whose wavefronts own 32 of T rows in
@@ -527,6 +548,19 @@ int launch_t(const SdpaBwdParams& p, hipStream_t s) {
     hipLaunchKernelGGL((bwd_f32_dkdv_kernel<D, 1, MT>), dim3((unsigned)(hk * ((p.Tk + 31) / 32))), dim3(64), 0,
                        s, p);
   return launch_status("bwd_f32_dkdv_kernel");
+}
+
+template <int D>
+int launch_packed(const SdpaBwdParams& p, hipStream_t s) {
+  const int64_t wide = packed_slots(p.total, p.num_seqs, 128), narrow = packed_slots(p.total, p.num_seqs, 32);
+  if (bwd_f32_waves(p.Hq, p.Tq) == 4)
+    hipLaunchKernelGGL((bwd_f32_dq_kernel<D, 4, 0, true>), dim3((unsigned)(wide * p.Hq)), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((bwd_f32_dq_kernel<D, 1, 0, true>), dim3((unsigned)(narrow * p.Hq)), dim3(64), 0, s, p);
+  if (int rc = launch_status("bwd_f32_dq_kernel (packed)")) return rc;
+  if (bwd_f32_waves(p.Hkv, p.Tk) == 4)
+    hipLaunchKernelGGL((bwd_f32_dkdv_kernel<D, 4, 0, true>), dim3((unsigned)(wide * p.Hkv)), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((bwd_f32_dkdv_kernel<D, 1, 0, true>), dim3((unsigned)(narrow * p.Hkv)), dim3(64), 0, s, p);
+  return launch_status("bwd_f32_dkdv_kernel (packed)");
 }
 
 template <int D>
@@ -564,6 +598,15 @@ int launch_bwd_f32(const SdpaBwdParams& p, hipStream_t s) {
     case 64: return launch_d<64>(p, s);
     case 96: return launch_d<96>(p, s);
     default: return launch_d<128>(p, s);
+  }
+}
+
+int launch_packed_bwd_f32(const SdpaBwdParams& p, hipStream_t s) {
+  switch (p.D) {
+    case 32: return launch_packed<32>(p, s);
+    case 64: return launch_packed<64>(p, s);
+    case 96: return launch_packed<96>(p, s);
+    default: return launch_packed<128>(p, s);
   }
 }
 

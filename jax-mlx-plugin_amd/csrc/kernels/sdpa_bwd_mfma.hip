@@ -44,6 +44,7 @@
 
 #include "sdpa_elem.h"
 #include "sdpa_mask.h"
+#include "sdpa_packed.h"
 #include "sdpa_tiles.h"
 
 #if defined(MFX_PHASE_TIMERS)
@@ -149,8 +150,10 @@ constexpr int kKvPf = 2;   // operand reads issued ahead of their MFMAs
 constexpr int kKvStages = 3;
 constexpr int kDkdvHeadGroup = 2;  // kv heads whose key blocks an XCD runs together
 
-template <int D, bool CAUSAL, int MASKT, int E>
+// PACKED: one sequence of a packed batch (sdpa_packed.h).
+template <int D, bool CAUSAL, int MASKT, int E, bool PACKED = false>
 __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
+  static_assert(!PACKED || MASKT == 0, "packed sequences have no additive mask");
   constexpr bool MASK = MASKT != 0;
   constexpr int TILE = kTile * D;    // elements of one Q or dO tile
   constexpr int TB = TILE * 2;       // its bytes
@@ -200,7 +203,14 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
   const int nkb = (p.Tk + kRows - 1) / kRows;
   const int id = blockIdx.x;
   int bhk, kblk;
-  if ((BHk & 7) == 0 && ((BHk >> 3) % kDkdvHeadGroup) == 0) {
+  if constexpr (PACKED) {
+    int slot;
+    PackedBlock pb;
+    packed_head(id, BHk, gridDim.x / BHk, bhk, slot);
+    if (!packed_block<kRows>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
+    kblk = pb.nb - 1 - pb.work;
+    packed_shift<2>(p, pb.start, pb.len);
+  } else if ((BHk & 7) == 0 && ((BHk >> 3) % kDkdvHeadGroup) == 0) {
     // Blocks are dealt to the 8 XCDs round-robin.  Each XCD takes its kv
     // heads in groups whose key blocks all run together (2 heads x 16 key
     // blocks fill an XCD's 32 CUs at config 3), so the group's Q / dO tiles,
@@ -227,7 +237,7 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
   // g * qs[1] + qt * 64 * qs[2] elements past the group's first head.
   const bf16* qp = static_cast<const bf16*>(p.q) + b * p.qs[0] + (int64_t)hk * G * p.qs[1];
   const bf16* gp = static_cast<const bf16*>(p.dout) + b * p.dos[0] + (int64_t)hk * G * p.dos[1];
-  const int64_t rbase = ((int64_t)b * p.Hq + (int64_t)hk * G) * Tq;  // lse / delta row of (g=0, q=0)
+  const int64_t rbase = ((int64_t)b * p.Hq + (int64_t)hk * G) * row_pitch<PACKED>(p);  // lse / delta row of (g=0, q=0)
   const float* lsep = p.lse + rbase;
   const float* dlp = p.delta + rbase;
   const int st_bytes = G * Tq * 4;
@@ -241,12 +251,26 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
   // rows past Tq read zeros or (inside the span) rows of the next head,
   // which are masked.
   Loader<D> qload(qp, p.qs[2], 0, D, wave, lane), gload(gp, p.dos[2], 0, D, wave, lane);
-  qload.nbytes = (int)(((int64_t)(G - 1) * p.qs[1] + (int64_t)(Tq - 1) * p.qs[2] + D) * 2);
-  gload.nbytes = (int)(((int64_t)(G - 1) * p.dos[1] + (int64_t)(Tq - 1) * p.dos[2] + D) * 2);
+  // (Packed, a head's resource is its own and ends with the sequence: what
+  // other sequences hold, or nobody has written, never meets the products.)
+  qload.nbytes = (int)(((PACKED ? 0 : (int64_t)(G - 1) * p.qs[1]) + (int64_t)(Tq - 1) * p.qs[2] + D) * 2);
+  gload.nbytes = (int)(((PACKED ? 0 : (int64_t)(G - 1) * p.dos[1]) + (int64_t)(Tq - 1) * p.dos[2] + D) * 2);
   auto tile_head = [&](int t) { return t / per_head; };
   auto tile_q = [&](int t) { return qt0 + t % per_head; };
   auto issue = [&](int t, int st) {
     const int g = tile_head(t), qt = tile_q(t);
+    if constexpr (PACKED) {
+      Loader<D> ql = qload, gl = gload;
+      ql.base += (int64_t)g * p.qs[1];
+      gl.base += (int64_t)g * p.dos[1];
+      ql.load_at((uint32_t)((int64_t)qt * kTile * p.qs[2] * 2), reinterpret_cast<bf16*>(smem + st * TB), wave);
+      gl.load_at((uint32_t)((int64_t)qt * kTile * p.dos[2] * 2), reinterpret_cast<bf16*>(smem + GB + st * TB), wave);
+      const int64_t row = (int64_t)g * row_pitch<PACKED>(p);
+      float* sl = reinterpret_cast<float*>(smem + LB + st * LS);
+      if (wave == 0) tiles::load_row64_f32(lsep + row, Tq * 4, (uint32_t)(qt * kTile * 4), sl, lane);
+      if (wave == 1) tiles::load_row64_f32(dlp + row, Tq * 4, (uint32_t)(qt * kTile * 4), sl + kTile, lane);
+      return;
+    }
     qload.load_at((uint32_t)(((int64_t)g * p.qs[1] + (int64_t)qt * kTile * p.qs[2]) * 2),
                   reinterpret_cast<bf16*>(smem + st * TB), wave);
     gload.load_at((uint32_t)(((int64_t)g * p.dos[1] + (int64_t)qt * kTile * p.dos[2]) * 2),
@@ -577,7 +601,7 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
 constexpr int kDqPf = 2;
 
 // Two workgroups per CU, except D = 128 with mask runs in registers (~300).
-template <int D, bool CAUSAL, int MASKT, int E>
+template <int D, bool CAUSAL, int MASKT, int E, bool PACKED = false>
 __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 1 : 2) void bwd_dq_mfma(SdpaBwdParams p) {
   constexpr bool MASK = MASKT != 0, RUNS = MASK && MASKT != kAnyMask;
   constexpr int TILE = kTile * D;  // elements of one K or V tile
@@ -596,7 +620,14 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
   const int BH = p.B * p.Hq;
   const int id = blockIdx.x;
   int bh, mblk;
-  if ((BH & 7) == 0) {
+  if constexpr (PACKED) {
+    int slot;
+    PackedBlock pb;
+    packed_head(id, BH, gridDim.x / BH, bh, slot);
+    if (!packed_block<kRows>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
+    mblk = pb.work;
+    packed_shift<2>(p, pb.start, pb.len);
+  } else if ((BH & 7) == 0) {
     // Heads dealt to the 8 XCDs round-robin, longest causal q-block first.
     const int xcd = id & 7, slot = id >> 3, bpx = BH >> 3;
     bh = (slot % bpx) * 8 + xcd;
@@ -625,7 +656,7 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
   bf16x8 qf[D / 16], gf[D / 16];
   load_frags<D>(static_cast<const bf16*>(p.q) + b * p.qs[0] + h * p.qs[1], p.qs[2], qi, Tq, half, qf);
   load_frags<D>(static_cast<const bf16*>(p.dout) + b * p.dos[0] + h * p.dos[1], p.dos[2], qi, Tq, half, gf);
-  const int64_t row = (int64_t)bh * Tq + min(qi, Tq - 1);
+  const int64_t row = (int64_t)bh * row_pitch<PACKED>(p) + min(qi, Tq - 1);
   const float lse = p.lse[row];
   // delta = rowsum(dO * O): this lane's 64 features, then its partner's.
   float dl;
@@ -844,6 +875,29 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
   }
 }
 
+#if defined(MFX_PACKED)
+template <int D, bool CAUSAL, int E>
+int launch_t(const SdpaBwdParams& p, hipStream_t s) {
+  const int64_t slots = packed_slots(p.total, p.num_seqs, kRows);
+  hipLaunchKernelGGL((bwd_dq_mfma<D, CAUSAL, 0, E, true>), dim3((unsigned)(slots * p.Hq)), dim3(kNT), 0, s, p);
+  if (int rc = launch_status("bwd_dq_mfma (packed)")) return rc;
+  hipLaunchKernelGGL((bwd_dkdv_mfma<D, CAUSAL, 0, E, true>), dim3((unsigned)(slots * p.Hkv)), dim3(kNT), 0, s, p);
+  return launch_status("bwd_dkdv_mfma (packed)");
+}
+
+template <int D, int E>
+int launch_d(const SdpaBwdParams& p, hipStream_t s) {
+  return p.causal ? launch_t<D, true, E>(p, s) : launch_t<D, false, E>(p, s);
+}
+
+}  // namespace
+
+// Packed sequences (the caller checked bwd_mfma_supports).
+int launch_packed_bwd_mfma(const SdpaBwdParams& p, hipStream_t s) {
+  if (p.dtype == MFX_F16) return p.D == 128 ? launch_d<128, 1>(p, s) : launch_d<64, 1>(p, s);
+  return p.D == 128 ? launch_d<128, 0>(p, s) : launch_d<64, 0>(p, s);
+}
+#else
 template <int D, bool CAUSAL, int MT, int E>
 int launch_t(const SdpaBwdParams& p, hipStream_t s) {
   const int64_t q_blocks = (int64_t)p.B * p.Hq * ((p.Tq + kRows - 1) / kRows);
@@ -907,6 +961,7 @@ int launch_bwd_mfma(const SdpaBwdParams& p, hipStream_t s) {
   if (p.dtype == MFX_F16) return p.D == 128 ? launch_d<128, 1>(p, s) : launch_d<64, 1>(p, s);
   return p.D == 128 ? launch_d<128, 0>(p, s) : launch_d<64, 0>(p, s);
 }
+#endif
 
 }  // namespace mfx
 

@@ -35,6 +35,11 @@ struct SdpaParams {
   // lse[(b * Hq + h) * Tq + i] = log2(sum_j exp2(s_ij)), written by the
   // flash and generic kernels when non-null (the backward pass reads it).
   float* lse;
+  // Packed sequences (sdpa_packed.h): their offsets, number and the tokens in
+  // all; lse is then [Hq][total].  Null otherwise.
+  const int32_t* seq_off;
+  int num_seqs;
+  int total;
 };
 
 // Backward pass (mfx_sdpa_bwd).  o / lse come from the recomputed forward
@@ -61,6 +66,9 @@ struct SdpaBwdParams {
   int causal;
   float scale;
   float scale_log2;
+  const int32_t* seq_off;  // packed sequences, as in SdpaParams
+  int num_seqs;
+  int total;
 };
 
 bool bwd_mfma_supports(const SdpaBwdParams& p);

@@ -59,6 +59,7 @@
 #include <type_traits>
 
 #include "sdpa_elem.h"
+#include "sdpa_packed.h"
 #include "sdpa_tiles.h"
 
 #if defined(MFX_PHASE_TIMERS)
@@ -203,8 +204,10 @@ constexpr int wait_v(int j, int MP, int pf) { return 2 * (pf < MP - 1 - j ? pf :
 // feature blocks, so the features DV .. D-1 of a tile (the next row's first
 // elements, or zeros past the tensor) are never read from LDS.  (256-wide
 // rows do not fit: the loop's state passes 512 registers.)
-template <int D, int DV, bool CAUSAL, int MT, int E>
+// PACKED: the rows of one sequence of a packed batch (sdpa_packed.h).
+template <int D, int DV, bool CAUSAL, int MT, int E, bool PACKED = false>
 __global__ __launch_bounds__(kNT, 2) void flash_bf16_pipe_kernel(SdpaParams p) {
+  static_assert(!PACKED || MT == 0, "packed sequences have no additive mask");
   static_assert(DV % 32 == 0 && DV <= D && D - DV < 64, "head size");
   constexpr int TILE = kBN * D;     // elements of one K or V tile
   constexpr int TB = TILE * 2;      // its bytes
@@ -237,7 +240,14 @@ __global__ __launch_bounds__(kNT, 2) void flash_bf16_pipe_kernel(SdpaParams p) {
   const int BH = p.B * p.Hq;
   const int id = blockIdx.x;
   int bh, mblk;
-  if ((BH & 7) == 0) {
+  if constexpr (PACKED) {
+    int slot;
+    PackedBlock pb;
+    packed_head(id, BH, gridDim.x / BH, bh, slot);
+    if (!packed_block<kBM>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
+    mblk = pb.work;
+    packed_shift<2>(p, pb.start, pb.len);
+  } else if ((BH & 7) == 0) {
     // Blocks are dealt to the 8 XCDs round-robin.  Each XCD works through
     // its heads in groups: all q-blocks of a group are issued together,
     // longest first, so they stream the group's K/V tiles at about the same
@@ -646,7 +656,7 @@ __global__ __launch_bounds__(kNT, 2) void flash_bf16_pipe_kernel(SdpaParams p) {
   PHASE(fence(); const unsigned c_epi = PhaseClock::now(); fence();)
   const float lt = l_run + __shfl_xor(l_run, 32, 64);
   const float inv = 1.0f / lt;
-  if (p.lse && half == 0 && qi < Tq) p.lse[(int64_t)bh * Tq + qi] = b_run + __log2f(lt);
+  if (p.lse && half == 0 && qi < Tq) p.lse[(int64_t)bh * row_pitch<PACKED>(p) + qi] = b_run + __log2f(lt);
   // Lane (l32, half) holds features dt*32 + g*8 + half*4 + e of row qi.
   // (Row addresses are formed from an opaque copy of the row index here, so
   // they are not hoisted into the tile loop, where more live registers
@@ -693,6 +703,25 @@ __global__ __launch_bounds__(kNT, 2) void flash_bf16_pipe_kernel(SdpaParams p) {
   PHASE(fence(); ph.write(lane, id * kNW + wave, bh, mblk, N, nw, c_epi);)
 }
 
+#if defined(MFX_PACKED)
+template <int D, int DV, int E>
+int launch_t(const SdpaParams& p, hipStream_t s) {
+  const int64_t blocks = packed_slots(p.total, p.num_seqs, kBM) * p.Hq;
+  if (p.causal)
+    hipLaunchKernelGGL((flash_bf16_pipe_kernel<D, DV, true, 0, E, true>), dim3((unsigned)blocks), dim3(kNT), 0, s, p);
+  else
+    hipLaunchKernelGGL((flash_bf16_pipe_kernel<D, DV, false, 0, E, true>), dim3((unsigned)blocks), dim3(kNT), 0, s, p);
+  return launch_status("flash_bf16_pipe_kernel (packed)");
+}
+
+template <int E>
+int launch_d(const SdpaParams& p, hipStream_t s) {
+  if (p.D == 128) return launch_t<128, 128, E>(p, s);
+  if (p.D == 96) return launch_t<128, 96, E>(p, s);
+  if (p.D == 64) return launch_t<64, 64, E>(p, s);
+  return launch_t<64, 32, E>(p, s);
+}
+#else
 template <int D, int DV, bool CAUSAL, int MT, int E>
 int launch_t(const SdpaParams& p, hipStream_t s) {
   const int nmb = (p.Tq + kBM - 1) / kBM;
@@ -734,10 +763,17 @@ int launch_d(const SdpaParams& p, hipStream_t s) {
   return launch_flash_bf16_pipe_wide(p, s);
 }
 #endif
+#endif
 
 }  // namespace
 
-#if defined(MFX_PIPE_WIDE)
+#if defined(MFX_PACKED)
+// Packed sequences, head size 32, 64, 96 or 128 (the caller checked
+// flash_bf16_supports).
+int launch_packed_flash16(const SdpaParams& p, hipStream_t s) {
+  return p.dtype == MFX_F16 ? launch_d<1>(p, s) : launch_d<0>(p, s);
+}
+#elif defined(MFX_PIPE_WIDE)
 // Head sizes 32 and 96 of launch_flash_bf16_pipe (their kernels are
 // instantiated in a translation unit of their own, so the two compile in
 // parallel).

@@ -8,6 +8,7 @@
 // so that every LDS read is a 16-byte (K) or conflict-free 4-byte (V) access
 // and V needs no transpose.  Tiles are 32 keys, double-buffered through LDS.
 #include "sdpa_f32.h"
+#include "sdpa_packed.h"
 
 // 8-byte raw buffer load, bound to the LLVM intrinsic itself: this
 // compiler's __builtin_amdgcn_raw_buffer_load_b64 lowers to a 4-byte load.
@@ -55,7 +56,8 @@ struct Cfg {
 // Two workgroups per CU (256 VGPRs) except masked D = 96 and 128, whose
 // extra mask state would spill at that bound, and D = 256 (Q and O alone
 // take 256 registers; 134 KB of LDS).
-template <int D, bool CAUSAL, bool MASK>
+// PACKED: one sequence of a packed batch (sdpa_packed.h).
+template <int D, bool CAUSAL, bool MASK, bool PACKED = false>
 __global__ __launch_bounds__(kNT, (D >= 256 || (D >= 96 && MASK)) ? 1 : 2) void flash_f32_kernel(SdpaParams p) {
   using C = Cfg<D, MASK>;
   __shared__ __attribute__((aligned(16))) float k_lds[2][C::KS * C::KROW];
@@ -71,7 +73,14 @@ __global__ __launch_bounds__(kNT, (D >= 256 || (D >= 96 && MASK)) ? 1 : 2) void 
   const int BH = p.B * p.Hq;
   const int id = blockIdx.x;
   int bh, mblk;
-  if ((BH & 7) == 0) {
+  if constexpr (PACKED) {
+    int slot;
+    PackedBlock pb;
+    packed_head(id, BH, gridDim.x / BH, bh, slot);
+    if (!packed_block<kBM>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
+    mblk = pb.work;
+    packed_shift<4>(p, pb.start, pb.len);
+  } else if ((BH & 7) == 0) {
     const int xcd = id & 7, slot = id >> 3;
     bh = (slot / nmb) * 8 + xcd;
     mblk = nmb - 1 - slot % nmb;
@@ -259,7 +268,7 @@ __global__ __launch_bounds__(kNT, (D >= 256 || (D >= 96 && MASK)) ? 1 : 2) void 
 
   const float lt = l_run + __shfl_xor(l_run, 32, 64);
   const float inv = 1.0f / lt;
-  if (p.lse && half == 0 && qi < Tq) p.lse[(int64_t)bh * Tq + qi] = m_run + __log2f(lt);
+  if (p.lse && half == 0 && qi < Tq) p.lse[(int64_t)bh * row_pitch<PACKED>(p) + qi] = m_run + __log2f(lt);
   if (qi < Tq) {
     float* orow = op + qi * os2;
 #pragma unroll
@@ -522,6 +531,14 @@ int launch_t(const SdpaParams& p, hipStream_t s) {
 }
 
 template <int D>
+int launch_packed(const SdpaParams& p, hipStream_t s) {
+  const dim3 grid((unsigned)(packed_slots(p.total, p.num_seqs, kBM) * p.Hq));
+  if (p.causal) hipLaunchKernelGGL((flash_f32_kernel<D, true, false, true>), grid, dim3(kNT), 0, s, p);
+  else hipLaunchKernelGGL((flash_f32_kernel<D, false, false, true>), grid, dim3(kNT), 0, s, p);
+  return launch_status("flash_f32_kernel (packed)");
+}
+
+template <int D>
 int launch_d(const SdpaParams& p, hipStream_t s) {
   const bool m = p.mask != nullptr;
   if (p.causal) return m ? launch_t<D, true, true>(p, s) : launch_t<D, true, false>(p, s);
@@ -552,6 +569,16 @@ int launch_flash_f32(const SdpaParams& p, hipStream_t s) {
     case 128: return launch_d<128>(p, s);
     case 256: return launch_d<256>(p, s);
     default: return launch_d<64>(p, s);
+  }
+}
+
+int launch_packed_f32(const SdpaParams& p, hipStream_t s) {
+  switch (p.D) {
+    case 32: return launch_packed<32>(p, s);
+    case 96: return launch_packed<96>(p, s);
+    case 128: return launch_packed<128>(p, s);
+    case 256: return launch_packed<256>(p, s);
+    default: return launch_packed<64>(p, s);
   }
 }
 

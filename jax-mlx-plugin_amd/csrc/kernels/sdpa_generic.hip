@@ -5,20 +5,27 @@
 // features lane, lane+64, ...  This kernel covers the shapes the MFMA and
 // split-KV kernels do not take; it is correct, not fast.
 #include "sdpa_common.h"
+#include "sdpa_packed.h"
 
 namespace mfx {
 namespace {
 
 constexpr int kMaxD = 256;
 
-template <typename T>
+template <typename T, bool PACKED = false>
 __global__ __launch_bounds__(64) void generic_kernel(SdpaParams p) {
   __shared__ float q_lds[kMaxD];
   __shared__ float p_lds[64];
   const int lane = threadIdx.x;
   const int64_t row = blockIdx.x;
-  const int t = (int)(row % p.Tq);
+  int t = (int)(row % p.Tq);
   const int bh = (int)(row / p.Tq);
+  if constexpr (PACKED) {
+    int start, len;
+    if (!packed_seq(p.seq_off, p.num_seqs, p.total, t, start, len)) return;
+    packed_shift<(int)sizeof(T)>(p, start, len);
+    t -= start;
+  }
   const int b = bh / p.Hq, h = bh % p.Hq, hk = h / p.group;
   const int D = p.D, Dv = p.Dv;
 
@@ -83,7 +90,7 @@ __global__ __launch_bounds__(64) void generic_kernel(SdpaParams p) {
     }
     __syncthreads();
   }
-  if (p.lse && lane == 0) p.lse[row] = m + __log2f(l);
+  if (p.lse && lane == 0) p.lse[(int64_t)bh * row_pitch<PACKED>(p) + t] = m + __log2f(l);
   T* orow = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + t * p.os[2];
 #pragma unroll
   for (int jj = 0; jj < kMaxD / 64; ++jj) {
@@ -105,6 +112,14 @@ int launch_generic(const SdpaParams& p, hipStream_t s) {
   else
     hipLaunchKernelGGL((generic_kernel<float>), dim3((unsigned)rows), dim3(64), 0, s, p);
   return launch_status("generic_kernel");
+}
+
+int launch_packed_generic(const SdpaParams& p, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)p.Hq * p.Tq));
+  if (p.dtype == MFX_BF16) hipLaunchKernelGGL((generic_kernel<bf16, true>), grid, dim3(64), 0, s, p);
+  else if (p.dtype == MFX_F16) hipLaunchKernelGGL((generic_kernel<_Float16, true>), grid, dim3(64), 0, s, p);
+  else hipLaunchKernelGGL((generic_kernel<float, true>), grid, dim3(64), 0, s, p);
+  return launch_status("generic_kernel (packed)");
 }
 
 }  // namespace mfx

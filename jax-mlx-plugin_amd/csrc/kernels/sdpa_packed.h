@@ -1,0 +1,215 @@
+// Packed sequences: where a workgroup of an attention kernel finds its rows.
+//
+// A packed batch is T tokens, sequence s of them from off[s] up to off[s + 1],
+// the offsets in device memory.  The host knows neither the lengths nor the
+// number of row blocks, only a bound: a sequence of n rows is at most
+// n / BM + 1 blocks, so T / BM + min(sequences, T) slots per head cover all.
+// Each workgroup finds its own (sequence, block) from its slot number, with
+// no launch before it, and slots without a block leave at once.
+//
+// Order.  Under a causal mask block b of a sequence walks b + 1 blocks of
+// keys (a block of keys, the blocks of queries behind it), so blocks are handed
+// out by that number, longest first, over all sequences: workgroups start in
+// slot order, and a long block started last would run alone.  With nb(s)
+// blocks in sequence s, above(w) = sum_s max(nb(s) - w, 0) blocks have work
+// past w; slot r belongs to the w with above(w + 1) <= r < above(w), found by
+// bisection, each lane holding the nb of its sequences, and to the
+// (r - above(w + 1))-th sequence of more than w blocks.  That takes a bisection
+// step of a few vector operations and one sum over the lanes (about 80
+// cycles), some 8 steps.  Past kLaneSeqs sequences a lane's share no longer
+// fits registers, and slots go to sequences in order: sequence s owns the slots
+// from (off[s] - off[0]) / BM + s, which are enough for it and need no count
+// of the blocks before.
+//
+// Offsets are taken as they come: each is clamped to 0 .. T and a sequence that
+// would end before it starts is empty, so no offsets lead outside the tensors.
+#pragma once
+
+#include <type_traits>
+
+#include "sdpa_common.h"
+
+namespace mfx {
+
+constexpr int kLaneSeqs = 8;  // sequences a lane holds: 512 in all
+
+struct PackedBlock {
+  int start, len;  // the sequence's first token and its length
+  int work;        // key blocks behind this one, 0 .. nb - 1 (see above)
+  int nb;          // its blocks
+};
+
+// Sum over the wavefront's 64 lanes, in every lane.
+__device__ __forceinline__ int wave_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes below, within 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // lane 15's and 47's into the 16 above
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // lane 31's into the upper half
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+__device__ __forceinline__ void packed_bounds(const int32_t* off, int total, int s, int& start, int& len) {
+  start = min(max(off[s], 0), total);
+  len = max(min(off[s + 1], total) - start, 0);
+}
+
+// Slot `r`'s block of BM rows; false: it has none.  Uniform over the
+// wavefront (every lane active).
+template <int BM>
+__device__ __forceinline__ bool packed_block(const int32_t* off, int n, int total, int r, PackedBlock& out) {
+  const int lane = threadIdx.x & 63;
+  int seq, work;
+  if (n <= 64 * kLaneSeqs) {
+    int nb[kLaneSeqs];
+#pragma unroll
+    for (int c = 0; c < kLaneSeqs; ++c) {
+      nb[c] = 0;
+      if (c * 64 < n) {
+        int a, len = 0;
+        if (c * 64 + lane < n) packed_bounds(off, total, c * 64 + lane, a, len);
+        nb[c] = (len + BM - 1) / BM;
+      }
+    }
+    auto above = [&](int w) {
+      int v = 0;
+#pragma unroll
+      for (int c = 0; c < kLaneSeqs; ++c)
+        if (c * 64 < n) v += max(nb[c] - w, 0);
+      return wave_sum(v);
+    };
+    if (above(0) <= r) return false;
+    int lo = 0, hi = (total + BM - 1) / BM;  // above(lo) > r >= above(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (above(mid) > r) lo = mid;
+      else hi = mid;
+    }
+    work = lo;
+    int j = r - above(lo + 1);
+    seq = 0;
+    bool found = false;
+#pragma unroll
+    for (int c = 0; c < kLaneSeqs; ++c) {
+      if (c * 64 < n && !found) {
+        const uint64_t m = __ballot(nb[c] > lo);
+        const int cnt = __popcll(m);
+        if (j < cnt) {
+          const bool mine = (m >> lane & 1) && __popcll(m & ((1ull << lane) - 1)) == j;
+          seq = c * 64 + __builtin_ctzll(__ballot(mine));
+          found = true;
+        }
+        j -= cnt;
+      }
+    }
+    packed_bounds(off, total, __builtin_amdgcn_readfirstlane(seq), out.start, out.len);
+    out.nb = (out.len + BM - 1) / BM;
+  } else {
+    // The last sequence whose first slot is at or before r, 64 at a time.
+    const int first = off[0];
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) / 64, s = lo + lane * step;
+      const bool at = s < hi && (int64_t)max(off[min(s, n)] - first, 0) / BM + s <= r;
+      const int cnt = max(__popcll(__ballot(at)), 1);
+      lo += (cnt - 1) * step;
+      hi = min(hi, lo + step);
+    }
+    seq = __builtin_amdgcn_readfirstlane(lo);
+    packed_bounds(off, total, seq, out.start, out.len);
+    const int64_t b = r - ((int64_t)max(off[seq] - first, 0) / BM + seq);
+    out.nb = (out.len + BM - 1) / BM;
+    if (b < 0 || b >= out.nb) return false;
+    work = out.nb - 1 - (int)b;
+  }
+  out.start = __builtin_amdgcn_readfirstlane(out.start);
+  out.len = __builtin_amdgcn_readfirstlane(out.len);
+  out.nb = __builtin_amdgcn_readfirstlane(out.nb);
+  out.work = __builtin_amdgcn_readfirstlane(work);
+  return true;
+}
+
+// The sequence that token t lies in; false: none.
+__device__ __forceinline__ bool packed_seq(const int32_t* off, int n, int total, int t, int& start, int& len) {
+  int lo = 0, hi = n;  // the last s with off[s] <= t
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (off[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  packed_bounds(off, total, lo, start, len);
+  return t >= start && t < start + len;
+}
+
+// Slots per head of a packed call (host): blocks of BM rows at most.
+inline int64_t packed_slots(int64_t total, int64_t n, int BM) { return total / BM + (n < total ? n : total); }
+
+// (head, slot) of a workgroup.  Workgroups are dealt to the 8 XCDs in turn;
+// with heads divisible by 8 each XCD takes a run of neighbouring heads, which
+// share K and V under grouped queries, four at a time side by side.
+__device__ __forceinline__ void packed_head(int id, int heads, int slots, int& head, int& slot) {
+  if ((heads & 7) == 0) {
+    const int per = heads >> 3, hg = (per & 3) == 0 ? 4 : (per & 1) == 0 ? 2 : 1;
+    const int i = id >> 3, r = i % (hg * slots);
+    head = (id & 7) * per + i / (hg * slots) * hg + r % hg;
+    slot = r / hg;
+  } else {
+    head = id % heads;
+    slot = id / heads;
+  }
+}
+
+// Points the params at the rows of one sequence (batch 1): SIZE-byte elements.
+template <int SIZE>
+__device__ __forceinline__ void packed_shift(SdpaParams& p, int start, int len) {
+  auto at = [&](auto*& ptr, int64_t stride) {
+    ptr = reinterpret_cast<std::remove_reference_t<decltype(ptr)>>(
+        reinterpret_cast<uintptr_t>(ptr) + (int64_t)start * stride * SIZE);
+  };
+  at(p.q, p.qs[2]);
+  at(p.k, p.ks[2]);
+  at(p.v, p.vs[2]);
+  at(p.out, p.os[2]);
+  if (p.lse) p.lse += start;
+  p.Tq = p.Tk = len;
+}
+template <int SIZE>
+__device__ __forceinline__ void packed_shift(SdpaBwdParams& p, int start, int len) {
+  auto at = [&](auto*& ptr, int64_t stride) {
+    ptr = reinterpret_cast<std::remove_reference_t<decltype(ptr)>>(
+        reinterpret_cast<uintptr_t>(ptr) + (int64_t)start * stride * SIZE);
+  };
+  at(p.q, p.qs[2]);
+  at(p.k, p.ks[2]);
+  at(p.v, p.vs[2]);
+  at(p.o, p.os[2]);
+  at(p.dout, p.dos[2]);
+  at(p.dq, p.dqs[2]);
+  at(p.dk, p.dks[2]);
+  at(p.dv, p.dvs[2]);
+  p.lse += start;
+  p.delta += start;
+  p.Tq = p.Tk = len;
+}
+
+// Rows of lse and delta from one head to the next.
+template <bool PACKED, class Params>
+__device__ __forceinline__ int row_pitch(const Params& p) {
+  if constexpr (PACKED) return p.total;
+  else return p.Tq;
+}
+
+// The kernels' packed instances (batch 1, Tq = Tk = the tokens, no mask).
+int launch_packed_flash16(const SdpaParams& p, hipStream_t s);
+int launch_packed_f32(const SdpaParams& p, hipStream_t s);
+int launch_packed_generic(const SdpaParams& p, hipStream_t s);
+int launch_packed_bwd_mfma(const SdpaBwdParams& p, hipStream_t s);
+int launch_packed_bwd_f32(const SdpaBwdParams& p, hipStream_t s);
+int launch_packed_bwd_generic(const SdpaBwdParams& p, hipStream_t s);
+// Copies a [1, H, total, D] tensor into rows of dp features (or back, rows in
+// a sequence only).
+int packed_pad_rows(const void* src, void* dst, const SdpaBwdParams& p, int H, int dp, const int64_t* st, bool unpad,
+                    hipStream_t s);
+
+}  // namespace mfx

@@ -137,6 +137,30 @@ class SdpaBwdArgs(ctypes.Structure):
     ]
 
 
+I64x3 = ctypes.c_int64 * 3
+
+
+class SdpaPackedArgs(ctypes.Structure):
+    """mfx_sdpa_packed_args (include/mfx_kernels.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "seq_offsets", "lse")]
+                + [(n, ctypes.c_int64) for n in ("T", "num_seqs", "Hq", "Hkv", "D")]
+                + [(n, I64x3) for n in ("q_strides", "k_strides", "v_strides", "o_strides")]
+                + [("scale", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("causal", "dtype", "reserved")])
+
+
+class SdpaPackedBwdArgs(ctypes.Structure):
+    """mfx_sdpa_packed_bwd_args (include/mfx_kernels.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout", "out", "lse", "dq", "dk", "dv", "seq_offsets",
+                                                "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int64) for n in ("T", "num_seqs", "Hq", "Hkv", "D")]
+                + [(n, I64x3) for n in ("q_strides", "k_strides", "v_strides", "do_strides", "o_strides",
+                                        "dq_strides", "dk_strides", "dv_strides")]
+                + [("scale", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("causal", "dtype", "reserved")])
+
+
 class QkNormRopeArgs(ctypes.Structure):
     """mfx_qk_norm_rope_args (include/mfx_kernels.h)."""
 
@@ -289,6 +313,13 @@ def load(path: str | os.PathLike | None = None, make_default: bool = False) -> c
     lib.mfx_sdpa_workspace_size.restype = ctypes.c_size_t
     lib.mfx_sdpa_kernel_name.argtypes = [ctypes.POINTER(SdpaArgs)]
     lib.mfx_sdpa_kernel_name.restype = ctypes.c_char_p
+    for name, args in (("mfx_sdpa_packed", SdpaPackedArgs), ("mfx_sdpa_packed_bwd", SdpaPackedBwdArgs)):
+        getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name + "_kernel_name").argtypes = [ctypes.POINTER(args)]
+        getattr(lib, name + "_kernel_name").restype = ctypes.c_char_p
+    lib.mfx_sdpa_packed_bwd_workspace_size.argtypes = [ctypes.POINTER(SdpaPackedBwdArgs)]
+    lib.mfx_sdpa_packed_bwd_workspace_size.restype = ctypes.c_size_t
     lib.mfx_rope_freqs.argtypes = [ctypes.c_double, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]
     lib.mfx_rope_freqs.restype = ctypes.c_int
     lib.mfx_qk_norm_rope.argtypes = [ctypes.POINTER(QkNormRopeArgs), ctypes.c_void_p]
@@ -615,7 +646,7 @@ def sdpa_bwd_workspace_size(q, k, v, **kw) -> int:
     return int(load().mfx_sdpa_bwd_workspace_size(ctypes.byref(a)))
 
 
-# ---- query / key norm with rotation ----------------------------------------------
+# ---- helpers of the operators below ----------------------------------------------
 
 def _on(t, *others):
     """Context in which work for t's device is launched: t's device made the
@@ -633,6 +664,129 @@ def _on(t, *others):
 def _ptr(t):
     return t.data_ptr() if t is not None else 0
 
+
+def _workspace(a, query, workspace, like):
+    """Sets a.workspace: the caller's, or one from torch's allocator for this
+    call (also inside a captured graph, whose pool then owns it)."""
+    if workspace is None:
+        need = int(getattr(load(), query)(ctypes.byref(a)))
+        if not need:
+            return None
+        workspace = _torch().empty(need, dtype=_torch().uint8, device=like.device)
+    a.workspace = workspace.data_ptr()
+    a.workspace_bytes = workspace.numel() * workspace.element_size()
+    return workspace
+
+
+# ---- packed sequences ------------------------------------------------------------
+
+_PACKED_PACK = struct.Struct("6P5q12qf3i").pack
+_PACKED_BWD_PACK = struct.Struct("11PN5q24qf3i").pack
+
+
+def _packed_dims(q, k, v, seq_offsets, *like_q):
+    """(T, sequences, Hq, Hkv, D) of checked [T, H, D] tensors."""
+    torch = _torch()
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("packed q, k and v are [T, heads, head size]")
+    T, Hq, D = q.shape
+    if k.shape != v.shape or k.shape[0] != T or k.shape[2] != D:
+        raise ValueError("k and v must agree with each other and with q in tokens and head size")
+    for t in (k, v, *like_q):
+        if t.dtype != q.dtype:
+            raise ValueError("packed tensors must share one dtype")
+    for t in like_q:
+        if t.shape != q.shape:
+            raise ValueError("out and its gradient must have q's shape")
+    if seq_offsets.dtype != torch.int32 or seq_offsets.dim() != 1 or not seq_offsets.is_contiguous():
+        raise TypeError("seq_offsets must be a contiguous int32 vector")
+    if seq_offsets.numel() < 1:
+        raise ValueError("seq_offsets has one more entry than there are sequences")
+    return T, seq_offsets.numel() - 1, Hq, k.shape[1], D
+
+
+def _htd(t):
+    s = t.stride()
+    return s[1], s[0], s[2]
+
+
+def _packed_lse(lse, Hq, T):
+    if lse.dtype != _torch().float32 or lse.numel() != Hq * T or not lse.is_contiguous():
+        raise ValueError("lse must be a contiguous f32 tensor of [heads, tokens]")
+
+
+def sdpa_packed_args(q, k, v, out, seq_offsets, *, scale=None, causal=True, lse=None) -> SdpaPackedArgs:
+    dims = _packed_dims(q, k, v, seq_offsets, out)
+    if lse is not None:
+        _packed_lse(lse, dims[2], dims[0])
+    return SdpaPackedArgs.from_buffer_copy(_PACKED_PACK(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), seq_offsets.data_ptr(), _ptr(lse), *dims, *_htd(q),
+        *_htd(k), *_htd(v), *_htd(out), _f32(1.0 / (dims[4] ** 0.5) if scale is None else scale), 1 if causal else 0,
+        dtype_code(q.dtype), 0))
+
+
+def sdpa_packed(q, k, v, seq_offsets, *, scale=None, causal=True, out=None, lse=None):
+    """Attention over packed sequences (mfx_sdpa_packed): q [T, Hq, D], k and v
+    [T, Hkv, D], sequence s the tokens seq_offsets[s] .. seq_offsets[s + 1]
+    (int32, on the device).  Rows in no sequence are not written (a fresh out
+    holds anything there).  lse: optional f32 [Hq, T] output for
+    sdpa_packed_bwd."""
+    torch = _torch()
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    a = sdpa_packed_args(q, k, v, out, seq_offsets, scale=scale, causal=causal, lse=lse)
+    with _on(q, k, v, out, seq_offsets, lse):
+        check(load().mfx_sdpa_packed(ctypes.byref(a), _stream_handle(q)))
+    return out
+
+
+def sdpa_packed_kernel_name(q, k, v, seq_offsets, **kw) -> str:
+    """Which kernel mfx_sdpa_packed picks for these tensors (host-only query)."""
+    name = load().mfx_sdpa_packed_kernel_name(ctypes.byref(sdpa_packed_args(q, k, v, q, seq_offsets, **kw)))
+    if name is None:
+        raise MfxError(-1, load().mfx_last_error().decode())
+    return name.decode()
+
+
+def sdpa_packed_bwd_args(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, *, scale=None,
+                         causal=True) -> SdpaPackedBwdArgs:
+    dims = _packed_dims(q, k, v, seq_offsets, dout, out, dq)
+    _packed_lse(lse, dims[2], dims[0])
+    if dk.shape != k.shape or dv.shape != v.shape or dk.dtype != q.dtype or dv.dtype != q.dtype:
+        raise ValueError("dk and dv must match k and v")
+    return SdpaPackedBwdArgs.from_buffer_copy(_PACKED_BWD_PACK(
+        *[t.data_ptr() for t in (q, k, v, dout, out, lse, dq, dk, dv, seq_offsets)], 0, 0, *dims,
+        *[x for t in (q, k, v, dout, out, dq, dk, dv) for x in _htd(t)],
+        _f32(1.0 / (dims[4] ** 0.5) if scale is None else scale), 1 if causal else 0, dtype_code(q.dtype), 0))
+
+
+def sdpa_packed_bwd(q, k, v, dout, out, lse, seq_offsets, *, scale=None, causal=True, dq=None, dk=None, dv=None,
+                    workspace=None):
+    """(dq, dk, dv) of sdpa_packed for the gradient dout of its output, from
+    its out and lse (mfx_sdpa_packed_bwd).  Rows in no sequence are not
+    written."""
+    torch = _torch()
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if g is None else g
+                  for t, g in ((q, dq), (k, dk), (v, dv)))
+    a = sdpa_packed_bwd_args(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, scale=scale, causal=causal)
+    with _on(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, workspace):
+        keep = _workspace(a, "mfx_sdpa_packed_bwd_workspace_size", workspace, q)  # noqa: F841 (until the launch)
+        check(load().mfx_sdpa_packed_bwd(ctypes.byref(a), _stream_handle(q)))
+    return dq, dk, dv
+
+
+def sdpa_packed_bwd_kernel_name(q, k, v, seq_offsets, **kw) -> str:
+    """Which backward kernels mfx_sdpa_packed_bwd picks (host-only query)."""
+    torch = _torch()
+    lse = torch.empty(q.shape[1], q.shape[0])
+    name = load().mfx_sdpa_packed_bwd_kernel_name(
+        ctypes.byref(sdpa_packed_bwd_args(q, k, v, q, q, lse, q, k, v, seq_offsets, **kw)))
+    if name is None:
+        raise MfxError(-1, load().mfx_last_error().decode())
+    return name.decode()
+
+
+# ---- query / key norm with rotation ----------------------------------------------
 
 def rope_table(rot: int, theta: float = 10000.0, *, inv_freq=None, device="cuda"):
     """The frequencies of a rotation of `rot` features, as qk_norm_rope takes
@@ -776,19 +930,6 @@ def qk_norm_rope_bwd(q, k, dq_out, dk_out, positions, table, *, q_weight=None, k
         keep = _workspace(a, "mfx_qk_norm_rope_bwd_workspace_size", workspace, first)  # noqa: F841 (until the launch)
         check(load().mfx_qk_norm_rope_bwd(ctypes.byref(a), _stream_handle(first)))
     return dq, dk, dqw, dkw
-
-
-def _workspace(a, query, workspace, like):
-    """Sets a.workspace: the caller's, or one from torch's allocator for this
-    call (also inside a captured graph, whose pool then owns it)."""
-    if workspace is None:
-        need = int(getattr(load(), query)(ctypes.byref(a)))
-        if not need:
-            return None
-        workspace = _torch().empty(need, dtype=_torch().uint8, device=like.device)
-    a.workspace = workspace.data_ptr()
-    a.workspace_bytes = workspace.numel() * workspace.element_size()
-    return workspace
 
 
 # ---- GEMM ----------------------------------------------------------------------
