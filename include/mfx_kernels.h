@@ -711,6 +711,77 @@ int mfx_gemm(const mfx_gemm_args* args, void* stream);
  * traces. */
 const char* mfx_gemm_kernel_name(const mfx_gemm_args* args);
 
+/*
+ * Softmax cross entropy of a linear head over a large vocabulary, the logits
+ * z = h W^T [T, V] never stored:
+ *   lse[t] = log(sum_v exp(z[t, v])),   loss[t] = lse[t] - z[t, targets[t]]
+ * h [T, H] and w [V, H] in `dtype` (f32, bf16, f16), rows spaced h_stride /
+ * w_stride elements; fp32 products and sums.  targets int32 or int64
+ * (target_dtype MFX_I32 / MFX_I64); a row whose target lies outside [0, V)
+ * does not count: its loss is 0 and it adds nothing to any gradient.  loss and
+ * lse (optional) are fp32 [T].  Not rounded between: what
+ * mfx_gemm, then mfx_log_softmax and a gather give without their roundings.
+ * Rows must be 16-byte aligned and H a multiple of 16 bytes.
+ * workspace: mfx_linear_xent_workspace_size() bytes, 256-byte aligned (8 bytes
+ * per row and tile of 128 or 256 columns), or NULL for library scratch.
+ * The reference's models form the logits and their log_softmax (callee
+ * @log_softmax, src/jax_mlx_pjrt.cpp:5624-5641).
+ */
+typedef struct {
+  const void* h;
+  const void* w;
+  const void* targets;
+  float* loss;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t T, H, V;
+  int64_t h_stride;
+  int64_t w_stride;
+  int32_t dtype;
+  int32_t target_dtype;
+} mfx_linear_xent_args;
+
+int mfx_linear_xent(const mfx_linear_xent_args* args, void* stream);
+
+size_t mfx_linear_xent_workspace_size(const mfx_linear_xent_args* args);
+
+/*
+ * Backward of mfx_linear_xent for the gradients dloss[T] (fp32) of the losses,
+ * from the forward's lse:
+ *   d = (exp(z - lse) - onehot(targets)) * dloss,   dh = d W,   dw = d^T h
+ * dh [T, H] of `dtype`, dw [V, H] of `dw_dtype` (`dtype` or MFX_F32); either
+ * may be NULL.  d is formed in pieces of the vocabulary (at most 512 MiB of it,
+ * or 256 columns) and rounded to `dtype`, in f16 times a power of two that
+ * fits the largest |dloss|.  Outputs must not share memory with the inputs.
+ * workspace: mfx_linear_xent_bwd_workspace_size() bytes, 256-byte aligned, or
+ * NULL for library scratch.  Deterministic: no atomics.
+ */
+typedef struct {
+  const void* h;
+  const void* w;
+  const void* targets;
+  const float* lse;
+  const float* dloss;
+  void* dh;
+  void* dw;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t T, H, V;
+  int64_t h_stride;
+  int64_t w_stride;
+  int64_t dh_stride;
+  int64_t dw_stride;
+  int32_t dtype;
+  int32_t target_dtype;
+  int32_t dw_dtype;
+  int32_t reserved;
+} mfx_linear_xent_bwd_args;
+
+int mfx_linear_xent_bwd(const mfx_linear_xent_bwd_args* args, void* stream);
+
+size_t mfx_linear_xent_bwd_workspace_size(const mfx_linear_xent_bwd_args* args);
+
 /* GEMM with a fused elementwise epilogue: out = epi(inputs) where epi's
  * input `c_input` is the GEMM result C = A B, read at the program's output
  * index (contiguous strides, fp32; its data pointer and gemm->c are

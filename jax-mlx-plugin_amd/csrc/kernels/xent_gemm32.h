@@ -1,0 +1,113 @@
+// The f32 product kernel of the linear cross entropy: C[m][n] = sum_k A(m, k)
+// B(n, k) on v_mfma_f32_32x32x2_f32, operands stored as in xent_gemm16.h, 128 x
+// 128 tiles of 32 k by 4 wavefronts of 64 x 64.
+//
+// A 32x32x2 product takes 64 cycles, so a tile's 16 products per 8 k and
+// wavefront leave 1024 cycles for 4 to 16 LDS reads: plain double buffering
+// (global -> registers -> LDS, one barrier a tile) keeps the matrix cores fed.
+// The k of products are permuted alike in both operands: step e of 8 k takes k =
+// half * 4 + e, so a k-contiguous row gives four steps in one 16-byte read.
+// Rows padded by 16 bytes (k-contiguous) or 32 (index-contiguous, whose two
+// halves read rows 4 apart) keep the reads off each other's banks.
+#pragma once
+
+#include "xent_tiles.h"
+
+namespace mfx {
+namespace xent {
+
+template <bool KC>
+struct Tile32 {
+  static constexpr int IDX = 128, NT = 256;
+  static constexpr int ROW = KC ? kBK32 + 4 : IDX + 8;        // floats
+  static constexpr int CPR = KC ? kBK32 / 4 : IDX / 4;        // 16-byte chunks per row
+  static constexpr int CH = IDX * kBK32 / 4 / NT;             // chunks per thread: 4
+  const float* p;
+  int64_t ld;
+  int idx0, total, K;
+  f32x4 r[CH];
+  __device__ __forceinline__ Tile32(const Operand& o, int i0, int n, int k)
+      : p(static_cast<const float*>(o.p)), ld(o.ld), idx0(i0), total(n), K(k) {}
+  // (K and an index-contiguous operand's rows are whole chunks, K % 4 == 0 and
+  // total % 4 == 0 or the row padded to it: checked on the host.)
+  __device__ __forceinline__ void load(int kt) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int c = threadIdx.x + i * NT, row = c / CPR, col = c % CPR * 4;
+      const int idx = idx0 + (KC ? row : col), k = kt * kBK32 + (KC ? col : row);
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      if (idx < total && k < K) v = *reinterpret_cast<const f32x4*>(p + (KC ? idx * ld + k : k * ld + idx));
+      r[i] = v;
+    }
+  }
+  __device__ __forceinline__ void store(float* lds) const {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int c = threadIdx.x + i * NT, row = c / CPR, col = c % CPR * 4;
+      *reinterpret_cast<f32x4*>(lds + row * ROW + col) = r[i];
+    }
+  }
+};
+
+// The four k of step c (of 8) that this lane's half holds, for index `idx`.
+template <bool KC>
+__device__ __forceinline__ f32x4 frag32(const float* lds, int idx, int c, int half) {
+  constexpr int ROW = Tile32<KC>::ROW;
+  const int k = c * 8 + half * 4;
+  if constexpr (KC) return *reinterpret_cast<const f32x4*>(lds + idx * ROW + k);
+  else return f32x4{lds[k * ROW + idx], lds[(k + 1) * ROW + idx], lds[(k + 2) * ROW + idx], lds[(k + 3) * ROW + idx]};
+}
+
+template <class C>
+__device__ __forceinline__ void gemm_tile32(const GemmShape& g, int m0, int n0, int kt0, int kt1, float* smem,
+                                            Acc<C>& acc) {
+  static_assert(C::BM == 128 && C::BN == 128 && C::NT == 256, "one tile form");
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+  const int wm = wave % C::WM, wn = wave / C::WM;
+  Tile32<C::A_KC> ta(g.a, m0, g.M, g.K);
+  Tile32<C::B_KC> tb(g.b, n0, g.N, g.K);
+  constexpr int HALF = C::STAGE / 8;  // floats of one operand's tile
+#pragma unroll
+  for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
+  ta.load(kt0);
+  tb.load(kt0);
+  ta.store(smem);
+  tb.store(smem + HALF);
+  __syncthreads();
+  for (int kt = kt0; kt < kt1; ++kt) {
+    const float* at = smem + ((kt - kt0) & 1) * 2 * HALF;
+    const float* bt = at + HALF;
+    float* const next = smem + ((kt - kt0 + 1) & 1) * 2 * HALF;
+    if (kt + 1 < kt1) {
+      ta.load(kt + 1);
+      tb.load(kt + 1);
+    }
+#pragma unroll
+    for (int c = 0; c < kBK32 / 8; ++c) {
+      f32x4 fa[C::FM], fb[C::FN];
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i) fa[i] = frag32<C::A_KC>(at, (wm * C::FM + i) * 32 + l32, c, half);
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j) fb[j] = frag32<C::B_KC>(bt, (wn * C::FN + j) * 32 + l32, c, half);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+          for (int i = 0; i < C::FM; ++i)
+            acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j][e], fa[i][e], acc[j][i], 0, 0, 0);
+    }
+    if (kt + 1 < kt1) {
+      ta.store(next);
+      tb.store(next + HALF);
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace xent
+}  // namespace mfx

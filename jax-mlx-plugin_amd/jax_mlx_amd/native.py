@@ -16,6 +16,7 @@ LIB_DIR = Path(__file__).resolve().parent / "lib"
 KERNELS_LIB = LIB_DIR / "libmfx_kernels.so"
 
 MFX_F32, MFX_BF16, MFX_F16 = 0, 1, 2
+MFX_I32, MFX_I64 = 3, 5
 MFX_OK = 0
 
 
@@ -211,6 +212,24 @@ class GemmArgs(ctypes.Structure):
     ]
 
 
+class LinearXentArgs(ctypes.Structure):
+    """mfx_linear_xent_args (include/mfx_kernels.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("h", "w", "targets", "loss", "lse", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int64) for n in ("T", "H", "V", "h_stride", "w_stride")]
+                + [(n, ctypes.c_int32) for n in ("dtype", "target_dtype")])
+
+
+class LinearXentBwdArgs(ctypes.Structure):
+    """mfx_linear_xent_bwd_args (include/mfx_kernels.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("h", "w", "targets", "lse", "dloss", "dh", "dw", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int64) for n in ("T", "H", "V", "h_stride", "w_stride", "dh_stride", "dw_stride")]
+                + [(n, ctypes.c_int32) for n in ("dtype", "target_dtype", "dw_dtype", "reserved")])
+
+
 MFX_MAX_RANK = 8
 MFX_EW_MAX_INPUTS = 8
 MFX_EW_MAX_INSTRS = 64
@@ -313,6 +332,11 @@ def load(path: str | os.PathLike | None = None, make_default: bool = False) -> c
     lib.mfx_sdpa_workspace_size.restype = ctypes.c_size_t
     lib.mfx_sdpa_kernel_name.argtypes = [ctypes.POINTER(SdpaArgs)]
     lib.mfx_sdpa_kernel_name.restype = ctypes.c_char_p
+    for name, args in (("mfx_linear_xent", LinearXentArgs), ("mfx_linear_xent_bwd", LinearXentBwdArgs)):
+        getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name + "_workspace_size").argtypes = [ctypes.POINTER(args)]
+        getattr(lib, name + "_workspace_size").restype = ctypes.c_size_t
     for name, args in (("mfx_sdpa_packed", SdpaPackedArgs), ("mfx_sdpa_packed_bwd", SdpaPackedBwdArgs)):
         getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
         getattr(lib, name).restype = ctypes.c_int
@@ -930,6 +954,85 @@ def qk_norm_rope_bwd(q, k, dq_out, dk_out, positions, table, *, q_weight=None, k
         keep = _workspace(a, "mfx_qk_norm_rope_bwd_workspace_size", workspace, first)  # noqa: F841 (until the launch)
         check(load().mfx_qk_norm_rope_bwd(ctypes.byref(a), _stream_handle(first)))
     return dq, dk, dqw, dkw
+
+
+# ---- cross entropy of a linear head ----------------------------------------------
+
+_XENT_PACK = struct.Struct("6PN5q2i").pack
+_XENT_BWD_PACK = struct.Struct("8PN7q4i").pack
+
+
+def _xent_dims(h, w, targets):
+    """((T, H, V), h_stride, w_stride, dtype, target dtype) of checked tensors."""
+    torch = _torch()
+    if w.dim() != 2 or h.dim() < 2 or w.shape[1] != h.shape[-1]:
+        raise ValueError("h is [..., H] and w [V, H]")
+    if w.dtype != h.dtype:
+        raise ValueError("h and w must share one dtype")
+    if targets.shape != h.shape[:-1] or not targets.is_contiguous():
+        raise ValueError("targets must be contiguous, one for each row of h")
+    if targets.dtype not in (torch.int32, torch.int64):
+        raise TypeError("targets must be int32 or int64")
+    if w.stride(1) != 1:
+        raise ValueError("last dimension must be contiguous")
+    T, H, hs = _rows_view(h)
+    # (One row may carry any stride.)
+    return ((T, H, w.shape[0]), hs if T > 1 else H, w.stride(0) if w.shape[0] > 1 else H, dtype_code(h.dtype),
+            MFX_I64 if targets.dtype == torch.int64 else MFX_I32)
+
+
+def _f32_rows(name, t, like):
+    if t.dtype != _torch().float32 or t.shape != like.shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous f32 tensor of the targets' shape")
+
+
+def linear_xent(h, w, targets, *, loss=None, lse=None, workspace=None):
+    """(loss, lse) of softmax cross entropy with logits h w^T, which are never
+    stored (mfx_linear_xent): h [..., H], w [V, H], targets [...] int32 or
+    int64.  A target outside [0, V) marks a row that does not count (loss 0).
+    loss and lse are f32 of the targets' shape."""
+    torch = _torch()
+    dims, hs, ws, code, tcode = _xent_dims(h, w, targets)
+    if loss is None:
+        loss = torch.empty(targets.shape, dtype=torch.float32, device=h.device)
+    if lse is None:
+        lse = torch.empty(targets.shape, dtype=torch.float32, device=h.device)
+    _f32_rows("loss", loss, targets)
+    _f32_rows("lse", lse, targets)
+    a = LinearXentArgs.from_buffer_copy(_XENT_PACK(h.data_ptr(), w.data_ptr(), targets.data_ptr(), loss.data_ptr(),
+                                                   lse.data_ptr(), 0, 0, *dims, hs, ws, code, tcode))
+    with _on(h, w, targets, loss, lse, workspace):
+        keep = _workspace(a, "mfx_linear_xent_workspace_size", workspace, h)  # noqa: F841 (until the launch)
+        check(load().mfx_linear_xent(ctypes.byref(a), _stream_handle(h)))
+    return loss, lse
+
+
+def linear_xent_bwd(h, w, targets, lse, dloss, *, need_dh=True, need_dw=True, dw_dtype=None, dh=None, dw=None,
+                    workspace=None):
+    """(dh, dw) of linear_xent for the gradients dloss of its losses, from its
+    lse (mfx_linear_xent_bwd).  dw has w's dtype or `dw_dtype` (f32); one not
+    needed is None and costs nothing."""
+    torch = _torch()
+    dims, hs, ws, code, tcode = _xent_dims(h, w, targets)
+    _f32_rows("lse", lse, targets)
+    _f32_rows("dloss", dloss, targets)
+    if dh is None and need_dh:
+        dh = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    if dw is None and need_dw:
+        dw = torch.empty(w.shape, dtype=dw_dtype or w.dtype, device=w.device)
+    if dh is not None and (dh.shape != h.shape or dh.dtype != h.dtype):
+        raise ValueError("dh must match h")
+    if dw is not None and (dw.shape != w.shape or dw.stride(1) != 1):
+        raise ValueError("dw must match w")
+    dhs = _rows_view(dh)[2] if dh is not None and dims[0] > 1 else dims[1]
+    dws = dw.stride(0) if dw is not None and dims[2] > 1 else dims[1]
+    a = LinearXentBwdArgs.from_buffer_copy(_XENT_BWD_PACK(
+        h.data_ptr(), w.data_ptr(), targets.data_ptr(), lse.data_ptr(), dloss.data_ptr(), _ptr(dh), _ptr(dw), 0, 0,
+        *dims, hs, ws, dhs, dws, code, tcode, dtype_code(dw.dtype) if dw is not None else code, 0))
+    with _on(h, w, targets, lse, dloss, dh, dw, workspace):
+        keep = _workspace(a, "mfx_linear_xent_bwd_workspace_size", workspace, h)  # noqa: F841 (until the launch)
+        check(load().mfx_linear_xent_bwd(ctypes.byref(a), _stream_handle(h)))
+    return dh, dw
 
 
 # ---- GEMM ----------------------------------------------------------------------
