@@ -34,7 +34,7 @@ namespace xent {
 
 // Wide tiles for what fills the device with them, else narrow ones.
 template <bool A_KC, bool B_KC, int E>
-using Wide = Config<256, 256, 2, 4, A_KC, B_KC, E>;
+using Wide = Config<256, 256, 2, 2, A_KC, B_KC, E>;
 template <bool A_KC, bool B_KC, int E>
 using Narrow = Config<128, 128, 2, 2, A_KC, B_KC, E>;
 
@@ -80,10 +80,13 @@ __device__ __forceinline__ int64_t target_of(const void* t, int wide, int row) {
   return wide ? static_cast<const int64_t*>(t)[row] : static_cast<const int32_t*>(t)[row];
 }
 
+// Column, within a wavefront's, of accumulator element e of block j.
+__device__ __forceinline__ int column(int j, int e, int half) { return j * 32 + (e >> 2) * 8 + half * 4 + (e & 3); }
+
 // ---- the logits' tiles -------------------------------------------------------
 
 template <class C, bool BWD>
-__global__ __launch_bounds__(C::NT, 2) void xent_logits_kernel(LossArgs p) {
+__global__ __launch_bounds__(C::NT, C::WAVES) void xent_logits_kernel(LossArgs p) {
   constexpr int FM = C::FM, FN = C::FN;
   __shared__ __attribute__((aligned(16))) char smem[C::SMEM];
   int tm, tn;
@@ -98,38 +101,67 @@ __global__ __launch_bounds__(C::NT, 2) void xent_logits_kernel(LossArgs p) {
   const int wm = wave % C::WM, wn = wave / C::WM;
   const int M = p.g.M, N = p.g.N;
   const int nw = n0 + wn * FN * 32;  // this wavefront's first column (of the piece)
+  // Block i's values, -inf in columns past N (of which only the last tile has
+  // any): 16 FN registers at a time, and the fences between blocks keep it so.
+  auto block = [&](int i, auto edge_tag, float (&z)[FN * 16]) __attribute__((always_inline)) {
+    fence();
+    int left = N - nw - half * 4;  // (opaque, so that no comparison is kept from block to block)
+    asm volatile("" : "+v"(left));
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        z[j * 16 + e] = acc[j][i][e];
+        if (decltype(edge_tag)::value && column(j, e, 0) >= left) z[j * 16 + e] = -INFINITY;
+      }
+  };
+  // The logit of this lane's column `t` (one of two lanes has it): few rows
+  // have their target in a wavefront's columns, so the others need not look.
+  auto pick = [&](const float (&z)[FN * 16], int64_t t, bool& mine) __attribute__((always_inline)) {
+    const int n = (int)(t - nw) - half * 4;
+    float x = 0.f;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x = column(j, e, 0) == n ? z[j * 16 + e] : x;
+    mine = n >= 0 && n < FN * 32 && (n & 4) == 0;
+    return x;
+  };
+  auto here = [&](int64_t t) { return __ballot(t >= nw && t < nw + FN * 32) != 0; };
 
   if constexpr (!BWD) {
     float* const red_m = reinterpret_cast<float*>(smem);  // [WN][BM]
     float* const red_l = red_m + C::WN * C::BM;
+    auto fold = [&](auto edge_tag) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int r = wm * FM * 32 + i * 32 + l32, row = m0 + r;
-      const int64_t t = row < M ? target_of(p.targets, p.target64, row) : -1;
-      float mx = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int n = nw + j * 32 + (e >> 2) * 8 + half * 4 + (e & 3);
-          const float z = acc[j][i][e];
-          if (n == t) p.picked[row] = z;
-          acc[j][i][e] = n < N ? z * kLog2e : -INFINITY;
-          mx = fmaxf(mx, acc[j][i][e]);
+      for (int i = 0; i < FM; ++i) {
+        const int r = wm * FM * 32 + i * 32 + l32, row = m0 + r;
+        const int64_t t = row < M ? target_of(p.targets, p.target64, row) : -1;
+        float z[FN * 16];
+        block(i, edge_tag, z);
+        if (here(t)) {
+          bool mine;
+          const float x = pick(z, t, mine);
+          if (mine) p.picked[row] = x;
         }
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float base = mx == -INFINITY ? 0.f : mx;
-      float l = 0.f;
+        float mx = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
+        for (int e = 0; e < FN * 16; ++e) mx = fmaxf(mx, z[e]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float base = mx == -INFINITY ? 0.f : mx * kLog2e;
+        float l[2] = {0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 16; ++e) l += __builtin_amdgcn_exp2f(acc[j][i][e] - base);
-      l += __shfl_xor(l, 32, 64);
-      if (half == 0) {
-        red_m[wn * C::BM + r] = mx;
-        red_l[wn * C::BM + r] = l;
+        for (int e = 0; e < FN * 16; ++e) l[e & 1] += __builtin_amdgcn_exp2f(fmaf(z[e], kLog2e, -base));
+        l[0] += l[1];
+        l[0] += __shfl_xor(l[0], 32, 64);
+        if (half == 0) {
+          red_m[wn * C::BM + r] = mx == -INFINITY ? mx : base;
+          red_l[wn * C::BM + r] = l[0];
+        }
       }
-    }
+    };
+    if (n0 + C::BN > N) fold(std::true_type{});
+    else fold(std::false_type{});
     __syncthreads();
     for (int r = threadIdx.x; r < C::BM; r += C::NT) {
       if (m0 + r >= M) continue;
@@ -150,37 +182,53 @@ __global__ __launch_bounds__(C::NT, 2) void xent_logits_kernel(LossArgs p) {
     constexpr int CPR = FN * 4;    // chunks per row
     constexpr int RPS = 64 / CPR;  // rows per store instruction
     bf16* const st = reinterpret_cast<bf16*>(smem) + wave * (FM * 32) * (FN * 32);
+    auto turn = [&](auto edge_tag) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int r = i * 32 + l32, row = m0 + wm * FM * 32 + r;
-      const int64_t t = row < M ? target_of(p.targets, p.target64, row) : -1;
-      const bool counts = t >= 0 && t < p.V;
-      const float lse = row < M ? p.lse[row] : 0.f;
-      const float w = counts ? p.dloss[row] * s : 0.f;
+      for (int i = 0; i < FM; ++i) {
+        int l = l32;  // (opaque: no address of a later block is formed early)
+        asm volatile("" : "+v"(l));
+        const int r = i * 32 + l, row = m0 + wm * FM * 32 + r;
+        int64_t t = row < M ? target_of(p.targets, p.target64, row) : -1;
+        const bool counts = t >= 0 && t < p.V;
+        t = counts ? t - p.v0 : -1;
+        const float lse2 = row < M ? p.lse[row] * kLog2e : 0.f;
+        const float w = counts ? p.dloss[row] * s : 0.f;
+        auto prob = [&](float x) __attribute__((always_inline)) { return __builtin_amdgcn_exp2f(fmaf(x, kLog2e, -lse2)); };
+        float z[FN * 16];
+        block(i, edge_tag, z);
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float o[4];
+          for (int g = 0; g < 4; ++g) {
+            float o[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int n = nw + j * 32 + g * 8 + half * 4 + e;
-            // (Subtracted first: z and lse may be large where their distance is not.)
-            float d = __builtin_amdgcn_exp2f((acc[j][i][g * 4 + e] - lse) * kLog2e);
-            if (p.v0 + n == t) d -= 1.f;
-            o[e] = counts && n < N ? d * w : 0.f;
+            for (int e = 0; e < 4; ++e) o[e] = counts ? prob(z[j * 16 + g * 4 + e]) * w : 0.f;
+            if constexpr (C::E == 2) {
+              if (row < M)
+                *reinterpret_cast<f32x4*>(static_cast<float*>(p.d) + (int64_t)row * p.ldd + nw +
+                                          column(j, g * 4, half)) = f32x4{o[0], o[1], o[2], o[3]};
+            } else {
+              const int c = j * 4 + g;
+              *reinterpret_cast<u32x2*>(st + r * (FN * 32) + (c ^ (r & (CPR - 1))) * 8 + half * 4) =
+                  u32x2{pack2<C::E & 1>(o[0], o[1]), pack2<C::E & 1>(o[2], o[3])};
+            }
           }
-          if constexpr (C::E == 2) {
-            if (row < M)
-              *reinterpret_cast<f32x4*>(static_cast<float*>(p.d) + (int64_t)row * p.ldd + nw + j * 32 + g * 8 +
-                                        half * 4) = f32x4{o[0], o[1], o[2], o[3]};
-          } else {
-            const int c = j * 4 + g;
-            *reinterpret_cast<u16x4*>(st + r * (FN * 32) + (c ^ (r & (CPR - 1))) * 8 + half * 4) =
-                u16x4{store_e<C::E>(o[0]), store_e<C::E>(o[1]), store_e<C::E>(o[2]), store_e<C::E>(o[3])};
+        // The target's entry, over the one just written.
+        if (here(t)) {
+          bool mine;
+          const float d = (prob(pick(z, t, mine)) - 1.f) * w;
+          const int n = (int)t - nw;
+          if (mine) {
+            if constexpr (C::E == 2) static_cast<float*>(p.d)[(int64_t)row * p.ldd + t] = d;
+            else
+              reinterpret_cast<uint16_t*>(st)[r * (FN * 32) + ((n >> 3) ^ (r & (CPR - 1))) * 8 + (n & 7)] =
+                  store_e<C::E & 1>(d);
           }
         }
-    }
+      }
+    };
+    if (n0 + C::BN > N) turn(std::true_type{});
+    else turn(std::false_type{});
     if constexpr (C::E == 2) return;
     const int mw = m0 + wm * FM * 32;
 #pragma unroll
@@ -252,7 +300,7 @@ __global__ __launch_bounds__(1024) void xent_scale(const float* __restrict__ dlo
 // ---- the gradients' products -------------------------------------------------
 
 template <class C>
-__global__ __launch_bounds__(C::NT, 2) void xent_grad_kernel(StoreArgs p) {
+__global__ __launch_bounds__(C::NT, C::WAVES) void xent_grad_kernel(StoreArgs p) {
   constexpr int FM = C::FM, FN = C::FN;
   __shared__ __attribute__((aligned(16))) char smem[C::SMEM];
   const int ntiles = p.g.tiles_m * p.g.tiles_n;
@@ -420,7 +468,7 @@ int launch_logits(const LossArgs& p, bool wide, hipStream_t s) {
   if constexpr (E == 2) {
     hipLaunchKernelGGL((xent_logits_kernel<Full<true, true>, BWD>), grid, dim3(256), 0, s, p);
   } else {
-    if (wide) hipLaunchKernelGGL((xent_logits_kernel<Wide<true, true, E>, BWD>), grid, dim3(512), 0, s, p);
+    if (wide) hipLaunchKernelGGL((xent_logits_kernel<Wide<true, true, E>, BWD>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((xent_logits_kernel<Narrow<true, true, E>, BWD>), grid, dim3(256), 0, s, p);
   }
   return launch_status("xent_logits_kernel");
@@ -435,7 +483,7 @@ int launch_grad(StoreArgs& p, int64_t range, bool wide, hipStream_t s) {
   if constexpr (E == 2) {
     hipLaunchKernelGGL((xent_grad_kernel<Full<A_KC, false>>), grid, dim3(256), 0, s, p);
   } else {
-    if (wide) hipLaunchKernelGGL((xent_grad_kernel<Wide<A_KC, false, E>>), grid, dim3(512), 0, s, p);
+    if (wide) hipLaunchKernelGGL((xent_grad_kernel<Wide<A_KC, false, E>>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((xent_grad_kernel<Narrow<A_KC, false, E>>), grid, dim3(256), 0, s, p);
   }
   return launch_status("xent_grad_kernel");

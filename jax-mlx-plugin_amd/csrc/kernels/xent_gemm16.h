@@ -3,30 +3,33 @@
 //   C[m][n] = sum_k A(m, k) B(n, k)        fp32 accumulation
 //
 // Each operand is stored either k-contiguous, [index][k], or index-contiguous,
-// [k][index]; what happens to a tile's sums is the Epilogue's business (a
+// [k][index]; what happens to a tile's sums is the epilogue's business (a
 // softmax's partial sums, a gradient, a store).  As in gemm16.hip the kernel
 // computes C^T on v_mfma_f32_32x32x16 (its A operand taken from B): an
 // accumulator lane then holds one row m and 16 columns n, so a row's maximum
 // and sum need one exchange between two lanes.
 //
-// Schedule.  Tiles of BM x BN outputs and 64 k; 256 x 256 with 8 wavefronts
-// of 128 x 64 each.  Per 64 k a CU then reads 192 KB from LDS beside 2.1 us *
-// its matrix rate of products, 75% of what the LDS delivers in that time
-// (128 x 128 tiles with 64 x 64 a wavefront read it all and stop at 0.6-0.87
-// PFLOP/s).  Two LDS stages (64 KB each at 256 x 256) are filled by LDS-DMA.  A
-// k-tile is four steps of 16 k, the operands of step s + 1 read while step s
-// multiplies.  The barrier sits before the last step's products, when its
-// operands are in registers and the stage is free: behind it the next tile's
-// first operands are read and the DMA of the tile after goes into this stage,
-// both under those products.  So a k-tile's loads have a whole k-tile to
-// land, and no product waits for a first LDS read.
+// Tiles of 256 x 256 outputs by 4 wavefronts of 128 x 128 (one a SIMD, the sums
+// in its 256 accumulation registers): 8 operand reads feed 16 products, half of
+// what 64 x 64 a wavefront needs.  k advances by 32 through four LDS stages
+// of 32 KB filled by LDS-DMA three tiles ahead.
+//
+// Schedule.  With one wavefront a SIMD nothing hides a stall, so every
+// instruction that is not a product goes between two products, which occupy the
+// matrix core for 32 cycles each: the operand reads of the next 16 k between
+// the first products of a step, a tile's 8 loads one to two products (a CU takes
+// their requests at about 90 bytes a cycle; together they would wait for each
+// other).  The one barrier a tile falls between products of its last step, whose
+// operands are in registers by then: behind it the next tile's stage is read
+// and the stage of the tile before it is loaded.
 //
 // Range.  A buffer resource is built per tile with the tile's own 64-bit base
 // (so no operand's size is limited) and the bytes left in the operand; rows
 // past the operand's end read as zeros.  A k past K inside a k-contiguous row
 // is pointed out of range per lane; index-contiguous columns past the last
 // read a neighbour row's values and reach only outputs that the epilogue
-// drops.
+// drops.  Tiles past the last are loaded out of range, so that the number of
+// loads in flight, which the waits count, does not depend on the tile.
 #pragma once
 
 #include "sdpa_tiles.h"
@@ -40,63 +43,78 @@ using tiles::s16x4;
 using tiles::tile_swz;
 
 constexpr uint32_t kOOR = 0x80000000u;
+constexpr int kStages = 4;
+
+// A k-contiguous tile's rows are 64 bytes, four to the 64 banks: chunk c of row r
+// at c ^ kc_swz(r) spreads the 16 rows that a 16-byte read serves at a time.
+__device__ __forceinline__ int kc_swz(int r) { return (r >> 2) & 3; }
 
 // One operand's tiles: IDX indices of a tile, NW wavefronts sharing the loads.
-// KC: [IDX rows][64 k], 128 bytes a row, chunk c of row r at c ^ tile_swz<64>(r).
-// else: [64 k][IDX], chunk c of row r at c ^ tile_swz<128>(r).
+// KC: [IDX rows][32 k], chunk c of row r at c ^ kc_swz(r).
+// else: [32 k][IDX], chunk c of row r at c ^ tile_swz<128>(r).
 template <bool KC, int IDX, int NW>
 struct Tile {
   static constexpr int ELEMS = IDX * kBK16;
-  static constexpr int RPI = KC ? 8 : 512 / IDX;           // rows one load instruction covers
+  static constexpr int RPI = KC ? 16 : 512 / IDX;  // rows one load instruction covers
   static constexpr int ROWS = KC ? IDX : kBK16;
   static constexpr int LOADS = ROWS / (RPI * NW);
   static_assert(LOADS >= 1 && LOADS * RPI * NW == ROWS, "whole loads");
-  // Rows that instructions of one wavefront are apart keep the swizzle.
-  static_assert(KC ? (RPI * NW) % 8 == 0 : (RPI * NW) % 16 == 0, "one source chunk per lane");
+  // Rows between instructions of a wavefront: whole swizzle periods (16), or
+  // half of one, which flips bit 3 of the source chunk.
+  static constexpr int STEP = RPI * NW;
+  static_assert(STEP % 16 == 0 || (!KC && STEP == 8), "one or two source chunks per lane");
+  static constexpr int NOFF = STEP % 16 == 0 ? 1 : 2;
 
-  const bf16* base;   // KC: row idx0, k 0; else: row 0, index idx0
-  int64_t ld;
-  int left;           // KC: indices from idx0 on; else: the same (columns)
-  int K;
-  uint32_t voff;      // this lane's byte offset in instruction 0
-  int lane_k;         // KC: k of the lane's chunk within a tile
+  const bf16* cur;      // the next tile's first element (KC: row idx0; else: index idx0)
+  int64_t next;         // elements from tile to tile
+  int k0, k_end, K;     // the next tile's first k; the k to stop at
+  int ld2;              // bytes from row to row
+  int last;             // KC: bytes from a tile's first element to its last row's end at k 0 = 0
+                        // else: bytes of the last row
+  uint32_t voff[NOFF];  // this lane's byte offset in instructions 0 and 1, less the rows between
+  int lane_k;           // KC: k of the lane's chunk within a tile
+#if defined(__HIP_DEVICE_COMPILE__)
+  __amdgpu_buffer_rsrc_t rsrc;
+#endif
+  uint32_t vo;          // KC: voff, or out of range past K
 
-  __device__ __forceinline__ Tile(const Operand& o, int idx0, int total, int k, int wave, int lane) {
-    ld = o.ld;
-    left = total - idx0;
-    K = k;
-    base = static_cast<const bf16*>(o.p) + (KC ? (int64_t)idx0 * o.ld : (int64_t)idx0);
-    constexpr int CPR = KC ? 8 : IDX / 8;  // chunks per row
-    const int row = wave * RPI + lane / CPR, slot = lane % CPR;
-    const int chunk = KC ? slot ^ tile_swz<64>(row) : slot ^ tile_swz<128>(row);
-    lane_k = chunk * 8;
-    voff = (uint32_t)(((int64_t)row * ld + chunk * 8) * 2);
-  }
   // (The range check drops the whole of a load that reaches past the extent: a
   // row ends with its last chunk, whose surplus elements are zeros or meet
   // zeros; rows are whole chunks wide.)
   static __device__ __forceinline__ int chunks(int n) { return (n + 7) & ~7; }
-  __device__ __forceinline__ void load(int kt, bf16* lds, int wave) const {
-#if defined(__HIP_DEVICE_COMPILE__)
-    const int k0 = kt * kBK16;
-    const bf16* from;
-    int64_t extent;
-    uint32_t vo = voff;
-    if constexpr (KC) {
-      from = base + k0;
-      extent = ((int64_t)(min(left, IDX) - 1) * ld + chunks(K - k0)) * 2;
-      if (k0 + lane_k >= K) vo = kOOR;
-    } else {
-      from = base + (int64_t)k0 * ld;
-      extent = ((int64_t)(min(K - k0, kBK16) - 1) * ld + chunks(left)) * 2;
-    }
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<bf16*>(from), (short)0, (int)(extent > 0x7fffffff ? 0x7fffffff : extent), 0x00020000);
-    const uint32_t step = (uint32_t)(RPI * NW * ld * 2);
+  __device__ __forceinline__ Tile(const Operand& o, int idx0, int total, int k, int kt0, int kt1, int wave, int lane) {
+    const int left = total - idx0;
+    K = k;
+    k0 = kt0 * kBK16;
+    k_end = min(K, kt1 * kBK16);
+    ld2 = (int)o.ld * 2;
+    next = KC ? kBK16 : kBK16 * o.ld;
+    cur = static_cast<const bf16*>(o.p) + (KC ? (int64_t)idx0 * o.ld + k0 : (int64_t)k0 * o.ld + idx0);
+    last = KC ? (min(left, IDX) - 1) * ld2 + chunks(K) * 2 : chunks(left) * 2;
+    constexpr int CPR = KC ? kBK16 / 8 : IDX / 8;  // chunks per row
+    const int row = wave * RPI + lane / CPR, slot = lane % CPR;
+    const int chunk = KC ? slot ^ kc_swz(row) : slot ^ tile_swz<128>(row);
+    lane_k = chunk * 8;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (tiles::lds_void_t*)(lds + (NW * i + wave) * 64 * 8), 16,
-                                               vo + (uint32_t)i * step, 0, 0, 0);
+    for (int i = 0; i < NOFF; ++i) voff[i] = (uint32_t)(row * ld2 + (chunk ^ (i * 8)) * 16);
+    vo = voff[0];
+  }
+  // Takes up the next tile: its resource (empty past k_end), then its loads one by one.
+  __device__ __forceinline__ void take() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    int extent = KC ? last - k0 * 2 : (min(K - k0, kBK16) - 1) * ld2 + last;
+    if (k0 >= k_end) extent = 0;
+    rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16*>(cur), (short)0, extent, 0x00020000);
+    if constexpr (KC) vo = k0 + lane_k < K ? voff[0] : kOOR;
+    cur += next;
+    k0 += kBK16;
+#endif
+  }
+  __device__ __forceinline__ void load(int i, bf16* lds, int wave) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const uint32_t v = NOFF == 1 ? vo : voff[i % NOFF];
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (tiles::lds_void_t*)(lds + (NW * i + wave) * 64 * 8), 16,
+                                             (NOFF == 1 && !KC ? voff[0] : v) + (uint32_t)(i * STEP * ld2), 0, 0, 0);
 #endif
   }
 };
@@ -120,18 +138,18 @@ struct Frag<false> {
 };
 
 // Fragments of NB neighbouring 32-index blocks of an operand's tile.  Byte
-// addresses are those of one stage; move() takes them to the other.
+// addresses are those of one stage; move() takes them to another.
 template <bool KC, int IDX, int NB>
 struct Reader {
-  static constexpr int NA = KC ? 4 : 2 * NB;
+  static constexpr int NA = KC ? 2 : 2 * NB;
+  static constexpr int READS = KC ? NB : 2 * NB;  // of a step
   uint32_t a[NA];
   __device__ __forceinline__ Reader(uint32_t tile, int blk0, int lane) {
     const int half = lane >> 5, l32 = lane & 31;
     if constexpr (KC) {
-      const int sw = tile_swz<64>(l32);
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-        a[ks] = tile + (uint32_t)((blk0 * 32 + l32) * 128 + ((2 * ks + half) ^ sw) * 16);
+      for (int ks = 0; ks < 2; ++ks)
+        a[ks] = tile + (uint32_t)((blk0 * 32 + l32) * 64 + ((2 * ks + half) ^ kc_swz(l32)) * 16);
     } else {
       const int tj = lane & 15, tg = (lane >> 4) & 1;
       const int r = 8 * half + (tj >> 2);
@@ -144,14 +162,12 @@ struct Reader {
       }
     }
   }
-  template <int KS, int B>
-  __device__ __forceinline__ void read(Frag<KC>& f) const {
-    if constexpr (KC) {
-      tiles::ds_b128<B * 4096>(f.v, a[KS]);
-    } else {
-      tiles::ds_tr<KS * 16 * IDX * 2>(f.lo, a[2 * B]);
-      tiles::ds_tr<KS * 16 * IDX * 2>(f.hi, a[2 * B + 1]);
-    }
+  // Read R of step KS.
+  template <int KS, int R>
+  __device__ __forceinline__ void read(Frag<KC> (&f)[NB]) const {
+    if constexpr (KC) tiles::ds_b128<R * 2048>(f[R].v, a[KS]);
+    else if constexpr (R & 1) tiles::ds_tr<KS * 16 * IDX * 2>(f[R / 2].hi, a[R]);
+    else tiles::ds_tr<KS * 16 * IDX * 2>(f[R / 2].lo, a[R]);
   }
   __device__ __forceinline__ void move(uint32_t by) {
 #pragma unroll
@@ -159,24 +175,39 @@ struct Reader {
   }
 };
 
+// s_waitcnt vmcnt(N), other counters left alone.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14);
+}
+
+// A barrier alone: __syncthreads would also wait for the loads in flight.
+__device__ __forceinline__ void barrier() {
+  fence();
+  __builtin_amdgcn_s_barrier();
+  fence();
+}
+
 // The sums of tile (m0, n0) over the k-tiles [kt0, kt1) (at least one).
 template <class C>
 __device__ __forceinline__ void gemm_tile16(const GemmShape& g, int m0, int n0, int kt0, int kt1, bf16* smem,
                                             Acc<C>& acc) {
-  constexpr int FM = C::FM, FN = C::FN;
+  constexpr int FM = C::FM, FN = C::FN, NQ = FM * FN;  // products of a step
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % C::WM, wn = wave / C::WM;
 
   using TA = Tile<C::A_KC, C::BM, C::NW>;
   using TB = Tile<C::B_KC, C::BN, C::NW>;
-  const TA ta(g.a, m0, g.M, g.K, wave, lane);
-  const TB tb(g.b, n0, g.N, g.K, wave, lane);
-  bf16* const sa = smem;
-  bf16* const sb = smem + TA::ELEMS;
+  constexpr int LA = TA::LOADS, NL = LA + TB::LOADS, STAGE = C::STAGE;
+  TA ta(g.a, m0, g.M, g.K, kt0, kt1, wave, lane);
+  TB tb(g.b, n0, g.N, g.K, kt0, kt1, wave, lane);
   const uint32_t lds = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem;
-  Reader<C::A_KC, C::BM, FM> ra(lds, wm * FM, lane);
-  Reader<C::B_KC, C::BN, FN> rb(lds + TA::ELEMS * 2, wn * FN, lane);
+  using RA = Reader<C::A_KC, C::BM, FM>;
+  using RB = Reader<C::B_KC, C::BN, FN>;
+  RA ra(lds, wm * FM, lane);
+  RB rb(lds + TA::ELEMS * 2, wn * FN, lane);
+  constexpr int NR = RA::READS + RB::READS;  // reads of a step
 
 #pragma unroll
   for (int j = 0; j < FN; ++j)
@@ -185,77 +216,123 @@ __device__ __forceinline__ void gemm_tile16(const GemmShape& g, int m0, int n0, 
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
 
-  auto load = [&](int kt, int st) {
-    ta.load(kt, sa + st * (C::STAGE / 2), wave);
-    tb.load(kt, sb + st * (C::STAGE / 2), wave);
-  };
   Frag<C::A_KC> fa[2][FM];
   Frag<C::B_KC> fb[2][FN];
-  auto read = [&](auto ks_tag, int set) {
-    constexpr int KS = decltype(ks_tag)::value;
-    tiles::static_for<0, FN>([&](auto j) { rb.template read<KS, decltype(j)::value>(fb[set][decltype(j)::value]); });
-    tiles::static_for<0, FM>([&](auto i) { ra.template read<KS, decltype(i)::value>(fa[set][decltype(i)::value]); });
+  auto stage = [&](int kt) { return smem + ((kt - kt0) & (kStages - 1)) * (STAGE / 2); };
+  // Reads and loads of product slot q: read r of step KS into set S, in order;
+  // (both directions of the wait below count on their order.)
+  auto read = [&](auto ks_tag, auto set_tag, auto r_tag) __attribute__((always_inline)) {
+    constexpr int KS = decltype(ks_tag)::value, S = decltype(set_tag)::value, r = decltype(r_tag)::value;
+    if constexpr (r < RB::READS) rb.template read<KS, r>(fb[S]);
+    else ra.template read<KS, r - RB::READS>(fa[S]);
   };
   // The operands of a step have landed: their uses come after this.
-  auto landed = [&](int set) {
+  auto landed = [&](auto set_tag) __attribute__((always_inline)) {
+    constexpr int S = decltype(set_tag)::value;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-    for (int j = 0; j < FN; ++j) fb[set][j].tie();
+    for (int j = 0; j < FN; ++j) fb[S][j].tie();
 #pragma unroll
-    for (int i = 0; i < FM; ++i) fa[set][i].tie();
+    for (int i = 0; i < FM; ++i) fa[S][i].tie();
     fence();
   };
-  auto multiply = [&](int set) {
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-#pragma unroll
-      for (int i = 0; i < FM; ++i) acc[j][i] = mfma16<C::E>(fb[set][j].bits(), fa[set][i].bits(), acc[j][i]);
+  // The products of set S in order, with between(q) ahead of product q.
+  auto multiply = [&](auto set_tag, auto between) __attribute__((always_inline)) {
+    constexpr int S = decltype(set_tag)::value;
+    tiles::static_for<0, NQ>([&](auto q_tag) {
+      constexpr int q = decltype(q_tag)::value, j = q / FM, i = q % FM;
+      between(q_tag);
+      fence();
+      acc[j][i] = mfma16<C::E>(fb[S][j].bits(), fa[S][i].bits(), acc[j][i]);
+      fence();
+    });
   };
+  // Those of the reads that fall to slot q when they are spread over the slots
+  // [from, to).
+  auto spread = [](auto q_tag, auto from_tag, auto to_tag, auto f) __attribute__((always_inline)) {
+    constexpr int q = decltype(q_tag)::value, a = decltype(from_tag)::value, b = decltype(to_tag)::value;
+    if constexpr (q >= a && q < b) tiles::static_for<(q - a) * NR / (b - a), (q - a + 1) * NR / (b - a)>(f);
+  };
+  auto load = [&](int l, bf16* to) __attribute__((always_inline)) {
+    if (l < LA) ta.load(l, to, wave);
+    else tb.load(l - LA, to + TA::ELEMS, wave);
+  };
+  // A tile's loads go out over the 2 NQ slots from one barrier to the next, the
+  // last of every EVERY.  Slot c of those.
+  constexpr int EVERY = 2 * NQ / NL, B0 = NQ >= 16 ? NQ / 4 : NQ / 2;  // B0: the slot of step 1 with the barrier
+  static_assert(EVERY * NL == 2 * NQ, "loads fill the slots");
+  auto slot_load = [&](int c, bf16* to) __attribute__((always_inline)) {
+    if (c % EVERY == EVERY - 1) load(c / EVERY, to);
+  };
+  constexpr int EARLY = (NQ - B0) / EVERY;  // loads of a tile that fall into step 1, behind the barrier
+  static_assert(EARLY * EVERY == NQ - B0, "whole turns in a step");
+  // The scalar and address work goes between products too, where it is free:
+  // A's next tile is taken up behind its last load, B's likewise, and the read
+  // addresses move on behind step 0's reads.
+  constexpr int TAKE_A = NQ * 5 / 8, MOVE_A = NQ * 3 / 4, MOVE_B = NQ * 3 / 4 + NQ / 16, TAKE_B = NQ - 2;
+  static_assert(LA * EVERY - (NQ - B0) <= TAKE_A && B0 <= TAKE_B && NQ / 2 <= MOVE_A, "behind the last use");
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
-  using I2 = std::integral_constant<int, 2>;
-  using I3 = std::integral_constant<int, 3>;
+  using Barrier = std::integral_constant<int, B0>;
+  using Half = std::integral_constant<int, NQ / 2>;
+  using Most = std::integral_constant<int, B0 + NQ / 2>;
 
-  load(kt0, 0);
-  tiles::wait_dma();
-  __syncthreads();
-  if (kt0 + 1 < kt1) load(kt0 + 1, 1);
-  read(I0{}, 0);
-  landed(0);
-  // Steps 0 to 2; the last step's operands are in set 1 behind them.
-  auto steps = [&]() __attribute__((always_inline)) {
-    read(I1{}, 1);
-    fence();
-    multiply(0);
-    landed(1);
-    read(I2{}, 0);
-    fence();
-    multiply(1);
-    landed(0);
-    read(I3{}, 1);
-    fence();
-    multiply(0);
-    landed(1);
-  };
-  // (The last tile runs behind the loop: with its branch inside, the sums would
-  // be live in two sets of registers.)
-  int by = C::STAGE;
-  for (int kt = kt0; kt < kt1 - 1; ++kt) {
-    steps();
-    // Tile kt + 1 is in its stage, and nobody reads this one any more.
-    tiles::wait_dma();
-    __syncthreads();
-    ra.move((uint32_t)by);
-    rb.move((uint32_t)by);
-    by = -by;
-    read(I0{}, 0);
-    if (kt + 2 < kt1) load(kt + 2, (kt - kt0) & 1);
-    fence();
-    multiply(1);
-    landed(0);
+  // Three tiles, and of the fourth what falls before step 0.
+  for (int t = 0; t < 3; ++t) {
+    ta.take();
+    tb.take();
+#pragma unroll
+    for (int l = 0; l < NL; ++l) load(l, stage(kt0 + t));
   }
-  steps();
-  multiply(1);
+  ta.take();
+  tb.take();
+#pragma unroll
+  for (int l = 0; l < EARLY; ++l) load(l, stage(kt0 + 3));
+  wait_loads<2 * NL + EARLY>();
+  barrier();
+  tiles::static_for<0, NR>([&](auto r) { read(I0{}, I0{}, r); });
+  landed(I0{});
+  uint32_t to = 3;  // the stage being loaded
+  for (int kt = kt0; kt < kt1 - 1; ++kt) {
+    bf16* const old = smem + to * (STAGE / 2);
+    to = (to + 1) & (kStages - 1);
+    bf16* const fresh = smem + to * (STAGE / 2);
+    const uint32_t by = to == 3 ? (uint32_t)(-3 * STAGE) : (uint32_t)STAGE;
+    // Step 0, reading step 1.
+    multiply(I0{}, [&](auto q_tag) __attribute__((always_inline)) {
+      constexpr int q = decltype(q_tag)::value;
+      spread(q_tag, I0{}, Half{}, [&](auto r) { read(I1{}, I1{}, r); });
+      slot_load(q + NQ - B0, old);
+      if constexpr (q == TAKE_A) ta.take();
+      if constexpr (q == MOVE_A) ra.move(by);
+      if constexpr (q == MOVE_B) rb.move(by);
+    });
+    landed(I1{});
+    // Step 1.  Its operands are in registers and nobody reads this stage any
+    // more; at its slot B0 tile kt + 1 has landed for everyone, and the loads
+    // go on with tile kt + 4 into this one.
+    multiply(I1{}, [&](auto q_tag) __attribute__((always_inline)) {
+      constexpr int q = decltype(q_tag)::value;
+      if constexpr (q < B0) {
+        slot_load(q + 2 * NQ - B0, old);
+      } else {
+        if constexpr (q == B0) {
+          wait_loads<2 * NL>();
+          barrier();
+        }
+        spread(q_tag, Barrier{}, Most{}, [&](auto r) { read(I0{}, I0{}, r); });
+        slot_load(q - B0, fresh);
+        if constexpr (q == TAKE_B) tb.take();
+      }
+    });
+    landed(I0{});
+  }
+  multiply(I0{}, [&](auto q_tag) __attribute__((always_inline)) {
+    spread(q_tag, I0{}, Half{}, [&](auto r) { read(I1{}, I1{}, r); });
+  });
+  landed(I1{});
+  multiply(I1{}, [](auto) {});
+  wait_loads<0>();  // (those out of range: the stages are the caller's now)
 }
 
 }  // namespace xent

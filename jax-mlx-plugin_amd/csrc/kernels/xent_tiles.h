@@ -7,7 +7,7 @@
 namespace mfx {
 namespace xent {
 
-constexpr int kBK16 = 64, kBK32 = 32;  // k per tile: 128 bytes
+constexpr int kBK16 = 32, kBK32 = 32;  // k per tile
 
 struct Operand {
   const void* p;
@@ -44,12 +44,13 @@ struct Config {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, E = E_;
   static constexpr bool A_KC = A_KC_, B_KC = B_KC_;
   static constexpr int NW = WM * WN, NT = NW * 64;
+  static constexpr int WAVES = BM == 256 ? 1 : 2;                 // per SIMD
   static constexpr int FM = BM / (32 * WM), FN = BN / (32 * WN);  // blocks of a wavefront
   static constexpr int BK = E == 2 ? kBK32 : kBK16;
-  // 16 bits: bytes of a stage, and of the two.  f32: tiles of 128 indices, the
-  // larger of the two forms' padded rows (xent_gemm32.h), two stages.
+  // Bytes of a stage, and of all: four in 16 bits; f32: two, tiles of 128
+  // indices in the larger of the two forms' padded rows (xent_gemm32.h).
   static constexpr int STAGE = E == 2 ? 2 * 128 * (kBK32 + 4) * 4 : (BM + BN) * kBK16 * 2;
-  static constexpr int SMEM = 2 * STAGE;
+  static constexpr int SMEM = (E == 2 ? 2 : 4) * STAGE;
 };
 
 template <class C>
