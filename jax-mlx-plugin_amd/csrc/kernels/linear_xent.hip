@@ -24,6 +24,7 @@
 // What bounds it: the matrix cores, 2 T H V flops a product, one product
 // forward and three backward.
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "xent_gemm16.h"
@@ -32,14 +33,22 @@
 namespace mfx {
 namespace xent {
 
-// Wide tiles for what fills the device with them, else narrow ones.
-template <bool A_KC, bool B_KC, int E>
-using Wide = Config<256, 256, 2, 2, A_KC, B_KC, E>;
-template <bool A_KC, bool B_KC, int E>
-using Narrow = Config<128, 128, 2, 2, A_KC, B_KC, E>;
+// Tile forms: 256 x 256, one workgroup a CU; 128 x 128, two; and 64 rows of A by
+// 128 of B (f32: 64 x 64), three.  f32 has the last two.
+enum Form { kWide, kNarrow, kSlim };
+constexpr int kFormM[3] = {256, 128, 64};
+constexpr int kFormN[2][3] = {{256, 128, 128}, {256, 128, 64}};  // 16 bits, f32
 
+template <Form F, bool A_KC, bool B_KC, int E>
+struct Pick;
+template <bool A_KC, bool B_KC, int E>
+struct Pick<kWide, A_KC, B_KC, E> : Config<256, 256, 2, 2, A_KC, B_KC, E> {};
+template <bool A_KC, bool B_KC, int E>
+struct Pick<kNarrow, A_KC, B_KC, E> : Config<128, 128, 2, 2, A_KC, B_KC, E> {};
+template <bool A_KC, bool B_KC, int E>
+struct Pick<kSlim, A_KC, B_KC, E> : Config<64, 128, 1, 4, A_KC, B_KC, E> {};
 template <bool A_KC, bool B_KC>
-using Full = Config<128, 128, 2, 2, A_KC, B_KC, 2>;
+struct Pick<kSlim, A_KC, B_KC, 2> : Config<64, 64, 2, 2, A_KC, B_KC, 2> {};
 
 template <class C>
 __device__ __forceinline__ void gemm_tile(const GemmShape& g, int m0, int n0, int kt0, int kt1, char* smem,
@@ -242,20 +251,31 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void xent_logits_kernel(LossArgs p
 }
 
 // lse and loss of each row from its tiles' partials: 64 rows a workgroup, a
-// row's tiles shared out over 4 wavefronts.
-__global__ __launch_bounds__(256) void xent_combine(const float* __restrict__ part_m, const float* __restrict__ part_l,
-                                                    const float* __restrict__ picked, const void* targets,
-                                                    int target64, int T, int V, int tiles, float* loss, float* lse) {
-  __shared__ float red_m[4][64], red_l[4][64];
+// row's tiles shared out over 16 wavefronts, four of them in flight at a time.
+constexpr int kCombine = 16;
+__global__ __launch_bounds__(64 * kCombine) void xent_combine(const float* __restrict__ part_m,
+                                                              const float* __restrict__ part_l,
+                                                              const float* __restrict__ picked, const void* targets,
+                                                              int target64, int T, int V, int tiles, float* loss,
+                                                              float* lse) {
+  __shared__ float red_m[kCombine][64], red_l[kCombine][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int row = blockIdx.x * 64 + lane;
   float m = -INFINITY, l = 0.f;
   if (row < T)
-    for (int i = w; i < tiles; i += 4) {
-      const float mi = part_m[(int64_t)i * T + row], li = part_l[(int64_t)i * T + row];
+    for (int i0 = w; i0 < tiles; i0 += 4 * kCombine) {
+      float mi[4], li[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * kCombine;
+        mi[u] = i < tiles ? part_m[(int64_t)i * T + row] : -INFINITY;
+        li[u] = i < tiles ? part_l[(int64_t)i * T + row] : 0.f;
+      }
       // (A NaN maximum is lost to fmaxf; its sum is NaN and stays.)
-      const float mn = fmaxf(m, mi), base = mn == -INFINITY ? 0.f : mn;
-      l = l * __builtin_amdgcn_exp2f(m - base) + li * __builtin_amdgcn_exp2f(mi - base);
+      const float mn = fmaxf(fmaxf(fmaxf(mi[0], mi[1]), fmaxf(mi[2], mi[3])), m), base = mn == -INFINITY ? 0.f : mn;
+      l *= __builtin_amdgcn_exp2f(m - base);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) l += li[u] * __builtin_amdgcn_exp2f(mi[u] - base);
       m = mn;
     }
   red_m[w][lane] = m;
@@ -263,13 +283,12 @@ __global__ __launch_bounds__(256) void xent_combine(const float* __restrict__ pa
   __syncthreads();
   if (w != 0 || row >= T) return;
 #pragma unroll
-  for (int i = 1; i < 4; ++i) m = fmaxf(m, red_m[i][lane]);
+  for (int i = 1; i < kCombine; ++i) m = fmaxf(m, red_m[i][lane]);
   const float base = m == -INFINITY ? 0.f : m;
   l = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) l += red_l[i][lane] * __builtin_amdgcn_exp2f(red_m[i][lane] - base);
-  // log(sum exp z) = (m + log2 sum) ln 2, in two parts so that a large m
-  // keeps the sum's digits.
+  for (int i = 0; i < kCombine; ++i) l += red_l[i][lane] * __builtin_amdgcn_exp2f(red_m[i][lane] - base);
+  // log(sum exp z) = m ln 2 + log(sum of 2^(z - m)).
   const float z = fmaf(m, 0.6931471805599453f, __logf(l));
   if (lse) lse[row] = z;
   const int64_t t = target_of(targets, target64, row);
@@ -397,41 +416,72 @@ constexpr size_t kPieceBytes = 512u << 20;  // of d at a time
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Wide tiles where they number at least a CU each; narrow ones (two to a CU)
-// reach more CUs below.  f32 has narrow ones only.
-bool wide_tiles(int E, int64_t M, int64_t N) {
-  return E != 2 && ceil_div(M, 256) * ceil_div(N, 256) >= device_cu_count();
-}
+// A product's tile form and, for a gradient's, its ranges of k.
+struct Way {
+  Form form;
+  int64_t range, ranges;  // k-tiles of one, and their number
+};
 
-GemmShape shape(Operand a, Operand b, int64_t M, int64_t N, int64_t K, bool wide) {
+GemmShape shape(Operand a, Operand b, int64_t M, int64_t N, int64_t K, int E, Form f) {
   GemmShape g{};
   g.a = a;
   g.b = b;
   g.M = (int)M;
   g.N = (int)N;
   g.K = (int)K;
-  const int t = wide ? 256 : 128;
-  g.tiles_m = (int)ceil_div(M, t);
-  g.tiles_n = (int)ceil_div(N, t);
+  g.tiles_m = (int)ceil_div(M, kFormM[f]);
+  g.tiles_n = (int)ceil_div(N, kFormN[E == 2][f]);
   g.splits = 1;
   return g;
 }
 
-// k-tiles per range of a gradient's product: all, or where its tiles are too
-// few for the CUs ranges (of 8 k-tiles at least) that fill them twice.
-int64_t range_tiles(int E, int64_t M, int64_t N, int64_t K) {
-  const int64_t kt = ceil_div(K, E == 2 ? kBK32 : kBK16);
-  if (wide_tiles(E, M, N)) return kt;
-  const int64_t tiles = ceil_div(M, 128) * ceil_div(N, 128), want = 2LL * device_cu_count();
-  const int64_t s = std::max<int64_t>(1, std::min(want / tiles, kt / 8));
-  return ceil_div(kt, s);
+// Microseconds that a form takes: a k-tile with `slots` workgroups on each CU,
+// each further round of workgroups, and once.  Fitted to the measured times of
+// 13 shapes from [33 x 4096 x 65537] to [8192 x 512 x 1000] in every form and
+// with 1 to 16 ranges; the chosen way took at most 13% more than the best of
+// them.
+struct Cost {
+  int slots;
+  float kt, each, once;
+};
+constexpr Cost kCost[2][3] = {{{1, 0.85f, 9.f, 0.f}, {2, 0.57f, 1.f, 6.f}, {3, 0.85f, 0.5f, 4.f}},
+                              {{1, 0.f, 0.f, 0.f}, {2, 4.6f, 2.f, 6.f}, {3, 1.95f, 1.f, 4.f}}};
+
+float way_us(const Cost& c, int64_t wgs, int64_t range, int64_t cus) {
+  const int64_t full = wgs / (c.slots * cus), rest = wgs % (c.slots * cus);
+  float t = c.once + (float)full * ((float)range * c.kt + c.each);
+  // (With fewer than `slots` workgroups on a CU each runs faster.)
+  if (rest) t += (float)range * c.kt * (0.25f + 0.75f * (float)ceil_div(rest, cus) / (float)c.slots) + c.each;
+  return t;
+}
+
+// The way that takes least by these: every form, and with `split` every number
+// of ranges up to 32 of at least 8 k-tiles, whose sums are written and read
+// again (8 bytes an output and range at 4 TB/s, and a launch more).
+Way choose(int E, int64_t M, int64_t N, int64_t K, bool split) {
+  const int64_t kt = ceil_div(K, E == 2 ? kBK32 : kBK16), cus = device_cu_count();
+  Way best{kNarrow, kt, 1};
+  float least = INFINITY;
+  for (int f = E == 2 ? kNarrow : kWide; f <= kSlim; ++f) {
+    const Cost& c = kCost[E == 2][f];
+    const int64_t tiles = ceil_div(M, kFormM[f]) * ceil_div(N, kFormN[E == 2][f]);
+    for (int64_t s = 1; s <= (split ? std::min<int64_t>(32, std::max<int64_t>(1, kt / 8)) : 1); ++s) {
+      const int64_t range = ceil_div(kt, s), ranges = ceil_div(kt, range);
+      float t = way_us(c, tiles * ranges, range, cus);
+      if (ranges > 1) t += 4.f + (float)ranges * (float)M * (float)N * 8.f / 4e6f;
+      if (t < least) {
+        least = t;
+        best = Way{(Form)f, range, ranges};
+      }
+    }
+  }
+  return best;
 }
 
 struct BwdPlan {
   int E;
   int64_t piece, pieces;
-  int64_t dh_range, dw_range;    // k-tiles per range
-  int64_t dh_ranges, dw_ranges;  // of a whole piece
+  Way dh, dw;  // of the first piece, the widest
   size_t d_bytes, dh_bytes, dw_bytes, total;
 };
 
@@ -440,52 +490,49 @@ int elem_of(int dtype) { return dtype == MFX_F32 ? 2 : dtype == MFX_F16 ? 1 : 0;
 BwdPlan plan_bwd(const mfx_linear_xent_bwd_args& a) {
   BwdPlan pl{};
   pl.E = elem_of(a.dtype);
-  const int size = dtype_size(a.dtype), bk = pl.E == 2 ? kBK32 : kBK16;
+  const int size = dtype_size(a.dtype);
   const int64_t vp = ceil_div(a.V, 256) * 256;
   const int64_t most = std::max<int64_t>(256, (int64_t)(kPieceBytes / size) / a.T / 256 * 256);
   pl.pieces = ceil_div(vp, most);
   pl.piece = ceil_div(ceil_div(vp, pl.pieces), 256) * 256;
   pl.pieces = ceil_div(vp, pl.piece);
-  const int64_t nv = std::min(pl.piece, a.V);  // columns of the first piece, the widest
+  const int64_t nv = std::min(pl.piece, a.V);
   pl.d_bytes = align256((size_t)a.T * pl.piece * size);
   if (a.dh) {
-    pl.dh_range = range_tiles(pl.E, a.T, a.H, nv);
-    pl.dh_ranges = ceil_div(ceil_div(nv, bk), pl.dh_range);
-    if (pl.pieces > 1 || pl.dh_ranges > 1) pl.dh_bytes = align256((size_t)pl.dh_ranges * a.T * a.H * 4);
+    pl.dh = choose(pl.E, a.T, a.H, nv, true);
+    if (pl.pieces > 1 || pl.dh.ranges > 1) pl.dh_bytes = align256((size_t)pl.dh.ranges * a.T * a.H * 4);
   }
   if (a.dw) {
-    pl.dw_range = range_tiles(pl.E, nv, a.H, a.T);
-    pl.dw_ranges = ceil_div(ceil_div(a.T, bk), pl.dw_range);
-    if (pl.dw_ranges > 1) pl.dw_bytes = align256((size_t)pl.dw_ranges * nv * a.H * 4);
+    pl.dw = choose(pl.E, nv, a.H, a.T, true);
+    if (pl.dw.ranges > 1) pl.dw_bytes = align256((size_t)pl.dw.ranges * nv * a.H * 4);
   }
   pl.total = 256 + pl.d_bytes + pl.dh_bytes + pl.dw_bytes;
   return pl;
 }
 
 template <int E, bool BWD>
-int launch_logits(const LossArgs& p, bool wide, hipStream_t s) {
+int launch_logits(const LossArgs& p, Form f, hipStream_t s) {
   const dim3 grid((unsigned)(p.g.tiles_m * p.g.tiles_n));
-  if constexpr (E == 2) {
-    hipLaunchKernelGGL((xent_logits_kernel<Full<true, true>, BWD>), grid, dim3(256), 0, s, p);
-  } else {
-    if (wide) hipLaunchKernelGGL((xent_logits_kernel<Wide<true, true, E>, BWD>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((xent_logits_kernel<Narrow<true, true, E>, BWD>), grid, dim3(256), 0, s, p);
-  }
+  if constexpr (E != 2)
+    if (f == kWide) hipLaunchKernelGGL((xent_logits_kernel<Pick<kWide, true, true, E>, BWD>), grid, dim3(256), 0, s, p);
+  if (f == kNarrow) hipLaunchKernelGGL((xent_logits_kernel<Pick<kNarrow, true, true, E>, BWD>), grid, dim3(256), 0, s, p);
+  if (f == kSlim) hipLaunchKernelGGL((xent_logits_kernel<Pick<kSlim, true, true, E>, BWD>), grid, dim3(256), 0, s, p);
   return launch_status("xent_logits_kernel");
 }
 
 template <bool A_KC, int E>
-int launch_grad(StoreArgs& p, int64_t range, bool wide, hipStream_t s) {
+int launch_grad(StoreArgs& p, const Way& way, hipStream_t s) {
   const int64_t kt = ceil_div(p.g.K, E == 2 ? kBK32 : kBK16);
-  p.g.kt_per_split = (int)std::min(range, kt);
+  p.g.kt_per_split = (int)std::min(way.range, kt);
   p.g.splits = (int)ceil_div(kt, p.g.kt_per_split);
   const dim3 grid((unsigned)(p.g.tiles_m * p.g.tiles_n * p.g.splits));
-  if constexpr (E == 2) {
-    hipLaunchKernelGGL((xent_grad_kernel<Full<A_KC, false>>), grid, dim3(256), 0, s, p);
-  } else {
-    if (wide) hipLaunchKernelGGL((xent_grad_kernel<Wide<A_KC, false, E>>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((xent_grad_kernel<Narrow<A_KC, false, E>>), grid, dim3(256), 0, s, p);
-  }
+  if constexpr (E != 2)
+    if (way.form == kWide)
+      hipLaunchKernelGGL((xent_grad_kernel<Pick<kWide, A_KC, false, E>>), grid, dim3(256), 0, s, p);
+  if (way.form == kNarrow)
+    hipLaunchKernelGGL((xent_grad_kernel<Pick<kNarrow, A_KC, false, E>>), grid, dim3(256), 0, s, p);
+  if (way.form == kSlim)
+    hipLaunchKernelGGL((xent_grad_kernel<Pick<kSlim, A_KC, false, E>>), grid, dim3(256), 0, s, p);
   return launch_status("xent_grad_kernel");
 }
 
@@ -519,8 +566,8 @@ int run_bwd(const mfx_linear_xent_bwd_args& a, const BwdPlan& pl, char* ws, hipS
     const int64_t v0 = i * pl.piece, nv = std::min(pl.piece, a.V - v0);
     const Operand w{static_cast<const char*>(a.w) + v0 * a.w_stride * size, a.w_stride};
     LossArgs z{};
-    bool wide = wide_tiles(E, a.T, nv);
-    z.g = shape(h, w, a.T, nv, a.H, wide);
+    const Way zw = choose(E, a.T, nv, a.H, false);
+    z.g = shape(h, w, a.T, nv, a.H, E, zw.form);
     z.targets = a.targets;
     z.target64 = t64;
     z.v0 = v0;
@@ -530,25 +577,23 @@ int run_bwd(const mfx_linear_xent_bwd_args& a, const BwdPlan& pl, char* ws, hipS
     z.scale = scale;
     z.d = d;
     z.ldd = pl.piece;
-    if (int rc = launch_logits<E, true>(z, wide, s)) return rc;
+    if (int rc = launch_logits<E, true>(z, zw.form, s)) return rc;
+    // (A narrower last piece keeps the first's ways: no more ranges than its.)
     if (a.dw) {
       StoreArgs p{};
-      wide = wide_tiles(E, nv, a.H);
-      p.g = shape(dl, h, nv, a.H, a.T, wide);
+      p.g = shape(dl, h, nv, a.H, a.T, E, pl.dw.form);
       p.scale = scale;
       p.c = static_cast<char*>(a.dw) + v0 * a.dw_stride * dtype_size(a.dw_dtype);
       p.ldc = a.dw_stride;
       p.c_f32 = a.dw_dtype == MFX_F32;
-      if (pl.dw_ranges > 1) p.part = dw_part;
-      if (int rc = launch_grad<false, E>(p, pl.dw_range, wide, s)) return rc;
+      if (pl.dw.ranges > 1) p.part = dw_part;
+      if (int rc = launch_grad<false, E>(p, pl.dw, s)) return rc;
       if (p.part)
-        if (int rc = launch_sum(dw_part, pl.dw_ranges, nv, a.H, p.c, p.ldc, a.dw_dtype, scale, s)) return rc;
+        if (int rc = launch_sum(dw_part, pl.dw.ranges, nv, a.H, p.c, p.ldc, a.dw_dtype, scale, s)) return rc;
     }
     if (a.dh) {
-      // (A narrower last piece has no more ranges than the first.)
       StoreArgs p{};
-      wide = wide_tiles(E, a.T, a.H);
-      p.g = shape(dl, w, a.T, a.H, nv, wide);
+      p.g = shape(dl, w, a.T, a.H, nv, E, pl.dh.form);
       p.scale = scale;
       p.c = a.dh;
       p.ldc = a.dh_stride;
@@ -557,23 +602,24 @@ int run_bwd(const mfx_linear_xent_bwd_args& a, const BwdPlan& pl, char* ws, hipS
         p.part = dh_part;
         p.add = i > 0;
       }
-      if (int rc = launch_grad<true, E>(p, pl.dh_range, wide, s)) return rc;
+      if (int rc = launch_grad<true, E>(p, pl.dh, s)) return rc;
     }
   }
-  if (a.dh && pl.dh_bytes) return launch_sum(dh_part, pl.dh_ranges, a.T, a.H, a.dh, a.dh_stride, a.dtype, scale, s);
+  if (a.dh && pl.dh_bytes) return launch_sum(dh_part, pl.dh.ranges, a.T, a.H, a.dh, a.dh_stride, a.dtype, scale, s);
   return MFX_OK;
 }
 
 // Forward workspace: the targets' logits, then the partials.
 struct FwdPlan {
-  bool wide;
+  Form form;
   int64_t tiles_n;
   size_t row_bytes, part_bytes;
 };
 FwdPlan plan_fwd(const mfx_linear_xent_args& a) {
   FwdPlan pl{};
-  pl.wide = wide_tiles(elem_of(a.dtype), a.T, a.V);
-  pl.tiles_n = ceil_div(a.V, pl.wide ? 256 : 128);
+  const int E = elem_of(a.dtype);
+  pl.form = choose(E, a.T, a.V, a.H, false).form;
+  pl.tiles_n = ceil_div(a.V, kFormN[E == 2][pl.form]);
   pl.row_bytes = align256((size_t)a.T * 4);
   pl.part_bytes = align256((size_t)pl.tiles_n * a.T * 4);
   return pl;
@@ -589,8 +635,8 @@ int check_common(int64_t T, int64_t H, int64_t V, int dtype, int target_dtype) {
   if (target_dtype != MFX_I32 && target_dtype != MFX_I64)
     return fail(MFX_E_UNSUPPORTED, "target dtype must be i32 or i64");
   if (T > lim - 256 || V > lim - 256 || H > lim - 256) return fail(MFX_E_UNSUPPORTED, "T, H or V too large");
-  if (ceil_div(T, 128) * ceil_div(V, 128) > lim || ceil_div(T, 128) * ceil_div(H, 128) > lim / 64 ||
-      ceil_div(V, 128) * ceil_div(H, 128) > lim / 64)
+  if (ceil_div(T, 64) * ceil_div(V, 64) > lim || ceil_div(T, 64) * ceil_div(H, 64) > lim / 32 ||
+      ceil_div(V, 64) * ceil_div(H, 64) > lim / 32)
     return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
   if (H % (dtype == MFX_F32 ? 4 : 8))
     return fail(MFX_E_UNSUPPORTED, "H must be a multiple of 16 bytes");
@@ -679,7 +725,8 @@ int mfx_linear_xent(const mfx_linear_xent_args* args, void* stream) {
                               "mfx_linear_xent_workspace_size", s, &ws))
     return rc;
   LossArgs z{};
-  z.g = shape(Operand{a.h, a.h_stride}, Operand{a.w, a.w_stride}, a.T, a.V, a.H, pl.wide);
+  z.g = shape(Operand{a.h, a.h_stride}, Operand{a.w, a.w_stride}, a.T, a.V, a.H, elem_of(a.dtype),
+              pl.form);
   z.targets = a.targets;
   z.target64 = a.target_dtype == MFX_I64;
   z.V = (int)a.V;
@@ -687,11 +734,11 @@ int mfx_linear_xent(const mfx_linear_xent_args* args, void* stream) {
   z.part_m = reinterpret_cast<float*>(ws + pl.row_bytes);
   z.part_l = reinterpret_cast<float*>(ws + pl.row_bytes + pl.part_bytes);
   int rc;
-  if (a.dtype == MFX_F32) rc = launch_logits<2, false>(z, pl.wide, s);
-  else if (a.dtype == MFX_F16) rc = launch_logits<1, false>(z, pl.wide, s);
-  else rc = launch_logits<0, false>(z, pl.wide, s);
+  if (a.dtype == MFX_F32) rc = launch_logits<2, false>(z, pl.form, s);
+  else if (a.dtype == MFX_F16) rc = launch_logits<1, false>(z, pl.form, s);
+  else rc = launch_logits<0, false>(z, pl.form, s);
   if (rc) return rc;
-  hipLaunchKernelGGL(xent_combine, dim3((unsigned)ceil_div(a.T, 64)), dim3(256), 0, s, z.part_m, z.part_l, z.picked,
+  hipLaunchKernelGGL(xent_combine, dim3((unsigned)ceil_div(a.T, 64)), dim3(64 * kCombine), 0, s, z.part_m, z.part_l, z.picked,
                      a.targets, z.target64, (int)a.T, (int)a.V, (int)pl.tiles_n, a.loss, a.lse);
   return launch_status("xent_combine");
 }

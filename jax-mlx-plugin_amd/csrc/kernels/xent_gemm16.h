@@ -51,7 +51,7 @@ __device__ __forceinline__ int kc_swz(int r) { return (r >> 2) & 3; }
 
 // One operand's tiles: IDX indices of a tile, NW wavefronts sharing the loads.
 // KC: [IDX rows][32 k], chunk c of row r at c ^ kc_swz(r).
-// else: [32 k][IDX], chunk c of row r at c ^ tile_swz<128>(r).
+// else: [32 k][IDX], chunk c of row r at c ^ tile_swz<IDX>(r).
 template <bool KC, int IDX, int NW>
 struct Tile {
   static constexpr int ELEMS = IDX * kBK16;
@@ -93,7 +93,7 @@ struct Tile {
     last = KC ? (min(left, IDX) - 1) * ld2 + chunks(K) * 2 : chunks(left) * 2;
     constexpr int CPR = KC ? kBK16 / 8 : IDX / 8;  // chunks per row
     const int row = wave * RPI + lane / CPR, slot = lane % CPR;
-    const int chunk = KC ? slot ^ kc_swz(row) : slot ^ tile_swz<128>(row);
+    const int chunk = KC ? slot ^ kc_swz(row) : slot ^ tile_swz<IDX>(row);
     lane_k = chunk * 8;
 #pragma unroll
     for (int i = 0; i < NOFF; ++i) voff[i] = (uint32_t)(row * ld2 + (chunk ^ (i * 8)) * 16);
@@ -157,8 +157,8 @@ struct Reader {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const int c = (blk0 + b) * 4 + chunk;
-        a[2 * b] = tile + (uint32_t)(r * IDX * 2 + (c ^ tile_swz<128>(r)) * 16 + sub);
-        a[2 * b + 1] = tile + (uint32_t)((r + 4) * IDX * 2 + (c ^ tile_swz<128>(r + 4)) * 16 + sub);
+        a[2 * b] = tile + (uint32_t)(r * IDX * 2 + (c ^ tile_swz<IDX>(r)) * 16 + sub);
+        a[2 * b + 1] = tile + (uint32_t)((r + 4) * IDX * 2 + (c ^ tile_swz<IDX>(r + 4)) * 16 + sub);
       }
     }
   }
@@ -257,20 +257,24 @@ __device__ __forceinline__ void gemm_tile16(const GemmShape& g, int m0, int n0, 
     if (l < LA) ta.load(l, to, wave);
     else tb.load(l - LA, to + TA::ELEMS, wave);
   };
-  // A tile's loads go out over the 2 NQ slots from one barrier to the next, the
-  // last of every EVERY.  Slot c of those.
-  constexpr int EVERY = 2 * NQ / NL, B0 = NQ >= 16 ? NQ / 4 : NQ / 2;  // B0: the slot of step 1 with the barrier
-  static_assert(EVERY * NL == 2 * NQ, "loads fill the slots");
-  auto slot_load = [&](int c, bf16* to) __attribute__((always_inline)) {
-    if (c % EVERY == EVERY - 1) load(c / EVERY, to);
+  // A tile's loads go out evenly over the 2 NQ slots from one barrier to the
+  // next: those of slot c.
+  constexpr int B0 = NQ >= 16 ? NQ / 4 : NQ / 2;  // the slot of step 1 with the barrier
+  auto slot_load = [&](auto c_tag, bf16* to) __attribute__((always_inline)) {
+    constexpr int c = decltype(c_tag)::value;
+#pragma unroll
+    for (int l = c * NL / (2 * NQ); l < (c + 1) * NL / (2 * NQ); ++l) load(l, to);
   };
-  constexpr int EARLY = (NQ - B0) / EVERY;  // loads of a tile that fall into step 1, behind the barrier
-  static_assert(EARLY * EVERY == NQ - B0, "whole turns in a step");
+  constexpr int EARLY = (NQ - B0) * NL / (2 * NQ);  // loads of a tile that fall into step 1, behind the barrier
   // The scalar and address work goes between products too, where it is free:
   // A's next tile is taken up behind its last load, B's likewise, and the read
   // addresses move on behind step 0's reads.
-  constexpr int TAKE_A = NQ * 5 / 8, MOVE_A = NQ * 3 / 4, MOVE_B = NQ * 3 / 4 + NQ / 16, TAKE_B = NQ - 2;
-  static_assert(LA * EVERY - (NQ - B0) <= TAKE_A && B0 <= TAKE_B && NQ / 2 <= MOVE_A, "behind the last use");
+  constexpr int TAKE_A = NQ * 5 / 8, MOVE_A = NQ * 3 / 4, MOVE_B = NQ * 3 / 4 + NQ / 16;
+  constexpr int TAKE_B = NQ >= 4 ? NQ - 2 : NQ - 1;
+  constexpr int LAST_A = (LA * 2 * NQ + NL - 1) / NL - 1;       // slot of A's last load
+  constexpr int FIRST_B = ((LA + 1) * 2 * NQ + NL - 1) / NL - 1;  // and of B's first
+  static_assert(LAST_A - (NQ - B0) <= TAKE_A && B0 <= TAKE_B && TAKE_B - B0 < FIRST_B && NQ / 2 <= MOVE_A,
+                "behind the last use and before the next");
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
   using Barrier = std::integral_constant<int, B0>;
@@ -302,7 +306,7 @@ __device__ __forceinline__ void gemm_tile16(const GemmShape& g, int m0, int n0, 
     multiply(I0{}, [&](auto q_tag) __attribute__((always_inline)) {
       constexpr int q = decltype(q_tag)::value;
       spread(q_tag, I0{}, Half{}, [&](auto r) { read(I1{}, I1{}, r); });
-      slot_load(q + NQ - B0, old);
+      slot_load(std::integral_constant<int, q + NQ - B0>{}, old);
       if constexpr (q == TAKE_A) ta.take();
       if constexpr (q == MOVE_A) ra.move(by);
       if constexpr (q == MOVE_B) rb.move(by);
@@ -314,14 +318,14 @@ __device__ __forceinline__ void gemm_tile16(const GemmShape& g, int m0, int n0, 
     multiply(I1{}, [&](auto q_tag) __attribute__((always_inline)) {
       constexpr int q = decltype(q_tag)::value;
       if constexpr (q < B0) {
-        slot_load(q + 2 * NQ - B0, old);
+        slot_load(std::integral_constant<int, q + 2 * NQ - B0>{}, old);
       } else {
         if constexpr (q == B0) {
           wait_loads<2 * NL>();
           barrier();
         }
         spread(q_tag, Barrier{}, Most{}, [&](auto r) { read(I0{}, I0{}, r); });
-        slot_load(q - B0, fresh);
+        slot_load(std::integral_constant<int, q - B0>{}, fresh);
         if constexpr (q == TAKE_B) tb.take();
       }
     });

@@ -1,9 +1,10 @@
 // The f32 product kernel of the linear cross entropy: C[m][n] = sum_k A(m, k)
-// B(n, k) on v_mfma_f32_32x32x2_f32, operands stored as in xent_gemm16.h, 128 x
-// 128 tiles of 32 k by 4 wavefronts of 64 x 64.
+// B(n, k) on v_mfma_f32_32x32x2_f32, operands stored as in xent_gemm16.h, tiles
+// of 32 k by 4 wavefronts: 128 x 128 outputs (64 x 64 a wavefront), or 64 x 64
+// where those are too few.
 //
-// A 32x32x2 product takes 64 cycles, so a tile's 16 products per 8 k and
-// wavefront leave 1024 cycles for 4 to 16 LDS reads: plain double buffering
+// A 32x32x2 product takes 64 cycles, so the 16 (4) products per 8 k and
+// wavefront leave 1024 (256) cycles for 4 to 16 (2 to 8) LDS reads: plain double buffering
 // (global -> registers -> LDS, one barrier a tile) keeps the matrix cores fed.
 // The k of products are permuted alike in both operands: step e of 8 k takes k =
 // half * 4 + e, so a k-contiguous row gives four steps in one 16-byte read.
@@ -16,12 +17,12 @@
 namespace mfx {
 namespace xent {
 
-template <bool KC>
+template <bool KC, int IDX>
 struct Tile32 {
-  static constexpr int IDX = 128, NT = 256;
+  static constexpr int NT = 256;
   static constexpr int ROW = KC ? kBK32 + 4 : IDX + 8;        // floats
   static constexpr int CPR = KC ? kBK32 / 4 : IDX / 4;        // 16-byte chunks per row
-  static constexpr int CH = IDX * kBK32 / 4 / NT;             // chunks per thread: 4
+  static constexpr int CH = IDX * kBK32 / 4 / NT;             // chunks per thread
   const float* p;
   int64_t ld;
   int idx0, total, K;
@@ -50,9 +51,9 @@ struct Tile32 {
 };
 
 // The four k of step c (of 8) that this lane's half holds, for index `idx`.
-template <bool KC>
+template <bool KC, int IDX>
 __device__ __forceinline__ f32x4 frag32(const float* lds, int idx, int c, int half) {
-  constexpr int ROW = Tile32<KC>::ROW;
+  constexpr int ROW = Tile32<KC, IDX>::ROW;
   const int k = c * 8 + half * 4;
   if constexpr (KC) return *reinterpret_cast<const f32x4*>(lds + idx * ROW + k);
   else return f32x4{lds[k * ROW + idx], lds[(k + 1) * ROW + idx], lds[(k + 2) * ROW + idx], lds[(k + 3) * ROW + idx]};
@@ -61,11 +62,11 @@ __device__ __forceinline__ f32x4 frag32(const float* lds, int idx, int c, int ha
 template <class C>
 __device__ __forceinline__ void gemm_tile32(const GemmShape& g, int m0, int n0, int kt0, int kt1, float* smem,
                                             Acc<C>& acc) {
-  static_assert(C::BM == 128 && C::BN == 128 && C::NT == 256, "one tile form");
+  static_assert(C::BM == C::BN && C::NT == 256, "square tiles by four wavefronts");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
   const int wm = wave % C::WM, wn = wave / C::WM;
-  Tile32<C::A_KC> ta(g.a, m0, g.M, g.K);
-  Tile32<C::B_KC> tb(g.b, n0, g.N, g.K);
+  Tile32<C::A_KC, C::BM> ta(g.a, m0, g.M, g.K);
+  Tile32<C::B_KC, C::BN> tb(g.b, n0, g.N, g.K);
   constexpr int HALF = C::STAGE / 8;  // floats of one operand's tile
 #pragma unroll
   for (int j = 0; j < C::FN; ++j)
@@ -90,9 +91,9 @@ __device__ __forceinline__ void gemm_tile32(const GemmShape& g, int m0, int n0, 
     for (int c = 0; c < kBK32 / 8; ++c) {
       f32x4 fa[C::FM], fb[C::FN];
 #pragma unroll
-      for (int i = 0; i < C::FM; ++i) fa[i] = frag32<C::A_KC>(at, (wm * C::FM + i) * 32 + l32, c, half);
+      for (int i = 0; i < C::FM; ++i) fa[i] = frag32<C::A_KC, C::BM>(at, (wm * C::FM + i) * 32 + l32, c, half);
 #pragma unroll
-      for (int j = 0; j < C::FN; ++j) fb[j] = frag32<C::B_KC>(bt, (wn * C::FN + j) * 32 + l32, c, half);
+      for (int j = 0; j < C::FN; ++j) fb[j] = frag32<C::B_KC, C::BN>(bt, (wn * C::FN + j) * 32 + l32, c, half);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll

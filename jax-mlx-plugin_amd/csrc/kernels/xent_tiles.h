@@ -44,12 +44,12 @@ struct Config {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, E = E_;
   static constexpr bool A_KC = A_KC_, B_KC = B_KC_;
   static constexpr int NW = WM * WN, NT = NW * 64;
-  static constexpr int WAVES = BM == 256 ? 1 : 2;                 // per SIMD
+  static constexpr int WAVES = BM == 256 ? 1 : BM == 128 ? 2 : 3;  // per SIMD
   static constexpr int FM = BM / (32 * WM), FN = BN / (32 * WN);  // blocks of a wavefront
   static constexpr int BK = E == 2 ? kBK32 : kBK16;
-  // Bytes of a stage, and of all: four in 16 bits; f32: two, tiles of 128
-  // indices in the larger of the two forms' padded rows (xent_gemm32.h).
-  static constexpr int STAGE = E == 2 ? 2 * 128 * (kBK32 + 4) * 4 : (BM + BN) * kBK16 * 2;
+  // Bytes of a stage, and of all: four in 16 bits; f32: two, in the larger of
+  // the two forms' padded rows (xent_gemm32.h).
+  static constexpr int STAGE = E == 2 ? 2 * BM * (kBK32 + (BM < 128 ? 8 : 4)) * 4 : (BM + BN) * kBK16 * 2;
   static constexpr int SMEM = (E == 2 ? 2 : 4) * STAGE;
 };
 
