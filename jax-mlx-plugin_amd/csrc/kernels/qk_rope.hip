@@ -23,9 +23,13 @@
 // half the rotated features apart the chunks hold the two members, for pairs
 // side by side they are neighbours), a row takes the power of two of lanes
 // that covers it (8 at D = 128 in 16 bits), and a wavefront owns a token and
-// walks its heads, queries first, so that a token's angles are formed once
-// for all its heads.  A call of few tokens splits the heads over more
-// wavefronts.  Everything is fp32 and rounded once, at the store.
+// walks the heads of its queries or of its keys (so one weight, and in the
+// backward one set of sums, is all a lane holds).  The token's angles are
+// formed once, a pair a lane, and handed round through LDS.  The next rows are
+// on their way while these are worked on, as they came (unpacked when their
+// turn comes: twice the registers would halve the wavefronts in flight).  A call
+// of few tokens splits the heads over more wavefronts.  Everything is fp32 and
+// rounded once, at the store.
 //
 // What bounds it: HBM, each row read once and written once (backward: two
 // rows read, one written).
@@ -48,22 +52,22 @@ struct Rows {  // one [B, H, T, D] tensor: strides (batch, head, seq) in element
   int64_t s[3];
 };
 
+struct Side {  // the queries', or the keys', part of a call
+  Rows in, grad, out;  // (grad: of the outputs; out: dq or dk in the backward)
+  const void* w;
+  int heads, per_wave, parts;  // heads a wavefront walks, and wavefronts for all
+};
+
 struct Params {
-  Rows q, k;    // inputs
-  Rows gq, gk;  // gradients of the outputs (backward)
-  Rows qo, ko;  // outputs (backward: dq, dk)
-  const void* qw;
-  const void* kw;
+  Side side[2];
   const int32_t* pos;
   const uint64_t* freqs;
-  float* partial;  // [workgroups][2][D], or null
+  float* partial;  // [workgroups][D], the queries' first, or null
   int64_t ps[3];   // positions: strides (axis, batch, seq)
-  int64_t tokens;  // B * T
-  int64_t T;
-  int Hq, H;       // query heads, all heads
+  uint32_t tokens;  // B * T, below 2^31
+  uint32_t T;
   int D, rot, pairs;  // pairs = rot / 2
   int bound[kMaxAxes];  // pair i belongs to the first axis with i < bound
-  int heads_per_wave;   // a multiple of the rows a wavefront holds at once
   float eps;
 };
 
@@ -77,8 +81,7 @@ struct Chunk<T, 1> {
 };
 
 template <typename T, int VEC>
-__device__ __forceinline__ void load_chunk(const T* p, float* v) {
-  const auto c = *reinterpret_cast<const typename Chunk<T, VEC>::type*>(p);
+__device__ __forceinline__ void unpack(const typename Chunk<T, VEC>::type& c, float* v) {
   if constexpr (VEC == 1) v[0] = to_f32(c);
   else
 #pragma unroll
@@ -116,13 +119,25 @@ __device__ __forceinline__ void cos_sin(uint64_t turns, float& c, float& s) {
   s = (quarter & 2) ? -b : b;
 }
 
+// A row's chunks of one lane, as they are in memory.
+template <typename T, int VEC, int NU>
+struct Raw {
+  typename Chunk<T, VEC>::type c[NU][2];
+  __device__ __forceinline__ void get(float (&v)[NU][2 * VEC]) const {
+#pragma unroll
+    for (int n = 0; n < NU; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) unpack<T, VEC>(c[n][h], &v[n][h * VEC]);
+  }
+};
+
 // What a lane owns of every row: NU units of 2 VEC features.  Unit u < units
 // of rotated pairs holds pairs u*VEC .. u*VEC + VEC-1; the units after them
 // the features from rot on.
 template <int VEC, int NU, int LPR, bool IL>
 struct Unit {
-  int off[NU][2];   // first feature of each chunk; -1: none
-  bool turn[NU];    // rotated
+  int off[NU][2];  // first feature of each chunk; -1: none
+  bool turn[NU];   // rotated
   float c[NU][VEC], s[NU][VEC];
   __device__ __forceinline__ Unit(const Params& p, int l) {
     const int rotated = p.pairs / VEC;
@@ -138,31 +153,36 @@ struct Unit {
         off[n][0] = f < p.D ? f : -1;
         off[n][1] = f + VEC < p.D ? f + VEC : -1;
       }
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        c[n][j] = 1.f;
-        s[n][j] = 0.f;
-      }
     }
   }
-  __device__ __forceinline__ void angles(const Params& p, int l, int64_t b, int64_t t) {
+  // cos and sin of token (b, t): pair lane, lane + 64, .. by each lane into the
+  // wavefront's `cs`, from where every lane takes those of its own pairs.
+  __device__ __forceinline__ void angles(const Params& p, int lane, int l, uint32_t b, uint32_t t,
+                                         float (&cs)[2][kMaxD / 2]) {
+    const int32_t* at = p.pos + b * p.ps[1] + t * p.ps[2];
+    __builtin_amdgcn_wave_barrier();
+    for (int i = lane; i < p.pairs; i += 64) {
+      const int axis = (i >= p.bound[0]) + (i >= p.bound[1]) + (i >= p.bound[2]);
+      const int64_t pos = at[axis * p.ps[0]];
+      cos_sin((uint64_t)pos * p.freqs[i], cs[0][i], cs[1][i]);
+    }
+    // (One wavefront: its LDS operations are in order.)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
-      if (!turn[n]) continue;
-      const int i0 = (n * LPR + l) * VEC;
-      const int32_t* at = p.pos + b * p.ps[1] + t * p.ps[2];
+      const int i0 = turn[n] ? (n * LPR + l) * VEC : 0;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const int i = i0 + j;
-        const int axis = (i >= p.bound[0]) + (i >= p.bound[1]) + (i >= p.bound[2]);
-        const int64_t pos = at[axis * p.ps[0]];
-        cos_sin((uint64_t)pos * p.freqs[i], c[n][j], s[n][j]);
+        c[n][j] = cs[0][i0 + j];
+        s[n][j] = cs[1][i0 + j];
       }
     }
   }
   // Rotates (forward) or turns back (!FWD) the unit's 2 VEC values.
   template <bool FWD>
   __device__ __forceinline__ void rotate(int n, float* v) const {
+    if (!turn[n]) return;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       const int ia = IL ? 2 * j : j, ib = IL ? 2 * j + 1 : VEC + j;
@@ -172,15 +192,14 @@ struct Unit {
     }
   }
   template <typename T>
-  __device__ __forceinline__ void load(const T* row, bool valid, float (&v)[NU][2 * VEC]) const {
+  __device__ __forceinline__ void load(const T* row, bool valid, Raw<T, VEC, NU>& r) const {
 #pragma unroll
     for (int n = 0; n < NU; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (valid && off[n][h] >= 0) load_chunk<T, VEC>(row + off[n][h], &v[n][h * VEC]);
-        else
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) v[n][h * VEC + j] = 0.f;
+        r.c[n][h] = typename Chunk<T, VEC>::type{};
+        if (valid && off[n][h] >= 0)
+          r.c[n][h] = *reinterpret_cast<const typename Chunk<T, VEC>::type*>(row + off[n][h]);
       }
   }
   template <typename T>
@@ -191,72 +210,72 @@ struct Unit {
       for (int h = 0; h < 2; ++h)
         if (off[n][h] >= 0) store_chunk<T, VEC>(row + off[n][h], &v[n][h * VEC]);
   }
+  template <typename PT>
+  __device__ __forceinline__ void weight(const void* w, float (&v)[NU][2 * VEC]) const {
+#pragma unroll
+    for (int n = 0; n < NU; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          v[n][h * VEC + j] = w && off[n][h] >= 0 ? to_f32(static_cast<const PT*>(w)[off[n][h] + j]) : 1.f;
+  }
 };
 
-template <typename PT, int VEC, int NU, class U>
-__device__ __forceinline__ void load_weight(const U& u, const void* w, float (&v)[NU][2 * VEC]) {
-#pragma unroll
-  for (int n = 0; n < NU; ++n)
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        v[n][h * VEC + j] = w && u.off[n][h] >= 0 ? to_f32(static_cast<const PT*>(w)[u.off[n][h] + j]) : 1.f;
+template <typename T>
+__device__ __forceinline__ T* row_of(const Rows& r, uint32_t b, int h, uint32_t t) {
+  return const_cast<T*>(static_cast<const T*>(r.p)) + b * r.s[0] + h * r.s[1] + t * r.s[2];
 }
 
-// Row of head hh (queries first) of a (q, k) tensor pair.
-template <typename T>
-__device__ __forceinline__ const T* row_of(const Rows& q, const Rows& k, int Hq, int hh, int64_t b, int64_t t) {
-  const bool isq = hh < Hq;
-  const T* base = static_cast<const T*>(isq ? q.p : k.p);
-  const int64_t* s = isq ? q.s : k.s;
-  return base + b * s[0] + (int64_t)(isq ? hh : hh - Hq) * s[1] + t * s[2];
+// This workgroup's side and heads [h0, h1): blockIdx.y counts the queries'
+// parts, then the keys'.
+__device__ __forceinline__ const Side& my_side(const Params& p, int& h0, int& h1) {
+  const bool key = (int)blockIdx.y >= p.side[0].parts;
+  const Side& sd = p.side[key];
+  h0 = ((int)blockIdx.y - (key ? p.side[0].parts : 0)) * sd.per_wave;
+  h1 = min(sd.heads, h0 + sd.per_wave);
+  return sd;
 }
 
 template <typename T, typename PT, int VEC, int NU, int LPR, bool IL>
 __global__ __launch_bounds__(kBlock) void qk_rope_kernel(Params p) {
   constexpr int RPW = 64 / LPR;  // rows a wavefront holds at once
+  __shared__ __attribute__((aligned(16))) float cs[kWaves][2][kMaxD / 2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l = lane % LPR, g = lane / LPR;
-  const int64_t tok = (int64_t)blockIdx.x * kWaves + wave;
+  const uint32_t tok = blockIdx.x * kWaves + wave;
   if (tok >= p.tokens) return;
-  const int64_t b = tok / p.T, t = tok % p.T;
-  const int h0 = blockIdx.y * p.heads_per_wave;
-  const int h1 = min(p.H, h0 + p.heads_per_wave);
+  const uint32_t b = tok / p.T, t = tok - b * p.T;
+  int h0, h1;
+  const Side& sd = my_side(p, h0, h1);
 
   Unit<VEC, NU, LPR, IL> u(p, l);
-  float x[NU][2 * VEC];
-  int hh = h0 + g;
-  if (hh < h1) u.load(row_of<T>(p.q, p.k, p.Hq, hh, b, t), true, x);
-  u.angles(p, l, b, t);
-  float qw[NU][2 * VEC], kw[NU][2 * VEC];
-  load_weight<PT, VEC, NU>(u, p.qw, qw);
-  load_weight<PT, VEC, NU>(u, p.kw, kw);
+  Raw<T, VEC, NU> raw;
+  u.load(row_of<T>(sd.in, b, min(h0 + g, h1 - 1), t), h0 + g < h1, raw);
+  float w[NU][2 * VEC];
+  u.template weight<PT>(sd.w, w);
+  u.angles(p, lane, l, b, t, cs[wave]);
   const float inv_d = 1.f / (float)p.D;
-  for (int hb = h0; hb < h1; hb += RPW, hh += RPW) {
-    // The next head's row travels while this one is worked on.
-    float nx[NU][2 * VEC];
-    const bool more = hh + RPW < h1;
-    u.load(row_of<T>(p.q, p.k, p.Hq, more ? hh + RPW : h0, b, t), more, nx);
-    float ss = 0.f;
+  for (int h = h0 + g; h < h1 + g; h += RPW) {
+    float x[NU][2 * VEC];
+    raw.get(x);
+    if (h - g + RPW < h1) u.load(row_of<T>(sd.in, b, min(h + RPW, h1 - 1), t), h + RPW < h1, raw);
+    if (p.eps >= 0.f) {
+      float ss = 0.f;
 #pragma unroll
-    for (int n = 0; n < NU; ++n)
+      for (int n = 0; n < NU; ++n)
 #pragma unroll
-      for (int j = 0; j < 2 * VEC; ++j) ss = fmaf(x[n][j], x[n][j], ss);
-    const float r = p.eps >= 0.f ? 1.f / sqrtf(group_sum<LPR>(ss) * inv_d + p.eps) : 1.f;
-    const bool isq = hh < p.Hq;
+        for (int j = 0; j < 2 * VEC; ++j) ss = fmaf(x[n][j], x[n][j], ss);
+      const float r = 1.f / sqrtf(group_sum<LPR>(ss) * inv_d + p.eps);
 #pragma unroll
-    for (int n = 0; n < NU; ++n) {
+      for (int n = 0; n < NU; ++n)
 #pragma unroll
-      for (int j = 0; j < 2 * VEC; ++j) x[n][j] = x[n][j] * r * (isq ? qw[n][j] : kw[n][j]);
-      if (u.turn[n]) u.template rotate<true>(n, x[n]);
+        for (int j = 0; j < 2 * VEC; ++j) x[n][j] = x[n][j] * r * w[n][j];
     }
-    if (hh < h1) u.store(const_cast<T*>(row_of<T>(p.qo, p.ko, p.Hq, hh, b, t)), x);
 #pragma unroll
-    for (int n = 0; n < NU; ++n)
-#pragma unroll
-      for (int j = 0; j < 2 * VEC; ++j) x[n][j] = nx[n][j];
+    for (int n = 0; n < NU; ++n) u.template rotate<true>(n, x[n]);
+    if (h < h1) u.store(row_of<T>(sd.out, b, h, t), x);
   }
 }
 
@@ -267,109 +286,127 @@ __global__ __launch_bounds__(kBlock) void qk_rope_kernel(Params p) {
 template <typename T, typename PT, int VEC, int NU, int LPR, bool IL>
 __global__ __launch_bounds__(kBlock) void qk_rope_bwd_kernel(Params p) {
   constexpr int RPW = 64 / LPR;
+  __shared__ __attribute__((aligned(16))) float cs[kWaves][2][kMaxD / 2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l = lane % LPR, g = lane / LPR;
+  int h0, h1;
+  const Side& sd = my_side(p, h0, h1);
   Unit<VEC, NU, LPR, IL> u(p, l);
-  float qw[NU][2 * VEC], kw[NU][2 * VEC], aq[NU][2 * VEC], ak[NU][2 * VEC];
-  load_weight<PT, VEC, NU>(u, p.qw, qw);
-  load_weight<PT, VEC, NU>(u, p.kw, kw);
+  float w[NU][2 * VEC], acc[NU][2 * VEC];
+  u.template weight<PT>(sd.w, w);
 #pragma unroll
   for (int n = 0; n < NU; ++n)
 #pragma unroll
-    for (int j = 0; j < 2 * VEC; ++j) aq[n][j] = ak[n][j] = 0.f;
+    for (int j = 0; j < 2 * VEC; ++j) acc[n][j] = 0.f;
   const float inv_d = 1.f / (float)p.D;
-  const int h0 = blockIdx.y * p.heads_per_wave;
-  const int h1 = min(p.H, h0 + p.heads_per_wave);
 
-  for (int64_t tok = (int64_t)blockIdx.x * kWaves + wave; tok < p.tokens; tok += (int64_t)gridDim.x * kWaves) {
-    const int64_t b = tok / p.T, t = tok % p.T;
-    u.angles(p, l, b, t);
-    for (int hb = h0; hb < h1; hb += RPW) {
-      const int hh = hb + g;
-      const bool valid = hh < h1, isq = hh < p.Hq;
-      float x[NU][2 * VEC], d[NU][2 * VEC];
-      u.load(row_of<T>(p.q, p.k, p.Hq, valid ? hh : h0, b, t), valid, x);
-      u.load(row_of<T>(p.gq, p.gk, p.Hq, valid ? hh : h0, b, t), valid, d);
+  // Rows of (token, heads from h on) travel while the ones before are worked
+  // on, across tokens too.
+  Raw<T, VEC, NU> rx, rd;
+  auto fetch = [&](uint32_t tok, int h) __attribute__((always_inline)) {
+    const uint32_t b = tok / p.T, t = tok - b * p.T;
+    const bool valid = h + g < h1;
+    const int hh = valid ? h + g : h0;
+    u.load(row_of<T>(sd.in, b, hh, t), valid, rx);
+    u.load(row_of<T>(sd.grad, b, hh, t), valid, rd);
+  };
+  const uint32_t stride = gridDim.x * kWaves;
+  uint32_t tok = blockIdx.x * kWaves + wave;
+  if (tok < p.tokens) fetch(tok, h0);
+  for (int hb = h0; tok < p.tokens;) {
+    const uint32_t b = tok / p.T, t = tok - b * p.T;
+    if (hb == h0) u.angles(p, lane, l, b, t, cs[wave]);
+    const bool same = hb + RPW < h1;
+    const uint32_t tok2 = same ? tok : tok + stride;
+    const int hb2 = same ? hb + RPW : h0;
+    float x[NU][2 * VEC], d[NU][2 * VEC];
+    rx.get(x);
+    rd.get(d);
+    if (tok2 < p.tokens) fetch(tok2, hb2);
+    const bool valid = hb + g < h1;
+#pragma unroll
+    for (int n = 0; n < NU; ++n) u.template rotate<false>(n, d[n]);
+    if (p.eps >= 0.f) {
       float ss = 0.f;
 #pragma unroll
-      for (int n = 0; n < NU; ++n) {
+      for (int n = 0; n < NU; ++n)
 #pragma unroll
         for (int j = 0; j < 2 * VEC; ++j) ss = fmaf(x[n][j], x[n][j], ss);
-        if (u.turn[n]) u.template rotate<false>(n, d[n]);
-      }
-      if (p.eps >= 0.f) {
-        // (An absent row adds nothing: with eps = 0 its r would be infinite.)
-        const float r = valid ? 1.f / sqrtf(group_sum<LPR>(ss) * inv_d + p.eps) : (group_sum<LPR>(ss), 0.f);
-        float dot = 0.f;
+      const float mean = group_sum<LPR>(ss) * inv_d;
+      // (An absent row adds nothing: with eps = 0 its r would be infinite.)
+      const float r = valid ? 1.f / sqrtf(mean + p.eps) : 0.f;
+      float dot = 0.f;
 #pragma unroll
-        for (int n = 0; n < NU; ++n)
+      for (int n = 0; n < NU; ++n)
 #pragma unroll
-          for (int j = 0; j < 2 * VEC; ++j) {
-            x[n][j] *= r;
-            const float dxh = d[n][j] * x[n][j];
-            if (isq) aq[n][j] += dxh;
-            else ak[n][j] += dxh;
-            d[n][j] *= isq ? qw[n][j] : kw[n][j];
-            dot = fmaf(d[n][j], x[n][j], dot);
-          }
-        const float m = group_sum<LPR>(dot) * inv_d;
+        for (int j = 0; j < 2 * VEC; ++j) {
+          x[n][j] *= r;
+          acc[n][j] = fmaf(d[n][j], x[n][j], acc[n][j]);
+          d[n][j] *= w[n][j];
+          dot = fmaf(d[n][j], x[n][j], dot);
+        }
+      const float m = group_sum<LPR>(dot) * inv_d;
 #pragma unroll
-        for (int n = 0; n < NU; ++n)
+      for (int n = 0; n < NU; ++n)
 #pragma unroll
-          for (int j = 0; j < 2 * VEC; ++j) d[n][j] = r * (d[n][j] - x[n][j] * m);
-      }
-      if (valid) u.store(const_cast<T*>(row_of<T>(p.qo, p.ko, p.Hq, hh, b, t)), d);
+        for (int j = 0; j < 2 * VEC; ++j) d[n][j] = r * (d[n][j] - x[n][j] * m);
     }
+    if (valid) u.store(row_of<T>(sd.out, b, hb + g, t), d);
+    tok = tok2;
+    hb = hb2;
   }
   if (!p.partial) return;  // (uniform over the grid)
   // Fold the rows a wavefront holds, then the wavefronts.
-  __shared__ float fold[kWaves][2][kMaxD];
+  __shared__ float fold[kWaves][kMaxD];
 #pragma unroll
   for (int n = 0; n < NU; ++n)
 #pragma unroll
     for (int j = 0; j < 2 * VEC; ++j) {
 #pragma unroll
-      for (int off = LPR; off < 64; off <<= 1) {
-        aq[n][j] += __shfl_xor(aq[n][j], off, 64);
-        ak[n][j] += __shfl_xor(ak[n][j], off, 64);
-      }
+      for (int off = LPR; off < 64; off <<= 1) acc[n][j] += __shfl_xor(acc[n][j], off, 64);
       const int h = j / VEC;
-      if (g == 0 && u.off[n][h] >= 0) {
-        fold[wave][0][u.off[n][h] + j % VEC] = aq[n][j];
-        fold[wave][1][u.off[n][h] + j % VEC] = ak[n][j];
-      }
+      if (g == 0 && u.off[n][h] >= 0) fold[wave][u.off[n][h] + j % VEC] = acc[n][j];
     }
   __syncthreads();
-  float* out = p.partial + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * p.D;
-  for (int i = threadIdx.x; i < 2 * p.D; i += kBlock) {
-    const int which = i / p.D, d = i % p.D;
+  float* out = p.partial + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * p.D;
+  for (int i = threadIdx.x; i < p.D; i += kBlock) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) s += fold[w][which][d];
+    for (int wv = 0; wv < kWaves; ++wv) s += fold[wv][i];
     out[i] = s;
   }
 }
 
-// dw[which][d] = sum over the G partial rows, 32 columns a workgroup, each
-// column's rows shared out over 32 threads and folded in order.
+// dw[d] = sum over the G0 partial rows of the queries (blockIdx.y 0) or the G1
+// behind them of the keys, 16 columns a workgroup, each column's rows shared
+// out over 64 threads (eight in flight at a time) and folded in order.
 template <typename PT>
-__global__ __launch_bounds__(1024) void qk_rope_params(const float* __restrict__ partial, int G, int D, PT* dqw,
-                                                       PT* dkw) {
-  __shared__ float fold[32][33];
-  const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + c;
+__global__ __launch_bounds__(1024) void qk_rope_params(const float* __restrict__ partial, int G0, int G1, int D,
+                                                       PT* dqw, PT* dkw) {
+  PT* const out = blockIdx.y ? dkw : dqw;
+  if (!out) return;
+  const int G = blockIdx.y ? G1 : G0;
+  if (blockIdx.y) partial += (int64_t)G0 * D;
+  __shared__ float fold[64][17];
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const int col = blockIdx.x * 16 + c;
   float s = 0.f;
-  if (col < 2 * D)
-    for (int i = r; i < G; i += 32) s += partial[(int64_t)i * 2 * D + col];
+  if (col < D)
+    for (int i0 = r; i0 < G; i0 += 8 * 64) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = i0 + u * 64 < G ? partial[(int64_t)(i0 + u * 64) * D + col] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += v[u];
+    }
   fold[r][c] = s;
   __syncthreads();
-  if (r != 0 || col >= 2 * D) return;
+  if (r != 0 || col >= D) return;
   float t = 0.f;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) t += fold[i][c];
-  PT* out = col < D ? dqw : dkw;
-  if (out) out[col < D ? col : col - D] = from_f32<PT>(t);
+  for (int i = 0; i < 64; ++i) t += fold[i][c];
+  out[col] = from_f32<PT>(t);
 }
 
 // ---- host ------------------------------------------------------------------
@@ -385,7 +422,7 @@ struct Plan {
   int vec = 1, nu = 1, lpr = 1;
   bool f32_params = true;
   dim3 grid;       // workgroups
-  int partials = 0;  // rows of partial sums (backward with weight gradients)
+  bool sums = false;  // the backward adds up weight gradients
 };
 
 bool float_dtype(int dt) { return dt == MFX_F32 || dt == MFX_BF16 || dt == MFX_F16; }
@@ -437,10 +474,10 @@ int plan_common(Plan& pl, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t
   p.pos = pos;
   p.freqs = freqs;
   for (int i = 0; i < 3; ++i) p.ps[i] = ps[i];
-  p.tokens = B * T;
-  p.T = T;
-  p.Hq = (int)Hq;
-  p.H = (int)(Hq + Hkv);
+  p.tokens = (uint32_t)(B * T);
+  p.T = (uint32_t)T;
+  p.side[0].heads = (int)Hq;
+  p.side[1].heads = (int)Hkv;
   p.D = (int)D;
   p.rot = (int)rot;
   p.pairs = (int)(rot / 2);
@@ -453,7 +490,8 @@ int plan_common(Plan& pl, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t
   for (int vec : widths) {
     if (D % vec || p.pairs % vec || (D - rot) % vec) continue;
     bool ok = true;
-    for (const Rows* r : {&p.q, &p.k, &p.gq, &p.gk, &p.qo, &p.ko}) ok = ok && chunked(*r, vec, size);
+    for (const Side& sd : p.side)
+      for (const Rows* r : {&sd.in, &sd.grad, &sd.out}) ok = ok && chunked(*r, vec, size);
     if (!ok) continue;
     pl.vec = vec;
     break;
@@ -465,18 +503,24 @@ int plan_common(Plan& pl, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t
   return MFX_OK;
 }
 
-// Heads a wavefront walks: all of them (its angles then serve the whole
-// token) unless the tokens are too few to fill the device with eight
-// wavefronts a CU, when they are split down to one pass of rows each.
-// Returns the number of parts.
-int split_heads(Plan& pl, int64_t waves) {
+// Wavefronts that the tokens should be shared out to: eight a CU.
+int64_t wanted_waves() { return 8LL * device_cu_count(); }
+
+// Heads a wavefront walks: all of a side (its angles then serve them all) unless
+// `waves` of them are fewer than wanted, when the heads are split down to one
+// pass of rows each.
+void split_heads(Plan& pl, int64_t waves) {
   const int rpw = 64 / pl.lpr;
-  const int passes = (pl.p.H + rpw - 1) / rpw;
-  const int64_t want = 8LL * device_cu_count();
-  int parts = waves > 0 && waves < want ? (int)std::min<int64_t>(passes, (want + waves - 1) / waves) : 1;
-  const int per = (passes + parts - 1) / parts;
-  pl.p.heads_per_wave = per * rpw;
-  return (passes + per - 1) / per;
+  for (Side& sd : pl.p.side) {
+    sd.parts = sd.per_wave = 0;
+    if (sd.heads == 0) continue;
+    const int passes = (sd.heads + rpw - 1) / rpw;
+    const int64_t want = wanted_waves();
+    const int parts = waves > 0 && waves < want ? (int)std::min<int64_t>(passes, (want + waves - 1) / waves) : 1;
+    const int per = (passes + parts - 1) / parts;
+    sd.per_wave = per * rpw;
+    sd.parts = (passes + per - 1) / per;
+  }
 }
 
 template <bool BWD, typename T, typename PT, int VEC, int NU, int LPR, bool IL>
@@ -526,19 +570,21 @@ int plan_fwd(const mfx_qk_norm_rope_args* a, Plan& pl) {
   if (any && ((a->Hq > 0 && (!a->q || !a->q_out)) || (a->Hkv > 0 && (!a->k || !a->k_out))))
     return fail(MFX_E_INVALID, "q, q_out (and with Hkv > 0 k, k_out) must be non-null");
   Params& p = pl.p;
+  Side &q = p.side[0], &k = p.side[1];
   int rc = MFX_OK;
-  if (a->Hq > 0 && ((rc = bind(p.q, a->q, a->q_strides, "q")) || (rc = bind(p.qo, a->q_out, a->qo_strides, "q_out"))))
+  if (a->Hq > 0 && ((rc = bind(q.in, a->q, a->q_strides, "q")) || (rc = bind(q.out, a->q_out, a->qo_strides, "q_out"))))
     return rc;
-  if (a->Hkv > 0 && ((rc = bind(p.k, a->k, a->k_strides, "k")) || (rc = bind(p.ko, a->k_out, a->ko_strides, "k_out"))))
+  if (a->Hkv > 0 && ((rc = bind(k.in, a->k, a->k_strides, "k")) || (rc = bind(k.out, a->k_out, a->ko_strides, "k_out"))))
     return rc;
-  p.qw = a->q_weight;
-  p.kw = a->k_weight;
+  q.w = a->q_weight;
+  k.w = a->k_weight;
   rc = plan_common(pl, a->B, a->T, a->Hq, a->Hkv, a->D, a->rot, a->positions, a->freqs, a->pos_strides, a->sections,
                    a->axes, a->eps, a->dtype, a->param_dtype, a->interleaved != 0, a->q_weight || a->k_weight);
   if (rc) return rc;
   if (p.tokens == 0) return MFX_OK;
-  const int64_t blocks = (p.tokens + kWaves - 1) / kWaves;
-  pl.grid = dim3((unsigned)blocks, (unsigned)split_heads(pl, p.tokens));
+  const int64_t blocks = ((int64_t)p.tokens + kWaves - 1) / kWaves;
+  split_heads(pl, p.tokens);
+  pl.grid = dim3((unsigned)blocks, (unsigned)(q.parts + k.parts));
   return MFX_OK;
 }
 
@@ -548,16 +594,17 @@ int plan_bwd(const mfx_qk_norm_rope_bwd_args* a, Plan& pl) {
   if (any && ((a->Hq > 0 && (!a->q || !a->dq_out || !a->dq)) || (a->Hkv > 0 && (!a->k || !a->dk_out || !a->dk))))
     return fail(MFX_E_INVALID, "q, dq_out, dq (and with Hkv > 0 k, dk_out, dk) must be non-null");
   Params& p = pl.p;
+  Side &q = p.side[0], &k = p.side[1];
   int rc = MFX_OK;
-  if (a->Hq > 0 && ((rc = bind(p.q, a->q, a->q_strides, "q")) || (rc = bind(p.gq, a->dq_out, a->dqo_strides, "dq_out")) ||
-                    (rc = bind(p.qo, a->dq, a->dq_strides, "dq"))))
+  if (a->Hq > 0 && ((rc = bind(q.in, a->q, a->q_strides, "q")) || (rc = bind(q.grad, a->dq_out, a->dqo_strides, "dq_out")) ||
+                    (rc = bind(q.out, a->dq, a->dq_strides, "dq"))))
     return rc;
-  if (a->Hkv > 0 && ((rc = bind(p.k, a->k, a->k_strides, "k")) ||
-                     (rc = bind(p.gk, a->dk_out, a->dko_strides, "dk_out")) ||
-                     (rc = bind(p.ko, a->dk, a->dk_strides, "dk"))))
+  if (a->Hkv > 0 && ((rc = bind(k.in, a->k, a->k_strides, "k")) ||
+                     (rc = bind(k.grad, a->dk_out, a->dko_strides, "dk_out")) ||
+                     (rc = bind(k.out, a->dk, a->dk_strides, "dk"))))
     return rc;
-  p.qw = a->q_weight;
-  p.kw = a->k_weight;
+  q.w = a->q_weight;
+  k.w = a->k_weight;
   const bool grads = a->dq_weight || a->dk_weight;
   rc = plan_common(pl, a->B, a->T, a->Hq, a->Hkv, a->D, a->rot, a->positions, a->freqs, a->pos_strides, a->sections,
                    a->axes, a->eps, a->dtype, a->param_dtype, a->interleaved != 0,
@@ -565,14 +612,14 @@ int plan_bwd(const mfx_qk_norm_rope_bwd_args* a, Plan& pl) {
   if (rc) return rc;
   // Workgroups: one token a wavefront up to kMaxPartials of them, then each
   // wavefront walks several (fewer partial rows to add up).
-  const int64_t blocks = std::min<int64_t>((p.tokens + kWaves - 1) / kWaves, kMaxPartials);
-  const int parts = split_heads(pl, blocks * kWaves);
-  pl.grid = dim3((unsigned)std::max<int64_t>(blocks, 1), (unsigned)parts);
-  pl.partials = grads && p.tokens > 0 ? (int)blocks * parts : 0;
+  const int64_t blocks = std::min<int64_t>(((int64_t)p.tokens + kWaves - 1) / kWaves, kMaxPartials);
+  split_heads(pl, blocks * kWaves);
+  pl.grid = dim3((unsigned)blocks, (unsigned)(q.parts + k.parts));
+  pl.sums = grads && p.tokens > 0;
   return MFX_OK;
 }
 
-size_t bwd_bytes(const Plan& pl) { return (size_t)pl.partials * 2 * pl.p.D * sizeof(float); }
+size_t bwd_bytes(const Plan& pl) { return pl.sums ? (size_t)pl.grid.x * pl.grid.y * pl.p.D * sizeof(float) : 0; }
 
 }  // namespace
 }  // namespace mfx
@@ -608,12 +655,14 @@ int mfx_qk_norm_rope(const mfx_qk_norm_rope_args* args, void* stream) {
 size_t mfx_qk_norm_rope_bwd_workspace_size(const mfx_qk_norm_rope_bwd_args* args) {
   mfx::Plan pl;
   if (mfx::plan_bwd(args, pl) != MFX_OK) return 0;
-  if (!pl.partials) return 0;
+  if (!pl.sums) return 0;
   // At any alignment: narrower chunks take more lanes a row, hence more parts
   // of the heads, up to one row each or what fills the device (split_heads).
-  const int64_t waves = (int64_t)pl.grid.x * mfx::kWaves, want = 8LL * mfx::device_cu_count();
-  const int64_t parts = waves < want ? std::min<int64_t>(pl.p.H, (want + waves - 1) / waves) : 1;
-  return (size_t)pl.grid.x * parts * 2 * pl.p.D * sizeof(float);
+  const int64_t waves = (int64_t)pl.grid.x * mfx::kWaves, want = mfx::wanted_waves();
+  int64_t parts = 0;
+  for (const mfx::Side& sd : pl.p.side)
+    if (sd.heads) parts += waves < want ? std::min<int64_t>(sd.heads, (want + waves - 1) / waves) : 1;
+  return (size_t)pl.grid.x * parts * pl.p.D * sizeof(float);
 }
 
 int mfx_qk_norm_rope_bwd(const mfx_qk_norm_rope_bwd_args* args, void* stream) {
@@ -637,15 +686,16 @@ int mfx_qk_norm_rope_bwd(const mfx_qk_norm_rope_bwd_args* args, void* stream) {
     if (int rc = launch_t<true>(pl, args->dtype, args->interleaved != 0, s)) return rc;
   if (!args->dq_weight && !args->dk_weight) return MFX_OK;
   // (Without tokens the weight gradients are empty sums.)
-  const dim3 grid((unsigned)((2 * pl.p.D + 31) / 32));
+  const dim3 grid((unsigned)((pl.p.D + 15) / 16), 2);
+  const int g0 = pl.sums ? (int)pl.grid.x * pl.p.side[0].parts : 0, g1 = pl.sums ? (int)pl.grid.x * pl.p.side[1].parts : 0;
   if (pl.f32_params)
-    hipLaunchKernelGGL((qk_rope_params<float>), grid, dim3(1024), 0, s, pl.p.partial, pl.partials, pl.p.D,
+    hipLaunchKernelGGL((qk_rope_params<float>), grid, dim3(1024), 0, s, pl.p.partial, g0, g1, pl.p.D,
                        static_cast<float*>(args->dq_weight), static_cast<float*>(args->dk_weight));
   else if (args->dtype == MFX_BF16)
-    hipLaunchKernelGGL((qk_rope_params<bf16>), grid, dim3(1024), 0, s, pl.p.partial, pl.partials, pl.p.D,
+    hipLaunchKernelGGL((qk_rope_params<bf16>), grid, dim3(1024), 0, s, pl.p.partial, g0, g1, pl.p.D,
                        static_cast<bf16*>(args->dq_weight), static_cast<bf16*>(args->dk_weight));
   else
-    hipLaunchKernelGGL((qk_rope_params<_Float16>), grid, dim3(1024), 0, s, pl.p.partial, pl.partials, pl.p.D,
+    hipLaunchKernelGGL((qk_rope_params<_Float16>), grid, dim3(1024), 0, s, pl.p.partial, g0, g1, pl.p.D,
                        static_cast<_Float16*>(args->dq_weight), static_cast<_Float16*>(args->dk_weight));
   return launch_status("qk_rope_params");
 }

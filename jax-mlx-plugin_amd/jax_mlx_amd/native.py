@@ -672,17 +672,21 @@ def sdpa_bwd_workspace_size(q, k, v, **kw) -> int:
 
 # ---- helpers of the operators below ----------------------------------------------
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(t, *others):
     """Context in which work for t's device is launched: t's device made the
-    current one if it is not.  The other tensors must live there too."""
-    torch = _torch()
-    _require_gpu(t, *others)
+    current one if it is not.  The other tensors (or None) must live there too."""
+    index = t.get_device()
+    if index < 0:
+        raise ValueError("tensor must live on the GPU (device memory)")
     for o in others:
-        if o is not None and o.device != t.device:
-            raise ValueError(f"tensors on {t.device} and {o.device}")
-    if torch.cuda.current_device() == t.device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+        if o is not None and o.get_device() != index:
+            raise ValueError(f"tensors on {t.device} and {o.device}: all must live on one GPU")
+    if _torch().cuda.current_device() == index:
+        return _HERE
+    return _torch().cuda.device(index)
 
 
 def _ptr(t):
@@ -710,23 +714,23 @@ _PACKED_BWD_PACK = struct.Struct("11PN5q24qf3i").pack
 
 def _packed_dims(q, k, v, seq_offsets, *like_q):
     """(T, sequences, Hq, Hkv, D) of checked [T, H, D] tensors."""
-    torch = _torch()
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+    shape, dt, ks = q.shape, q.dtype, k.shape
+    if len(shape) != 3 or len(ks) != 3:
         raise ValueError("packed q, k and v are [T, heads, head size]")
-    T, Hq, D = q.shape
-    if k.shape != v.shape or k.shape[0] != T or k.shape[2] != D:
+    T, Hq, D = shape
+    if ks != v.shape or ks[0] != T or ks[2] != D:
         raise ValueError("k and v must agree with each other and with q in tokens and head size")
-    for t in (k, v, *like_q):
-        if t.dtype != q.dtype:
-            raise ValueError("packed tensors must share one dtype")
+    if k.dtype != dt or v.dtype != dt:
+        raise ValueError("packed tensors must share one dtype")
     for t in like_q:
-        if t.shape != q.shape:
-            raise ValueError("out and its gradient must have q's shape")
-    if seq_offsets.dtype != torch.int32 or seq_offsets.dim() != 1 or not seq_offsets.is_contiguous():
+        if t.shape != shape or t.dtype != dt:
+            raise ValueError("out and the gradients must have q's shape and dtype")
+    if seq_offsets.dtype != _torch().int32 or seq_offsets.dim() != 1 or not seq_offsets.is_contiguous():
         raise TypeError("seq_offsets must be a contiguous int32 vector")
-    if seq_offsets.numel() < 1:
+    n = seq_offsets.numel()
+    if n < 1:
         raise ValueError("seq_offsets has one more entry than there are sequences")
-    return T, seq_offsets.numel() - 1, Hq, k.shape[1], D
+    return T, n - 1, Hq, ks[1], D
 
 
 def _htd(t):
@@ -757,7 +761,7 @@ def sdpa_packed(q, k, v, seq_offsets, *, scale=None, causal=True, out=None, lse=
     sdpa_packed_bwd."""
     torch = _torch()
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     a = sdpa_packed_args(q, k, v, out, seq_offsets, scale=scale, causal=causal, lse=lse)
     with _on(q, k, v, out, seq_offsets, lse):
         check(load().mfx_sdpa_packed(ctypes.byref(a), _stream_handle(q)))
@@ -790,7 +794,7 @@ def sdpa_packed_bwd(q, k, v, dout, out, lse, seq_offsets, *, scale=None, causal=
     its out and lse (mfx_sdpa_packed_bwd).  Rows in no sequence are not
     written."""
     torch = _torch()
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if g is None else g
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) if g is None else g
                   for t, g in ((q, dq), (k, dk), (v, dv)))
     a = sdpa_packed_bwd_args(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, scale=scale, causal=causal)
     with _on(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, workspace):
@@ -832,77 +836,85 @@ _QK_PACK = struct.Struct("8P6q16q3q4i4ifi").pack
 _QK_BWD_PACK = struct.Struct("13PN6q24q3q4i4ifi").pack
 
 
-def _head_rows(t, layout):
-    """((B, H, T, D), strides) of [T, H, D] tokens or a 4-D tensor."""
-    if t.dim() == 3:
-        s = t.stride()
-        return (1, t.shape[1], t.shape[0], t.shape[2]), (t.shape[0] * s[0], s[1], s[0], s[2])
-    if t.dim() != 4:
-        raise ValueError("queries and keys are [T, H, D] or 4-D")
-    return _dims(t, layout), _strides4(t, layout)
+def _head_strides(t, layout):
+    """(batch, head, seq, feature) strides of [T, H, D] tokens or a 4-D tensor."""
+    s = t.stride()
+    if len(s) == 3:
+        return (0, s[1], s[0], s[2])
+    return s if layout == "bhtd" else (s[0], s[2], s[1], s[3])
+
+
+_NO_ROWS = (0, 0, 0, 1)
 
 
 def _qk_fields(q, k, positions, table, q_weight, k_weight, eps, sections, interleaved, layout, more):
-    """Checked (pointers of positions and table, dims, strides of q, k and of
-    the (q-shaped, k-shaped) pairs in `more`, the rest) for the packed structs."""
-    torch = _torch()
-    if q is None and k is None:
-        raise ValueError("q or k is needed")
+    """Checked (pointers of positions and table, dims, the rest) for the packed
+    structs; the rest starts with the strides of q, k and of the (q-shaped,
+    k-shaped) pairs in `more`."""
     first = q if q is not None else k
-    (B, _, T, D), _ = _head_rows(first, layout)
-    heads, strides = [0, 0], []
-    for pair in ((q, k), *more):
-        for i, t in enumerate(pair):
-            like = (q, k)[i]
-            if (t is None) != (like is None):
-                raise ValueError("q and k each need their outputs (and gradients)")
-            if t is None:
-                strides.append((0, 0, 0, 1))
+    if first is None:
+        raise ValueError("q or k is needed")
+    shape, dt = first.shape, first.dtype
+    if len(shape) == 3:
+        B, (T, H, D) = 1, shape
+    elif len(shape) != 4:
+        raise ValueError("queries and keys are [T, H, D] or 4-D")
+    elif layout == "bhtd":
+        B, H, T, D = shape
+    elif layout == "bthd":
+        B, T, H, D = shape
+    else:
+        raise ValueError(f"layout must be 'bhtd' or 'bthd', got {layout!r}")
+    Hq, Hkv = (H, 0) if k is None else (0, H)
+    if q is not None and k is not None:
+        at = 1 if len(shape) == 3 or layout == "bhtd" else 2
+        ks = k.shape
+        if k.dtype != dt or len(ks) != len(shape) or ks[:at] != shape[:at] or ks[at + 1:] != shape[at + 1:]:
+            raise ValueError("q and k must agree in dtype, batch, tokens and head size")
+        Hq, Hkv = H, ks[at]
+    strides = ()
+    for a, b in ((q, k), *more):
+        for t, like in ((a, q), (b, k)):
+            if t is None or like is None:
+                if t is not like:
+                    raise ValueError("q and k each need their outputs (and gradients)")
+                strides += _NO_ROWS
                 continue
-            if t.shape != like.shape or t.dtype != first.dtype or t.dim() != first.dim():
-                raise ValueError("q and k (and their outputs and gradients) must agree in shape and dtype")
-            (b, h, n, d), st = _head_rows(t, layout)
-            if (b, n, d) != (B, T, D):
-                raise ValueError("q and k must agree in batch, tokens and head size")
-            heads[i] = h
-            strides.append(st)
-    rot = 2 * table.numel() if table is not None else 0
-    ps, axes, secs = (0, 0, 0), 1, (rot // 2, 0, 0, 0)
-    if rot:
-        if table.dtype != torch.int64 or table.dim() != 1 or not table.is_contiguous():
+            if t.shape != like.shape or t.dtype != dt:
+                raise ValueError("outputs and gradients must have q's and k's shape and dtype")
+            strides += _head_strides(t, layout)
+    rot, ps, axes, secs, pp, tp = 0, (0, 0, 0), 1, (0, 0, 0, 0), 0, 0
+    if table is not None:
+        rot = 2 * table.numel()
+        if table.dtype != _torch().int64 or not table.is_contiguous():
             raise ValueError("table must come from rope_table")
-        if positions is None or positions.dtype != torch.int32:
+        if positions is None or positions.dtype != _torch().int32:
             raise TypeError("positions must be an int32 tensor")
-        p = positions
-        if sections is not None:
-            secs = tuple(int(x) for x in sections)
-            axes = len(secs)
-            if not 1 <= axes <= 4:
-                raise ValueError("sections of 1 to 4 axes")
-            if p.dim() < 2 or p.shape[0] != axes:
-                raise ValueError("positions must be [axes, T] or [axes, B, T]")
-            secs = secs + (0,) * (4 - axes)
-            tail, ts, a0 = p.shape[1:], p.stride()[1:], p.stride(0)
+        pshape, ps = positions.shape, positions.stride()
+        if sections is None:
+            secs = (rot // 2, 0, 0, 0)
+            ps = (0, *ps)
         else:
-            tail, ts, a0 = p.shape, p.stride(), 0
-        if tuple(tail) == (T,):
-            ps = (a0, 0, ts[0])
-        elif tuple(tail) == (B, T):
-            ps = (a0, ts[0], ts[1])
-        else:
-            raise ValueError(f"positions {tuple(p.shape)} do not fit {B} x {T} tokens")
+            axes = len(sections)
+            if not 1 <= axes <= 4 or len(pshape) < 2 or pshape[0] != axes:
+                raise ValueError("positions with sections must be [axes, T] or [axes, B, T], 1 to 4 axes")
+            secs = (*sections, 0, 0, 0)[:4]
+            pshape = pshape[1:]
+        if len(pshape) == 1 and pshape[0] == T:
+            ps = (ps[0], 0, ps[1])
+        elif len(pshape) != 2 or pshape[0] != B or pshape[1] != T:
+            raise ValueError(f"positions {tuple(positions.shape)} do not fit {B} x {T} tokens")
+        pp, tp = positions.data_ptr(), table.data_ptr()
     pd = None
     for w in (q_weight, k_weight):
-        if w is None:
-            continue
-        if w.shape != (D,) or not w.is_contiguous() or (pd is not None and w.dtype != pd):
-            raise ValueError("weights must be contiguous [head size] vectors of one dtype")
-        pd = w.dtype
-    code = dtype_code(first.dtype)
-    return ((_ptr(positions) if rot else 0, _ptr(table) if rot else 0), (B, T, heads[0], heads[1], D, rot),
-            tuple([x for st in strides for x in st]) + tuple(ps) + secs
-            + (axes, 1 if interleaved else 0, code, dtype_code(pd) if pd is not None else code,
-               -1.0 if eps is None else _f32(eps), 0))
+        if w is not None:
+            if w.numel() != D or w.dim() != 1 or not w.is_contiguous() or (pd is not None and w.dtype != pd):
+                raise ValueError("weights must be contiguous [head size] vectors of one dtype")
+            pd = w.dtype
+    code = dtype_code(dt)
+    return (pp, tp), (B, T, Hq, Hkv, D, rot), (*strides, *ps, *secs, axes, 1 if interleaved else 0, code,
+                                               code if pd is None else dtype_code(pd),
+                                               -1.0 if eps is None else _f32(eps), 0)
 
 
 def qk_norm_rope(q, k, positions, table, *, q_weight=None, k_weight=None, eps=1e-6, sections=None, interleaved=False,
