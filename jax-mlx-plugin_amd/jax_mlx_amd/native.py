@@ -693,6 +693,13 @@ def _ptr(t):
     return t.data_ptr() if t is not None else 0
 
 
+def _fresh(t):
+    """A new contiguous tensor like t (None for None)."""
+    if t is None:
+        return None
+    return _torch().empty_like(t, memory_format=_torch().contiguous_format)
+
+
 def _workspace(a, query, workspace, like):
     """Sets a.workspace: the caller's, or one from torch's allocator for this
     call (also inside a captured graph, whose pool then owns it)."""
@@ -759,9 +766,8 @@ def sdpa_packed(q, k, v, seq_offsets, *, scale=None, causal=True, out=None, lse=
     (int32, on the device).  Rows in no sequence are not written (a fresh out
     holds anything there).  lse: optional f32 [Hq, T] output for
     sdpa_packed_bwd."""
-    torch = _torch()
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = _fresh(q)
     a = sdpa_packed_args(q, k, v, out, seq_offsets, scale=scale, causal=causal, lse=lse)
     with _on(q, k, v, out, seq_offsets, lse):
         check(load().mfx_sdpa_packed(ctypes.byref(a), _stream_handle(q)))
@@ -793,9 +799,7 @@ def sdpa_packed_bwd(q, k, v, dout, out, lse, seq_offsets, *, scale=None, causal=
     """(dq, dk, dv) of sdpa_packed for the gradient dout of its output, from
     its out and lse (mfx_sdpa_packed_bwd).  Rows in no sequence are not
     written."""
-    torch = _torch()
-    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) if g is None else g
-                  for t, g in ((q, dq), (k, dk), (v, dv)))
+    dq, dk, dv = (_fresh(t) if g is None else g for t, g in ((q, dq), (k, dk), (v, dv)))
     a = sdpa_packed_bwd_args(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, scale=scale, causal=causal)
     with _on(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, workspace):
         keep = _workspace(a, "mfx_sdpa_packed_bwd_workspace_size", workspace, q)  # noqa: F841 (until the launch)
@@ -847,59 +851,66 @@ def _head_strides(t, layout):
 _NO_ROWS = (0, 0, 0, 1)
 
 
+def _same(given, like):
+    """A caller's output or gradient (or None) against the tensor it belongs to."""
+    if (given is None) != (like is None):
+        raise ValueError("q and k each need their outputs (and gradients)")
+    if given is not None and (given.shape != like.shape or given.dtype != like.dtype):
+        raise ValueError("outputs and gradients must have q's and k's shape and dtype")
+    return given
+
+
 def _qk_fields(q, k, positions, table, q_weight, k_weight, eps, sections, interleaved, layout, more):
     """Checked (pointers of positions and table, dims, the rest) for the packed
-    structs; the rest starts with the strides of q, k and of the (q-shaped,
-    k-shaped) pairs in `more`."""
+    structs; the rest starts with the strides of q, k and of the tensors in
+    `more` (shaped like q and k in turn)."""
     first = q if q is not None else k
     if first is None:
         raise ValueError("q or k is needed")
-    shape, dt = first.shape, first.dtype
+    shape = first.shape
     if len(shape) == 3:
-        B, (T, H, D) = 1, shape
+        T, H, D = shape
+        B, at = 1, 1
     elif len(shape) != 4:
         raise ValueError("queries and keys are [T, H, D] or 4-D")
     elif layout == "bhtd":
         B, H, T, D = shape
+        at = 1
     elif layout == "bthd":
         B, T, H, D = shape
+        at = 2
     else:
         raise ValueError(f"layout must be 'bhtd' or 'bthd', got {layout!r}")
-    Hq, Hkv = (H, 0) if k is None else (0, H)
-    if q is not None and k is not None:
-        at = 1 if len(shape) == 3 or layout == "bhtd" else 2
+    code = dtype_code(first.dtype)
+    if q is None:
+        Hq, Hkv = 0, H
+    elif k is None:
+        Hq, Hkv = H, 0
+    else:
         ks = k.shape
-        if k.dtype != dt or len(ks) != len(shape) or ks[:at] != shape[:at] or ks[at + 1:] != shape[at + 1:]:
+        Hq, Hkv = H, ks[at] if len(ks) == len(shape) else 0
+        if k.dtype != first.dtype or (*shape[:at], Hkv, *shape[at + 1:]) != ks:
             raise ValueError("q and k must agree in dtype, batch, tokens and head size")
-        Hq, Hkv = H, ks[at]
     strides = ()
-    for a, b in ((q, k), *more):
-        for t, like in ((a, q), (b, k)):
-            if t is None or like is None:
-                if t is not like:
-                    raise ValueError("q and k each need their outputs (and gradients)")
-                strides += _NO_ROWS
-                continue
-            if t.shape != like.shape or t.dtype != dt:
-                raise ValueError("outputs and gradients must have q's and k's shape and dtype")
-            strides += _head_strides(t, layout)
-    rot, ps, axes, secs, pp, tp = 0, (0, 0, 0), 1, (0, 0, 0, 0), 0, 0
+    for t in (q, k, *more):
+        strides += _NO_ROWS if t is None else _head_strides(t, layout)
+    pp = tp = rot = 0
+    ps, axes, secs = (0, 0, 0), 1, (0, 0, 0, 0)
     if table is not None:
-        rot = 2 * table.numel()
-        if table.dtype != _torch().int64 or not table.is_contiguous():
+        torch = _torch()
+        rot = 2 * table.shape[0]
+        if table.dtype != torch.int64 or table.dim() != 1 or not table.is_contiguous():
             raise ValueError("table must come from rope_table")
-        if positions is None or positions.dtype != _torch().int32:
+        if positions is None or positions.dtype != torch.int32:
             raise TypeError("positions must be an int32 tensor")
         pshape, ps = positions.shape, positions.stride()
         if sections is None:
-            secs = (rot // 2, 0, 0, 0)
-            ps = (0, *ps)
+            secs, ps = (rot // 2, 0, 0, 0), (0, *ps)
         else:
             axes = len(sections)
             if not 1 <= axes <= 4 or len(pshape) < 2 or pshape[0] != axes:
                 raise ValueError("positions with sections must be [axes, T] or [axes, B, T], 1 to 4 axes")
-            secs = (*sections, 0, 0, 0)[:4]
-            pshape = pshape[1:]
+            secs, pshape = (*sections, 0, 0, 0)[:4], pshape[1:]
         if len(pshape) == 1 and pshape[0] == T:
             ps = (ps[0], 0, ps[1])
         elif len(pshape) != 2 or pshape[0] != B or pshape[1] != T:
@@ -908,10 +919,9 @@ def _qk_fields(q, k, positions, table, q_weight, k_weight, eps, sections, interl
     pd = None
     for w in (q_weight, k_weight):
         if w is not None:
-            if w.numel() != D or w.dim() != 1 or not w.is_contiguous() or (pd is not None and w.dtype != pd):
+            if w.shape != (D,) or not w.is_contiguous() or (pd is not None and w.dtype != pd):
                 raise ValueError("weights must be contiguous [head size] vectors of one dtype")
             pd = w.dtype
-    code = dtype_code(dt)
     return (pp, tp), (B, T, Hq, Hkv, D, rot), (*strides, *ps, *secs, axes, 1 if interleaved else 0, code,
                                                code if pd is None else dtype_code(pd),
                                                -1.0 if eps is None else _f32(eps), 0)
@@ -929,14 +939,11 @@ def qk_norm_rope(q, k, positions, table, *, q_weight=None, k_weight=None, eps=1e
     (None: no rotation, positions unused).  eps None: no norm.  interleaved:
     pairs side by side instead of half the rotated features apart.  The
     outputs are contiguous unless given (q_out may be q, k_out k)."""
-    torch = _torch()
     first = q if q is not None else k
-    if q is not None and q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if k is not None and k_out is None:
-        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    q_out = _fresh(q) if q_out is None else _same(q_out, q)
+    k_out = _fresh(k) if k_out is None else _same(k_out, k)
     ptrs, dims, rest = _qk_fields(q, k, positions, table, q_weight, k_weight, eps, sections, interleaved, layout,
-                                  ((q_out, k_out),))
+                                  (q_out, k_out))
     a = QkNormRopeArgs.from_buffer_copy(_QK_PACK(_ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), _ptr(q_weight),
                                                  _ptr(k_weight), *ptrs, *dims, *rest))
     with _on(first, q, k, q_out, k_out, q_weight, k_weight, positions, table):
@@ -951,12 +958,10 @@ def qk_norm_rope_bwd(q, k, dq_out, dk_out, positions, table, *, q_weight=None, k
     A weight's gradient has its dtype; None for an absent weight."""
     torch = _torch()
     first = q if q is not None else k
-    if q is not None and dq is None:
-        dq = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if k is not None and dk is None:
-        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+    dq = _fresh(q) if dq is None else _same(dq, q)
+    dk = _fresh(k) if dk is None else _same(dk, k)
     ptrs, dims, rest = _qk_fields(q, k, positions, table, q_weight, k_weight, eps, sections, interleaved, layout,
-                                  ((dq_out, dk_out), (dq, dk)))
+                                  (_same(dq_out, q), _same(dk_out, k), dq, dk))
     dqw = torch.empty_like(q_weight) if q_weight is not None else None
     dkw = torch.empty_like(k_weight) if k_weight is not None else None
     a = QkNormRopeBwdArgs.from_buffer_copy(_QK_BWD_PACK(
