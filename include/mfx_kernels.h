@@ -478,7 +478,10 @@ const char* mfx_sdpa_packed_kernel_name(const mfx_sdpa_packed_args* args);
  * Backward of mfx_sdpa_packed from the forward's out and lse: dq, dk, dv, dk
  * and dv of a kv head summed over its query heads.  Rows in no sequence are
  * left as they were.  dq, dk and dv must not share memory with the inputs or
- * each other.  Workspace: mfx_sdpa_packed_bwd_workspace_size() bytes, 256-byte
+ * each other.  In 16 bits P and dS meet the matrix cores rounded to `dtype`, as
+ * in mfx_sdpa_bwd: bf16 gradients are off by 0.0025 of their size (root mean
+ * square), of which their own rounding is 0.0017.
+ * Workspace: mfx_sdpa_packed_bwd_workspace_size() bytes, 256-byte
  * aligned, or NULL for library scratch.  Deterministic: no atomics.
  */
 typedef struct {
@@ -752,8 +755,7 @@ size_t mfx_linear_xent_workspace_size(const mfx_linear_xent_args* args);
  *   d = (exp(z - lse) - onehot(targets)) * dloss,   dh = d W,   dw = d^T h
  * dh [T, H] of `dtype`, dw [V, H] of `dw_dtype` (`dtype` or MFX_F32); either
  * may be NULL.  d is formed in pieces of the vocabulary (at most 512 MiB of it,
- * or 256 columns) and rounded to `dtype`, in f16 times a power of two that
- * fits the largest |dloss|.  Outputs must not share memory with the inputs.
+ * or 256 columns) and, over the largest |dloss|, rounded to `dtype`.  Outputs must not share memory with the inputs.
  * workspace: mfx_linear_xent_bwd_workspace_size() bytes, 256-byte aligned, or
  * NULL for library scratch.  Deterministic: no atomics.
  */

@@ -6,20 +6,25 @@
 //
 // h [T, H] and W [V, H] in bf16, f16 or f32; all sums and the softmax in fp32.
 //
-// Forward: the product kernel (xent_gemm16.h, xent_gemm32.h) over tiles of T x V whose
-// epilogue leaves each row's maximum and sum of exponentials over the tile's
+// Forward: the product kernel (xent_gemm16.h, xent_gemm32.h) over tiles of
+// T x V whose epilogue leaves each row's maximum and sum of exponentials over the tile's
 // columns, and the target's logit; xent_combine folds a row's tiles.  The
 // partials are 8 bytes per row and 256 columns.
 //
 // Backward, in pieces of the vocabulary: the piece's logits again, whose
 // epilogue turns them into d, rounded to the inputs' type, in a workspace of
-// T x piece (f32 for f32 inputs, nothing is rounded there); then dW of the piece = d^T h and dh (+)= d W of the piece.  A
-// piece is as wide as kPieceBytes of d allow, so that the fp32 dh is added to
+// T x piece (f32 for f32 inputs, nothing is rounded there); then dW of the
+// piece = d^T h and dh (+)= d W of the piece.  A piece is as wide as kPieceBytes of d allow, so that the fp32 dh is added to
 // in few rounds and its products are long.  Rounding d costs half a step of
 // each entry (independent from entry to entry), as rounding the gradient of
 // stored 16-bit logits would; the target's entry is rounded after the
-// subtraction.  f16 would lose small entries below 2^-24: d is held times a
-// power of two that takes the largest |dloss| to 2^15, removed at the end.
+// subtraction.  d is held over the largest |dloss|, c, which the sums are
+// multiplied by at the end: with the usual equal weights the target's entry is
+// p - 1 then, which for an unlikely target rounds to -1 almost exactly, where
+// (p - 1) dloss would carry dloss's own rounding into every row alike
+// (8192 x 4096 x 65537: dh and dW off by 0.0028 of their size with it, 0.0019
+// without, 0.0017 of which is their own rounding).  f16 holds it times 2^15
+// besides, or entries below 2^-24 would be lost.
 //
 // What bounds it: the matrix cores, 2 T H V flops a product, one product
 // forward and three backward.
@@ -69,8 +74,7 @@ struct LossArgs {
   float* picked;         // [T]: the target's logit
   // backward
   const float* lse;
-  const float* dloss;
-  const float* scale;    // f16: the power of two d is held times (null: 1)
+  const float* weight;   // dloss, in 16 bits over c (times 2^15)
   void* d;               // [T][ldd]
   int64_t ldd;
 };
@@ -82,7 +86,7 @@ struct StoreArgs {
   void* c;               // [M][ldc]
   int64_t ldc;
   int c_f32;             // c is fp32, else the inputs' type
-  const float* scale;    // divides c (null: 1)
+  const float* scale;    // multiplies c (null: 1)
 };
 
 __device__ __forceinline__ int64_t target_of(const void* t, int wide, int row) {
@@ -184,7 +188,6 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void xent_logits_kernel(LossArgs p
       p.part_l[(int64_t)tn * M + m0 + r] = l;
     }
   } else {
-    const float s = p.scale ? *p.scale : 1.f;
     // 16 bits: through LDS, whole rows of the wavefront's block at a time: 16-byte
     // chunk c of row r at slot c ^ (r % chunks).  d's rows are whole tiles
     // wide, so only rows need a check.
@@ -201,7 +204,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void xent_logits_kernel(LossArgs p
         const bool counts = t >= 0 && t < p.V;
         t = counts ? t - p.v0 : -1;
         const float lse2 = row < M ? p.lse[row] * kLog2e : 0.f;
-        const float w = counts ? p.dloss[row] * s : 0.f;
+        const float w = counts ? p.weight[row] : 0.f;
         auto prob = [&](float x) __attribute__((always_inline)) { return __builtin_amdgcn_exp2f(fmaf(x, kLog2e, -lse2)); };
         float z[FN * 16];
         block(i, edge_tag, z);
@@ -295,25 +298,27 @@ __global__ __launch_bounds__(64 * kCombine) void xent_combine(const float* __res
   loss[row] = t >= 0 && t < V ? z - picked[row] : 0.f;
 }
 
-// The power of two that takes the largest |dloss| of the rows that count to
-// at most 2^15.
-__global__ __launch_bounds__(1024) void xent_scale(const float* __restrict__ dloss, const void* targets, int target64,
-                                                   int T, int V, float* scale) {
+// weight[t] = dloss[t] / c * times for the rows that count, c their largest
+// |dloss| (1 if that is 0 or not finite); *scale = c / times.
+__global__ __launch_bounds__(1024) void xent_weights(const float* __restrict__ dloss, const void* targets,
+                                                     int target64, int T, int V, float times, float* weight,
+                                                     float* scale) {
   __shared__ float red[16];
   float m = 0.f;
   for (int i = threadIdx.x; i < T; i += 1024) {
+    const float g = fabsf(dloss[i]);
     const int64_t t = target_of(targets, target64, i);
-    if (t >= 0 && t < V) m = fmaxf(m, fabsf(dloss[i]));
+    if (t >= 0 && t < V) m = fmaxf(m, g);
   }
   m = group_max<64>(m);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x != 0) return;
+  m = red[0];
 #pragma unroll
   for (int i = 1; i < 16; ++i) m = fmaxf(m, red[i]);
-  int e = 0;
-  if (m > 0.f && m < INFINITY) e = (int)((__float_as_uint(m) >> 23) & 255) - 126;  // m < 2^e
-  *scale = __uint_as_float((uint32_t)(127 + min(max(15 - e, -100), 100)) << 23);
+  const float c = m > 0.f && m < INFINITY ? m : 1.f;
+  for (int i = threadIdx.x; i < T; i += 1024) weight[i] = dloss[i] / c * times;
+  if (threadIdx.x == 0) *scale = c / times;
 }
 
 // ---- the gradients' products -------------------------------------------------
@@ -337,7 +342,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void xent_grad_kernel(StoreArgs p)
   const int wm = wave % C::WM, wn = wave / C::WM;
   const int M = p.g.M, N = p.g.N;
   const int mw = m0 + wm * FM * 32, nw = n0 + wn * FN * 32;
-  const float mul = p.scale ? 1.f / *p.scale : 1.f;  // (a power of two)
+  const float mul = p.scale ? *p.scale : 1.f;
   if (C::E == 2 || p.part || p.c_f32) {
     float* const out = p.part ? p.part + (int64_t)sp * M * N : static_cast<float*>(p.c);
     const int64_t ld = p.part ? N : p.ldc;
@@ -390,7 +395,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void xent_grad_kernel(StoreArgs p)
   }
 }
 
-// c = the fp32 sums of the ranges, added in order, over the scale.
+// c = the fp32 sums of the ranges, added in order, times c.
 template <typename T>
 __global__ __launch_bounds__(256) void xent_sum(const float* __restrict__ part, int splits, int64_t M, int N, T* c,
                                                 int64_t ldc, const float* scale) {
@@ -399,7 +404,7 @@ __global__ __launch_bounds__(256) void xent_sum(const float* __restrict__ part, 
   const int64_t e = q * 4, m = e / N, n = e % N;
   f32x4 v = *reinterpret_cast<const f32x4*>(part + e);
   for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(part + s * M * N + e);
-  const float mul = scale ? 1.f / *scale : 1.f;
+  const float mul = scale ? *scale : 1.f;
   typedef T t4 __attribute__((ext_vector_type(4)));
   t4 o;
 #pragma unroll
@@ -482,7 +487,7 @@ struct BwdPlan {
   int E;
   int64_t piece, pieces;
   Way dh, dw;  // of the first piece, the widest
-  size_t d_bytes, dh_bytes, dw_bytes, total;
+  size_t row_bytes, d_bytes, dh_bytes, dw_bytes, total;
 };
 
 int elem_of(int dtype) { return dtype == MFX_F32 ? 2 : dtype == MFX_F16 ? 1 : 0; }
@@ -506,7 +511,8 @@ BwdPlan plan_bwd(const mfx_linear_xent_bwd_args& a) {
     pl.dw = choose(pl.E, nv, a.H, a.T, true);
     if (pl.dw.ranges > 1) pl.dw_bytes = align256((size_t)pl.dw.ranges * nv * a.H * 4);
   }
-  pl.total = 256 + pl.d_bytes + pl.dh_bytes + pl.dw_bytes;
+  if (pl.E != 2) pl.row_bytes = 256 + align256((size_t)a.T * 4);
+  pl.total = pl.row_bytes + pl.d_bytes + pl.dh_bytes + pl.dw_bytes;
   return pl;
 }
 
@@ -552,15 +558,17 @@ int launch_sum(const float* part, int64_t splits, int64_t M, int64_t N, void* c,
 
 template <int E>
 int run_bwd(const mfx_linear_xent_bwd_args& a, const BwdPlan& pl, char* ws, hipStream_t s) {
-  float* const scale = E == 1 ? reinterpret_cast<float*>(ws) : nullptr;
-  char* const d = ws + 256;
+  float* const scale = E != 2 ? reinterpret_cast<float*>(ws) : nullptr;
+  float* const weight = E != 2 ? reinterpret_cast<float*>(ws + 256) : nullptr;
+  char* const d = ws + pl.row_bytes;
   float* const dh_part = reinterpret_cast<float*>(d + pl.d_bytes);
   float* const dw_part = reinterpret_cast<float*>(d + pl.d_bytes + pl.dh_bytes);
   const Operand h{a.h, a.h_stride}, dl{d, pl.piece};
   const int t64 = a.target_dtype == MFX_I64, size = dtype_size(a.dtype);
-  if (E == 1) {
-    hipLaunchKernelGGL(xent_scale, dim3(1), dim3(1024), 0, s, a.dloss, a.targets, t64, (int)a.T, (int)a.V, scale);
-    if (int rc = launch_status("xent_scale")) return rc;
+  if (E != 2) {
+    hipLaunchKernelGGL(xent_weights, dim3(1), dim3(1024), 0, s, a.dloss, a.targets, t64, (int)a.T, (int)a.V,
+                       E == 1 ? 32768.f : 1.f, weight, scale);
+    if (int rc = launch_status("xent_weights")) return rc;
   }
   for (int64_t i = 0; i < pl.pieces; ++i) {
     const int64_t v0 = i * pl.piece, nv = std::min(pl.piece, a.V - v0);
@@ -573,8 +581,7 @@ int run_bwd(const mfx_linear_xent_bwd_args& a, const BwdPlan& pl, char* ws, hipS
     z.v0 = v0;
     z.V = (int)a.V;
     z.lse = a.lse;
-    z.dloss = a.dloss;
-    z.scale = scale;
+    z.weight = weight ? weight : a.dloss;
     z.d = d;
     z.ldd = pl.piece;
     if (int rc = launch_logits<E, true>(z, zw.form, s)) return rc;
