@@ -416,7 +416,8 @@ __global__ __launch_bounds__(256) void xent_sum(const float* __restrict__ part, 
 
 namespace {
 
-constexpr size_t kPieceBytes = 512u << 20;  // of d at a time
+constexpr size_t kPieceBytes = 512u << 20;      // of d at a time
+constexpr int64_t kMaxStride = int64_t(1) << 21;  // a tile's 256 rows are addressed within 31 bits
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -497,7 +498,8 @@ BwdPlan plan_bwd(const mfx_linear_xent_bwd_args& a) {
   pl.E = elem_of(a.dtype);
   const int size = dtype_size(a.dtype);
   const int64_t vp = ceil_div(a.V, 256) * 256;
-  const int64_t most = std::max<int64_t>(256, (int64_t)(kPieceBytes / size) / a.T / 256 * 256);
+  int64_t most = std::max<int64_t>(256, (int64_t)(kPieceBytes / size) / a.T / 256 * 256);
+  most = std::min(most, kMaxStride);
   pl.pieces = ceil_div(vp, most);
   pl.piece = ceil_div(ceil_div(vp, pl.pieces), 256) * 256;
   pl.pieces = ceil_div(vp, pl.piece);
@@ -654,8 +656,7 @@ int check_matrix(const void* ptr, int64_t stride, int64_t H, int size, const cha
   if (stride < H) return fail(MFX_E_INVALID, std::string(what) + ": row stride must be >= H");
   if ((uintptr_t)ptr % 16 || stride % (16 / size))
     return fail(MFX_E_UNSUPPORTED, std::string(what) + ": rows must be 16-byte aligned");
-  // (A tile's 256 rows are addressed within 31 bits.)
-  if (stride >= (int64_t(1) << 21)) return fail(MFX_E_UNSUPPORTED, std::string(what) + ": row stride too large");
+  if (stride >= kMaxStride) return fail(MFX_E_UNSUPPORTED, std::string(what) + ": row stride too large");
   return MFX_OK;
 }
 

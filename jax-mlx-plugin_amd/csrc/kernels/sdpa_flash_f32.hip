@@ -312,7 +312,7 @@ __device__ __forceinline__ void ldn(__amdgpu_buffer_rsrc_t r, int off, float (&v
   }
 }
 
-template <int D, bool CAUSAL, bool MASK>
+template <int D, bool CAUSAL, bool MASK, bool PACKED = false>
 __global__ __launch_bounds__(64 * kSW) void flash_f32_split_kernel(SdpaParams p) {
   __shared__ float red_m[kSW][32], red_l[kSW][32];
   // [split][query][feature]; a 4-float pad keeps the 16-byte rows of one
@@ -327,7 +327,15 @@ __global__ __launch_bounds__(64 * kSW) void flash_f32_split_kernel(SdpaParams p)
   const int l32 = lane & 31;
 
   const int nmb = (p.Tq + 31) / 32;
-  const int bh = blockIdx.x / nmb, mblk = blockIdx.x % nmb;
+  int bh = blockIdx.x / nmb, mblk = blockIdx.x % nmb;
+  if constexpr (PACKED) {
+    int slot;
+    PackedBlock pb;
+    packed_head(blockIdx.x, p.Hq, gridDim.x / p.Hq, bh, slot);
+    if (!packed_block<32>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
+    mblk = pb.work;
+    packed_shift<4>(p, pb.start, pb.len);
+  }
   const int b = bh / p.Hq, h = bh % p.Hq, hk = h / p.group;
   const float* qp = static_cast<const float*>(p.q) + b * p.qs[0] + h * p.qs[1];
   const float* kp = static_cast<const float*>(p.k) + b * p.ks[0] + hk * p.ks[1];
@@ -493,7 +501,7 @@ __global__ __launch_bounds__(64 * kSW) void flash_f32_split_kernel(SdpaParams p)
       *reinterpret_cast<f32x4*>(&o_part[wave][l32][(g * 8 + half * 4) * NDT + j * 4]) =
           f32x4{run[j * 4], run[j * 4 + 1], run[j * 4 + 2], run[j * 4 + 3]};
   }
-  if (p.lse && wave == 0 && half == 0 && qi < Tq) p.lse[(int64_t)bh * Tq + qi] = M + __log2f(L);
+  if (p.lse && wave == 0 && half == 0 && qi < Tq) p.lse[(int64_t)bh * row_pitch<PACKED>(p) + qi] = M + __log2f(L);
   __syncthreads();
   constexpr int C4 = D / 4;  // float4 columns per row
 #pragma unroll
@@ -530,8 +538,29 @@ int launch_t(const SdpaParams& p, hipStream_t s) {
   return launch_status("flash_f32_kernel");
 }
 
+// Packed, the key-split variant where the 128-row workgroups number fewer than
+// two per CU, as above; a wavefront's tiles are known for the mean sequence
+// only.  (Six sequences of 1 to 128 tokens, 8 heads of 64: 16 us on the
+// 128-row kernel, 9 on this.)
+bool packed_use_split(const SdpaParams& p) {
+  for (int64_t st : {p.qs[2], p.ks[2], p.vs[2]})
+    if (st < p.D || st >= (int64_t(1) << 24)) return false;
+  return packed_slots(p.total, p.num_seqs, kBM) * p.Hq < 2LL * device_cu_count() &&
+         p.total <= (int64_t)p.num_seqs * 32 * 4 * 8;
+}
+
 template <int D>
 int launch_packed(const SdpaParams& p, hipStream_t s) {
+  if constexpr (D <= 128) {
+    if (packed_use_split(p)) {
+      const dim3 grid((unsigned)(packed_slots(p.total, p.num_seqs, 32) * p.Hq));
+      if (p.causal)
+        hipLaunchKernelGGL((flash_f32_split_kernel<D, true, false, true>), grid, dim3(64 * kSW), 0, s, p);
+      else
+        hipLaunchKernelGGL((flash_f32_split_kernel<D, false, false, true>), grid, dim3(64 * kSW), 0, s, p);
+      return launch_status("flash_f32_split_kernel (packed)");
+    }
+  }
   const dim3 grid((unsigned)(packed_slots(p.total, p.num_seqs, kBM) * p.Hq));
   if (p.causal) hipLaunchKernelGGL((flash_f32_kernel<D, true, false, true>), grid, dim3(kNT), 0, s, p);
   else hipLaunchKernelGGL((flash_f32_kernel<D, false, false, true>), grid, dim3(kNT), 0, s, p);

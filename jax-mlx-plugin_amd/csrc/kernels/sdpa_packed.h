@@ -3,7 +3,8 @@
 // A packed batch is T tokens, sequence s of them from off[s] up to off[s + 1],
 // the offsets in device memory.  The host knows neither the lengths nor the
 // number of row blocks, only a bound: a sequence of n rows is at most
-// n / BM + 1 blocks, so T / BM + min(sequences, T) slots per head cover all.
+// n / BM + 1 blocks, so T / BM slots per head and one for each sequence that
+// can hold a token cover all.
 // Each workgroup finds its own (sequence, block) from its slot number, with
 // no launch before it, and slots without a block leave at once.
 //
@@ -19,7 +20,7 @@
 // cycles), some 8 steps.  Past kLaneSeqs sequences a lane's share no longer
 // fits registers, and slots go to sequences in order: sequence s owns the slots
 // from (off[s] - off[0]) / BM + s, which are enough for it and need no count
-// of the blocks before.
+// of the blocks before (empty sequences own one too).
 //
 // Offsets are taken as they come: each is clamped to 0 .. T and a sequence that
 // would end before it starts is empty, so no offsets lead outside the tensors.
@@ -53,6 +54,13 @@ __device__ __forceinline__ int wave_sum(int v) {
 __device__ __forceinline__ void packed_bounds(const int32_t* off, int total, int s, int& start, int& len) {
   start = min(max(off[s], 0), total);
   len = max(min(off[s + 1], total) - start, 0);
+}
+
+// First slot of sequence s, which starts at `at`, when slots go in order.
+template <int BM>
+__device__ __forceinline__ int64_t packed_slot(int at, int first, int s) {
+  const int64_t d = (int64_t)at - first;
+  return (d > 0 ? d : 0) / BM + s;
 }
 
 // Slot `r`'s block of BM rows; false: it has none.  Uniform over the
@@ -111,14 +119,14 @@ __device__ __forceinline__ bool packed_block(const int32_t* off, int n, int tota
     int lo = 0, hi = n;
     while (hi - lo > 1) {
       const int step = (hi - lo + 63) / 64, s = lo + lane * step;
-      const bool at = s < hi && (int64_t)max(off[min(s, n)] - first, 0) / BM + s <= r;
+      const bool at = s < hi && packed_slot<BM>(off[min(s, n)], first, s) <= r;
       const int cnt = max(__popcll(__ballot(at)), 1);
       lo += (cnt - 1) * step;
       hi = min(hi, lo + step);
     }
     seq = __builtin_amdgcn_readfirstlane(lo);
     packed_bounds(off, total, seq, out.start, out.len);
-    const int64_t b = r - ((int64_t)max(off[seq] - first, 0) / BM + seq);
+    const int64_t b = r - packed_slot<BM>(off[seq], first, seq);
     out.nb = (out.len + BM - 1) / BM;
     if (b < 0 || b >= out.nb) return false;
     work = out.nb - 1 - (int)b;
@@ -142,8 +150,11 @@ __device__ __forceinline__ bool packed_seq(const int32_t* off, int n, int total,
   return t >= start && t < start + len;
 }
 
-// Slots per head of a packed call (host): blocks of BM rows at most.
-inline int64_t packed_slots(int64_t total, int64_t n, int BM) { return total / BM + (n < total ? n : total); }
+// Slots per head of a packed call (host): blocks of BM rows at most, and past
+// 64 kLaneSeqs sequences a slot for every empty one too.
+inline int64_t packed_slots(int64_t total, int64_t n, int BM) {
+  return total / BM + (n <= 64 * kLaneSeqs && total < n ? total : n);
+}
 
 // (head, slot) of a workgroup.  Workgroups are dealt to the 8 XCDs in turn;
 // with heads divisible by 8 each XCD takes a run of neighbouring heads, which

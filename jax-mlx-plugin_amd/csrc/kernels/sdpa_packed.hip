@@ -26,7 +26,7 @@ int check_common(const Args* a) {
   if (a->Hq % a->Hkv != 0) return fail(MFX_E_INVALID, "Hq must be a multiple of Hkv");
   const int64_t lim = 0x7fffffffLL;
   if (a->T > lim || a->num_seqs >= lim || a->Hq > 65535 ||
-      (a->T / 32 + (a->num_seqs < a->T ? a->num_seqs : a->T) + 1) * a->Hq > lim || a->T * a->Hq > lim)
+      packed_slots(a->T, a->num_seqs, 32) * a->Hq > lim || a->T * a->Hq > lim)
     return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
   if (a->dtype != MFX_F32 && a->dtype != MFX_BF16 && a->dtype != MFX_F16)
     return fail(MFX_E_UNSUPPORTED, "dtype must be f32, bf16 or f16");

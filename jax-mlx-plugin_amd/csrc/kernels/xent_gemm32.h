@@ -4,13 +4,16 @@
 // where those are too few.
 //
 // A 32x32x2 product takes 64 cycles, so the 16 (4) products per 8 k and
-// wavefront leave 1024 (256) cycles for 4 to 16 (2 to 8) LDS reads: plain double buffering
-// (global -> registers -> LDS, one barrier a tile) keeps the matrix cores fed.
+// wavefront leave 1024 (256) cycles for 4 to 16 (2 to 8) LDS reads: plain double
+// buffering (global -> registers -> LDS, one barrier a tile), with two tiles in
+// registers, keeps the matrix cores fed.
 // The k of products are permuted alike in both operands: step e of 8 k takes k =
 // half * 4 + e, so a k-contiguous row gives four steps in one 16-byte read.
 // Rows padded by 16 bytes (k-contiguous) or 32 (index-contiguous, whose two
 // halves read rows 4 apart) keep the reads off each other's banks.
 #pragma once
+
+#include <type_traits>
 
 #include "xent_tiles.h"
 
@@ -26,26 +29,26 @@ struct Tile32 {
   const float* p;
   int64_t ld;
   int idx0, total, K;
-  f32x4 r[CH];
+  f32x4 r[2][CH];  // two tiles on their way
   __device__ __forceinline__ Tile32(const Operand& o, int i0, int n, int k)
       : p(static_cast<const float*>(o.p)), ld(o.ld), idx0(i0), total(n), K(k) {}
   // (K and an index-contiguous operand's rows are whole chunks, K % 4 == 0 and
   // total % 4 == 0 or the row padded to it: checked on the host.)
-  __device__ __forceinline__ void load(int kt) {
+  __device__ __forceinline__ void load(int kt, int set) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = threadIdx.x + i * NT, row = c / CPR, col = c % CPR * 4;
       const int idx = idx0 + (KC ? row : col), k = kt * kBK32 + (KC ? col : row);
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
       if (idx < total && k < K) v = *reinterpret_cast<const f32x4*>(p + (KC ? idx * ld + k : k * ld + idx));
-      r[i] = v;
+      r[set][i] = v;
     }
   }
-  __device__ __forceinline__ void store(float* lds) const {
+  __device__ __forceinline__ void store(float* lds, int set) const {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = threadIdx.x + i * NT, row = c / CPR, col = c % CPR * 4;
-      *reinterpret_cast<f32x4*>(lds + row * ROW + col) = r[i];
+      *reinterpret_cast<f32x4*>(lds + row * ROW + col) = r[set][i];
     }
   }
 };
@@ -74,19 +77,23 @@ __device__ __forceinline__ void gemm_tile32(const GemmShape& g, int m0, int n0, 
     for (int i = 0; i < C::FM; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
-  ta.load(kt0);
-  tb.load(kt0);
-  ta.store(smem);
-  tb.store(smem + HALF);
+  // Tile kt multiplies from its LDS stage while kt + 1 is in registers (stored
+  // at the end) and kt + 2 on its way: a tile's products alone (1024 cycles at
+  // 64 x 64) do not cover a load.
+  ta.load(kt0, 0);
+  tb.load(kt0, 0);
+  ta.load(kt0 + 1, 1);  // (past K: zeros)
+  tb.load(kt0 + 1, 1);
+  ta.store(smem, 0);
+  tb.store(smem + HALF, 0);
   __syncthreads();
-  for (int kt = kt0; kt < kt1; ++kt) {
-    const float* at = smem + ((kt - kt0) & 1) * 2 * HALF;
+  auto tile = [&](int kt, auto set_tag) __attribute__((always_inline)) {
+    constexpr int S = decltype(set_tag)::value;  // kt's stage and, for kt + 2, register set
+    const float* at = smem + S * 2 * HALF;
     const float* bt = at + HALF;
-    float* const next = smem + ((kt - kt0 + 1) & 1) * 2 * HALF;
-    if (kt + 1 < kt1) {
-      ta.load(kt + 1);
-      tb.load(kt + 1);
-    }
+    float* const next = smem + (S ^ 1) * 2 * HALF;
+    ta.load(kt + 2, S);
+    tb.load(kt + 2, S);
 #pragma unroll
     for (int c = 0; c < kBK32 / 8; ++c) {
       f32x4 fa[C::FM], fb[C::FN];
@@ -102,12 +109,16 @@ __device__ __forceinline__ void gemm_tile32(const GemmShape& g, int m0, int n0, 
           for (int i = 0; i < C::FM; ++i)
             acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j][e], fa[i][e], acc[j][i], 0, 0, 0);
     }
-    if (kt + 1 < kt1) {
-      ta.store(next);
-      tb.store(next + HALF);
-    }
+    ta.store(next, S ^ 1);
+    tb.store(next + HALF, S ^ 1);
     __syncthreads();
+  };
+  int kt = kt0;
+  for (; kt + 1 < kt1; kt += 2) {
+    tile(kt, std::integral_constant<int, 0>{});
+    tile(kt + 1, std::integral_constant<int, 1>{});
   }
+  if (kt < kt1) tile(kt, std::integral_constant<int, 0>{});
 }
 
 }  // namespace xent

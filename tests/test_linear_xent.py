@@ -122,6 +122,12 @@ def test_several_pieces(cuda, nat):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+def test_more_classes_than_a_piece_has_columns(cuda, nat, name):
+    check_all(cuda, nat, name, *make(cuda, name, 3, 8, (1 << 21) + 1001, seed=11))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
 def test_int32_targets_strides_and_parts(cuda, nat, name):
     torch = cuda

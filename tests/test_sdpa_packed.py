@@ -149,6 +149,17 @@ def test_many_sequences(cuda, nat):
 
 
 @pytest.mark.gpu
+def test_more_sequences_than_tokens(cuda, nat):
+    """Empty sequences beside a few tokens, under and over 512 of them."""
+    for n, at in ((400, (0, 200, 399)), (1500, (3, 700, 1499))):
+        lens = [0] * n
+        for i, s in enumerate(at):
+            lens[s] = (1, 40, 150)[i]
+        for name in ("bf16", "f32"):
+            check_all(cuda, nat, name, lens, 2, 1, 64, tail=2, seed=n)
+
+
+@pytest.mark.gpu
 def test_longer_sequences(cuda, nat):
     check_all(cuda, nat, "bf16", [1500, 20, 700], 8, 2, 128)
 
