@@ -482,7 +482,9 @@ const char* mfx_sdpa_packed_kernel_name(const mfx_sdpa_packed_args* args);
  * in mfx_sdpa_bwd: bf16 gradients are off by 0.0025 of their size (root mean
  * square), of which their own rounding is 0.0017.
  * Workspace: mfx_sdpa_packed_bwd_workspace_size() bytes, 256-byte
- * aligned, or NULL for library scratch.  Deterministic: no atomics.
+ * aligned, or NULL for library scratch.  Deterministic.  (Under a causal mask
+ * the sums of a long sequence's first keys may be split, by T, num_seqs and the
+ * offsets: their last bits depend on what the sequence is packed with.)
  */
 typedef struct {
   const void* q;

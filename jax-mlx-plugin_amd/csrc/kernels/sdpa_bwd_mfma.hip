@@ -2,7 +2,8 @@
 // 64 or 128 (D == Dv), fp32 accumulation, v_mfma_f32_32x32x16_bf16 (f16: the
 // _f16 form) throughout.
 //
-// Two kernels, each owning its outputs (deterministic, no atomics):
+// Two kernels, each owning its outputs (deterministic; atomics only count the
+// shares of a packed batch's longest key blocks, which are added in order):
 //
 // dkdv: workgroup = 4 wavefronts = 128 keys of one (batch, kv head); each
 //   wavefront owns 32 keys.  Its K and V rows stay in registers as the B
@@ -148,7 +149,18 @@ __device__ __forceinline__ void load_frags(const bf16* base, int64_t stride, int
 // and the wavefront with the most visible blocks sets the pace anyway.
 constexpr int kKvPf = 2;   // operand reads issued ahead of their MFMAs
 constexpr int kKvStages = 3;
+constexpr int kPartTiles = 8;  // packed: a share of a key block's tiles is at least so many
 constexpr int kDkdvHeadGroup = 2;  // kv heads whose key blocks an XCD runs together
+
+// Four f32, written through to where every XCD sees them and read from there
+// (cache policy bit 4, sc1: past this XCD's L2).
+constexpr int kThrough = 1 << 4;
+__device__ __forceinline__ void put_sums(__amdgpu_buffer_rsrc_t to, int at, f32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), to, at, 0, kThrough);
+}
+__device__ __forceinline__ f32x4 get_sums(__amdgpu_buffer_rsrc_t from, int at) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, kThrough));
+}
 
 // PACKED: one sequence of a packed batch (sdpa_packed.h).
 template <int D, bool CAUSAL, int MASKT, int E, bool PACKED = false>
@@ -203,10 +215,20 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
   const int nkb = (p.Tk + kRows - 1) / kRows;
   const int id = blockIdx.x;
   int bhk, kblk;
+  int nparts = 1, part = 0, share = 0, block = 0;  // packed: shares of the key block's tiles (see packed_share)
   if constexpr (PACKED) {
     int slot;
     PackedBlock pb;
     packed_head(id, BHk, gridDim.x / BHk, bhk, slot);
+    if (CAUSAL && p.parts > 1) {
+      const PackedShare ps = packed_share<kRows>(p, 2 * p.group, kPartTiles, slot);
+      if (ps.parts > 1 && slot >= p.part_shares) return;  // (offsets that overlap: the workspace ends here)
+      share = slot * BHk + bhk;
+      block = ps.block * BHk + bhk;
+      slot = ps.block;
+      part = ps.part;
+      nparts = ps.parts;
+    }
     if (!packed_block<kRows>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
     kblk = pb.nb - 1 - pb.work;
     packed_shift<2>(p, pb.start, pb.len);
@@ -245,7 +267,11 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
   const int qt0 = CAUSAL ? (kblk * kRows) / kTile : 0;
   const int nqt = (Tq + kTile - 1) / kTile;
   const int per_head = nqt > qt0 ? nqt - qt0 : 0;
-  const int ntiles = G * per_head;
+  int ntiles = G * per_head, t_first = 0;
+  if constexpr (PACKED) {
+    t_first = ntiles * part / nparts;
+    ntiles = ntiles * (part + 1) / nparts - t_first;
+  }
 
   // Resource extents end with the last element of the group's last row, so
   // rows past Tq read zeros or (inside the span) rows of the next head,
@@ -255,8 +281,8 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
   // other sequences hold, or nobody has written, never meets the products.)
   qload.nbytes = (int)(((PACKED ? 0 : (int64_t)(G - 1) * p.qs[1]) + (int64_t)(Tq - 1) * p.qs[2] + D) * 2);
   gload.nbytes = (int)(((PACKED ? 0 : (int64_t)(G - 1) * p.dos[1]) + (int64_t)(Tq - 1) * p.dos[2] + D) * 2);
-  auto tile_head = [&](int t) { return t / per_head; };
-  auto tile_q = [&](int t) { return qt0 + t % per_head; };
+  auto tile_head = [&](int t) { return (t_first + t) / per_head; };
+  auto tile_q = [&](int t) { return qt0 + (t_first + t) % per_head; };
   auto issue = [&](int t, int st) {
     const int g = tile_head(t), qt = tile_q(t);
     if constexpr (PACKED) {
@@ -540,6 +566,62 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
   }
 
   PHASE(ph_fence(); ph_set(kPhCEpi, ph_now()); ph_fence();)
+  if constexpr (PACKED) {
+    if (nparts > 1) {
+      // Each share's sums go to the workspace as they lie in registers; the
+      // workgroup that counts itself last adds them in the shares' order, so
+      // the result does not depend on which one that is.  (Of two shares the
+      // order does not matter, and the last one's stay where they are.)  The
+      // sums go past the L2s, so no fence has to write one back: with fences
+      // the join of a batch's shares took longer than it saved.
+      const bool pair = nparts == 2;
+      __shared__ int others;
+      constexpr int kShare = kRows * D * 8;  // bytes: dK and dV of a key block
+      char* const own = reinterpret_cast<char*>(p.part_sums) + (int64_t)share * kShare;
+      const int at = wave * (kShare / 4) + lane * 16;
+      int* const count = p.part_count + block;
+      if (tid == 0) others = __hip_atomic_load(count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      if (!pair || others != 1) {
+        const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(own, 0, kShare, 0x00020000);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f32x4 a, c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = dk[dt][i * 4 + e], c[e] = dv[dt][i * 4 + e];
+            put_sums(to, at + (dt * 4 + i) * 2048, a);
+            put_sums(to, at + (dt * 4 + i) * 2048 + 1024, c);
+          }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) others = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (others != nparts - 1) return;
+      }
+      if (!pair) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dk[dt][i] = dv[dt][i] = 0.f;
+      }
+      for (int n = 0; n < nparts; ++n) {
+        if (pair && n == part) continue;
+        const __amdgpu_buffer_rsrc_t from =
+            __builtin_amdgcn_make_buffer_rsrc(own + (int64_t)(n - part) * BHk * kShare, 0, kShare, 0x00020000);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x4 a = get_sums(from, at + (dt * 4 + i) * 2048);
+            const f32x4 c = get_sums(from, at + (dt * 4 + i) * 2048 + 1024);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dk[dt][i * 4 + e] += a[e], dv[dt][i * 4 + e] += c[e];
+          }
+      }
+    }
+  }
   // Every wavefront's last Y has read its Q / dO stage: the stages take the
   // dK and dV rows on their way out.  (The first key comes from an opaque
   // copy here, so no address is hoisted into the loop.)
@@ -623,6 +705,8 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
   if constexpr (PACKED) {
     int slot;
     PackedBlock pb;
+    // (No share of a key block has been counted yet.)
+    if (id * kNT + tid < p.part_shares * p.Hkv) p.part_count[id * kNT + tid] = 0;
     packed_head(id, BH, gridDim.x / BH, bh, slot);
     if (!packed_block<kRows>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
     mblk = pb.work;
@@ -881,7 +965,8 @@ int launch_t(const SdpaBwdParams& p, hipStream_t s) {
   const int64_t slots = packed_slots(p.total, p.num_seqs, kRows);
   hipLaunchKernelGGL((bwd_dq_mfma<D, CAUSAL, 0, E, true>), dim3((unsigned)(slots * p.Hq)), dim3(kNT), 0, s, p);
   if (int rc = launch_status("bwd_dq_mfma (packed)")) return rc;
-  hipLaunchKernelGGL((bwd_dkdv_mfma<D, CAUSAL, 0, E, true>), dim3((unsigned)(slots * p.Hkv)), dim3(kNT), 0, s, p);
+  const unsigned shares = (unsigned)((slots + p.part_extra) * p.Hkv);
+  hipLaunchKernelGGL((bwd_dkdv_mfma<D, CAUSAL, 0, E, true>), dim3(shares), dim3(kNT), 0, s, p);
   return launch_status("bwd_dkdv_mfma (packed)");
 }
 

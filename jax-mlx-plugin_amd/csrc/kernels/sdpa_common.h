@@ -69,6 +69,12 @@ struct SdpaBwdParams {
   const int32_t* seq_off;  // packed sequences, as in SdpaParams
   int num_seqs;
   int total;
+  // Packed, matrix cores: dK / dV of a key block in up to `parts` shares
+  // (packed_share): at most part_shares of one head belong to blocks of more
+  // than one, and at most part_extra workgroups a head come of it.
+  int parts, part_quarters, part_shares, part_extra;
+  float* part_sums;
+  int* part_count;
 };
 
 bool bwd_mfma_supports(const SdpaBwdParams& p);

@@ -2,6 +2,7 @@
 // selection for attention over packed sequences.  The kernels are the packed
 // instances of those of mfx_sdpa_fwd and mfx_sdpa_bwd (sdpa_packed.h): a
 // workgroup finds its sequence on the device and then runs the same tiles.
+#include <algorithm>
 #include <cmath>
 
 #include "sdpa_packed.h"
@@ -10,6 +11,10 @@ namespace mfx {
 namespace {
 
 enum class Kind { kNone, kFlash16, kFlashF32, kMfma16, kMfmaF32, kPadded16, kGeneric };
+
+// dK / dV on the matrix cores: up to kPartBlocks key blocks (four a CU) some
+// are shared, at most kMaxParts ways (packed_share).
+constexpr int kPartBlocks = 4 * kCus, kMaxParts = 8;
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -80,6 +85,7 @@ struct BwdPlan {
   SdpaBwdParams p{};
   Kind kind = Kind::kNone;
   size_t row_bytes = 0;            // delta
+  size_t count_bytes = 0, sum_bytes = 0;  // key blocks in shares: their counts and sums
   int dp = 0;                      // kPadded16: features of the padded copies
   size_t q_pad = 0, kv_pad = 0;    // bytes of one
 };
@@ -153,11 +159,40 @@ int plan_bwd(const mfx_sdpa_packed_bwd_args* a, BwdPlan& pl) {
       pl.kv_pad = align256((size_t)p.Hkv * p.total * dp * 2);
     }
   }
+  if (pl.kind == Kind::kMfma16 || pl.kind == Kind::kPadded16) {
+    const int64_t slots = packed_slots(p.total, p.num_seqs, kBwdKeyBlock), blocks = slots * p.Hkv;
+    // A key block walks all queries behind it for every head of its group, and
+    // the longest ones alone can last longer than a CU's part of the whole
+    // (backward of one sequence of 4096 tokens, 32 heads on 8: 730 us with whole
+    // blocks, 602 with shares of at most three quarters of that part, 646 of
+    // one; 512 tokens: 100 and 59; 3000 tokens in 2, 8 heads on 1: 580 and 144).
+    // With more than two blocks a CU smaller ones fill the gaps and joining
+    // shares costs more (8192 tokens in 1: 1990 whole, 2055 in three quarters;
+    // in 8 of 96 .. 2500: 622, 614, and 607 in shares of one part).
+    p.parts = 1;
+    if (p.causal && blocks <= kPartBlocks && p.num_seqs <= 64 * kLaneSeqs)
+      p.parts = (int)std::min<int64_t>(kMaxParts, kPartBlocks / blocks + 1);
+    if (p.parts > 1) {
+      p.part_quarters = blocks <= 2 * kCus ? 3 : 4;
+      // A block in k shares walks more than (k - 1) `most`, and all of a head
+      // no more than `all`: so many blocks are shared at most, and so many
+      // shares added.  (Of offsets that are no offsets there may be more
+      // blocks than slots, but no workgroups behind slots + part_extra.)
+      const int64_t all = kCus * 4 / p.part_quarters / p.Hkv + 1;
+      p.part_extra = (int)std::min(slots * (p.parts - 1), all);
+      p.part_shares = (int)std::min(slots, all) + p.part_extra;
+      const int64_t n = (int64_t)p.part_shares * p.Hkv;
+      pl.count_bytes = align256(n * sizeof(int));
+      pl.sum_bytes = (size_t)n * 2 * kBwdKeyBlock * (pl.dp ? pl.dp : p.D) * sizeof(float);
+    }
+  }
   return MFX_OK;
 }
 
 size_t bwd_bytes(const BwdPlan& pl) {
-  return pl.kind == Kind::kNone ? 0 : pl.row_bytes + (pl.dp ? 4 * pl.q_pad + 4 * pl.kv_pad : 0);
+  return pl.kind == Kind::kNone
+             ? 0
+             : pl.row_bytes + pl.count_bytes + pl.sum_bytes + (pl.dp ? 4 * pl.q_pad + 4 * pl.kv_pad : 0);
 }
 
 int run_padded(const BwdPlan& pl, char* w, hipStream_t s) {
@@ -268,10 +303,15 @@ int mfx_sdpa_packed_bwd(const mfx_sdpa_packed_bwd_args* args, void* stream) {
     if (!ws) return MFX_E_HIP;
   }
   pl.p.delta = reinterpret_cast<float*>(ws);
+  ws += pl.row_bytes;
+  pl.p.part_count = reinterpret_cast<int*>(ws);
+  ws += pl.count_bytes;
+  pl.p.part_sums = reinterpret_cast<float*>(ws);
+  ws += pl.sum_bytes;
   switch (pl.kind) {
     case Kind::kMfma16: return launch_packed_bwd_mfma(pl.p, s);
     case Kind::kMfmaF32: return launch_packed_bwd_f32(pl.p, s);
-    case Kind::kPadded16: return run_padded(pl, ws + pl.row_bytes, s);
+    case Kind::kPadded16: return run_padded(pl, ws, s);
     default: return launch_packed_bwd_generic(pl.p, s);
   }
 }

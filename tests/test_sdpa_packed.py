@@ -165,6 +165,54 @@ def test_longer_sequences(cuda, nat):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    # name, lengths, heads, head size: key blocks of one share up to eight.
+    ("bf16", [1411], 8, 1, 128),
+    ("f16", [1000, 300, 77], 8, 1, 64),
+    ("bf16", [700, 0, 129, 640], 6, 2, 96),
+    ("bf16", [1300] + [40] * 70, 8, 2, 64),
+    ("f16", [900, 901], 4, 4, 128),
+], ids=lambda c: f"{c[0]}-{len(c[1])}-{c[2]}on{c[3]}-{c[4]}")
+def test_shared_key_blocks(cuda, nat, case):
+    name, lens, Hq, Hkv, D = case
+    check_all(cuda, nat, name, lens, Hq, Hkv, D, tail=5)
+
+
+@pytest.mark.gpu
+def test_shared_key_blocks_repeat(cuda, nat):
+    """Shares of a key block are counted in a workspace that may hold anything,
+    by eager and captured calls, and give the same bits each time."""
+    torch = cuda
+    q, k, v, g, off = make(torch, "bf16", [1000, 24, 512], 8, 1, 128)
+    T = q.shape[0]
+    lse = torch.zeros(8, T, device="cuda")
+    o = torch.empty_like(q)
+    ws = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+
+    def step():
+        nat.sdpa_packed(q, k, v, off, out=o, lse=lse)
+        return nat.sdpa_packed_bwd(q, k, v, g, o, lse, off, workspace=ws)
+
+    ws.fill_(255)
+    first = [t.clone() for t in step()]
+    for fill in (0, 1, 127):
+        ws.fill_(fill)
+        assert all(torch.equal(a, b) for a, b in zip(first, step()))
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = step()
+    for lens in ([1536, 0, 0], [1000, 24, 512], [3, 1200, 333]):
+        off.copy_(torch.tensor([0] + lens).cumsum(0))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        ws.fill_(85)
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("layout", ["thd", "htd"])
 @pytest.mark.parametrize("name,D", [("bf16", 64), ("f16", 96), ("f32", 64), ("bf16", 80)])
 def test_sequences_do_not_see_each_other(cuda, nat, name, D, layout):
@@ -244,6 +292,24 @@ def test_offsets_out_of_order_stay_inside(cuda, nat, name, D, off):
     nat.sdpa_packed_bwd(q, k, v, g, o, lse, offs, dq=dq, dk=dk, dv=dv)
     for t in big:
         assert (t[:100] == 5).all() and (t[400:] == 5).all()
+
+
+@pytest.mark.gpu
+def test_overlapping_offsets_stay_inside_the_workspace(cuda, nat):
+    """400 sequences that are each the whole batch have more key blocks than the
+    workspace has shares for."""
+    torch = cuda
+    q, k, v, g, _ = make(torch, "bf16", [512], 8, 1, 64)
+    lse = torch.zeros(8, 512, device="cuda")
+    off = torch.tensor([0, 512] * 200, device="cuda", dtype=torch.int32)
+    out, dq, dk, dv = (torch.zeros_like(t) for t in (q, q, k, v))
+    args = nat.sdpa_packed_bwd_args(q, k, v, g, out, lse, dq, dk, dv, off)
+    import ctypes
+
+    need = int(nat.load().mfx_sdpa_packed_bwd_workspace_size(ctypes.byref(args)))
+    ws = torch.full((need + (1 << 26),), 7, dtype=torch.uint8, device="cuda")
+    nat.sdpa_packed_bwd(q, k, v, g, out, lse, off, dq=dq, dk=dk, dv=dv, workspace=ws[:need])
+    assert (ws[need:] == 7).all()
 
 
 @pytest.mark.gpu
