@@ -723,12 +723,13 @@ const char* mfx_gemm_kernel_name(const mfx_gemm_args* args);
  * h [T, H] and w [V, H] in `dtype` (f32, bf16, f16), rows spaced h_stride /
  * w_stride elements; fp32 products and sums.  targets int32 or int64
  * (target_dtype MFX_I32 / MFX_I64); a row whose target lies outside [0, V)
- * does not count: its loss is 0 and it adds nothing to any gradient.  loss and
+ * does not count: its loss is 0 and it adds nothing to any gradient (its row of
+ * h has to be finite for that: dw = d^T h holds 0 times it).  loss and
  * lse (optional) are fp32 [T].  Not rounded between: what
  * mfx_gemm, then mfx_log_softmax and a gather give without their roundings.
  * Rows must be 16-byte aligned and H a multiple of 16 bytes.
  * workspace: mfx_linear_xent_workspace_size() bytes, 256-byte aligned (8 bytes
- * per row and tile of 128 or 256 columns), or NULL for library scratch.
+ * per row and tile of 64 to 256 columns), or NULL for library scratch.
  * The reference's models form the logits and their log_softmax (callee
  * @log_softmax, src/jax_mlx_pjrt.cpp:5624-5641).
  */
@@ -757,7 +758,8 @@ size_t mfx_linear_xent_workspace_size(const mfx_linear_xent_args* args);
  *   d = (exp(z - lse) - onehot(targets)) * dloss,   dh = d W,   dw = d^T h
  * dh [T, H] of `dtype`, dw [V, H] of `dw_dtype` (`dtype` or MFX_F32); either
  * may be NULL.  d is formed in pieces of the vocabulary (at most 512 MiB of it,
- * or 256 columns) and, over the largest |dloss|, rounded to `dtype`.  Outputs must not share memory with the inputs.
+ * or 256 columns) and, over the largest |dloss|, rounded to `dtype`.  Outputs
+ * must not share memory with the inputs.
  * workspace: mfx_linear_xent_bwd_workspace_size() bytes, 256-byte aligned, or
  * NULL for library scratch.  Deterministic: no atomics.
  */

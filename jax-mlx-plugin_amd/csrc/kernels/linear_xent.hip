@@ -305,10 +305,19 @@ __global__ __launch_bounds__(1024) void xent_weights(const float* __restrict__ d
                                                      float* scale) {
   __shared__ float red[16];
   float m = 0.f;
-  for (int i = threadIdx.x; i < T; i += 1024) {
-    const float g = fabsf(dloss[i]);
-    const int64_t t = target_of(targets, target64, i);
-    if (t >= 0 && t < V) m = fmaxf(m, g);
+  // (Eight rows in flight at a time.)
+  for (int i0 = threadIdx.x; i0 < T; i0 += 8 * 1024) {
+    float g[8];
+    int64_t t[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = min(i0 + u * 1024, T - 1);
+      g[u] = dloss[i];
+      t[u] = target_of(targets, target64, i);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (t[u] >= 0 && t[u] < V) m = fmaxf(m, fabsf(g[u]));
   }
   m = group_max<64>(m);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
@@ -317,7 +326,14 @@ __global__ __launch_bounds__(1024) void xent_weights(const float* __restrict__ d
 #pragma unroll
   for (int i = 1; i < 16; ++i) m = fmaxf(m, red[i]);
   const float c = m > 0.f && m < INFINITY ? m : 1.f;
-  for (int i = threadIdx.x; i < T; i += 1024) weight[i] = dloss[i] / c * times;
+  for (int i0 = threadIdx.x; i0 < T; i0 += 8 * 1024) {
+    float g[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) g[u] = dloss[min(i0 + u * 1024, T - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i0 + u * 1024 < T) weight[i0 + u * 1024] = g[u] / c * times;
+  }
   if (threadIdx.x == 0) *scale = c / times;
 }
 
