@@ -729,7 +729,7 @@ const char* mfx_gemm_kernel_name(const mfx_gemm_args* args);
  * mfx_gemm, then mfx_log_softmax and a gather give without their roundings.
  * Rows must be 16-byte aligned and H a multiple of 16 bytes.
  * workspace: mfx_linear_xent_workspace_size() bytes, 256-byte aligned (8 bytes
- * per row and tile of 64 to 256 columns), or NULL for library scratch.
+ * per row and tile of 32 to 256 columns), or NULL for library scratch.
  * The reference's models form the logits and their log_softmax (callee
  * @log_softmax, src/jax_mlx_pjrt.cpp:5624-5641).
  */

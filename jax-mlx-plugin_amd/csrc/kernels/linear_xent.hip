@@ -38,11 +38,12 @@
 namespace mfx {
 namespace xent {
 
-// Tile forms: 256 x 256, one workgroup a CU; 128 x 128, two; and 64 rows of A by
-// 128 of B (f32: 64 x 64), three.  f32 has the last two.
-enum Form { kWide, kNarrow, kSlim };
-constexpr int kFormM[3] = {256, 128, 64};
-constexpr int kFormN[2][3] = {{256, 128, 128}, {256, 128, 64}};  // 16 bits, f32
+// Tile forms: 256 x 256, one workgroup a CU; 128 x 128, two; 64 rows of A by
+// 128 of B (f32: 64 x 64), three; and 32 x 32, four.  16 bits have the first
+// three, f32 the last three.
+enum Form { kWide, kNarrow, kSlim, kBlock };
+constexpr int kFormM[4] = {256, 128, 64, 32};
+constexpr int kFormN[2][4] = {{256, 128, 128, 0}, {0, 128, 64, 32}};  // 16 bits, f32
 
 template <Form F, bool A_KC, bool B_KC, int E>
 struct Pick;
@@ -54,11 +55,14 @@ template <bool A_KC, bool B_KC, int E>
 struct Pick<kSlim, A_KC, B_KC, E> : Config<64, 128, 1, 4, A_KC, B_KC, E> {};
 template <bool A_KC, bool B_KC>
 struct Pick<kSlim, A_KC, B_KC, 2> : Config<64, 64, 2, 2, A_KC, B_KC, 2> {};
+template <bool A_KC, bool B_KC>
+struct Pick<kBlock, A_KC, B_KC, 2> : Config<32, 32, 1, 1, A_KC, B_KC, 2, 4> {};
 
 template <class C>
 __device__ __forceinline__ void gemm_tile(const GemmShape& g, int m0, int n0, int kt0, int kt1, char* smem,
                                           Acc<C>& acc) {
-  if constexpr (C::E == 2) gemm_tile32<C>(g, m0, n0, kt0, kt1, reinterpret_cast<float*>(smem), acc);
+  if constexpr (C::KW > 1) gemm_block32<C>(g, m0, n0, kt0, kt1, reinterpret_cast<float*>(smem), acc);
+  else if constexpr (C::E == 2) gemm_tile32<C>(g, m0, n0, kt0, kt1, reinterpret_cast<float*>(smem), acc);
   else gemm_tile16<C>(g, m0, n0, kt0, kt1, reinterpret_cast<bf16*>(smem), acc);
 }
 
@@ -111,8 +115,9 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void xent_logits_kernel(LossArgs p
 
   const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave % C::WM, wn = wave / C::WM;
-  const int M = p.g.M, N = p.g.N;
+  const int wm = wave % C::WM, wn = wave / C::WM % C::WN;
+  // (Wavefronts without sums have no rows.)
+  const int M = wave < C::WM * C::WN ? p.g.M : 0, N = p.g.N;
   const int nw = n0 + wn * FN * 32;  // this wavefront's first column (of the piece)
   // Block i's values, -inf in columns past N (of which only the last tile has
   // any): 16 FN registers at a time, and the fences between blocks keep it so.
@@ -167,7 +172,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void xent_logits_kernel(LossArgs p
         for (int e = 0; e < FN * 16; ++e) l[e & 1] += __builtin_amdgcn_exp2f(fmaf(z[e], kLog2e, -base));
         l[0] += l[1];
         l[0] += __shfl_xor(l[0], 32, 64);
-        if (half == 0) {
+        if (half == 0 && (C::KW == 1 || row < M)) {
           red_m[wn * C::BM + r] = mx == -INFINITY ? mx : base;
           red_l[wn * C::BM + r] = l[0];
         }
@@ -355,8 +360,9 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void xent_grad_kernel(StoreArgs p)
 
   const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave % C::WM, wn = wave / C::WM;
-  const int M = p.g.M, N = p.g.N;
+  const int wm = wave % C::WM, wn = wave / C::WM % C::WN;
+  // (Wavefronts without sums have no rows.)
+  const int M = wave < C::WM * C::WN ? p.g.M : 0, N = p.g.N;
   const int mw = m0 + wm * FM * 32, nw = n0 + wn * FN * 32;
   const float mul = p.scale ? *p.scale : 1.f;
   if (C::E == 2 || p.part || p.c_f32) {
@@ -444,6 +450,10 @@ struct Way {
   int64_t range, ranges;  // k-tiles of one, and their number
 };
 
+// A type's first and last form.
+constexpr int first_form(int E) { return E == 2 ? kNarrow : kWide; }
+constexpr int last_form(int E) { return E == 2 ? kBlock : kSlim; }
+
 GemmShape shape(Operand a, Operand b, int64_t M, int64_t N, int64_t K, int E, Form f) {
   GemmShape g{};
   g.a = a;
@@ -459,15 +469,15 @@ GemmShape shape(Operand a, Operand b, int64_t M, int64_t N, int64_t K, int E, Fo
 
 // Microseconds that a form takes: a k-tile with `slots` workgroups on each CU,
 // each further round of workgroups, and once.  Fitted to the measured times of
-// 13 shapes from [33 x 4096 x 65537] to [8192 x 512 x 1000] in every form and
+// 18 shapes from [33 x 4096 x 65537] to [8192 x 512 x 1000] in every form and
 // with 1 to 16 ranges; the chosen way took at most 13% more than the best of
 // them.
 struct Cost {
   int slots;
   float kt, each, once;
 };
-constexpr Cost kCost[2][3] = {{{1, 0.85f, 9.f, 0.f}, {2, 0.57f, 1.f, 6.f}, {3, 0.85f, 0.5f, 4.f}},
-                              {{1, 0.f, 0.f, 0.f}, {2, 4.6f, 2.f, 6.f}, {3, 1.95f, 1.f, 4.f}}};
+constexpr Cost kCost[2][4] = {{{1, 0.85f, 9.f, 0.f}, {2, 0.57f, 1.f, 6.f}, {3, 0.85f, 0.5f, 4.f}, {}},
+                              {{}, {2, 4.6f, 2.f, 6.f}, {3, 1.95f, 1.f, 4.f}, {4, 0.8f, 1.f, 4.f}}};
 
 float way_us(const Cost& c, int64_t wgs, int64_t range, int64_t cus) {
   const int64_t full = wgs / (c.slots * cus), rest = wgs % (c.slots * cus);
@@ -484,7 +494,7 @@ Way choose(int E, int64_t M, int64_t N, int64_t K, bool split) {
   const int64_t kt = ceil_div(K, E == 2 ? kBK32 : kBK16), cus = device_cu_count();
   Way best{kNarrow, kt, 1};
   float least = INFINITY;
-  for (int f = E == 2 ? kNarrow : kWide; f <= kSlim; ++f) {
+  for (int f = first_form(E); f <= last_form(E); ++f) {
     const Cost& c = kCost[E == 2][f];
     const int64_t tiles = ceil_div(M, kFormM[f]) * ceil_div(N, kFormN[E == 2][f]);
     for (int64_t s = 1; s <= (split ? std::min<int64_t>(32, std::max<int64_t>(1, kt / 8)) : 1); ++s) {
@@ -541,6 +551,9 @@ int launch_logits(const LossArgs& p, Form f, hipStream_t s) {
     if (f == kWide) hipLaunchKernelGGL((xent_logits_kernel<Pick<kWide, true, true, E>, BWD>), grid, dim3(256), 0, s, p);
   if (f == kNarrow) hipLaunchKernelGGL((xent_logits_kernel<Pick<kNarrow, true, true, E>, BWD>), grid, dim3(256), 0, s, p);
   if (f == kSlim) hipLaunchKernelGGL((xent_logits_kernel<Pick<kSlim, true, true, E>, BWD>), grid, dim3(256), 0, s, p);
+  if constexpr (E == 2)
+    if (f == kBlock)
+      hipLaunchKernelGGL((xent_logits_kernel<Pick<kBlock, true, true, E>, BWD>), grid, dim3(256), 0, s, p);
   return launch_status("xent_logits_kernel");
 }
 
@@ -557,6 +570,9 @@ int launch_grad(StoreArgs& p, const Way& way, hipStream_t s) {
     hipLaunchKernelGGL((xent_grad_kernel<Pick<kNarrow, A_KC, false, E>>), grid, dim3(256), 0, s, p);
   if (way.form == kSlim)
     hipLaunchKernelGGL((xent_grad_kernel<Pick<kSlim, A_KC, false, E>>), grid, dim3(256), 0, s, p);
+  if constexpr (E == 2)
+    if (way.form == kBlock)
+      hipLaunchKernelGGL((xent_grad_kernel<Pick<kBlock, A_KC, false, E>>), grid, dim3(256), 0, s, p);
   return launch_status("xent_grad_kernel");
 }
 

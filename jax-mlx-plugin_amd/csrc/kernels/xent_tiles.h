@@ -38,19 +38,21 @@ __device__ __forceinline__ void map_tile(int id, int tiles_m, int tiles_n, int& 
   tn = t / rows;
 }
 
-// E: 0 bf16, 1 f16, 2 f32.
-template <int BM_, int BN_, int WM_, int WN_, bool A_KC_, bool B_KC_, int E_>
+// E: 0 bf16, 1 f16, 2 f32.  KW wavefronts share each block's k; the first of
+// them (wave < WM * WN) ends with the sums.
+template <int BM_, int BN_, int WM_, int WN_, bool A_KC_, bool B_KC_, int E_, int KW_ = 1>
 struct Config {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, E = E_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, E = E_, KW = KW_;
   static constexpr bool A_KC = A_KC_, B_KC = B_KC_;
-  static constexpr int NW = WM * WN, NT = NW * 64;
-  static constexpr int WAVES = BM == 256 ? 1 : BM == 128 ? 2 : 3;  // per SIMD
+  static constexpr int NW = WM * WN * KW, NT = NW * 64;
+  static constexpr int WAVES = BM == 256 ? 1 : BM == 128 ? 2 : BM == 64 ? 3 : 4;  // per SIMD
   static constexpr int FM = BM / (32 * WM), FN = BN / (32 * WN);  // blocks of a wavefront
   static constexpr int BK = E == 2 ? kBK32 : kBK16;
   // Bytes of a stage, and of all: four in 16 bits; f32: two, in the larger of
   // the two forms' padded rows (xent_gemm32.h).
   static constexpr int STAGE = E == 2 ? 2 * BM * (kBK32 + (BM < 128 ? 8 : 4)) * 4 : (BM + BN) * kBK16 * 2;
-  static constexpr int SMEM = (E == 2 ? 2 : 4) * STAGE;
+  // With KW > 1 one for each wavefront.
+  static constexpr int SMEM = (KW > 1 ? KW : E == 2 ? 2 : 4) * STAGE;
 };
 
 template <class C>

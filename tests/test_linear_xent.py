@@ -99,6 +99,14 @@ def test_wide_tiles_and_ranges(cuda, nat, name, T, H, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,H,V", [(33, 1028, 8001), (100, 2052, 300), (1, 4, 33), (70, 132, 31), (700, 200, 1501),
+                                   (2100, 256, 4001), (4093, 260, 4095)])
+def test_f32_tile_forms(cuda, nat, T, H, V):
+    """32 x 32 blocks, 64 x 64 and 128 x 128 tiles, ragged on every side."""
+    check_all(cuda, nat, "f32", *make(cuda, "f32", T, H, V, seed=4))
+
+
+@pytest.mark.gpu
 def test_several_pieces(cuda, nat):
     """d beyond its budget: a vocabulary in pieces, dh added up over them.
     (Against the same call on column blocks small enough for one piece.)"""
