@@ -52,7 +52,8 @@ __device__ __forceinline__ int kc_swz(int r) { return (r >> 2) & 3; }
 // One operand's tiles: IDX indices of a tile, NW wavefronts sharing the loads.
 // KC: [IDX rows][32 k], chunk c of row r at c ^ kc_swz(r).
 // else: [32 k][IDX], chunk c of row r at c ^ tile_swz<IDX>(r).
-template <bool KC, int IDX, int NW>
+// ROT: the tiles of k are walked round from a later one (its number `at`).
+template <bool KC, int IDX, int NW, bool ROT = false>
 struct Tile {
   static constexpr int ELEMS = IDX * kBK16;
   static constexpr int RPI = KC ? 16 : 512 / IDX;  // rows one load instruction covers
@@ -73,6 +74,7 @@ struct Tile {
                         // else: bytes of the last row
   uint32_t voff[NOFF];  // this lane's byte offset in instructions 0 and 1, less the rows between
   int lane_k;           // KC: k of the lane's chunk within a tile
+  int turn;             // ROT: tiles left
 #if defined(__HIP_DEVICE_COMPILE__)
   __amdgpu_buffer_rsrc_t rsrc;
 #endif
@@ -82,11 +84,13 @@ struct Tile {
   // row ends with its last chunk, whose surplus elements are zeros or meet
   // zeros; rows are whole chunks wide.)
   static __device__ __forceinline__ int chunks(int n) { return (n + 7) & ~7; }
-  __device__ __forceinline__ Tile(const Operand& o, int idx0, int total, int k, int kt0, int kt1, int wave, int lane) {
+  __device__ __forceinline__ Tile(const Operand& o, int idx0, int total, int k, int kt0, int kt1, int wave, int lane,
+                                  int at = 0) {
     const int left = total - idx0;
     K = k;
-    k0 = kt0 * kBK16;
+    k0 = (kt0 + at) * kBK16;
     k_end = min(K, kt1 * kBK16);
+    turn = kt1 - kt0;
     ld2 = (int)o.ld * 2;
     next = KC ? kBK16 : kBK16 * o.ld;
     cur = static_cast<const bf16*>(o.p) + (KC ? (int64_t)idx0 * o.ld + k0 : (int64_t)k0 * o.ld + idx0);
@@ -103,11 +107,18 @@ struct Tile {
   __device__ __forceinline__ void take() {
 #if defined(__HIP_DEVICE_COMPILE__)
     int extent = KC ? last - k0 * 2 : (min(K - k0, kBK16) - 1) * ld2 + last;
-    if (k0 >= k_end) extent = 0;
+    if (ROT ? turn-- <= 0 : k0 >= k_end) extent = 0;
     rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16*>(cur), (short)0, extent, 0x00020000);
     if constexpr (KC) vo = k0 + lane_k < K ? voff[0] : kOOR;
     cur += next;
     k0 += kBK16;
+    if constexpr (ROT) {
+      static_assert(KC, "steps along a row");
+      if (k0 >= k_end) {  // (one range: k from 0)
+        cur -= k0;
+        k0 = 0;
+      }
+    }
 #endif
   }
   __device__ __forceinline__ void load(int i, bf16* lds, int wave) const {
@@ -197,11 +208,18 @@ __device__ __forceinline__ void gemm_tile16(const GemmShape& g, int m0, int n0, 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % C::WM, wn = wave / C::WM;
 
-  using TA = Tile<C::A_KC, C::BM, C::NW>;
-  using TB = Tile<C::B_KC, C::BN, C::NW>;
+  // Few rows against many: the reads of B set the time, and workgroups that all
+  // walk the same 64 bytes of their rows crowd on a part of the memory channels
+  // (rows are often a power of two apart).  Neighbouring tiles start one tile of
+  // k apart: [33 x 4096] by [65537 x 4096] 151 us from the same k, 142 so; 2%
+  // slower where B fits the last cache.
+  constexpr bool ROT = C::BM == 64 && C::A_KC && C::B_KC;
+  using TA = Tile<C::A_KC, C::BM, C::NW, ROT>;
+  using TB = Tile<C::B_KC, C::BN, C::NW, ROT>;
+  const int at = ROT ? n0 / C::BN % (kt1 - kt0) : 0;
   constexpr int LA = TA::LOADS, NL = LA + TB::LOADS, STAGE = C::STAGE;
-  TA ta(g.a, m0, g.M, g.K, kt0, kt1, wave, lane);
-  TB tb(g.b, n0, g.N, g.K, kt0, kt1, wave, lane);
+  TA ta(g.a, m0, g.M, g.K, kt0, kt1, wave, lane, at);
+  TB tb(g.b, n0, g.N, g.K, kt0, kt1, wave, lane, at);
   const uint32_t lds = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem;
   using RA = Reader<C::A_KC, C::BM, FM>;
   using RB = Reader<C::B_KC, C::BN, FN>;
