@@ -7,15 +7,16 @@
 // h [T, H] and W [V, H] in bf16, f16 or f32; all sums and the softmax in fp32.
 //
 // Forward: the product kernel (xent_gemm16.h, xent_gemm32.h) over tiles of
-// T x V whose epilogue leaves each row's maximum and sum of exponentials over the tile's
-// columns, and the target's logit; xent_combine folds a row's tiles.  The
-// partials are 8 bytes per row and 256 columns.
+// T x V whose epilogue leaves each row's maximum and sum of exponentials over
+// the tile's columns, and the target's logit; xent_combine folds a row's tiles.
+// The partials are 8 bytes per row and tile of 32 to 256 columns.
 //
 // Backward, in pieces of the vocabulary: the piece's logits again, whose
 // epilogue turns them into d, rounded to the inputs' type, in a workspace of
 // T x piece (f32 for f32 inputs, nothing is rounded there); then dW of the
-// piece = d^T h and dh (+)= d W of the piece.  A piece is as wide as kPieceBytes of d allow, so that the fp32 dh is added to
-// in few rounds and its products are long.  Rounding d costs half a step of
+// piece = d^T h and dh (+)= d W of the piece.  A piece is as wide as kPieceBytes
+// of d allow, so that the fp32 dh is added to in few rounds and its products
+// are long.  Rounding d costs half a step of
 // each entry (independent from entry to entry), as rounding the gradient of
 // stored 16-bit logits would; the target's entry is rounded after the
 // subtraction.  d is held over the largest |dloss|, c, which the sums are
@@ -27,7 +28,11 @@
 // besides, or entries below 2^-24 would be lost.
 //
 // What bounds it: the matrix cores, 2 T H V flops a product, one product
-// forward and three backward.
+// forward and three backward.  bf16, T 8192, H 4096, V 65537: forward 3.5 ms (1.24
+// PFLOP/s, matrix cores 71% busy), backward 10.5 ms (1.25; logits 63%, dW 66%, dh
+// 73%); a library product of these sizes runs at 1.25 - 1.58 beside them, by the
+// clock.  T 4096, H 2048, V 32000: 0.46 and 1.36 ms (1.17, 1.19).  Few rows
+// (T 33) read W once: 132 us for 537 MB, 4.1 TB/s.
 #include <algorithm>
 #include <cmath>
 #include <string>

@@ -32,7 +32,12 @@
 // rounded once, at the store.
 //
 // What bounds it: HBM, each row read once and written once (backward: two
-// rows read, one written).
+// rows read, one written).  8192 tokens of 32 + 8 heads of 128, bf16: forward
+// 32 us (168 MB, 5.2 TB/s; a copy runs at 4.8), backward 47 us (253 MB, 5.4
+// TB/s) and 4 us for the weights' sums.  64 tokens: 5 us, one pass of rows after
+// the other (position, angles, row, store), which is why their heads are split.
+// Angles formed by every lane for its own pairs, in place of once a token: 46
+// and 103 us.
 #include <algorithm>
 #include <cmath>
 

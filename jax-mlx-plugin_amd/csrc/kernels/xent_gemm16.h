@@ -21,7 +21,11 @@
 // their requests at about 90 bytes a cycle; together they would wait for each
 // other).  The one barrier a tile falls between products of its last step, whose
 // operands are in registers by then: behind it the next tile's stage is read
-// and the stage of the tile before it is loaded.
+// and the stage of the tile before it is loaded.  Measured on products of 8192
+// x 4096 x 16384: matrix cores 66 - 75% busy; without the loads' issue the
+// kernels take 13 - 17% fewer cycles, without LDS reads as well another 5%,
+// without the barrier no fewer.  (Wavefronts that load in different slots: 0 -
+// 4% faster by kernel, not steadily.)
 //
 // Range.  A buffer resource is built per tile with the tile's own 64-bit base
 // (so no operand's size is limited) and the bytes left in the operand; rows
