@@ -483,8 +483,9 @@ const char* mfx_sdpa_packed_kernel_name(const mfx_sdpa_packed_args* args);
  * square), of which their own rounding is 0.0017.
  * Workspace: mfx_sdpa_packed_bwd_workspace_size() bytes, 256-byte
  * aligned, or NULL for library scratch.  Deterministic.  (Under a causal mask
- * the sums of a long sequence's first keys may be split, by T, num_seqs and the
- * offsets: their last bits depend on what the sequence is packed with.)
+ * the sums of a long sequence's first keys and last queries may be split, by T,
+ * num_seqs and the offsets: their last bits depend on what the sequence is
+ * packed with.)
  */
 typedef struct {
   const void* q;

@@ -149,7 +149,7 @@ __device__ __forceinline__ void load_frags(const bf16* base, int64_t stride, int
 // and the wavefront with the most visible blocks sets the pace anyway.
 constexpr int kKvPf = 2;   // operand reads issued ahead of their MFMAs
 constexpr int kKvStages = 3;
-constexpr int kPartTiles = 8;  // packed: a share of a key block's tiles is at least so many
+constexpr int kPartTiles = 8;  // packed: blocks of so many tiles have one share
 constexpr int kDkdvHeadGroup = 2;  // kv heads whose key blocks an XCD runs together
 
 // Four f32, written through to where every XCD sees them and read from there
@@ -160,6 +160,62 @@ __device__ __forceinline__ void put_sums(__amdgpu_buffer_rsrc_t to, int at, f32x
 }
 __device__ __forceinline__ f32x4 get_sums(__amdgpu_buffer_rsrc_t from, int at) {
   return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, kThrough));
+}
+
+// Joins the shares of a block: this one's sums, N accumulators acc(0) .., go to
+// the workspace as they lie in registers; the workgroup that counts itself
+// last adds them in the shares' order, so the result does not depend on which
+// one that is, and returns true.  (Of two shares the order does not matter,
+// and the last one's stay where they are.)  The sums go past the L2s, so no
+// fence has to write one back: with fences the join of a batch's shares took
+// longer than it saved.
+template <int N, class Acc>
+__device__ __forceinline__ bool join_shares(const PackedShares& sh, int share, int block, int part, int nparts,
+                                            int heads, Acc acc) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool pair = nparts == 2;
+  __shared__ int others;
+  constexpr int kWave = N * 64 * 16 * 4, kShare = kWave * (kNT / 64);  // bytes
+  char* const own = reinterpret_cast<char*>(sh.sums) + (int64_t)share * kShare;
+  const int at = wave * kWave + lane * 16;
+  int* const count = sh.count + block;
+  if (tid == 0) others = __hip_atomic_load(count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (!pair || others != 1) {
+    const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(own, 0, kShare, 0x00020000);
+    static_for<0, N>([&](auto n) {
+      f32x16& v = acc(n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        put_sums(to, at + (n * 4 + i) * 1024, f32x4{v[i * 4], v[i * 4 + 1], v[i * 4 + 2], v[i * 4 + 3]});
+    });
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) others = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (others != nparts - 1) return false;
+  }
+  if (!pair)
+    static_for<0, N>([&](auto n) {
+      f32x16& v = acc(n);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+    });
+  for (int s = 0; s < nparts; ++s) {
+    if (pair && s == part) continue;
+    const __amdgpu_buffer_rsrc_t from =
+        __builtin_amdgcn_make_buffer_rsrc(own + (int64_t)(s - part) * heads * kShare, 0, kShare, 0x00020000);
+    static_for<0, N>([&](auto n) {
+      f32x16& v = acc(n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 a = get_sums(from, at + (n * 4 + i) * 1024);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i * 4 + e] += a[e];
+      }
+    });
+  }
+  return true;
 }
 
 // PACKED: one sequence of a packed batch (sdpa_packed.h).
@@ -220,9 +276,9 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
     int slot;
     PackedBlock pb;
     packed_head(id, BHk, gridDim.x / BHk, bhk, slot);
-    if (CAUSAL && p.parts > 1) {
-      const PackedShare ps = packed_share<kRows>(p, 2 * p.group, kPartTiles, slot);
-      if (ps.parts > 1 && slot >= p.part_shares) return;  // (offsets that overlap: the workspace ends here)
+    if (CAUSAL && p.key_shares.parts > 1) {
+      const PackedShare ps = packed_share<kRows>(p, p.key_shares, BHk, kCus, 2 * p.group, kPartTiles, slot);
+      if (ps.parts > 1 && slot >= p.key_shares.shares) return;  // (offsets that overlap: the workspace ends here)
       share = slot * BHk + bhk;
       block = ps.block * BHk + bhk;
       slot = ps.block;
@@ -568,58 +624,11 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
   PHASE(ph_fence(); ph_set(kPhCEpi, ph_now()); ph_fence();)
   if constexpr (PACKED) {
     if (nparts > 1) {
-      // Each share's sums go to the workspace as they lie in registers; the
-      // workgroup that counts itself last adds them in the shares' order, so
-      // the result does not depend on which one that is.  (Of two shares the
-      // order does not matter, and the last one's stay where they are.)  The
-      // sums go past the L2s, so no fence has to write one back: with fences
-      // the join of a batch's shares took longer than it saved.
-      const bool pair = nparts == 2;
-      __shared__ int others;
-      constexpr int kShare = kRows * D * 8;  // bytes: dK and dV of a key block
-      char* const own = reinterpret_cast<char*>(p.part_sums) + (int64_t)share * kShare;
-      const int at = wave * (kShare / 4) + lane * 16;
-      int* const count = p.part_count + block;
-      if (tid == 0) others = __hip_atomic_load(count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __syncthreads();
-      if (!pair || others != 1) {
-        const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(own, 0, kShare, 0x00020000);
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f32x4 a, c;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) a[e] = dk[dt][i * 4 + e], c[e] = dv[dt][i * 4 + e];
-            put_sums(to, at + (dt * 4 + i) * 2048, a);
-            put_sums(to, at + (dt * 4 + i) * 2048 + 1024, c);
-          }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (tid == 0) others = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __syncthreads();
-        if (others != nparts - 1) return;
-      }
-      if (!pair) {
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) dk[dt][i] = dv[dt][i] = 0.f;
-      }
-      for (int n = 0; n < nparts; ++n) {
-        if (pair && n == part) continue;
-        const __amdgpu_buffer_rsrc_t from =
-            __builtin_amdgcn_make_buffer_rsrc(own + (int64_t)(n - part) * BHk * kShare, 0, kShare, 0x00020000);
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const f32x4 a = get_sums(from, at + (dt * 4 + i) * 2048);
-            const f32x4 c = get_sums(from, at + (dt * 4 + i) * 2048 + 1024);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dk[dt][i * 4 + e] += a[e], dv[dt][i * 4 + e] += c[e];
-          }
-      }
+      auto acc = [&](auto n) -> f32x16& {
+        if constexpr (n < D / 32) return dk[n];
+        else return dv[n - D / 32];
+      };
+      if (!join_shares<2 * (D / 32)>(p.key_shares, share, block, part, nparts, BHk, acc)) return;
     }
   }
   // Every wavefront's last Y has read its Q / dO stage: the stages take the
@@ -702,12 +711,22 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
   const int BH = p.B * p.Hq;
   const int id = blockIdx.x;
   int bh, mblk;
+  int nparts = 1, part = 0, share = 0, block_id = 0;  // packed: shares of the block's tiles
   if constexpr (PACKED) {
     int slot;
     PackedBlock pb;
     // (No share of a key block has been counted yet.)
-    if (id * kNT + tid < p.part_shares * p.Hkv) p.part_count[id * kNT + tid] = 0;
+    if (id * kNT + tid < p.key_shares.shares * p.Hkv) p.key_shares.count[id * kNT + tid] = 0;
     packed_head(id, BH, gridDim.x / BH, bh, slot);
+    if (CAUSAL && p.query_shares.parts > 1) {
+      const PackedShare ps = packed_share<kRows>(p, p.query_shares, BH, 2 * kCus, 2, kPartTiles, slot);
+      if (ps.parts > 1 && slot >= p.query_shares.shares) return;  // (as in bwd_dkdv_mfma)
+      share = slot * BH + bh;
+      block_id = ps.block * BH + bh;
+      slot = ps.block;
+      part = ps.part;
+      nparts = ps.parts;
+    }
     if (!packed_block<kRows>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
     mblk = pb.work;
     packed_shift<2>(p, pb.start, pb.len);
@@ -729,13 +748,17 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
   const bf16* vp = static_cast<const bf16*>(p.v) + b * p.vs[0] + hk * p.vs[1];
   int kv_end = Tk;
   if (CAUSAL) kv_end = min(Tk, min(Tq, (mblk + 1) * kRows));
-  const int ntiles = (kv_end + kTile - 1) / kTile;
+  int t0 = 0, ntiles = (kv_end + kTile - 1) / kTile;
+  if constexpr (PACKED) {
+    t0 = ntiles * part / nparts;
+    ntiles = ntiles * (part + 1) / nparts;
+  }
   const Loader<D> kload(kp, p.ks[2], Tk, D, wave, lane), vload(vp, p.vs[2], Tk, D, wave, lane);
   auto issue = [&](int t, int st) {
     kload.load(t, smem + (2 * st) * TILE, wave);
     vload.load(t, smem + (2 * st + 1) * TILE, wave);
   };
-  if (ntiles > 0) issue(0, 0);
+  if (ntiles > 0) issue(t0, 0);
 
   bf16x8 qf[D / 16], gf[D / 16];
   load_frags<D>(static_cast<const bf16*>(p.q) + b * p.qs[0] + h * p.qs[1], p.qs[2], qi, Tq, half, qf);
@@ -934,7 +957,7 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
 
   wait_dma();
   __syncthreads();
-  for (int t = 0; t < ntiles; t += 2) {
+  for (int t = t0; t < ntiles; t += 2) {
     if (t + 1 < ntiles) issue(t + 1, 1);
     step(t, std::integral_constant<int, 0>{});
     wait_dma();
@@ -946,6 +969,12 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
     __syncthreads();
   }
 
+  if constexpr (PACKED) {
+    if (nparts > 1) {
+      auto acc = [&](auto n) -> f32x16& { return dq[n]; };
+      if (!join_shares<D / 32>(p.query_shares, share, block_id, part, nparts, BH, acc)) return;
+    }
+  }
   // Every step ended at a barrier after its reads and with no load in
   // flight: the stages take the dQ rows on their way out.  (The first row
   // comes from an opaque copy here, so no address is hoisted into the loop.)
@@ -960,13 +989,24 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
 }
 
 #if defined(MFX_PACKED)
+__global__ __launch_bounds__(kNT) void clear_counts(int* count, int n) {
+  const int i = blockIdx.x * kNT + threadIdx.x;
+  if (i < n) count[i] = 0;
+}
+
 template <int D, bool CAUSAL, int E>
 int launch_t(const SdpaBwdParams& p, hipStream_t s) {
   const int64_t slots = packed_slots(p.total, p.num_seqs, kRows);
-  hipLaunchKernelGGL((bwd_dq_mfma<D, CAUSAL, 0, E, true>), dim3((unsigned)(slots * p.Hq)), dim3(kNT), 0, s, p);
+  const PackedShares &qs = p.query_shares, &ks = p.key_shares;
+  if (qs.parts > 1) {
+    const int n = qs.shares * p.Hq;
+    hipLaunchKernelGGL(clear_counts, dim3((unsigned)((n + kNT - 1) / kNT)), dim3(kNT), 0, s, qs.count, n);
+    if (int rc = launch_status("clear_counts")) return rc;
+  }
+  const unsigned queries = (unsigned)((slots + qs.extra) * p.Hq), keys = (unsigned)((slots + ks.extra) * p.Hkv);
+  hipLaunchKernelGGL((bwd_dq_mfma<D, CAUSAL, 0, E, true>), dim3(queries), dim3(kNT), 0, s, p);
   if (int rc = launch_status("bwd_dq_mfma (packed)")) return rc;
-  const unsigned shares = (unsigned)((slots + p.part_extra) * p.Hkv);
-  hipLaunchKernelGGL((bwd_dkdv_mfma<D, CAUSAL, 0, E, true>), dim3(shares), dim3(kNT), 0, s, p);
+  hipLaunchKernelGGL((bwd_dkdv_mfma<D, CAUSAL, 0, E, true>), dim3(keys), dim3(kNT), 0, s, p);
   return launch_status("bwd_dkdv_mfma (packed)");
 }
 

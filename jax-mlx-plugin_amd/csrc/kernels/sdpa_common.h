@@ -46,6 +46,15 @@ struct SdpaParams {
 // pass or from the caller's forward call: o [B][Hq][Tq][Dv] of `dtype` at
 // element strides os (feature stride 1), lse and delta [B][Hq][Tq] fp32
 // (log2 units for lse; delta = rowsum(dO * o)).
+// Blocks of a packed call in shares (sdpa_packed.h, packed_share): up to
+// `parts` of one block, at most `shares` of one head belong to blocks of more
+// than one, and at most `extra` workgroups a head come of it.
+struct PackedShares {
+  int parts, quarters, shares, extra;
+  int* count;   // [shares][heads]: those of a block that are done
+  float* sums;  // [shares][heads]
+};
+
 struct SdpaBwdParams {
   const void* q;
   const void* k;
@@ -69,12 +78,7 @@ struct SdpaBwdParams {
   const int32_t* seq_off;  // packed sequences, as in SdpaParams
   int num_seqs;
   int total;
-  // Packed, matrix cores: dK / dV of a key block in up to `parts` shares
-  // (packed_share): at most part_shares of one head belong to blocks of more
-  // than one, and at most part_extra workgroups a head come of it.
-  int parts, part_quarters, part_shares, part_extra;
-  float* part_sums;
-  int* part_count;
+  PackedShares key_shares, query_shares;  // packed, matrix cores
 };
 
 bool bwd_mfma_supports(const SdpaBwdParams& p);

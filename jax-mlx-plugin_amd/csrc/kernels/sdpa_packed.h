@@ -139,21 +139,23 @@ __device__ __forceinline__ bool packed_block(const int32_t* off, int n, int tota
   return true;
 }
 
-// Key blocks in shares.  Under a causal mask a block with work w walks
-// `tiles` (w + 1) tiles of queries; one that walks more than `most` is shared
-// by as many workgroups as bring each to `most` or less, at most p.parts.
-// `most` is p.part_quarters quarters of what a CU gets of all tiles of all
-// heads, or `least` if that is more.  Blocks are handed out by w, longest
-// first, so those of most shares come first: with n(k) blocks of k shares or
-// more, whose w is (k - 1) most / tiles or more, slot r falls to block and
-// share by a walk over k, and no workgroup is without work before the last.
-// (Every other workgroup leaving at once leaves half the shader engines
-// without work: a batch of 8192 tokens took 1.4 times as long.)
+// Blocks in shares.  Under a causal mask a block with work w walks
+// `tiles` (w + 1) tiles; one that walks more than `most` is shared
+// by as many workgroups as bring each to `most` or less, at most sh.parts.
+// `most` is sh.quarters quarters of what each of `room` workgroups at a time
+// gets of all tiles of `heads` heads, or `least` if that is more.  Blocks are
+// handed out by w, longest first, so those of most shares come first: with
+// n(k) blocks of k shares or more, whose w is (k - 1) most / tiles or more,
+// slot r falls to block and share by a walk over k, and no workgroup is
+// without work before the last.  (Every other workgroup leaving at once leaves
+// half the shader engines without work: a batch of 8192 tokens took 1.4 times
+// as long.)
 struct PackedShare {
   int block, part, parts;
 };
 template <int BM, class Params>
-__device__ __forceinline__ PackedShare packed_share(const Params& p, int tiles, int least, int r) {
+__device__ __forceinline__ PackedShare packed_share(const Params& p, const PackedShares& sh, int heads, int room,
+                                                    int tiles, int least, int r) {
   int nb[kLaneSeqs];
   int work = 0;
 #pragma unroll
@@ -167,11 +169,11 @@ __device__ __forceinline__ PackedShare packed_share(const Params& p, int tiles, 
       work += nb[c] * (nb[c] + 1) / 2;
     }
   }
-  const int64_t all = (int64_t)wave_sum(work) * tiles * p.Hkv * p.part_quarters;
-  const int most = max((int)min((all + 4 * kCus - 1) / (4 * kCus), (int64_t)1 << 27), least);
+  const int64_t all = (int64_t)wave_sum(work) * tiles * heads * sh.quarters;
+  const int most = max((int)min((all + 4 * room - 1) / (4 * room), (int64_t)1 << 27), least);
   PackedShare out{0, 0, 1};
   int before = 0, base = 0;
-  for (int k = p.parts; k > 1; --k) {
+  for (int k = sh.parts; k > 1; --k) {
     const int w = (k - 1) * most / tiles;
     int v = 0;
 #pragma unroll
@@ -269,7 +271,7 @@ int launch_packed_flash16(const SdpaParams& p, hipStream_t s);
 int launch_packed_f32(const SdpaParams& p, hipStream_t s);
 int launch_packed_generic(const SdpaParams& p, hipStream_t s);
 int launch_packed_bwd_mfma(const SdpaBwdParams& p, hipStream_t s);
-constexpr int kBwdKeyBlock = 128;  // keys a workgroup of it owns
+constexpr int kBwdBlock = 128;  // keys (or queries) a workgroup of it owns
 int launch_packed_bwd_f32(const SdpaBwdParams& p, hipStream_t s);
 int launch_packed_bwd_generic(const SdpaBwdParams& p, hipStream_t s);
 // Copies a [1, H, total, D] tensor into rows of dp features (or back, rows in

@@ -18,8 +18,8 @@ namespace {
 
 enum class Kind { kNone, kFlash16, kFlashF32, kMfma16, kMfmaF32, kPadded16, kGeneric };
 
-// dK / dV on the matrix cores: up to kPartBlocks key blocks (four a CU) some
-// are shared, at most kMaxParts ways (packed_share).
+// Backward on the matrix cores: up to kPartBlocks blocks (four a CU) some are
+// shared, at most kMaxParts ways (packed_share).
 constexpr int kPartBlocks = 4 * kCus, kMaxParts = 8;
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -91,10 +91,29 @@ struct BwdPlan {
   SdpaBwdParams p{};
   Kind kind = Kind::kNone;
   size_t row_bytes = 0;            // delta
-  size_t count_bytes = 0, sum_bytes = 0;  // key blocks in shares: their counts and sums
+  size_t count_bytes = 0, sum_bytes = 0;  // blocks in shares: their counts and sums
   int dp = 0;                      // kPadded16: features of the padded copies
   size_t q_pad = 0, kv_pad = 0;    // bytes of one
 };
+
+// Shares of a head's `slots` blocks, `room` of which run at a time: some while
+// there are no more than kPartBlocks blocks, up to kMaxParts ways.
+void plan_shares(PackedShares& sh, int64_t slots, int heads, int room, size_t block_bytes, BwdPlan& pl) {
+  const int64_t blocks = slots * heads;
+  if (blocks > kPartBlocks) return;
+  sh.parts = (int)std::min<int64_t>(kMaxParts, kPartBlocks / blocks + 1);
+  sh.quarters = blocks <= 2 * kCus ? 3 : 4;
+  // A block in k shares walks more than (k - 1) `most`, and all of a head
+  // no more than `all`: so many blocks are shared at most, and so many
+  // shares added.  (Of offsets that are no offsets there may be more
+  // blocks than slots, but no workgroups behind slots + extra.)
+  const int64_t all = room * 4 / sh.quarters / heads + 1;
+  sh.extra = (int)std::min(slots * (sh.parts - 1), all);
+  sh.shares = (int)std::min(slots, all) + sh.extra;
+  const int64_t n = (int64_t)sh.shares * heads;
+  pl.count_bytes += align256(n * sizeof(int));
+  pl.sum_bytes += n * block_bytes;
+}
 
 int plan_bwd(const mfx_sdpa_packed_bwd_args* a, BwdPlan& pl) {
   if (!a) return fail(MFX_E_INVALID, "null args");
@@ -165,9 +184,8 @@ int plan_bwd(const mfx_sdpa_packed_bwd_args* a, BwdPlan& pl) {
       pl.kv_pad = align256((size_t)p.Hkv * p.total * dp * 2);
     }
   }
-  if (pl.kind == Kind::kMfma16 || pl.kind == Kind::kPadded16) {
-    const int64_t slots = packed_slots(p.total, p.num_seqs, kBwdKeyBlock), blocks = slots * p.Hkv;
-    // A key block walks all queries behind it for every head of its group, and
+  if ((pl.kind == Kind::kMfma16 || pl.kind == Kind::kPadded16) && p.causal && p.num_seqs <= 64 * kLaneSeqs) {
+    // dK, dV: a key block walks all queries behind it for every head of its group, and
     // the longest ones alone can last longer than a CU's part of the whole
     // (backward of one sequence of 4096 tokens, 32 heads on 8: 730 us with whole
     // blocks, 602 with shares of at most three quarters of that part, 646 of
@@ -175,22 +193,16 @@ int plan_bwd(const mfx_sdpa_packed_bwd_args* a, BwdPlan& pl) {
     // With more than two blocks a CU smaller ones fill the gaps and joining
     // shares costs more (8192 tokens in 1: 1990 whole, 2055 in three quarters;
     // in 8 of 96 .. 2500: 622, 614, and 607 in shares of one part).
-    p.parts = 1;
-    if (p.causal && blocks <= kPartBlocks && p.num_seqs <= 64 * kLaneSeqs)
-      p.parts = (int)std::min<int64_t>(kMaxParts, kPartBlocks / blocks + 1);
-    if (p.parts > 1) {
-      p.part_quarters = blocks <= 2 * kCus ? 3 : 4;
-      // A block in k shares walks more than (k - 1) `most`, and all of a head
-      // no more than `all`: so many blocks are shared at most, and so many
-      // shares added.  (Of offsets that are no offsets there may be more
-      // blocks than slots, but no workgroups behind slots + part_extra.)
-      const int64_t all = kCus * 4 / p.part_quarters / p.Hkv + 1;
-      p.part_extra = (int)std::min(slots * (p.parts - 1), all);
-      p.part_shares = (int)std::min(slots, all) + p.part_extra;
-      const int64_t n = (int64_t)p.part_shares * p.Hkv;
-      pl.count_bytes = align256(n * sizeof(int));
-      pl.sum_bytes = (size_t)n * 2 * kBwdKeyBlock * (pl.dp ? pl.dp : p.D) * sizeof(float);
-    }
+    const int64_t slots = packed_slots(p.total, p.num_seqs, kBwdBlock);
+    const size_t block_bytes = (size_t)kBwdBlock * (pl.dp ? pl.dp : p.D) * sizeof(float);
+    plan_shares(p.key_shares, slots, p.Hkv, kCus, 2 * block_bytes, pl);
+    // dQ: blocks of queries, of which two run on a CU; counts that nothing before
+    // it clears cost a launch, 2 to 4 us.  (Whole backward, shares of queries and
+    // none: 8192 tokens, 4 heads on 1, 457 and 524 us; 12289 in 2 heads, 420 and
+    // 564; 1500 + 700, 4 heads, 86 and 100.  But 8192, 8 on 2, 698 and 686; four
+    // of 512, 8 heads, 55 and 51.)
+    if (p.total > 2048 && slots * p.Hq <= 2 * kCus)
+      plan_shares(p.query_shares, slots, p.Hq, 2 * kCus, block_bytes, pl);
   }
   return MFX_OK;
 }
@@ -310,10 +322,13 @@ int mfx_sdpa_packed_bwd(const mfx_sdpa_packed_bwd_args* args, void* stream) {
   }
   pl.p.delta = reinterpret_cast<float*>(ws);
   ws += pl.row_bytes;
-  pl.p.part_count = reinterpret_cast<int*>(ws);
-  ws += pl.count_bytes;
-  pl.p.part_sums = reinterpret_cast<float*>(ws);
-  ws += pl.sum_bytes;
+  for (PackedShares* sh : {&pl.p.key_shares, &pl.p.query_shares}) {
+    const size_t n = (size_t)sh->shares * (sh == &pl.p.key_shares ? pl.p.Hkv : pl.p.Hq);
+    sh->count = reinterpret_cast<int*>(ws);
+    ws += align256(n * sizeof(int));
+    sh->sums = reinterpret_cast<float*>(ws);
+    ws += n * kBwdBlock * (pl.dp ? pl.dp : pl.p.D) * (sh == &pl.p.key_shares ? 2 : 1) * sizeof(float);
+  }
   switch (pl.kind) {
     case Kind::kMfma16: return launch_packed_bwd_mfma(pl.p, s);
     case Kind::kMfmaF32: return launch_packed_bwd_f32(pl.p, s);

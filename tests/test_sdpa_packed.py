@@ -172,6 +172,10 @@ def test_longer_sequences(cuda, nat):
     ("bf16", [700, 0, 129, 640], 6, 2, 96),
     ("bf16", [1300] + [40] * 70, 8, 2, 64),
     ("f16", [900, 901], 4, 4, 128),
+    # and query blocks too (more than 2048 tokens, few heads).
+    ("bf16", [2111, 200], 2, 1, 128),
+    ("f16", [1200, 3, 1025], 2, 2, 64),
+    ("bf16", [2300], 1, 1, 32),
 ], ids=lambda c: f"{c[0]}-{len(c[1])}-{c[2]}on{c[3]}-{c[4]}")
 def test_shared_key_blocks(cuda, nat, case):
     name, lens, Hq, Hkv, D = case
@@ -183,7 +187,7 @@ def test_shared_key_blocks_repeat(cuda, nat):
     """Shares of a key block are counted in a workspace that may hold anything,
     by eager and captured calls, and give the same bits each time."""
     torch = cuda
-    q, k, v, g, off = make(torch, "bf16", [1000, 24, 512], 8, 1, 128)
+    q, k, v, g, off = make(torch, "bf16", [2000, 24, 512], 8, 1, 128)
     T = q.shape[0]
     lse = torch.zeros(8, T, device="cuda")
     o = torch.empty_like(q)
@@ -203,7 +207,7 @@ def test_shared_key_blocks_repeat(cuda, nat):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=s):
             out = step()
-    for lens in ([1536, 0, 0], [1000, 24, 512], [3, 1200, 333]):
+    for lens in ([2536, 0, 0], [2000, 24, 512], [3, 2200, 333]):
         off.copy_(torch.tensor([0] + lens).cumsum(0))
         graph.replay()
         torch.cuda.synchronize()
@@ -295,13 +299,14 @@ def test_offsets_out_of_order_stay_inside(cuda, nat, name, D, off):
 
 
 @pytest.mark.gpu
-def test_overlapping_offsets_stay_inside_the_workspace(cuda, nat):
-    """400 sequences that are each the whole batch have more key blocks than the
+@pytest.mark.parametrize("T,Hq", [(512, 8), (2100, 2)])
+def test_overlapping_offsets_stay_inside_the_workspace(cuda, nat, T, Hq):
+    """200 sequences that are each the whole batch have more blocks than the
     workspace has shares for."""
     torch = cuda
-    q, k, v, g, _ = make(torch, "bf16", [512], 8, 1, 64)
-    lse = torch.zeros(8, 512, device="cuda")
-    off = torch.tensor([0, 512] * 200, device="cuda", dtype=torch.int32)
+    q, k, v, g, _ = make(torch, "bf16", [T], Hq, 1, 64)
+    lse = torch.zeros(Hq, T, device="cuda")
+    off = torch.tensor([0, T] * 200, device="cuda", dtype=torch.int32)
     out, dq, dk, dv = (torch.zeros_like(t) for t in (q, q, k, v))
     args = nat.sdpa_packed_bwd_args(q, k, v, g, out, lse, dq, dk, dv, off)
     import ctypes
