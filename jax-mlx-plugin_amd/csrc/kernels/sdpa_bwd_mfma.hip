@@ -716,7 +716,8 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
     int slot;
     PackedBlock pb;
     // (No share of a key block has been counted yet.)
-    if (id * kNT + tid < p.key_shares.shares * p.Hkv) p.key_shares.count[id * kNT + tid] = 0;
+    const int64_t c = packed_cleared(blockIdx.x, tid, kNT, (int64_t)p.key_shares.shares * p.Hkv);
+    if (c >= 0) p.key_shares.count[c] = 0;
     packed_head(id, BH, gridDim.x / BH, bh, slot);
     if (CAUSAL && p.query_shares.parts > 1) {
       const PackedShare ps = packed_share<kRows>(p, p.query_shares, BH, 2 * kCus, 2, kPartTiles, slot);

@@ -28,6 +28,7 @@
 
 #include <type_traits>
 
+#include "packed_index.h"
 #include "sdpa_common.h"
 
 namespace mfx {
