@@ -439,8 +439,9 @@ const char* mfx_sdpa_bwd_kernel_name(const mfx_sdpa_bwd_args* args);
  * seq_offsets: num_seqs + 1 non-decreasing int32 values within 0 .. T, in
  * device memory (the host never reads them: a captured call may be replayed
  * with others).  Sequences may be empty.  Rows of out and lse in no sequence
- * (before the first, behind the last) are left as they were.  Offsets out of
- * order or range lead to no access outside the tensors; which rows are
+ * (before the first, behind the last) are left as they were, or with zero_rest
+ * those of out become zeros: what takes out next goes over every row.  Offsets
+ * out of order or range lead to no access outside the tensors; which rows are
  * computed then is unspecified.
  *
  * No sequence sees another's rows, whatever they hold; within a sequence rows
@@ -462,7 +463,7 @@ typedef struct {
   float scale;
   int32_t causal;
   int32_t dtype;
-  int32_t reserved;
+  int32_t zero_rest;
 } mfx_sdpa_packed_args;
 
 int mfx_sdpa_packed(const mfx_sdpa_packed_args* args, void* stream);
@@ -477,7 +478,9 @@ const char* mfx_sdpa_packed_kernel_name(const mfx_sdpa_packed_args* args);
 /*
  * Backward of mfx_sdpa_packed from the forward's out and lse: dq, dk, dv, dk
  * and dv of a kv head summed over its query heads.  Rows in no sequence are
- * left as they were.  dq, dk and dv must not share memory with the inputs or
+ * left as they were, or become zeros in those of dq (1), dk (2) and dv (4)
+ * whose bit zero_rest holds: sums over every row, as of a norm's weights, follow
+ * them.  dq, dk and dv must not share memory with the inputs or
  * each other.  In 16 bits P and dS meet the matrix cores rounded to `dtype`, as
  * in mfx_sdpa_bwd: bf16 gradients are off by 0.0025 of their size (root mean
  * square), of which their own rounding is 0.0017.
@@ -512,7 +515,7 @@ typedef struct {
   float scale;
   int32_t causal;
   int32_t dtype;
-  int32_t reserved;
+  int32_t zero_rest;
 } mfx_sdpa_packed_bwd_args;
 
 int mfx_sdpa_packed_bwd(const mfx_sdpa_packed_bwd_args* args, void* stream);

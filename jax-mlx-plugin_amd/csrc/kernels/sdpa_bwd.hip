@@ -79,7 +79,10 @@ __global__ __launch_bounds__(64) void bwd_dq_generic(SdpaBwdParams p) {
   const float lse = p.lse[row], dl = p.delta[row];
   if constexpr (PACKED) {
     int start, len;
-    if (!packed_seq(p.seq_off, p.num_seqs, p.total, i, start, len)) return;
+    if (!packed_seq(p.seq_off, p.num_seqs, p.total, i, start, len)) {
+      if (p.zero_rest & 1) packed_zero_row<T>(p.dq, p.dqs, h, i, p.D);
+      return;
+    }
     packed_shift<(int)sizeof(T)>(p, start, len);
     i -= start;
   }
@@ -143,7 +146,11 @@ __global__ __launch_bounds__(64) void bwd_dkdv_generic(SdpaBwdParams p) {
   const int b = bhk / p.Hkv, hk = bhk % p.Hkv;
   if constexpr (PACKED) {
     int start, len;
-    if (!packed_seq(p.seq_off, p.num_seqs, p.total, j, start, len)) return;
+    if (!packed_seq(p.seq_off, p.num_seqs, p.total, j, start, len)) {
+      if (p.zero_rest & 2) packed_zero_row<T>(p.dk, p.dks, hk, j, p.D);
+      if (p.zero_rest & 4) packed_zero_row<T>(p.dv, p.dvs, hk, j, p.Dv);
+      return;
+    }
     packed_shift<(int)sizeof(T)>(p, start, len);
     j -= start;
   }
@@ -207,24 +214,27 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 // stride 1) into contiguous rows of Dp >= D features, the rest zero; or back
 // (unpad: the first D features of each contiguous row to the strided rows).
 // One thread per 16-byte chunk (D and Dp multiples of 8 elements).  off, when
-// given: the offsets of n packed sequences; rows in none of them stay out of
-// the rows written back.
+// given: the offsets of `seqs` packed sequences; rows in none of them stay out
+// of the rows written back, or with `zero` are zeros there.
 template <bool UNPAD>
 __global__ __launch_bounds__(256) void pad_rows_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst,
                                                        int64_t rows, int D, int Dp, int H, int T, int64_t s0,
                                                        int64_t s1, int64_t s2, const int32_t* off = nullptr,
-                                                       int seqs = 0) {
+                                                       int seqs = 0, bool zero = false) {
   const int cpr = Dp / 8;  // chunks per padded row
   const int64_t n = rows * cpr;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / cpr;
     const int c = (int)(i % cpr) * 8;
     const int t = (int)(r % T);
-    if (UNPAD && off && (t < off[0] || t >= off[seqs])) continue;
+    const bool rest = UNPAD && off && (t < off[0] || t >= off[seqs]);
+    if (rest && !zero) continue;
     const int64_t bh = r / T;
     const int64_t strided = (bh / H) * s0 + (bh % H) * s1 + t * s2 + c;
     if constexpr (UNPAD) {
-      if (c < D) *reinterpret_cast<uint4*>(dst + strided) = *reinterpret_cast<const uint4*>(src + r * Dp + c);
+      if (c < D)
+        *reinterpret_cast<uint4*>(dst + strided) =
+            rest ? uint4{0u, 0u, 0u, 0u} : *reinterpret_cast<const uint4*>(src + r * Dp + c);
     } else {
       uint4 v = {0u, 0u, 0u, 0u};
       if (c < D) v = *reinterpret_cast<const uint4*>(src + strided);
@@ -427,10 +437,10 @@ int pad_rows(const void* src, void* dst, const BwdPlan& pl, int H, int T, const 
   const unsigned blocks = (unsigned)std::min<int64_t>((chunks + 255) / 256, 4096);
   if (unpad)
     hipLaunchKernelGGL((pad_rows_kernel<true>), dim3(blocks), dim3(256), 0, s, static_cast<const uint16_t*>(src),
-                       static_cast<uint16_t*>(dst), rows, pl.p.D, pl.dp, H, T, st[0], st[1], st[2], nullptr, 0);
+                       static_cast<uint16_t*>(dst), rows, pl.p.D, pl.dp, H, T, st[0], st[1], st[2], nullptr, 0, false);
   else
     hipLaunchKernelGGL((pad_rows_kernel<false>), dim3(blocks), dim3(256), 0, s, static_cast<const uint16_t*>(src),
-                       static_cast<uint16_t*>(dst), rows, pl.p.D, pl.dp, H, T, st[0], st[1], st[2], nullptr, 0);
+                       static_cast<uint16_t*>(dst), rows, pl.p.D, pl.dp, H, T, st[0], st[1], st[2], nullptr, 0, false);
   return launch_status("pad_rows_kernel");
 }
 
@@ -452,17 +462,17 @@ int launch_packed_bwd_generic(const SdpaBwdParams& p, hipStream_t s) {
 }
 
 int packed_pad_rows(const void* src, void* dst, const SdpaBwdParams& p, int H, int dp, const int64_t* st, bool unpad,
-                    hipStream_t s) {
+                    bool zero, hipStream_t s) {
   const int64_t rows = (int64_t)H * p.total;
   const unsigned blocks = (unsigned)std::min<int64_t>((rows * (dp / 8) + 255) / 256, 4096);
   auto* in = static_cast<const uint16_t*>(src);
   auto* out = static_cast<uint16_t*>(dst);
   if (unpad)
     hipLaunchKernelGGL((pad_rows_kernel<true>), dim3(blocks), dim3(256), 0, s, in, out, rows, p.D, dp, H, p.total,
-                       st[0], st[1], st[2], p.seq_off, p.num_seqs);
+                       st[0], st[1], st[2], p.seq_off, p.num_seqs, zero);
   else
     hipLaunchKernelGGL((pad_rows_kernel<false>), dim3(blocks), dim3(256), 0, s, in, out, rows, p.D, dp, H, p.total,
-                       st[0], st[1], st[2], p.seq_off, p.num_seqs);
+                       st[0], st[1], st[2], p.seq_off, p.num_seqs, zero);
   return launch_status("pad_rows_kernel (packed)");
 }
 

@@ -275,6 +275,7 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
   if constexpr (PACKED) {
     int slot;
     PackedBlock pb;
+    const PackedRest rest(p.seq_off, p.num_seqs, p.total);
     packed_head(id, BHk, gridDim.x / BHk, bhk, slot);
     if (CAUSAL && p.key_shares.parts > 1) {
       const PackedShare ps = packed_share<kRows>(p, p.key_shares, BHk, kCus, 2 * p.group, kPartTiles, slot);
@@ -285,7 +286,10 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
       part = ps.part;
       nparts = ps.parts;
     }
-    if (!packed_block<kRows>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
+    const bool any = packed_block<kRows>(p.seq_off, p.num_seqs, p.total, slot, pb);
+    if (p.zero_rest & 2) packed_zero_rest<2, kNT>(rest, p.dk, p.dks, p.Hkv, D);
+    if (p.zero_rest & 4) packed_zero_rest<2, kNT>(rest, p.dv, p.dvs, p.Hkv, D);
+    if (!any) return;
     kblk = pb.nb - 1 - pb.work;
     packed_shift<2>(p, pb.start, pb.len);
   } else if ((BHk & 7) == 0 && ((BHk >> 3) % kDkdvHeadGroup) == 0) {
@@ -718,6 +722,7 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
     // (No share of a key block has been counted yet.)
     const int64_t c = packed_cleared(blockIdx.x, tid, kNT, (int64_t)p.key_shares.shares * p.Hkv);
     if (c >= 0) p.key_shares.count[c] = 0;
+    const PackedRest rest(p.seq_off, p.num_seqs, p.total);
     packed_head(id, BH, gridDim.x / BH, bh, slot);
     if (CAUSAL && p.query_shares.parts > 1) {
       const PackedShare ps = packed_share<kRows>(p, p.query_shares, BH, 2 * kCus, 2, kPartTiles, slot);
@@ -728,7 +733,9 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
       part = ps.part;
       nparts = ps.parts;
     }
-    if (!packed_block<kRows>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
+    const bool any = packed_block<kRows>(p.seq_off, p.num_seqs, p.total, slot, pb);
+    if (p.zero_rest & 1) packed_zero_rest<2, kNT>(rest, p.dq, p.dqs, p.Hq, D);
+    if (!any) return;
     mblk = pb.work;
     packed_shift<2>(p, pb.start, pb.len);
   } else if ((BH & 7) == 0) {

@@ -40,6 +40,7 @@ struct SdpaParams {
   const int32_t* seq_off;
   int num_seqs;
   int total;
+  int zero_rest;  // packed: rows of out in no sequence become zeros
 };
 
 // Backward pass (mfx_sdpa_bwd).  o / lse come from the recomputed forward
@@ -78,6 +79,7 @@ struct SdpaBwdParams {
   const int32_t* seq_off;  // packed sequences, as in SdpaParams
   int num_seqs;
   int total;
+  int zero_rest;  // packed: those of dq (1), dk (2), dv (4) become zeros
   PackedShares key_shares, query_shares;  // packed, matrix cores
 };
 

@@ -243,8 +243,11 @@ __global__ __launch_bounds__(kNT, 2) void flash_bf16_pipe_kernel(SdpaParams p) {
   if constexpr (PACKED) {
     int slot;
     PackedBlock pb;
+    const PackedRest rest(p.seq_off, p.num_seqs, p.total);
     packed_head(id, BH, gridDim.x / BH, bh, slot);
-    if (!packed_block<kBM>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
+    const bool any = packed_block<kBM>(p.seq_off, p.num_seqs, p.total, slot, pb);
+    if (p.zero_rest) packed_zero_rest<2, kNT>(rest, p.out, p.os, p.Hq, p.Dv);
+    if (!any) return;
     mblk = pb.work;
     packed_shift<2>(p, pb.start, pb.len);
   } else if ((BH & 7) == 0) {

@@ -76,8 +76,11 @@ __global__ __launch_bounds__(kNT, (D >= 256 || (D >= 96 && MASK)) ? 1 : 2) void 
   if constexpr (PACKED) {
     int slot;
     PackedBlock pb;
+    const PackedRest rest(p.seq_off, p.num_seqs, p.total);
     packed_head(id, BH, gridDim.x / BH, bh, slot);
-    if (!packed_block<kBM>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
+    const bool any = packed_block<kBM>(p.seq_off, p.num_seqs, p.total, slot, pb);
+    if (p.zero_rest) packed_zero_rest<4, kNT>(rest, p.out, p.os, p.Hq, D);
+    if (!any) return;
     mblk = pb.work;
     packed_shift<4>(p, pb.start, pb.len);
   } else if ((BH & 7) == 0) {
@@ -331,8 +334,11 @@ __global__ __launch_bounds__(64 * kSW) void flash_f32_split_kernel(SdpaParams p)
   if constexpr (PACKED) {
     int slot;
     PackedBlock pb;
+    const PackedRest rest(p.seq_off, p.num_seqs, p.total);
     packed_head(blockIdx.x, p.Hq, gridDim.x / p.Hq, bh, slot);
-    if (!packed_block<32>(p.seq_off, p.num_seqs, p.total, slot, pb)) return;
+    const bool any = packed_block<32>(p.seq_off, p.num_seqs, p.total, slot, pb);
+    if (p.zero_rest) packed_zero_rest<4, 64 * kSW>(rest, p.out, p.os, p.Hq, D);
+    if (!any) return;
     mblk = pb.work;
     packed_shift<4>(p, pb.start, pb.len);
   }

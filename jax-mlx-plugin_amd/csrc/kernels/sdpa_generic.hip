@@ -22,7 +22,10 @@ __global__ __launch_bounds__(64) void generic_kernel(SdpaParams p) {
   const int bh = (int)(row / p.Tq);
   if constexpr (PACKED) {
     int start, len;
-    if (!packed_seq(p.seq_off, p.num_seqs, p.total, t, start, len)) return;
+    if (!packed_seq(p.seq_off, p.num_seqs, p.total, t, start, len)) {
+      if (p.zero_rest) packed_zero_row<T>(p.out, p.os, bh, t, p.Dv);
+      return;
+    }
     packed_shift<(int)sizeof(T)>(p, start, len);
     t -= start;
   }

@@ -22,6 +22,24 @@ enum class Kind { kNone, kFlash16, kFlashF32, kMfma16, kMfmaF32, kPadded16, kGen
 // shared, at most kMaxParts ways (packed_share).
 constexpr int kPartBlocks = 4 * kCus, kMaxParts = 8;
 
+// Zeros in all of a [heads, T, D] tensor: a call without sequences.
+template <int SIZE>
+__global__ __launch_bounds__(256) void packed_zero_all(void* out, int64_t s1, int64_t s2, int T, int heads, int D) {
+  const int64_t st[4] = {0, s1, s2, 1};
+  packed_zero_rest<SIZE, 256>(PackedRest(T), out, st, heads, D);
+}
+
+int zero_all(void* out, const int64_t* st, int64_t T, int64_t heads, int64_t D, int dtype, hipStream_t s) {
+  if (!out) return fail(MFX_E_INVALID, "outputs must be non-null");
+  if (st[2] != 1) return fail(MFX_E_INVALID, "feature (last) strides must be 1");
+  const dim3 grid((unsigned)std::min<int64_t>((T * heads + 3) / 4, 4096));
+  if (dtype == MFX_F32)
+    hipLaunchKernelGGL(packed_zero_all<4>, grid, dim3(256), 0, s, out, st[0], st[1], (int)T, (int)heads, (int)D);
+  else
+    hipLaunchKernelGGL(packed_zero_all<2>, grid, dim3(256), 0, s, out, st[0], st[1], (int)T, (int)heads, (int)D);
+  return launch_status("packed_zero_all");
+}
+
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 // (head, token, feature) strides as the kernels' (batch, head, seq, feature).
@@ -79,6 +97,7 @@ int plan_fwd(const mfx_sdpa_packed_args* a, SdpaParams& p, Kind& kind) {
   p.split_len = p.Tk;
   p.seq_off = a->seq_offsets;
   p.num_seqs = (int)a->num_seqs;
+  p.zero_rest = a->zero_rest;
   // (The 31-bit extents that the supports functions bound by Tk hold for every
   // sequence then; the row-block kernels of head size 256 are f32 only.)
   kind = p.D != 256 && flash_bf16_supports(p) ? Kind::kFlash16
@@ -154,6 +173,7 @@ int plan_bwd(const mfx_sdpa_packed_bwd_args* a, BwdPlan& pl) {
   p.scale_log2 = a->scale * kLog2e;
   p.seq_off = a->seq_offsets;
   p.num_seqs = (int)a->num_seqs;
+  p.zero_rest = a->zero_rest;
   pl.row_bytes = align256((size_t)p.Hq * p.total * sizeof(float));
   pl.kind = Kind::kGeneric;
   if (bwd_mfma_supports(p)) {
@@ -216,6 +236,7 @@ size_t bwd_bytes(const BwdPlan& pl) {
 int run_padded(const BwdPlan& pl, char* w, hipStream_t s) {
   const SdpaBwdParams& p = pl.p;
   SdpaBwdParams pp = p;
+  pp.zero_rest = 0;  // (the copies' rows in no sequence reach no output)
   pp.D = pp.Dv = pl.dp;
   for (auto* st : {&pp.qs, &pp.ks, &pp.vs, &pp.dos, &pp.os, &pp.dqs, &pp.dks, &pp.dvs}) {
     (*st)[1] = (int64_t)p.total * pl.dp;
@@ -227,6 +248,7 @@ int run_padded(const BwdPlan& pl, char* w, hipStream_t s) {
     void* dst;
     int H;
     const int64_t* st;
+    bool zero;
   };
   const Copy in[5] = {{p.q, w, p.Hq, p.qs},
                       {p.dout, w + pl.q_pad, p.Hq, p.dos},
@@ -234,7 +256,7 @@ int run_padded(const BwdPlan& pl, char* w, hipStream_t s) {
                       {p.k, wk, p.Hkv, p.ks},
                       {p.v, wk + pl.kv_pad, p.Hkv, p.vs}};
   for (const Copy& c : in)
-    if (int rc = packed_pad_rows(c.src, c.dst, p, c.H, pl.dp, c.st, false, s)) return rc;
+    if (int rc = packed_pad_rows(c.src, c.dst, p, c.H, pl.dp, c.st, false, false, s)) return rc;
   pp.q = in[0].dst;
   pp.dout = in[1].dst;
   pp.o = in[2].dst;
@@ -244,9 +266,11 @@ int run_padded(const BwdPlan& pl, char* w, hipStream_t s) {
   pp.dk = wk + 2 * pl.kv_pad;
   pp.dv = wk + 3 * pl.kv_pad;
   if (int rc = launch_packed_bwd_mfma(pp, s)) return rc;
-  const Copy out[3] = {{pp.dq, p.dq, p.Hq, p.dqs}, {pp.dk, p.dk, p.Hkv, p.dks}, {pp.dv, p.dv, p.Hkv, p.dvs}};
+  const Copy out[3] = {{pp.dq, p.dq, p.Hq, p.dqs, (p.zero_rest & 1) != 0},
+                       {pp.dk, p.dk, p.Hkv, p.dks, (p.zero_rest & 2) != 0},
+                       {pp.dv, p.dv, p.Hkv, p.dvs, (p.zero_rest & 4) != 0}};
   for (const Copy& c : out)
-    if (int rc = packed_pad_rows(c.src, c.dst, p, c.H, pl.dp, c.st, true, s)) return rc;
+    if (int rc = packed_pad_rows(c.src, c.dst, p, c.H, pl.dp, c.st, true, c.zero, s)) return rc;
   return MFX_OK;
 }
 
@@ -284,7 +308,9 @@ int mfx_sdpa_packed(const mfx_sdpa_packed_args* args, void* stream) {
   if (int rc = plan_fwd(args, p, kind)) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (kind) {
-    case Kind::kNone: return MFX_OK;
+    case Kind::kNone:
+      if (args->T == 0 || !args->zero_rest) return MFX_OK;
+      return zero_all(args->out, args->o_strides, args->T, args->Hq, args->D, args->dtype, s);
     case Kind::kFlash16: return launch_packed_flash16(p, s);
     case Kind::kFlashF32: return launch_packed_f32(p, s);
     default: return launch_packed_generic(p, s);
@@ -307,8 +333,21 @@ int mfx_sdpa_packed_bwd(const mfx_sdpa_packed_bwd_args* args, void* stream) {
   using namespace mfx;
   BwdPlan pl;
   if (int rc = plan_bwd(args, pl)) return rc;
-  if (pl.kind == Kind::kNone) return MFX_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (pl.kind == Kind::kNone) {
+    struct Out {
+      void* p;
+      const int64_t* st;
+      int64_t heads;
+    };
+    const Out outs[3] = {{args->dq, args->dq_strides, args->Hq},
+                         {args->dk, args->dk_strides, args->Hkv},
+                         {args->dv, args->dv_strides, args->Hkv}};
+    for (int i = 0; i < 3; ++i)
+      if (args->T > 0 && (args->zero_rest >> i & 1))
+        if (int rc = zero_all(outs[i].p, outs[i].st, args->T, outs[i].heads, args->D, args->dtype, s)) return rc;
+    return MFX_OK;
+  }
   const size_t need = bwd_bytes(pl);
   char* ws = nullptr;
   if (args->workspace) {

@@ -147,7 +147,7 @@ class SdpaPackedArgs(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "seq_offsets", "lse")]
                 + [(n, ctypes.c_int64) for n in ("T", "num_seqs", "Hq", "Hkv", "D")]
                 + [(n, I64x3) for n in ("q_strides", "k_strides", "v_strides", "o_strides")]
-                + [("scale", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("causal", "dtype", "reserved")])
+                + [("scale", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("causal", "dtype", "zero_rest")])
 
 
 class SdpaPackedBwdArgs(ctypes.Structure):
@@ -159,7 +159,7 @@ class SdpaPackedBwdArgs(ctypes.Structure):
                 + [(n, ctypes.c_int64) for n in ("T", "num_seqs", "Hq", "Hkv", "D")]
                 + [(n, I64x3) for n in ("q_strides", "k_strides", "v_strides", "do_strides", "o_strides",
                                         "dq_strides", "dk_strides", "dv_strides")]
-                + [("scale", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("causal", "dtype", "reserved")])
+                + [("scale", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("causal", "dtype", "zero_rest")])
 
 
 class QkNormRopeArgs(ctypes.Structure):
@@ -750,25 +750,27 @@ def _packed_lse(lse, Hq, T):
         raise ValueError("lse must be a contiguous f32 tensor of [heads, tokens]")
 
 
-def sdpa_packed_args(q, k, v, out, seq_offsets, *, scale=None, causal=True, lse=None) -> SdpaPackedArgs:
+def sdpa_packed_args(q, k, v, out, seq_offsets, *, scale=None, causal=True, lse=None, zero_rest=0) -> SdpaPackedArgs:
     dims = _packed_dims(q, k, v, seq_offsets, out)
     if lse is not None:
         _packed_lse(lse, dims[2], dims[0])
     return SdpaPackedArgs.from_buffer_copy(_PACKED_PACK(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), seq_offsets.data_ptr(), _ptr(lse), *dims, *_htd(q),
         *_htd(k), *_htd(v), *_htd(out), _f32(1.0 / (dims[4] ** 0.5) if scale is None else scale), 1 if causal else 0,
-        dtype_code(q.dtype), 0))
+        dtype_code(q.dtype), zero_rest))
 
 
 def sdpa_packed(q, k, v, seq_offsets, *, scale=None, causal=True, out=None, lse=None):
     """Attention over packed sequences (mfx_sdpa_packed): q [T, Hq, D], k and v
     [T, Hkv, D], sequence s the tokens seq_offsets[s] .. seq_offsets[s + 1]
-    (int32, on the device).  Rows in no sequence are not written (a fresh out
-    holds anything there).  lse: optional f32 [Hq, T] output for
+    (int32, on the device).  Rows in no sequence are zeros in an out made here;
+    a given out keeps its own there (and what takes it next goes over every
+    row: they should be finite).  lse: optional f32 [Hq, T] output for
     sdpa_packed_bwd."""
-    if out is None:
+    made = out is None
+    if made:
         out = _fresh(q)
-    a = sdpa_packed_args(q, k, v, out, seq_offsets, scale=scale, causal=causal, lse=lse)
+    a = sdpa_packed_args(q, k, v, out, seq_offsets, scale=scale, causal=causal, lse=lse, zero_rest=1 if made else 0)
     with _on(q, k, v, out, seq_offsets, lse):
         check(load().mfx_sdpa_packed(ctypes.byref(a), _stream_handle(q)))
     return out
@@ -782,8 +784,8 @@ def sdpa_packed_kernel_name(q, k, v, seq_offsets, **kw) -> str:
     return name.decode()
 
 
-def sdpa_packed_bwd_args(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, *, scale=None,
-                         causal=True) -> SdpaPackedBwdArgs:
+def sdpa_packed_bwd_args(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, *, scale=None, causal=True,
+                         zero_rest=0) -> SdpaPackedBwdArgs:
     dims = _packed_dims(q, k, v, seq_offsets, dout, out, dq)
     _packed_lse(lse, dims[2], dims[0])
     if dk.shape != k.shape or dv.shape != v.shape or dk.dtype != q.dtype or dv.dtype != q.dtype:
@@ -791,16 +793,19 @@ def sdpa_packed_bwd_args(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, *, sc
     return SdpaPackedBwdArgs.from_buffer_copy(_PACKED_BWD_PACK(
         *[t.data_ptr() for t in (q, k, v, dout, out, lse, dq, dk, dv, seq_offsets)], 0, 0, *dims,
         *[x for t in (q, k, v, dout, out, dq, dk, dv) for x in _htd(t)],
-        _f32(1.0 / (dims[4] ** 0.5) if scale is None else scale), 1 if causal else 0, dtype_code(q.dtype), 0))
+        _f32(1.0 / (dims[4] ** 0.5) if scale is None else scale), 1 if causal else 0, dtype_code(q.dtype), zero_rest))
 
 
 def sdpa_packed_bwd(q, k, v, dout, out, lse, seq_offsets, *, scale=None, causal=True, dq=None, dk=None, dv=None,
                     workspace=None):
     """(dq, dk, dv) of sdpa_packed for the gradient dout of its output, from
-    its out and lse (mfx_sdpa_packed_bwd).  Rows in no sequence are not
-    written."""
+    its out and lse (mfx_sdpa_packed_bwd).  Rows in no sequence are zeros in
+    the gradients made here; given ones keep their own there (which a sum over
+    every row, as qk_norm_rope_bwd's for its weights, takes in)."""
+    made = (1 if dq is None else 0) | (2 if dk is None else 0) | (4 if dv is None else 0)
     dq, dk, dv = (_fresh(t) if g is None else g for t, g in ((q, dq), (k, dk), (v, dv)))
-    a = sdpa_packed_bwd_args(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, scale=scale, causal=causal)
+    a = sdpa_packed_bwd_args(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, scale=scale, causal=causal,
+                             zero_rest=made)
     with _on(q, k, v, dout, out, lse, dq, dk, dv, seq_offsets, workspace):
         keep = _workspace(a, "mfx_sdpa_packed_bwd_workspace_size", workspace, q)  # noqa: F841 (until the launch)
         check(load().mfx_sdpa_packed_bwd(ctypes.byref(a), _stream_handle(q)))
