@@ -149,7 +149,6 @@ __device__ __forceinline__ void load_frags(const bf16* base, int64_t stride, int
 // and the wavefront with the most visible blocks sets the pace anyway.
 constexpr int kKvPf = 2;   // operand reads issued ahead of their MFMAs
 constexpr int kKvStages = 3;
-constexpr int kPartTiles = 8;  // packed: blocks of so many tiles have one share
 constexpr int kDkdvHeadGroup = 2;  // kv heads whose key blocks an XCD runs together
 
 // Four f32, written through to where every XCD sees them and read from there

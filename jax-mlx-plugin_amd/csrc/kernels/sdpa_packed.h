@@ -35,6 +35,7 @@ namespace mfx {
 
 constexpr int kCus = 256;
 constexpr int kLaneSeqs = 8;  // sequences a lane holds: 512 in all
+constexpr int kPartTiles = 8;  // blocks of so many tiles have one share
 
 struct PackedBlock {
   int start, len;  // the sequence's first token and its length

@@ -115,13 +115,17 @@ struct BwdPlan {
   size_t q_pad = 0, kv_pad = 0;    // bytes of one
 };
 
-// Shares of a head's `slots` blocks, `room` of which run at a time: some while
-// there are no more than kPartBlocks blocks, up to kMaxParts ways.
-void plan_shares(PackedShares& sh, int64_t slots, int heads, int room, size_t block_bytes, BwdPlan& pl) {
+// Shares of a head's `slots` blocks, `room` of which run at a time and which
+// walk `tiles` more from one to the next: some while there are no more than
+// kPartBlocks blocks, up to kMaxParts ways, and if any block can have them (their
+// sums are two or more blocks a head: 268 MB for 100 tokens of 1024 heads).
+void plan_shares(PackedShares& sh, int64_t slots, int heads, int room, int64_t tiles, size_t block_bytes, BwdPlan& pl) {
   const int64_t blocks = slots * heads;
   if (blocks > kPartBlocks) return;
+  const int quarters = blocks <= 2 * kCus ? 3 : 4;
+  if (!packed_shares_possible(pl.p.total, kBwdBlock, heads, quarters, room, tiles, kPartTiles)) return;
   sh.parts = (int)std::min<int64_t>(kMaxParts, kPartBlocks / blocks + 1);
-  sh.quarters = blocks <= 2 * kCus ? 3 : 4;
+  sh.quarters = quarters;
   // A block in k shares walks more than (k - 1) `most`, and all of a head
   // no more than `all`: so many blocks are shared at most, and so many
   // shares added.  (Of offsets that are no offsets there may be more
@@ -215,14 +219,14 @@ int plan_bwd(const mfx_sdpa_packed_bwd_args* a, BwdPlan& pl) {
     // in 8 of 96 .. 2500: 622, 614, and 607 in shares of one part).
     const int64_t slots = packed_slots(p.total, p.num_seqs, kBwdBlock);
     const size_t block_bytes = (size_t)kBwdBlock * (pl.dp ? pl.dp : p.D) * sizeof(float);
-    plan_shares(p.key_shares, slots, p.Hkv, kCus, 2 * block_bytes, pl);
+    plan_shares(p.key_shares, slots, p.Hkv, kCus, 2 * (int64_t)p.group, 2 * block_bytes, pl);
     // dQ: blocks of queries, of which two run on a CU; counts that nothing before
     // it clears cost a launch, 2 to 4 us.  (Whole backward, shares of queries and
     // none: 8192 tokens, 4 heads on 1, 457 and 524 us; 12289 in 2 heads, 420 and
     // 564; 1500 + 700, 4 heads, 86 and 100.  But 8192, 8 on 2, 698 and 686; four
     // of 512, 8 heads, 55 and 51.)
     if (p.total > 2048 && slots * p.Hq <= 2 * kCus)
-      plan_shares(p.query_shares, slots, p.Hq, 2 * kCus, block_bytes, pl);
+      plan_shares(p.query_shares, slots, p.Hq, 2 * kCus, 2, block_bytes, pl);
   }
   return MFX_OK;
 }
