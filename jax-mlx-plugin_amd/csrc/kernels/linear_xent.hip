@@ -426,17 +426,17 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void xent_grad_kernel(StoreArgs p)
 template <typename T>
 __global__ __launch_bounds__(256) void xent_sum(const float* __restrict__ part, int splits, int64_t M, int N, T* c,
                                                 int64_t ldc, const float* scale) {
-  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (q >= M * N / 4) return;
-  const int64_t e = q * 4, m = e / N, n = e % N;
-  f32x4 v = *reinterpret_cast<const f32x4*>(part + e);
-  for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(part + s * M * N + e);
-  const float mul = scale ? *scale : 1.f;
-  typedef T t4 __attribute__((ext_vector_type(4)));
-  t4 o;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < M * N / 4; q += (int64_t)gridDim.x * 256) {
+    const int64_t e = q * 4, m = e / N, n = e % N;
+    f32x4 v = *reinterpret_cast<const f32x4*>(part + e);
+    for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(part + s * M * N + e);
+    const float mul = scale ? *scale : 1.f;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 o;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) o[j] = from_f32<T>(v[j] * mul);
-  *reinterpret_cast<t4*>(c + m * ldc + n) = o;
+    for (int j = 0; j < 4; ++j) o[j] = from_f32<T>(v[j] * mul);
+    *reinterpret_cast<t4*>(c + m * ldc + n) = o;
+  }
 }
 
 // ---- host ----------------------------------------------------------------------
@@ -448,6 +448,10 @@ constexpr int64_t kMaxStride = int64_t(1) << 21;  // a tile's 256 rows are addre
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Workgroups of 256 for `n` threads' work; the kernel's threads go on in
+// strides of the grid past 2^28 (a launch holds fewer than 2^32).
+dim3 strided_grid(int64_t n) { return dim3((unsigned)std::min<int64_t>(ceil_div(n, 256), 1 << 20)); }
 
 // A product's tile form and, for a gradient's, its ranges of k.
 struct Way {
@@ -583,7 +587,7 @@ int launch_grad(StoreArgs& p, const Way& way, hipStream_t s) {
 
 int launch_sum(const float* part, int64_t splits, int64_t M, int64_t N, void* c, int64_t ldc, int dtype,
                const float* scale, hipStream_t s) {
-  const dim3 grid((unsigned)ceil_div(M * N / 4, 256));
+  const dim3 grid = strided_grid(M * N / 4);
   const int n = (int)splits, w = (int)N;
   if (dtype == MFX_F32)
     hipLaunchKernelGGL((xent_sum<float>), grid, dim3(256), 0, s, part, n, M, w, static_cast<float*>(c), ldc, scale);
@@ -740,8 +744,8 @@ int take_workspace(void* given, size_t given_bytes, size_t need, const char* que
 // dw of no rows.
 template <typename T>
 __global__ __launch_bounds__(256) void xent_zero(T* c, int64_t rows, int64_t n, int64_t ldc) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < rows * n) c[i / n * ldc + i % n] = from_f32<T>(0.f);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * n; i += (int64_t)gridDim.x * 256)
+    c[i / n * ldc + i % n] = from_f32<T>(0.f);
 }
 
 }  // namespace
@@ -802,7 +806,7 @@ int mfx_linear_xent_bwd(const mfx_linear_xent_bwd_args* args, void* stream) {
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a.T == 0) {
     if (!a.dw) return MFX_OK;
-    const dim3 grid((unsigned)ceil_div(a.V * a.H, 256));
+    const dim3 grid = strided_grid(a.V * a.H);
     if (a.dw_dtype == MFX_F32)
       hipLaunchKernelGGL((xent_zero<float>), grid, dim3(256), 0, s, static_cast<float*>(a.dw), a.V, a.H, a.dw_stride);
     else  // (zero has the same bits in both 16-bit types)

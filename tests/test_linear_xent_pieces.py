@@ -117,3 +117,43 @@ def test_bounds_catch(name):
     short = dw - (grads(torch.where(torch.arange(T) >= T - 64, dloss, 0.0) + 1e-30)[1])
     assert bad(dh, short)[1] > 0.05
     assert bad((dh.double() - dh.double() * 0.05).to(dh.dtype), dw)[0] > 0.5
+
+
+@pytest.mark.gpu
+def test_no_rows_of_many_weights(cuda):
+    """2^32 weights: as many threads as one launch cannot hold."""
+    torch = cuda
+    from jax_mlx_amd import native as nat
+
+    w = torch.empty(1 << 18, 1 << 14, device="cuda", dtype=torch.bfloat16)
+    z, t = torch.empty(0, device="cuda"), torch.empty(0, device="cuda", dtype=torch.int64)
+    dw = torch.ones_like(w)
+    nat.linear_xent_bwd(w[:0], w, t, z, z, need_dh=False, dw=dw)
+    assert not dw.any()
+
+
+@pytest.mark.gpu
+def test_sums_of_more_entries_than_a_grid(cuda):
+    """dh of 2^31 entries, added over pieces: the last sum's threads take
+    several each.  Rows apart have the gradients of their own, so some are
+    compared."""
+    torch = cuda
+    from jax_mlx_amd import native as nat
+
+    T, H, V = (1 << 19) + 3, 4096, 700
+    g = torch.Generator("cuda").manual_seed(8)
+    w = (torch.randn(V, H, device="cuda", generator=g) * H ** -0.5).to(torch.bfloat16)
+    h = torch.empty(T, H, device="cuda", dtype=torch.bfloat16)
+    for a in range(0, T, 1 << 16):
+        h[a:a + (1 << 16)] = torch.randn(min(1 << 16, T - a), H, device="cuda", generator=g)
+    t = torch.randint(0, V, (T,), device="cuda", generator=g)
+    dloss = torch.rand(T, device="cuda", generator=g)
+    assert T * 256 * 2 <= 512 << 20 < T * V * 2
+    _, lse = nat.linear_xent(h, w, t)
+    dh = torch.full_like(h, float("nan"))
+    nat.linear_xent_bwd(h, w, t, lse, dloss, need_dw=False, dh=dh)
+    assert dh.isfinite().all()
+    for a in (0, 70000, 262143, 400000, T - 200):
+        s = slice(a, a + 200)
+        ref, bound, _, _ = bounds(torch, "bf16", h[s], w, t[s], dloss[s])
+        assert not out_of_bounds(torch, "bf16", dh[s], ref, bound).any(), a
