@@ -29,6 +29,10 @@ inline int launch_status(const char* what) {
   return MFX_OK;
 }
 
+// A launch holds fewer than 2^32 threads; HIP refuses more, but with an error of
+// its own and after what was launched before.
+inline bool launch_fits(int64_t blocks, int threads) { return blocks * threads <= 0xffffffffLL; }
+
 inline int dtype_size(int dt) {
   switch (dt) {
     case MFX_F32: return 4;

@@ -508,6 +508,7 @@ Way choose(int E, int64_t M, int64_t N, int64_t K, bool split) {
     const int64_t tiles = ceil_div(M, kFormM[f]) * ceil_div(N, kFormN[E == 2][f]);
     for (int64_t s = 1; s <= (split ? std::min<int64_t>(32, std::max<int64_t>(1, kt / 8)) : 1); ++s) {
       const int64_t range = ceil_div(kt, s), ranges = ceil_div(kt, range);
+      if (!launch_fits(tiles * ranges, 256)) continue;
       float t = way_us(c, tiles * ranges, range, cus);
       if (ranges > 1) t += 4.f + (float)ranges * (float)M * (float)N * 8.f / 4e6f;
       if (t < least) {
@@ -685,8 +686,11 @@ int check_common(int64_t T, int64_t H, int64_t V, int dtype, int target_dtype) {
   if (target_dtype != MFX_I32 && target_dtype != MFX_I64)
     return fail(MFX_E_UNSUPPORTED, "target dtype must be i32 or i64");
   if (T > lim - 256 || V > lim - 256 || H > lim - 256) return fail(MFX_E_UNSUPPORTED, "T, H or V too large");
-  if (ceil_div(T, 64) * ceil_div(V, 64) > lim || ceil_div(T, 64) * ceil_div(H, 64) > lim / 32 ||
-      ceil_div(V, 64) * ceil_div(H, 64) > lim / 32)
+  // (The widest tiles' launches have to fit; `choose` passes over others that do not.)
+  const int64_t b = kFormM[first_form(elem_of(dtype))];
+  const int64_t t = ceil_div(T, b), v = ceil_div(V, b), k = ceil_div(H, b);
+  if (!launch_fits(t * v, 256) || !launch_fits(t * k, 256) || !launch_fits(v * k, 256) ||
+      !launch_fits(ceil_div(T, 64), 64 * kCombine))
     return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
   if (H % (dtype == MFX_F32 ? 4 : 8))
     return fail(MFX_E_UNSUPPORTED, "H must be a multiple of 16 bytes");

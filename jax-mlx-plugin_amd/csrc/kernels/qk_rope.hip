@@ -588,6 +588,7 @@ int plan_fwd(const mfx_qk_norm_rope_args* a, Plan& pl) {
   if (rc) return rc;
   if (p.tokens == 0) return MFX_OK;
   const int64_t blocks = ((int64_t)p.tokens + kWaves - 1) / kWaves;
+  if (!launch_fits(blocks, kBlock)) return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
   split_heads(pl, p.tokens);
   pl.grid = dim3((unsigned)blocks, (unsigned)(q.parts + k.parts));
   return MFX_OK;

@@ -64,6 +64,17 @@ int check_common(const Args* a) {
   return MFX_OK;
 }
 
+// Whether the launches of a call fit: a wavefront a row, or workgroups of 256
+// threads for blocks of 128 rows (the f32 ones of 64 threads for 32 rows have no
+// more threads, and shares are only added to few blocks).
+template <class Params>
+int check_launch(const Params& p, Kind kind) {
+  const int64_t rows = (int64_t)p.Hq * p.total;
+  const bool fits = kind == Kind::kGeneric ? launch_fits((rows + 3) / 4, 256)
+                                           : launch_fits(packed_slots(p.total, p.num_seqs, 128) * p.Hq, 256);
+  return fits ? MFX_OK : fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
+}
+
 int plan_fwd(const mfx_sdpa_packed_args* a, SdpaParams& p, Kind& kind) {
   if (!a) return fail(MFX_E_INVALID, "null args");
   if (int rc = check_common(a)) return rc;
@@ -103,7 +114,7 @@ int plan_fwd(const mfx_sdpa_packed_args* a, SdpaParams& p, Kind& kind) {
   kind = p.D != 256 && flash_bf16_supports(p) ? Kind::kFlash16
          : flash_f32_supports(p)              ? Kind::kFlashF32
                                               : Kind::kGeneric;
-  return MFX_OK;
+  return check_launch(p, kind);
 }
 
 struct BwdPlan {
@@ -208,6 +219,7 @@ int plan_bwd(const mfx_sdpa_packed_bwd_args* a, BwdPlan& pl) {
       pl.kv_pad = align256((size_t)p.Hkv * p.total * dp * 2);
     }
   }
+  if (int rc = check_launch(p, pl.kind)) return rc;
   if ((pl.kind == Kind::kMfma16 || pl.kind == Kind::kPadded16) && p.causal && p.num_seqs <= 64 * kLaneSeqs) {
     // dK, dV: a key block walks all queries behind it for every head of its group, and
     // the longest ones alone can last longer than a CU's part of the whole
