@@ -298,7 +298,8 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) void bwd_f32_dq_kernel(Sd
     const PackedRest rest(p.seq_off, p.num_seqs, p.total);
     packed_head(blockIdx.x, p.Hq, gridDim.x / p.Hq, bh, slot);
     const bool any = packed_block<32 * NW>(p.seq_off, p.num_seqs, p.total, slot, pb);
-    if (p.zero_rest & 1) packed_zero_rest<4, 64 * NW>(rest, p.dq, p.dqs, p.Hq, D);
+    if (packed_rest_here() && (p.zero_rest & 1))
+      packed_zero_rest<4, 64 * NW>(rest, p.dq, p.dqs, p.Hq, D);
     if (!any) return;
     blk = pb.work;
     packed_shift<4>(p, pb.start, pb.len);
@@ -408,8 +409,10 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) void bwd_f32_dkdv_kernel(
     const PackedRest rest(p.seq_off, p.num_seqs, p.total);
     packed_head(blockIdx.x, p.Hkv, gridDim.x / p.Hkv, bhk, slot);
     const bool any = packed_block<32 * NW>(p.seq_off, p.num_seqs, p.total, slot, pb);
-    if (p.zero_rest & 2) packed_zero_rest<4, 64 * NW>(rest, p.dk, p.dks, p.Hkv, D);
-    if (p.zero_rest & 4) packed_zero_rest<4, 64 * NW>(rest, p.dv, p.dvs, p.Hkv, D);
+    if (packed_rest_here()) {
+      if (p.zero_rest & 2) packed_zero_rest<4, 64 * NW>(rest, p.dk, p.dks, p.Hkv, D);
+      if (p.zero_rest & 4) packed_zero_rest<4, 64 * NW>(rest, p.dv, p.dvs, p.Hkv, D);
+    }
     if (!any) return;
     blk = pb.nb - 1 - pb.work;
     packed_shift<4>(p, pb.start, pb.len);

@@ -286,8 +286,10 @@ __global__ __launch_bounds__(kNT, 1) void bwd_dkdv_mfma(SdpaBwdParams p) {
       nparts = ps.parts;
     }
     const bool any = packed_block<kRows>(p.seq_off, p.num_seqs, p.total, slot, pb);
-    if (p.zero_rest & 2) packed_zero_rest<2, kNT>(rest, p.dk, p.dks, p.Hkv, D);
-    if (p.zero_rest & 4) packed_zero_rest<2, kNT>(rest, p.dv, p.dvs, p.Hkv, D);
+    if (packed_rest_here()) {
+      if (p.zero_rest & 2) packed_zero_rest<2, kNT>(rest, p.dk, p.dks, p.Hkv, D);
+      if (p.zero_rest & 4) packed_zero_rest<2, kNT>(rest, p.dv, p.dvs, p.Hkv, D);
+    }
     if (!any) return;
     kblk = pb.nb - 1 - pb.work;
     packed_shift<2>(p, pb.start, pb.len);
@@ -733,7 +735,8 @@ __global__ __launch_bounds__(kNT, D == 128 && MASKT != 0 && MASKT != kAnyMask ? 
       nparts = ps.parts;
     }
     const bool any = packed_block<kRows>(p.seq_off, p.num_seqs, p.total, slot, pb);
-    if (p.zero_rest & 1) packed_zero_rest<2, kNT>(rest, p.dq, p.dqs, p.Hq, D);
+    if (packed_rest_here() && (p.zero_rest & 1))
+      packed_zero_rest<2, kNT>(rest, p.dq, p.dqs, p.Hq, D);
     if (!any) return;
     mblk = pb.work;
     packed_shift<2>(p, pb.start, pb.len);

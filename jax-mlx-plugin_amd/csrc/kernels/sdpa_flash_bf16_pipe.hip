@@ -246,7 +246,8 @@ __global__ __launch_bounds__(kNT, 2) void flash_bf16_pipe_kernel(SdpaParams p) {
     const PackedRest rest(p.seq_off, p.num_seqs, p.total);
     packed_head(id, BH, gridDim.x / BH, bh, slot);
     const bool any = packed_block<kBM>(p.seq_off, p.num_seqs, p.total, slot, pb);
-    if (p.zero_rest) packed_zero_rest<2, kNT>(rest, p.out, p.os, p.Hq, p.Dv);
+    if (packed_rest_here() && p.zero_rest)
+      packed_zero_rest<2, kNT>(rest, p.out, p.os, p.Hq, p.Dv);
     if (!any) return;
     mblk = pb.work;
     packed_shift<2>(p, pb.start, pb.len);

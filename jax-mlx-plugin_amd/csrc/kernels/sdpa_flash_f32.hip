@@ -79,7 +79,8 @@ __global__ __launch_bounds__(kNT, (D >= 256 || (D >= 96 && MASK)) ? 1 : 2) void 
     const PackedRest rest(p.seq_off, p.num_seqs, p.total);
     packed_head(id, BH, gridDim.x / BH, bh, slot);
     const bool any = packed_block<kBM>(p.seq_off, p.num_seqs, p.total, slot, pb);
-    if (p.zero_rest) packed_zero_rest<4, kNT>(rest, p.out, p.os, p.Hq, D);
+    if (packed_rest_here() && p.zero_rest)
+      packed_zero_rest<4, kNT>(rest, p.out, p.os, p.Hq, D);
     if (!any) return;
     mblk = pb.work;
     packed_shift<4>(p, pb.start, pb.len);
@@ -337,7 +338,8 @@ __global__ __launch_bounds__(64 * kSW) void flash_f32_split_kernel(SdpaParams p)
     const PackedRest rest(p.seq_off, p.num_seqs, p.total);
     packed_head(blockIdx.x, p.Hq, gridDim.x / p.Hq, bh, slot);
     const bool any = packed_block<32>(p.seq_off, p.num_seqs, p.total, slot, pb);
-    if (p.zero_rest) packed_zero_rest<4, 64 * kSW>(rest, p.out, p.os, p.Hq, D);
+    if (packed_rest_here() && p.zero_rest)
+      packed_zero_rest<4, 64 * kSW>(rest, p.out, p.os, p.Hq, D);
     if (!any) return;
     mblk = pb.work;
     packed_shift<4>(p, pb.start, pb.len);

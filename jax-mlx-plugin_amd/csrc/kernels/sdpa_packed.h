@@ -217,16 +217,23 @@ struct PackedRest {
   __device__ __forceinline__ PackedRest(int t) : first(0), last(0), total(t) {}  // no sequences
 };
 
-// Zeros in those rows of a [heads, total, D] tensor, shared out over the
-// grid's workgroups of NT threads, a row a wavefront.  (The products and sums
-// that take the tensor next go over every row.)
+// The last workgroups of a grid zero those rows: their blocks are the shortest,
+// or they have none, and the others need not wait for what to do (4 us of a
+// 500 us backward, in which every workgroup asked).
+constexpr uint32_t kRestGroups = 2 * kCus;
+__device__ __forceinline__ bool packed_rest_here() { return blockIdx.x + kRestGroups >= gridDim.x; }
+
+// Zeros in those rows of a [heads, total, D] tensor, shared out over these
+// workgroups of NT threads, a row a wavefront.  (The products and sums that
+// take the tensor next go over every row.)
 template <int SIZE, int NT>
 __device__ __forceinline__ void packed_zero_rest(const PackedRest& rest, void* out, const int64_t (&st)[4], int heads,
                                                  int D) {
   const int total = rest.total, first = min(max(rest.first, 0), total), last = max(min(rest.last, total), first);
   // (Fewer than 2^31 rows, and 2^32 threads in the grid: checked on the host.)
   const uint32_t rows = (uint32_t)(first + total - last) * (uint32_t)heads;
-  for (uint32_t r = blockIdx.x * (NT / 64) + (threadIdx.x >> 6); r < rows; r += gridDim.x * (NT / 64)) {
+  const uint32_t groups = min((uint32_t)gridDim.x, kRestGroups), group = blockIdx.x + groups - gridDim.x;
+  for (uint32_t r = group * (NT / 64) + (threadIdx.x >> 6); r < rows; r += groups * (NT / 64)) {
     int t = (int)(r / (uint32_t)heads);
     const int h = (int)(r - (uint32_t)t * (uint32_t)heads);
     if (t >= first) t += last - first;

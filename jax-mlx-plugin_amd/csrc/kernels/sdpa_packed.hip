@@ -32,7 +32,7 @@ __global__ __launch_bounds__(256) void packed_zero_all(void* out, int64_t s1, in
 int zero_all(void* out, const int64_t* st, int64_t T, int64_t heads, int64_t D, int dtype, hipStream_t s) {
   if (!out) return fail(MFX_E_INVALID, "outputs must be non-null");
   if (st[2] != 1) return fail(MFX_E_INVALID, "feature (last) strides must be 1");
-  const dim3 grid((unsigned)std::min<int64_t>((T * heads + 3) / 4, 4096));
+  const dim3 grid((unsigned)std::min<int64_t>((T * heads + 3) / 4, kRestGroups));
   if (dtype == MFX_F32)
     hipLaunchKernelGGL(packed_zero_all<4>, grid, dim3(256), 0, s, out, st[0], st[1], (int)T, (int)heads, (int)D);
   else
