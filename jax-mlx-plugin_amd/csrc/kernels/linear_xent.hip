@@ -24,15 +24,16 @@
 // p - 1 then, which for an unlikely target rounds to -1 almost exactly, where
 // (p - 1) dloss would carry dloss's own rounding into every row alike
 // (8192 x 4096 x 65537: dh and dW off by 0.0028 of their size with it, 0.0019
-// without, 0.0017 of which is their own rounding).  f16 holds it times 2^15
+// without, 0.0017 of which is their own rounding; an f32 dW by 0.0010).  Two
+// terms of d would take that away for twice the products of dh and dW.  f16 holds it times 2^15
 // besides, or entries below 2^-24 would be lost.
 //
 // What bounds it: the matrix cores, 2 T H V flops a product, one product
-// forward and three backward.  bf16, T 8192, H 4096, V 65537: forward 3.5 ms (1.24
-// PFLOP/s, matrix cores 71% busy), backward 10.5 ms (1.25; logits 63%, dW 66%, dh
+// forward and three backward.  bf16, T 8192, H 4096, V 65537: forward 3.6 ms (1.22
+// PFLOP/s, matrix cores 71% busy), backward 11.0 ms (1.20; logits 63%, dW 66%, dh
 // 73%); a library product of these sizes runs at 1.25 - 1.58 beside them, by the
-// clock.  T 4096, H 2048, V 32000: 0.46 and 1.36 ms (1.17, 1.19).  Few rows
-// (T 33) read W once: 132 us for 537 MB, 4.1 TB/s.
+// clock.  T 4096, H 2048, V 32000: 0.47 and 1.41 ms (1.13, 1.14).  Few rows
+// (T 33) read W once: 131 us for 537 MB, 4.1 TB/s.
 #include <algorithm>
 #include <cmath>
 #include <string>

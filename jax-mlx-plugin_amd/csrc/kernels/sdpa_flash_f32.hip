@@ -547,9 +547,15 @@ int launch_t(const SdpaParams& p, hipStream_t s) {
 }
 
 // Packed, the key-split variant where the 128-row workgroups number fewer than
-// two per CU, as above; a wavefront's tiles are known for the mean sequence
-// only.  (Six sequences of 1 to 128 tokens, 8 heads of 64: 16 us on the
-// 128-row kernel, 9 on this.)
+// two per CU, as above, and the mean sequence (empty ones counted) is 1024
+// tokens or less: the host does not know the longest, nor need it, for a few long
+// sequences leave the 128-row kernel most CUs idle.  128-row kernel and this (us): six
+// of 1 to 128 tokens, 8 heads of 64, 16 and 9; 4096 tokens beside three empty
+// sequences 304 and 166, 8 heads on 2 of 128 556 and 307; 2000 + 16 of 8, 274 and 95.
+// Many short sequences near two workgroups a CU are the worst for it: 30 of 64,
+// 8 on 2 of 128, 17.5 and 22.6; 20 of 100, 28 and 32.  (A mean past 1024 keeps
+// the 128-row kernel, the unpacked rule, though 4096 tokens alone take what they
+// take beside empty sequences.)
 bool packed_use_split(const SdpaParams& p) {
   for (int64_t st : {p.qs[2], p.ks[2], p.vs[2]})
     if (st < p.D || st >= (int64_t(1) << 24)) return false;

@@ -20,7 +20,10 @@
 // cycles), some 8 steps.  Past kLaneSeqs sequences a lane's share no longer
 // fits registers, and slots go to sequences in order: sequence s owns the slots
 // from (off[s] - off[0]) / BM + s, which are enough for it and need no count
-// of the blocks before (empty sequences own one too).
+// of the blocks before (empty sequences own one too).  What the order is worth
+// there is less than what it costs to find: one sequence of 4096 tokens and 511 of
+// 8, 32 heads on 8 of 128, forward 355 us and backward 1033, with 512 of 8 295
+// and 941; one of 8192 and 500 of 4 707 and 2392, 520 of 4 653 and 2320.
 //
 // Offsets are taken as they come: each is clamped to 0 .. T and a sequence that
 // would end before it starts is empty, so no offsets lead outside the tensors.
@@ -33,7 +36,7 @@
 
 namespace mfx {
 
-constexpr int kCus = 256;
+constexpr int kCus = 256;  // of the whole MI355X (a partition with fewer is only shared out finer than it needs)
 constexpr int kLaneSeqs = 8;  // sequences a lane holds: 512 in all
 constexpr int kPartTiles = 8;  // blocks of so many tiles have one share
 

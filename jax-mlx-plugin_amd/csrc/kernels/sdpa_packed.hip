@@ -5,9 +5,15 @@
 //
 // What bounds them is what bounds those: the matrix cores and the vector work
 // between their products.  bf16, 32 heads on 8, D 128, causal: 16 sequences of 1
-// .. 4096 tokens 340 - 365 us (0.84 - 0.90 PFLOP/s of visible pairs), 4095 + 12289
-// 1.22 - 1.42 ms (1.1 to 0.97 PFLOP/s, by the clock); eight of 96 .. 2500 forward
-// 145, dQ 204, dK / dV 348 us (378 before the longest key blocks were shared).
+// .. 4096 tokens 330 - 365 us (0.83 - 0.92 PFLOP/s of visible pairs), 4095 + 12289
+// 1.23 - 1.42 ms (1.1 to 0.97 PFLOP/s, by the clock); eight of 96 .. 2500 forward
+// 146, dQ 207, dK / dV 357 us (in shares of the longest key blocks; whole 7% more).
+//
+// Roundings.  P, and in the backward dS, meet the matrix cores in the inputs'
+// type, as in the unpacked kernels; sums, the softmax and delta are fp32.  Of
+// the outputs' size (bf16, against 64 bits, their own rounding 0.0016): out off by
+// 0.0020, dq and dk by 0.0025.  Second terms of P or dS would cost a product each
+// of the two forward and seven backward.
 #include <algorithm>
 #include <cmath>
 
