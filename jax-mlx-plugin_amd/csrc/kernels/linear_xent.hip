@@ -25,8 +25,8 @@
 // (p - 1) dloss would carry dloss's own rounding into every row alike
 // (8192 x 4096 x 65537: dh and dW off by 0.0028 of their size with it, 0.0019
 // without, 0.0017 of which is their own rounding; an f32 dW by 0.0010).  Two
-// terms of d would take that away for twice the products of dh and dW.  f16 holds it times 2^15
-// besides, or entries below 2^-24 would be lost.
+// terms of d would take that away for twice the products of dh and dW.  f16
+// holds d times 2^15 besides, or entries below 2^-24 would be lost.
 //
 // What bounds it: the matrix cores, 2 T H V flops a product, one product
 // forward and three backward.  bf16, T 8192, H 4096, V 65537: forward 3.6 ms (1.22

@@ -247,7 +247,7 @@ __global__ __launch_bounds__(kNT, 2) void flash_bf16_pipe_kernel(SdpaParams p) {
     packed_head(id, BH, gridDim.x / BH, bh, slot);
     const bool any = packed_block<kBM>(p.seq_off, p.num_seqs, p.total, slot, pb);
     if (packed_rest_here() && p.zero_rest)
-      packed_zero_rest<2, kNT>(rest, p.out, p.os, p.Hq, p.Dv);
+      packed_zero_rest<2, kNT>(rest, p.out, p.os, p.Hq, DV);
     if (!any) return;
     mblk = pb.work;
     packed_shift<2>(p, pb.start, pb.len);

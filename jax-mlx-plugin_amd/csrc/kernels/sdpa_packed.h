@@ -217,7 +217,6 @@ __device__ __forceinline__ bool packed_seq(const int32_t* off, int n, int total,
 struct PackedRest {
   int first, last, total;
   __device__ __forceinline__ PackedRest(const int32_t* off, int n, int t) : first(off[0]), last(off[n]), total(t) {}
-  __device__ __forceinline__ PackedRest(int t) : first(0), last(0), total(t) {}  // no sequences
 };
 
 // The last workgroups of a grid zero those rows: their blocks are the shortest,
@@ -226,22 +225,26 @@ struct PackedRest {
 constexpr uint32_t kRestGroups = 2 * kCus;
 __device__ __forceinline__ bool packed_rest_here() { return blockIdx.x + kRestGroups >= gridDim.x; }
 
-// Zeros in those rows of a [heads, total, D] tensor, shared out over these
-// workgroups of NT threads, a row a wavefront.  (The products and sums that
-// take the tensor next go over every row.)
+// Zeros in those rows of a [heads, total, D] tensor of whole, aligned 16-byte
+// chunks, shared out over these workgroups of NT threads; up to 64 chunks a row.
+// (The products and sums that take the tensor next go over every row.)
 template <int SIZE, int NT>
 __device__ __forceinline__ void packed_zero_rest(const PackedRest& rest, void* out, const int64_t (&st)[4], int heads,
                                                  int D) {
   const int total = rest.total, first = min(max(rest.first, 0), total), last = max(min(rest.last, total), first);
   // (Fewer than 2^31 rows, and 2^32 threads in the grid: checked on the host.)
   const uint32_t rows = (uint32_t)(first + total - last) * (uint32_t)heads;
+  if (rows == 0) return;
   const uint32_t groups = min((uint32_t)gridDim.x, kRestGroups), group = blockIdx.x + groups - gridDim.x;
-  for (uint32_t r = group * (NT / 64) + (threadIdx.x >> 6); r < rows; r += groups * (NT / 64)) {
+  const uint32_t chunks = D * SIZE / 16, per = NT / chunks;  // of a row; rows a workgroup takes at a time
+  const uint32_t mine = threadIdx.x / chunks, chunk = threadIdx.x - mine * chunks;
+  if (mine >= per) return;
+  for (uint32_t r = group * per + mine; r < rows; r += groups * per) {
     int t = (int)(r / (uint32_t)heads);
     const int h = (int)(r - (uint32_t)t * (uint32_t)heads);
     if (t >= first) t += last - first;
-    auto* row = static_cast<std::conditional_t<SIZE == 2, uint16_t, uint32_t>*>(out) + h * st[1] + t * st[2];
-    for (int d = threadIdx.x & 63; d < D; d += 64) row[d] = 0;
+    char* const row = static_cast<char*>(out) + (h * st[1] + t * st[2]) * SIZE;
+    *reinterpret_cast<u32x4*>(row + chunk * 16) = u32x4{0, 0, 0, 0};
   }
 }
 

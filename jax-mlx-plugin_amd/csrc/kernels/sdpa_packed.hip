@@ -12,8 +12,8 @@
 // Roundings.  P, and in the backward dS, meet the matrix cores in the inputs'
 // type, as in the unpacked kernels; sums, the softmax and delta are fp32.  Of
 // the outputs' size (bf16, against 64 bits, their own rounding 0.0016): out off by
-// 0.0020, dq and dk by 0.0025.  Second terms of P or dS would cost a product each
-// of the two forward and seven backward.
+// 0.0020, dq and dk by 0.0025.  A second term of P or dS would cost another product
+// beside the forward's two, or two beside the backward's seven.
 #include <algorithm>
 #include <cmath>
 
@@ -29,20 +29,23 @@ enum class Kind { kNone, kFlash16, kFlashF32, kMfma16, kMfmaF32, kPadded16, kGen
 constexpr int kPartBlocks = 4 * kCus, kMaxParts = 8;
 
 // Zeros in all of a [heads, T, D] tensor: a call without sequences.
-template <int SIZE>
-__global__ __launch_bounds__(256) void packed_zero_all(void* out, int64_t s1, int64_t s2, int T, int heads, int D) {
+template <typename T>
+__global__ __launch_bounds__(256) void packed_zero_all(void* out, int64_t s1, int64_t s2, int64_t rows, int heads,
+                                                       int D) {
   const int64_t st[4] = {0, s1, s2, 1};
-  packed_zero_rest<SIZE, 256>(PackedRest(T), out, st, heads, D);
+  for (int64_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.x * 4)
+    packed_zero_row<T>(out, st, (int)(r % heads), (int)(r / heads), D);
 }
 
 int zero_all(void* out, const int64_t* st, int64_t T, int64_t heads, int64_t D, int dtype, hipStream_t s) {
   if (!out) return fail(MFX_E_INVALID, "outputs must be non-null");
   if (st[2] != 1) return fail(MFX_E_INVALID, "feature (last) strides must be 1");
-  const dim3 grid((unsigned)std::min<int64_t>((T * heads + 3) / 4, kRestGroups));
+  const int64_t rows = T * heads;
+  const dim3 grid((unsigned)std::min<int64_t>((rows + 3) / 4, 4096));
   if (dtype == MFX_F32)
-    hipLaunchKernelGGL(packed_zero_all<4>, grid, dim3(256), 0, s, out, st[0], st[1], (int)T, (int)heads, (int)D);
-  else
-    hipLaunchKernelGGL(packed_zero_all<2>, grid, dim3(256), 0, s, out, st[0], st[1], (int)T, (int)heads, (int)D);
+    hipLaunchKernelGGL(packed_zero_all<float>, grid, dim3(256), 0, s, out, st[0], st[1], rows, (int)heads, (int)D);
+  else  // (zero has the same bits in both 16-bit types)
+    hipLaunchKernelGGL(packed_zero_all<bf16>, grid, dim3(256), 0, s, out, st[0], st[1], rows, (int)heads, (int)D);
   return launch_status("packed_zero_all");
 }
 
