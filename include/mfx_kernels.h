@@ -797,6 +797,62 @@ int mfx_linear_xent_bwd(const mfx_linear_xent_bwd_args* args, void* stream);
 
 size_t mfx_linear_xent_bwd_workspace_size(const mfx_linear_xent_bwd_args* args);
 
+/*
+ * Embedding lookup with scaling:
+ *   out[t] = scale * w[ids[t]],   zeros for an id outside [0, V)
+ * w [V, H] of `dtype`, out [T, H] of `out_dtype` (each f32, bf16 or f16; fp32
+ * arithmetic, one rounding), rows spaced w_stride / out_stride elements, any
+ * alignment; ids int32 or int64 (ids_dtype MFX_I32 / MFX_I64), contiguous.
+ * No counterpart in the reference, whose models take embedded inputs.
+ */
+typedef struct {
+  const void* w;
+  const void* ids;
+  void* out;
+  int64_t T, H, V;
+  int64_t w_stride;
+  int64_t out_stride;
+  float scale;
+  int32_t dtype;
+  int32_t out_dtype;
+  int32_t ids_dtype;
+} mfx_embedding_args;
+
+int mfx_embedding(const mfx_embedding_args* args, void* stream);
+
+/*
+ * Backward of mfx_embedding: the table's gradient
+ *   dw[v] = (accumulate ? dw[v] : 0) + scale * sum over t with ids[t] = v of dout[t]
+ * dout [T, H] of `dtype`, dw [V, H] of `dw_dtype` (any of the three types
+ * each).  The tokens are sorted by id: every row is written once, its tokens
+ * added in fp32 in their order, or in pieces of 64 sorted positions where there are
+ * more (deterministic, no atomics on memory).  accumulate: rows without tokens are
+ * left alone, the others rounded once (a head tied to the table: pass
+ * mfx_linear_xent_bwd's dw).  dw must not share memory with dout or ids.
+ * workspace: mfx_embedding_bwd_workspace_size() bytes, 256-byte aligned (4
+ * bytes a token and a row, H / 8 bytes a token), or NULL for library scratch.
+ */
+typedef struct {
+  const void* dout;
+  const void* ids;
+  void* dw;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t T, H, V;
+  int64_t dout_stride;
+  int64_t dw_stride;
+  float scale;
+  int32_t dtype;
+  int32_t dw_dtype;
+  int32_t ids_dtype;
+  int32_t accumulate;
+  int32_t reserved;
+} mfx_embedding_bwd_args;
+
+int mfx_embedding_bwd(const mfx_embedding_bwd_args* args, void* stream);
+
+size_t mfx_embedding_bwd_workspace_size(const mfx_embedding_bwd_args* args);
+
 /* GEMM with a fused elementwise epilogue: out = epi(inputs) where epi's
  * input `c_input` is the GEMM result C = A B, read at the program's output
  * index (contiguous strides, fp32; its data pointer and gemm->c are

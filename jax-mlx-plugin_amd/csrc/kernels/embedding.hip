@@ -1,0 +1,526 @@
+// Embedding lookup and the gradient of its table (no counterpart in the
+// reference, whose models take embedded inputs):
+//
+//   out[t] = scale * w[ids[t]]              (zeros for an id outside [0, V))
+//   dw[v]  = [dw[v] +] scale * sum over t with ids[t] = v of dout[t]
+//
+// Both are bound by memory: the forward reads and writes T rows, the backward
+// reads T rows and writes V.  Sums are fp32, each output rounded once.
+//
+// The backward sorts the tokens by id, so that each row of dw is written once,
+// by one owner, without atomics, its tokens added in their order:
+//   embed_index  Each workgroup owns a run of up to 960 rows of the table and
+//     looks at every id (they are few against the rows of dout, and in the L2
+//     after the first look): a count of the ids below its rows is where its tokens
+//     start in the sorted order, counts of its own rows (by wavefront, each
+//     walking a share of the tokens) give every row's start, and a second look
+//     puts its tokens there in order.  One launch, where a radix sort takes three
+//     for each digit.
+//   embed_rows   A group of lanes owns a piece of a row of dw: sums its
+//     tokens' rows and writes it (zeros for a row without tokens).  A row of
+//     more than kRun tokens (a padding or end token, in the worst case all of
+//     them) is cut at multiples of kRun positions of the sorted order, a group for
+//     each, into fp32 partials;
+//   embed_fold   adds those of a row in order and writes it.
+#include <algorithm>
+#include <cmath>
+
+#include "rowvec.h"
+#include "workspace.h"
+
+namespace mfx {
+namespace embed {
+namespace {
+
+using namespace rowvec;
+
+constexpr int kRun = 64;          // tokens that one group adds up
+constexpr int kScanWaves = 16;    // of embed_index
+constexpr int kScanRows = 960;    // table rows of one of its workgroups, at most (60 KB of counts)
+constexpr int kFoldWaves = 8;
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Elements a lane takes at a time: 16 bytes of the narrower type.
+template <typename A, typename B>
+constexpr int kVec = sizeof(A) == 4 && sizeof(B) == 4 ? 4 : 8;
+
+// Group of LANES lanes of this launch (of fewer than 2^32 threads), uniform (a
+// scalar) over a wavefront where the group is one.
+template <int LANES>
+__device__ __forceinline__ uint32_t group_id() {
+  if constexpr (LANES == 64)
+    return blockIdx.x * (kBlock / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  else
+    return blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
+}
+
+__device__ __forceinline__ int64_t load_id(const void* ids, int ids64, int64_t t) {
+  return ids64 ? static_cast<const int64_t*>(ids)[t] : (int64_t)static_cast<const int32_t*>(ids)[t];
+}
+
+struct LookupArgs {
+  const void* w;
+  const void* ids;
+  void* out;
+  int64_t T, V, ws, os;
+  int H, segs, ids64;
+  float scale;
+};
+
+template <typename TI, typename TO, int LANES, int NV>
+__global__ __launch_bounds__(kBlock) void embed_lookup(LookupArgs a) {
+  constexpr int VEC = kVec<TI, TO>;
+  const uint32_t g = group_id<LANES>(), row = g / (uint32_t)a.segs;
+  const int64_t t = row;
+  if (t >= a.T) return;
+  const int col = (int)(g - row * a.segs) * (LANES * NV * VEC) + (int)(threadIdx.x % LANES) * VEC;
+  const int64_t id = load_id(a.ids, a.ids64, t);
+  const bool valid = id >= 0 && id < a.V;
+  const TI* src = static_cast<const TI*>(a.w) + (valid ? id : 0) * a.ws;
+  TO* dst = static_cast<TO*>(a.out) + t * a.os;
+  float v[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    // (An id outside the table reads nothing: V may be 0.)
+    load_run<TI, VEC>(src, col + i * LANES * VEC, valid ? a.H : 0, 0.f, v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[i][j] *= a.scale;
+    store_run<TO, VEC>(dst, col + i * LANES * VEC, a.H, v[i]);
+  }
+}
+
+// ---- the order of the tokens -----------------------------------------------------
+
+// order[]: the tokens with an id in [0, V) by id, those of one id ascending;
+// start[v]: where row v's begin, start[V] their number.
+__global__ __launch_bounds__(kScanWaves * 64) void embed_index(const void* ids, int ids64, int64_t T, int64_t V,
+                                                               int rows, int32_t* order, int32_t* start) {
+  extern __shared__ int32_t count[];  // [wavefront][row]: tokens, then the next one's place
+  __shared__ int32_t below_w[kScanWaves], scan_w[kScanWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t v0 = (int64_t)blockIdx.x * rows;
+  const int mine = (int)min((int64_t)rows, V - v0);
+  for (int i = tid; i < kScanWaves * rows; i += kScanWaves * 64) count[i] = 0;
+  __syncthreads();
+
+  // This wavefront's tokens.
+  const int64_t per = (T + kScanWaves * 64 - 1) / (kScanWaves * 64) * 64;
+  const int64_t t0 = min(T, wave * per), t1 = min(T, t0 + per);
+  int32_t* const own = count + wave * rows;
+  constexpr int U = 8;  // looks in flight
+  int32_t below = 0;
+  for (int64_t t = t0; t < t1; t += 64 * U) {
+    int64_t id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = t + u * 64 + lane;
+      id[u] = at < t1 ? load_id(ids, ids64, at) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = id[u] - v0;
+      if (id[u] >= 0 && r < 0) ++below;
+      else if (id[u] >= 0 && r < mine) atomicAdd(own + r, 1);
+    }
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) below += __shfl_xor(below, off, 64);
+  if (lane == 0) below_w[wave] = below;
+  __syncthreads();
+
+  // Thread r: row r's tokens, their start, and each wavefront's.
+  int32_t n = 0;
+  if (tid < mine)
+    for (int w = 0; w < kScanWaves; ++w) n += count[w * rows + tid];
+  int32_t upto = n;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int32_t o = __shfl_up(upto, off, 64);
+    if (lane >= off) upto += o;
+  }
+  if (lane == 63) scan_w[wave] = upto;
+  __syncthreads();
+  int32_t at = upto - n;
+  for (int w = 0; w < kScanWaves; ++w) {
+    at += below_w[w];
+    if (w < wave) at += scan_w[w];
+  }
+  if (tid < mine) {
+    start[v0 + tid] = at;
+    if (v0 + tid == V - 1) start[V] = at + n;
+    for (int w = 0; w < kScanWaves; ++w) {
+      const int32_t c = count[w * rows + tid];
+      count[w * rows + tid] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+
+  for (int64_t t = t0; t < t1; t += 64 * U) {
+    int64_t id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = t + u * 64 + lane;
+      id[u] = k < t1 ? load_id(ids, ids64, k) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r64 = id[u] - v0;
+      const int r = id[u] >= 0 && r64 >= 0 && r64 < mine ? (int)r64 : -1;
+      // One id of the 64 at a time: its lanes in order.
+      uint64_t left = __ballot(r >= 0);
+      while (left) {
+        const int row = __builtin_amdgcn_readlane(r, __ffsll((unsigned long long)left) - 1);
+        const uint64_t same = __ballot(r == row);
+        const int32_t place = own[row];
+        if (r == row) {
+          const int before = __popcll(same & ((1ull << lane) - 1));
+          order[place + before] = (int32_t)(t + u * 64 + lane);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (lane == 0) own[row] = place + __popcll(same);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        left &= ~same;
+      }
+    }
+  }
+}
+
+// ---- the sums --------------------------------------------------------------------
+
+struct SumArgs {
+  const void* dout;
+  const void* ids;
+  void* dw;
+  const int32_t* order;
+  const int32_t* start;
+  float* part;       // [2 blocks][part_ld]: of the run at a block's first, and at its last position
+  int64_t V, ds, gs, part_ld;
+  int64_t blocks;    // of kRun positions (0: no row can have more tokens)
+  int H, segs, ids64, add;
+  float scale;
+};
+
+// Sum of the rows of dout at positions [s, e) of the order.
+template <typename T, int LANES, int NV, int VEC>
+__device__ __forceinline__ void sum_rows(const SumArgs& a, int64_t s, int64_t e, int col, float (&acc)[NV][VEC]) {
+  constexpr int U = NV == 1 ? 8 : 4;  // rows in flight
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[i][j] = 0.f;
+  const T* const dout = static_cast<const T*>(a.dout);
+  for (int64_t p = s; p < e; p += U) {
+    float v[U][NV][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = p + u < e;
+      const T* row = dout + (int64_t)(in ? a.order[p + u] : 0) * a.ds;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) load_run<T, VEC>(row, col + i * LANES * VEC, in ? a.H : 0, 0.f, v[u][i]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[i][j] += v[u][i][j];
+  }
+}
+
+template <typename TO, int VEC>
+__device__ __forceinline__ void write_row(const SumArgs& a, int64_t v, int col, const float (&acc)[VEC]) {
+  TO* const row = static_cast<TO*>(a.dw) + v * a.gs;
+  float o[VEC];
+  if (a.add) {
+    load_run<TO, VEC>(row, col, a.H, 0.f, o);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) o[j] = fmaf(acc[j], a.scale, o[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) o[j] = acc[j] * a.scale;
+  }
+  store_run<TO, VEC>(row, col, a.H, o);
+}
+
+template <typename TI, typename TO, int LANES, int NV>
+__global__ __launch_bounds__(kBlock) void embed_rows(SumArgs a) {
+  constexpr int VEC = kVec<TI, TO>;
+  const uint32_t g = group_id<LANES>(), which = g / (uint32_t)a.segs;
+  int64_t task = which;
+  const int col = (int)(g - which * a.segs) * (LANES * NV * VEC) + (int)(threadIdx.x % LANES) * VEC;
+  float acc[NV][VEC];
+  // The blocks of long runs first: they take longest.
+  if (task < 2 * a.blocks) {
+    const int64_t n = a.start[a.V], p0 = (task >> 1) * kRun, p1 = min(p0 + kRun, n);
+    if (p0 >= n) return;
+    const int64_t first = load_id(a.ids, a.ids64, a.order[p0]), last = load_id(a.ids, a.ids64, a.order[p1 - 1]);
+    if ((task & 1) && first == last) return;
+    const int64_t v = task & 1 ? last : first;
+    const int64_t s = a.start[v], e = a.start[v + 1];
+    if (e - s <= kRun) return;
+    sum_rows<TI, LANES, NV, VEC>(a, max(s, p0), min(e, p1), col, acc);
+    float* const to = a.part + task * a.part_ld;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4)
+        if (col + i * LANES * VEC + j < a.H)  // (part_ld is H rounded up to whole chunks)
+          *reinterpret_cast<f32x4*>(to + col + i * LANES * VEC + j) =
+              f32x4{acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]};
+    return;
+  }
+  task -= 2 * a.blocks;
+  if (task >= a.V) return;
+  const int64_t s = a.start[task], e = a.start[task + 1];
+  if (e - s > kRun || (a.add && s == e)) return;
+  sum_rows<TI, LANES, NV, VEC>(a, s, e, col, acc);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) write_row<TO, VEC>(a, task, col + i * LANES * VEC, acc[i]);
+}
+
+// Workgroup (block, segment): the long run that starts in the block, if any.
+template <typename TO>
+__global__ __launch_bounds__(kFoldWaves * 64) void embed_fold(SumArgs a) {
+  constexpr int VEC = 8, SEG = 64 * VEC;
+  __shared__ float sums[kFoldWaves][SEG];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t segs = (a.H + SEG - 1) / SEG, b = blockIdx.x / segs;
+  const int col = (int)(blockIdx.x - b * segs) * SEG + lane * VEC;
+  const int64_t n = a.start[a.V], p0 = b * kRun, p1 = min(p0 + kRun, n);
+  if (p0 >= n) return;
+  const int64_t v = load_id(a.ids, a.ids64, a.order[p1 - 1]);
+  const int64_t s = a.start[v], e = a.start[v + 1];
+  if (s < p0 || e - s <= kRun) return;
+  // Its partials: this block's, then the first-position ones of the blocks up to its end.
+  const int64_t end = (e - 1) / kRun, parts = end - b + 1;
+  const int64_t q0 = b + wave * parts / kFoldWaves, q1 = b + (wave + 1) * parts / kFoldWaves;
+  float acc[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+  if (col < a.H) {
+    constexpr int U = 4;
+    for (int64_t q = q0; q < q1; q += U) {
+      f32x4 x[U][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        // (Past the last: the last again, not added.)
+        const int64_t k = min(q + u, q1 - 1), slot = 2 * k + (k == b && s > p0 ? 1 : 0);
+        const f32x4* from = reinterpret_cast<const f32x4*>(a.part + slot * a.part_ld + col);
+        x[u][0] = from[0];
+        x[u][1] = from[1];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (q + u < q1)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) acc[j] += x[u][j / 4][j % 4];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) sums[wave][lane * VEC + j] = acc[j];
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int w = 1; w < kFoldWaves; ++w)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[j] += sums[w][lane * VEC + j];
+  if constexpr (sizeof(TO) == 4) {
+    const float lo[4] = {acc[0], acc[1], acc[2], acc[3]}, hi[4] = {acc[4], acc[5], acc[6], acc[7]};
+    write_row<TO, 4>(a, v, col, lo);
+    write_row<TO, 4>(a, v, col + 4, hi);
+  } else {
+    write_row<TO, 8>(a, v, col, acc);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------
+
+bool float_dtype(int dt) { return dt == MFX_F32 || dt == MFX_BF16 || dt == MFX_F16; }
+
+// Lanes of a group and 16-byte chunks a lane takes: 16 lanes for rows that a
+// wavefront would leave mostly idle; four chunks a lane where that still makes
+// eight wavefronts a CU (a launch of fewer is bound by latency and wants as many as
+// it can have).
+struct Split {
+  int lanes, nv, segs;
+};
+Split split(int64_t rows, int64_t H, int vec, int most) {
+  Split s{H <= 16 * vec ? 16 : 64, 1, 1};
+  if (s.lanes == 64) {
+    const int64_t chunks = ceil_div(H, 64 * vec);
+    while (s.nv * 2 <= most && s.nv < chunks && rows * ceil_div(chunks, s.nv * 2) >= 8LL * device_cu_count()) s.nv *= 2;
+  }
+  s.segs = (int)ceil_div(H, (int64_t)s.lanes * vec * s.nv);
+  return s;
+}
+
+int vec_of(int a, int b) { return a == MFX_F32 && b == MFX_F32 ? 4 : 8; }
+
+int check_common(int64_t T, int64_t H, int64_t V, int dtype, int other, int ids_dtype, float scale, const char* what) {
+  const int64_t lim = 0x7fffffffLL - 4096;
+  if (T < 0 || H <= 0 || V <= 0) return fail(MFX_E_INVALID, "T must be >= 0, H and V positive");
+  if (!float_dtype(dtype) || !float_dtype(other))
+    return fail(MFX_E_UNSUPPORTED, std::string("dtype and ") + what + " must be f32, bf16 or f16");
+  if (ids_dtype != MFX_I32 && ids_dtype != MFX_I64) return fail(MFX_E_UNSUPPORTED, "ids dtype must be i32 or i64");
+  if (!std::isfinite(scale)) return fail(MFX_E_INVALID, "scale must be finite");
+  if (T > lim || V > lim || H > lim) return fail(MFX_E_UNSUPPORTED, "T, H or V too large");
+  return MFX_OK;
+}
+
+// (Rows that are only read may overlap: a gradient broadcast over the tokens.)
+int check_rows(const void* p, int64_t stride, int64_t rows, int64_t H, int dtype, const char* what, bool written) {
+  if (!p) return fail(MFX_E_INVALID, std::string(what) + " must be non-null");
+  if ((uintptr_t)p % dtype_size(dtype)) return fail(MFX_E_INVALID, std::string(what) + " must be aligned to its type");
+  if (rows > 1 && stride < (written ? H : 0))
+    return fail(MFX_E_INVALID, std::string(what) + (written ? ": row stride must be >= H" : ": row stride must be >= 0"));
+  return MFX_OK;
+}
+
+int check_ids(const void* ids, int dtype) {
+  if (!ids) return fail(MFX_E_INVALID, "ids must be non-null");
+  if ((uintptr_t)ids % (dtype == MFX_I64 ? 8 : 4)) return fail(MFX_E_INVALID, "ids must be aligned to their type");
+  return MFX_OK;
+}
+
+struct FwdPlan {
+  Split sp;
+  int64_t grid;
+};
+int plan_fwd(const mfx_embedding_args* a, FwdPlan& pl) {
+  if (!a) return fail(MFX_E_INVALID, "null args");
+  if (int rc = check_common(a->T, a->H, a->V, a->dtype, a->out_dtype, a->ids_dtype, a->scale, "out_dtype")) return rc;
+  if (a->T == 0) return MFX_OK;
+  if (int rc = check_ids(a->ids, a->ids_dtype)) return rc;
+  if (int rc = check_rows(a->w, a->w_stride, a->V, a->H, a->dtype, "w", false)) return rc;
+  if (int rc = check_rows(a->out, a->out_stride, a->T, a->H, a->out_dtype, "out", true)) return rc;
+  pl.sp = split(a->T, a->H, vec_of(a->dtype, a->out_dtype), 4);
+  pl.grid = ceil_div(a->T * pl.sp.segs, kBlock / pl.sp.lanes);
+  if (!launch_fits(pl.grid, kBlock)) return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
+  return MFX_OK;
+}
+
+struct BwdPlan {
+  Split sp;
+  int64_t blocks, grid, fold, part_ld;
+  int rows;
+  int64_t scans;
+  size_t order_bytes, start_bytes, part_bytes, total;
+};
+int plan_bwd(const mfx_embedding_bwd_args* a, BwdPlan& pl) {
+  if (!a) return fail(MFX_E_INVALID, "null args");
+  if (int rc = check_common(a->T, a->H, a->V, a->dtype, a->dw_dtype, a->ids_dtype, a->scale, "dw_dtype")) return rc;
+  if (int rc = check_rows(a->dw, a->dw_stride, a->V, a->H, a->dw_dtype, "dw", true)) return rc;
+  if (a->T > 0) {
+    if (int rc = check_ids(a->ids, a->ids_dtype)) return rc;
+    if (int rc = check_rows(a->dout, a->dout_stride, a->T, a->H, a->dtype, "dout", false)) return rc;
+  }
+  pl.sp = split(a->V, a->H, vec_of(a->dtype, a->dw_dtype), 2);
+  pl.blocks = a->T > kRun ? ceil_div(a->T, kRun) : 0;
+  pl.grid = ceil_div((2 * pl.blocks + a->V) * pl.sp.segs, kBlock / pl.sp.lanes);
+  pl.fold = pl.blocks * ceil_div(a->H, 512);
+  // A workgroup of the index for each CU, of at most 960 rows (a thread each).
+  pl.rows = (int)std::min<int64_t>(kScanRows, ceil_div(a->V, device_cu_count()));
+  pl.scans = ceil_div(a->V, pl.rows);
+  if (!launch_fits(pl.grid, kBlock) || !launch_fits(pl.fold, kFoldWaves * 64) ||
+      !launch_fits(pl.scans, kScanWaves * 64))
+    return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
+  pl.part_ld = ceil_div(a->H, 8) * 8;
+  pl.order_bytes = align256((size_t)a->T * 4);
+  pl.start_bytes = align256(((size_t)a->V + 1) * 4);
+  pl.part_bytes = (size_t)pl.blocks * 2 * pl.part_ld * 4;
+  pl.total = pl.order_bytes + pl.start_bytes + pl.part_bytes;
+  return MFX_OK;
+}
+
+template <typename TI, typename TO>
+void launch_lookup(const LookupArgs& p, const FwdPlan& pl, hipStream_t s) {
+  const dim3 grid((unsigned)pl.grid), block(kBlock);
+  if (pl.sp.lanes == 16) hipLaunchKernelGGL((embed_lookup<TI, TO, 16, 1>), grid, block, 0, s, p);
+  else if (pl.sp.nv == 1) hipLaunchKernelGGL((embed_lookup<TI, TO, 64, 1>), grid, block, 0, s, p);
+  else if (pl.sp.nv == 2) hipLaunchKernelGGL((embed_lookup<TI, TO, 64, 2>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((embed_lookup<TI, TO, 64, 4>), grid, block, 0, s, p);
+}
+
+template <typename TI, typename TO>
+void launch_rows(const SumArgs& p, const BwdPlan& pl, hipStream_t s) {
+  const dim3 grid((unsigned)pl.grid), block(kBlock);
+  if (pl.sp.lanes == 16) hipLaunchKernelGGL((embed_rows<TI, TO, 16, 1>), grid, block, 0, s, p);
+  else if (pl.sp.nv == 1) hipLaunchKernelGGL((embed_rows<TI, TO, 64, 1>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((embed_rows<TI, TO, 64, 2>), grid, block, 0, s, p);
+}
+
+// f(TI{}, TO{}) for a pair of element types.
+template <class F>
+void with_types(int in, int out, F f) {
+  auto second = [&](auto t) {
+    if (out == MFX_F32) f(t, float{});
+    else if (out == MFX_BF16) f(t, bf16{});
+    else f(t, _Float16{});
+  };
+  if (in == MFX_F32) second(float{});
+  else if (in == MFX_BF16) second(bf16{});
+  else second(_Float16{});
+}
+
+}  // namespace
+}  // namespace embed
+}  // namespace mfx
+
+extern "C" {
+
+int mfx_embedding(const mfx_embedding_args* args, void* stream) {
+  using namespace mfx;
+  using namespace mfx::embed;
+  FwdPlan pl;
+  if (int rc = plan_fwd(args, pl)) return rc;
+  const mfx_embedding_args& a = *args;
+  if (a.T == 0) return MFX_OK;
+  const LookupArgs p{a.w, a.ids, a.out, a.T, a.V, a.w_stride, a.out_stride, (int)a.H, pl.sp.segs,
+                     a.ids_dtype == MFX_I64, a.scale};
+  with_types(a.dtype, a.out_dtype, [&](auto ti, auto to) {
+    launch_lookup<decltype(ti), decltype(to)>(p, pl, static_cast<hipStream_t>(stream));
+  });
+  return launch_status("embed_lookup");
+}
+
+size_t mfx_embedding_bwd_workspace_size(const mfx_embedding_bwd_args* args) {
+  mfx::embed::BwdPlan pl;
+  return mfx::embed::plan_bwd(args, pl) == MFX_OK ? pl.total : 0;
+}
+
+int mfx_embedding_bwd(const mfx_embedding_bwd_args* args, void* stream) {
+  using namespace mfx;
+  using namespace mfx::embed;
+  BwdPlan pl;
+  if (int rc = plan_bwd(args, pl)) return rc;
+  const mfx_embedding_bwd_args& a = *args;
+  if (a.T == 0 && a.accumulate) return MFX_OK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = nullptr;
+  if (int rc = take_workspace(a.workspace, a.workspace_bytes, pl.total, "mfx_embedding_bwd_workspace_size", s, &ws))
+    return rc;
+  int32_t* const order = reinterpret_cast<int32_t*>(ws);
+  int32_t* const start = reinterpret_cast<int32_t*>(ws + pl.order_bytes);
+  const int ids64 = a.ids_dtype == MFX_I64;
+  hipLaunchKernelGGL(embed_index, dim3((unsigned)pl.scans), dim3(kScanWaves * 64), (size_t)kScanWaves * pl.rows * 4, s,
+                     a.ids, ids64, a.T, a.V, pl.rows, order, start);
+  if (int rc = launch_status("embed_index")) return rc;
+  const SumArgs p{a.dout, a.ids, a.dw, order, start, reinterpret_cast<float*>(ws + pl.order_bytes + pl.start_bytes),
+                  a.V, a.dout_stride, a.dw_stride, pl.part_ld, pl.blocks, (int)a.H, pl.sp.segs, ids64,
+                  a.accumulate != 0, a.scale};
+  with_types(a.dtype, a.dw_dtype, [&](auto ti, auto to) { launch_rows<decltype(ti), decltype(to)>(p, pl, s); });
+  if (int rc = launch_status("embed_rows")) return rc;
+  if (!pl.blocks) return MFX_OK;
+  const dim3 grid((unsigned)pl.fold), block(kFoldWaves * 64);
+  if (a.dw_dtype == MFX_F32) hipLaunchKernelGGL((embed_fold<float>), grid, block, 0, s, p);
+  else if (a.dw_dtype == MFX_BF16) hipLaunchKernelGGL((embed_fold<bf16>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((embed_fold<_Float16>), grid, block, 0, s, p);
+  return launch_status("embed_fold");
+}
+
+}  // extern "C"

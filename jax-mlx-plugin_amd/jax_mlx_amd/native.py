@@ -230,6 +230,24 @@ class LinearXentBwdArgs(ctypes.Structure):
                 + [(n, ctypes.c_int32) for n in ("dtype", "target_dtype", "dw_dtype", "reserved")])
 
 
+class EmbeddingArgs(ctypes.Structure):
+    """mfx_embedding_args (include/mfx_kernels.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("w", "ids", "out")]
+                + [(n, ctypes.c_int64) for n in ("T", "H", "V", "w_stride", "out_stride")]
+                + [("scale", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("dtype", "out_dtype", "ids_dtype")])
+
+
+class EmbeddingBwdArgs(ctypes.Structure):
+    """mfx_embedding_bwd_args (include/mfx_kernels.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("dout", "ids", "dw", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int64) for n in ("T", "H", "V", "dout_stride", "dw_stride")]
+                + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("dtype", "dw_dtype", "ids_dtype", "accumulate", "reserved")])
+
+
 MFX_MAX_RANK = 8
 MFX_EW_MAX_INPUTS = 8
 MFX_EW_MAX_INSTRS = 64
@@ -332,7 +350,10 @@ def load(path: str | os.PathLike | None = None, make_default: bool = False) -> c
     lib.mfx_sdpa_workspace_size.restype = ctypes.c_size_t
     lib.mfx_sdpa_kernel_name.argtypes = [ctypes.POINTER(SdpaArgs)]
     lib.mfx_sdpa_kernel_name.restype = ctypes.c_char_p
-    for name, args in (("mfx_linear_xent", LinearXentArgs), ("mfx_linear_xent_bwd", LinearXentBwdArgs)):
+    lib.mfx_embedding.argtypes = [ctypes.POINTER(EmbeddingArgs), ctypes.c_void_p]
+    lib.mfx_embedding.restype = ctypes.c_int
+    for name, args in (("mfx_linear_xent", LinearXentArgs), ("mfx_linear_xent_bwd", LinearXentBwdArgs),
+                       ("mfx_embedding_bwd", EmbeddingBwdArgs)):
         getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name + "_workspace_size").argtypes = [ctypes.POINTER(args)]
@@ -1055,6 +1076,78 @@ def linear_xent_bwd(h, w, targets, lse, dloss, *, need_dh=True, need_dw=True, dw
         keep = _workspace(a, "mfx_linear_xent_bwd_workspace_size", workspace, h)  # noqa: F841 (until the launch)
         check(load().mfx_linear_xent_bwd(ctypes.byref(a), _stream_handle(h)))
     return dh, dw
+
+
+# ---- embedding -------------------------------------------------------------------
+
+_EMBED_PACK = struct.Struct("3P5qf3i").pack
+_EMBED_BWD_PACK = struct.Struct("4PN5qf5i").pack
+
+
+def _token_rows(name, t, ids, H):
+    """(dtype code, row stride) of t [..., H], a row for each of ids."""
+    if t.shape != (*ids.shape, H):
+        raise ValueError(f"{name} must be {(*ids.shape, H)}, got {tuple(t.shape)}")
+    n, _, stride = _rows_view(t)
+    # (One row may carry any stride.)
+    return dtype_code(t.dtype), stride if n > 1 else H
+
+
+def _table_rows(name, w):
+    """(V, H, dtype code, row stride) of a table [V, H]."""
+    if w.dim() != 2 or w.shape[1] == 0 or w.stride(1) != 1:
+        raise ValueError(f"{name} must be [V, H] with a contiguous last dimension")
+    return *w.shape, dtype_code(w.dtype), w.stride(0) if w.shape[0] > 1 else w.shape[1]
+
+
+def _ids_code(ids):
+    torch = _torch()
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError("ids must be int32 or int64")
+    if not ids.is_contiguous():
+        raise ValueError("ids must be contiguous")
+    return MFX_I64 if ids.dtype == torch.int64 else MFX_I32
+
+
+def embedding(ids, w, *, scale=1.0, out_dtype=None, out=None):
+    """out [..., H] = scale * w[ids] (mfx_embedding): ids [...] int32 or int64,
+    w [V, H]; an id outside [0, V) gives zeros.  out has w's dtype, out_dtype, or
+    its own if given."""
+    torch = _torch()
+    icode = _ids_code(ids)
+    V, H, code, ws = _table_rows("w", w)
+    if out is None:
+        out = torch.empty((*ids.shape, H), dtype=out_dtype or w.dtype, device=w.device)
+    ocode, os_ = _token_rows("out", out, ids, H)
+    a = EmbeddingArgs.from_buffer_copy(_EMBED_PACK(w.data_ptr(), ids.data_ptr(), out.data_ptr(), ids.numel(), H, V, ws,
+                                                   os_, _f32(scale), code, ocode, icode))
+    with _on(w, ids, out):
+        check(load().mfx_embedding(ctypes.byref(a), _stream_handle(w)))
+    return out
+
+
+def embedding_bwd(ids, dout, num_rows=None, *, scale=1.0, dw_dtype=None, dw=None, accumulate=False, workspace=None):
+    """dw [num_rows, H], the gradient of embedding's table for the gradient
+    dout [..., H] of its output (mfx_embedding_bwd), in dout's dtype, dw_dtype, or
+    that of a given dw; accumulate adds to a given dw (a table tied to the head:
+    linear_xent_bwd's dw)."""
+    torch = _torch()
+    icode = _ids_code(ids)
+    if dw is None:
+        if num_rows is None or accumulate:
+            raise ValueError("num_rows, or a dw (to accumulate into), is needed")
+        dw = torch.empty(num_rows, dout.shape[-1], dtype=dw_dtype or dout.dtype, device=dout.device)
+    elif num_rows not in (None, dw.shape[0]):
+        raise ValueError(f"dw has {dw.shape[0]} rows, not {num_rows}")
+    V, H, wcode, ws = _table_rows("dw", dw)
+    code, ds = _token_rows("dout", dout, ids, H)
+    a = EmbeddingBwdArgs.from_buffer_copy(_EMBED_BWD_PACK(
+        dout.data_ptr(), ids.data_ptr(), dw.data_ptr(), 0, 0, ids.numel(), H, V, ds, ws, _f32(scale), code, wcode,
+        icode, 1 if accumulate else 0, 0))
+    with _on(dw, dout, ids, workspace):
+        keep = _workspace(a, "mfx_embedding_bwd_workspace_size", workspace, dw)  # noqa: F841 (until the launch)
+        check(load().mfx_embedding_bwd(ctypes.byref(a), _stream_handle(dw)))
+    return dw
 
 
 # ---- GEMM ----------------------------------------------------------------------
