@@ -853,6 +853,113 @@ int mfx_embedding_bwd(const mfx_embedding_bwd_args* args, void* stream);
 
 size_t mfx_embedding_bwd_workspace_size(const mfx_embedding_bwd_args* args);
 
+/* Which rows share a row of the gate of mfx_residual_norm. */
+enum {
+  MFX_GATE_NONE = 0,     /* no gate */
+  MFX_GATE_FEATURE = 1,  /* gate [H], one row for all */
+  MFX_GATE_SEQUENCE = 2, /* gate [num_seqs, H], a row for each sequence */
+  MFX_GATE_TOKEN = 3,    /* gate [T, H], a row for each token */
+};
+
+/*
+ * The norm behind a block, its gate, the residual sum and the norm before the
+ * next block:
+ *   z = y / rms(y) * (weight_offset + post_weight)   (post_eps < 0: z = y)
+ *   r = alpha x + beta gate * z
+ *   h = r / rms(r) * (weight_offset + pre_weight)    (pre_eps < 0: no h)
+ * with rms(v) = sqrt(mean(v^2) + its eps) over a row.  The residual stream x, r
+ * [T, H] is in `res_dtype` (`dtype` or MFX_F32), the block's y, h in `dtype`
+ * (f32, bf16, f16); fp32 arithmetic, h of the unrounded r, each output rounded
+ * once.  Weights [H] of `param_dtype` or NULL (all ones, no offset); the gate
+ * of `gate_dtype`, rows gate_stride apart.  MFX_GATE_SEQUENCE: token t belongs to the
+ * sequence s with seq_offsets[s] <= t < seq_offsets[s + 1] (int32 [num_seqs + 1],
+ * read on the device); a row in no sequence takes no part of y, whatever it
+ * holds (r = alpha x).  Rows at any alignment, H up to 32768.  r may be x and h
+ * may be y; otherwise outputs share no memory with inputs.
+ * The reference's counterpart are the elementwise programs around its
+ * rms_norm (src/jax_mlx_pjrt.cpp:4408-4446).
+ */
+typedef struct {
+  const void* x;
+  const void* y;
+  const void* gate;
+  const int32_t* seq_offsets;
+  const void* post_weight;
+  const void* pre_weight;
+  void* r;
+  void* h;
+  int64_t T, H, num_seqs;
+  int64_t x_stride;
+  int64_t y_stride;
+  int64_t gate_stride;
+  int64_t r_stride;
+  int64_t h_stride;
+  float alpha;
+  float beta;
+  float weight_offset;
+  float post_eps;
+  float pre_eps;
+  int32_t res_dtype;
+  int32_t dtype;
+  int32_t param_dtype;
+  int32_t gate_mode;
+  int32_t gate_dtype;
+} mfx_residual_norm_args;
+
+int mfx_residual_norm(const mfx_residual_norm_args* args, void* stream);
+
+/*
+ * Backward of mfx_residual_norm from its inputs x, y, gate and weights and
+ * the gradients dr of r (res_dtype) and dh of h (dtype), either NULL if there
+ * is none: dx (res_dtype), dy (dtype) and, unless NULL, dgate (of the gate's shape
+ * and type), dpost_weight, dpre_weight ([H] of param_dtype), fp32 sums over the
+ * rows that share them.  Rows in no sequence get dy = 0.  dx may be dr or x, dy may
+ * be dh or y.  Nothing is kept from the forward; deterministic, no atomics.
+ * workspace: mfx_residual_norm_bwd_workspace_size() bytes, 256-byte aligned
+ * (fp32 rows of H: up to 16 a compute unit for each weight's gradient, as many
+ * and one for each sequence for a gate by sequence), or NULL for library scratch.
+ */
+typedef struct {
+  const void* x;
+  const void* y;
+  const void* gate;
+  const int32_t* seq_offsets;
+  const void* post_weight;
+  const void* pre_weight;
+  const void* dr;
+  const void* dh;
+  void* dx;
+  void* dy;
+  void* dgate;
+  void* dpost_weight;
+  void* dpre_weight;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t T, H, num_seqs;
+  int64_t x_stride;
+  int64_t y_stride;
+  int64_t gate_stride;
+  int64_t dr_stride;
+  int64_t dh_stride;
+  int64_t dx_stride;
+  int64_t dy_stride;
+  int64_t dgate_stride;
+  float alpha;
+  float beta;
+  float weight_offset;
+  float post_eps;
+  float pre_eps;
+  int32_t res_dtype;
+  int32_t dtype;
+  int32_t param_dtype;
+  int32_t gate_mode;
+  int32_t gate_dtype;
+} mfx_residual_norm_bwd_args;
+
+int mfx_residual_norm_bwd(const mfx_residual_norm_bwd_args* args, void* stream);
+
+size_t mfx_residual_norm_bwd_workspace_size(const mfx_residual_norm_bwd_args* args);
+
 /* GEMM with a fused elementwise epilogue: out = epi(inputs) where epi's
  * input `c_input` is the GEMM result C = A B, read at the program's output
  * index (contiguous strides, fp32; its data pointer and gemm->c are

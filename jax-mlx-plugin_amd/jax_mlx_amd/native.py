@@ -248,6 +248,32 @@ class EmbeddingBwdArgs(ctypes.Structure):
                 + [(n, ctypes.c_int32) for n in ("dtype", "dw_dtype", "ids_dtype", "accumulate", "reserved")])
 
 
+MFX_GATE_NONE, MFX_GATE_FEATURE, MFX_GATE_SEQUENCE, MFX_GATE_TOKEN = 0, 1, 2, 3
+
+_RESIDUAL_SCALARS = ([(n, ctypes.c_float) for n in ("alpha", "beta", "weight_offset", "post_eps", "pre_eps")]
+                     + [(n, ctypes.c_int32) for n in ("res_dtype", "dtype", "param_dtype", "gate_mode", "gate_dtype")])
+
+
+class ResidualNormArgs(ctypes.Structure):
+    """mfx_residual_norm_args (include/mfx_kernels.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "y", "gate", "seq_offsets", "post_weight", "pre_weight", "r", "h")]
+                + [(n, ctypes.c_int64) for n in ("T", "H", "num_seqs", "x_stride", "y_stride", "gate_stride",
+                                                 "r_stride", "h_stride")]
+                + _RESIDUAL_SCALARS)
+
+
+class ResidualNormBwdArgs(ctypes.Structure):
+    """mfx_residual_norm_bwd_args (include/mfx_kernels.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "y", "gate", "seq_offsets", "post_weight", "pre_weight", "dr",
+                                                "dh", "dx", "dy", "dgate", "dpost_weight", "dpre_weight", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int64) for n in ("T", "H", "num_seqs", "x_stride", "y_stride", "gate_stride",
+                                                 "dr_stride", "dh_stride", "dx_stride", "dy_stride", "dgate_stride")]
+                + _RESIDUAL_SCALARS)
+
+
 MFX_MAX_RANK = 8
 MFX_EW_MAX_INPUTS = 8
 MFX_EW_MAX_INSTRS = 64
@@ -350,10 +376,11 @@ def load(path: str | os.PathLike | None = None, make_default: bool = False) -> c
     lib.mfx_sdpa_workspace_size.restype = ctypes.c_size_t
     lib.mfx_sdpa_kernel_name.argtypes = [ctypes.POINTER(SdpaArgs)]
     lib.mfx_sdpa_kernel_name.restype = ctypes.c_char_p
-    lib.mfx_embedding.argtypes = [ctypes.POINTER(EmbeddingArgs), ctypes.c_void_p]
-    lib.mfx_embedding.restype = ctypes.c_int
+    for name, args in (("mfx_embedding", EmbeddingArgs), ("mfx_residual_norm", ResidualNormArgs)):
+        getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        getattr(lib, name).restype = ctypes.c_int
     for name, args in (("mfx_linear_xent", LinearXentArgs), ("mfx_linear_xent_bwd", LinearXentBwdArgs),
-                       ("mfx_embedding_bwd", EmbeddingBwdArgs)):
+                       ("mfx_embedding_bwd", EmbeddingBwdArgs), ("mfx_residual_norm_bwd", ResidualNormBwdArgs)):
         getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name + "_workspace_size").argtypes = [ctypes.POINTER(args)]
@@ -1148,6 +1175,112 @@ def embedding_bwd(ids, dout, num_rows=None, *, scale=1.0, dw_dtype=None, dw=None
         keep = _workspace(a, "mfx_embedding_bwd_workspace_size", workspace, dw)  # noqa: F841 (until the launch)
         check(load().mfx_embedding_bwd(ctypes.byref(a), _stream_handle(dw)))
     return dw
+
+
+# ---- norms around a block --------------------------------------------------------
+
+_RESIDUAL_PACK = struct.Struct("8P8q5f5i").pack
+_RESIDUAL_BWD_PACK = struct.Struct("14PN11q5f5i").pack
+
+
+def _rows_of(name, t, like, dtype=None):
+    """Row stride of t, which has like's shape (and dtype, if given)."""
+    if t.shape != like.shape or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{name} must be {tuple(like.shape)}{'' if dtype is None else f' of {dtype}'}")
+    n, H, stride = _rows_view(t)
+    return stride if n > 1 else H
+
+
+def _residual_fields(x, y, gate, seq_offsets, post_weight, pre_weight, post_eps, pre_eps, alpha, beta, weight_offset):
+    """Checked (pointers, dims, strides of x, y and gate, scalars) of both directions."""
+    if x.dim() < 2 or x.shape[-1] == 0:
+        raise ValueError("x and y are [..., H]")
+    if any(eps is not None and not eps >= 0.0 for eps in (post_eps, pre_eps)):
+        raise ValueError("eps must be >= 0 (None: no norm)")
+    xs, ys = _rows_of("x", x, x), _rows_of("y", y, x)
+    H = x.shape[-1]
+    T = x.numel() // H
+    pd = None
+    for w in (post_weight, pre_weight):
+        if w is not None:
+            if w.shape != (H,) or not w.is_contiguous() or (pd is not None and w.dtype != pd):
+                raise ValueError("weights must be contiguous [H] vectors of one dtype")
+            pd = w.dtype
+    mode, S, gs, off = MFX_GATE_NONE, 0, H, 0
+    if seq_offsets is not None:
+        if gate is None:
+            raise ValueError("seq_offsets belong to a gate")
+        if seq_offsets.dtype != _torch().int32 or seq_offsets.dim() != 1 or not seq_offsets.is_contiguous():
+            raise TypeError("seq_offsets must be a contiguous int32 vector")
+        S = seq_offsets.numel() - 1
+        if S < 0 or gate.shape != (S, H) or gate.stride(1) != 1:
+            raise ValueError("a gate by sequence is [sequences, H], seq_offsets one entry more")
+        mode, gs, off = MFX_GATE_SEQUENCE, gate.stride(0) if S > 1 else H, seq_offsets.data_ptr()
+    elif gate is not None and gate.dim() == 1:
+        if gate.shape != (H,) or not gate.is_contiguous():
+            raise ValueError("a gate for all rows is a contiguous [H] vector")
+        mode = MFX_GATE_FEATURE
+    elif gate is not None:
+        mode, gs = MFX_GATE_TOKEN, _rows_of("a gate by token", gate, x)
+    code = dtype_code(y.dtype)
+    return ((x.data_ptr(), y.data_ptr(), _ptr(gate), off, _ptr(post_weight), _ptr(pre_weight)), (T, H, S),
+            (xs, ys, gs), (_f32(alpha), _f32(beta), _f32(weight_offset), -1.0 if post_eps is None else _f32(post_eps),
+                           -1.0 if pre_eps is None else _f32(pre_eps), dtype_code(x.dtype), code,
+                           code if pd is None else dtype_code(pd), mode, code if gate is None else dtype_code(gate.dtype)))
+
+
+def residual_norm(x, y, *, gate=None, seq_offsets=None, post_weight=None, pre_weight=None, post_eps=None,
+                  pre_eps=1e-6, alpha=1.0, beta=1.0, weight_offset=0.0, r=None, h=None):
+    """(r, h) of a residual stream x and a block's output y, [..., H]
+    (mfx_residual_norm): r = alpha x + beta gate * norm(y), h = norm(r).
+
+    post_eps None: y itself in place of its norm; pre_eps None: h is None.
+    Norms divide by the root mean square and multiply by weight_offset +
+    their weight [H] (None: by nothing).  gate: [H], [..., H] like x, or with
+    seq_offsets (int32 [sequences + 1], on the device) [sequences, H]; tokens in no
+    sequence keep r = alpha x.  x and r may be f32 beside 16-bit y and h.  r may be
+    x, h may be y."""
+    torch = _torch()
+    ptrs, dims, strides, scalars = _residual_fields(x, y, gate, seq_offsets, post_weight, pre_weight, post_eps,
+                                                    pre_eps, alpha, beta, weight_offset)
+    if r is None:
+        r = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if h is None and pre_eps is not None:
+        h = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    elif h is not None and pre_eps is None:
+        raise ValueError("h needs its norm (pre_eps)")
+    a = ResidualNormArgs.from_buffer_copy(_RESIDUAL_PACK(
+        *ptrs, r.data_ptr(), _ptr(h), *dims, *strides, _rows_of("r", r, x, x.dtype),
+        dims[1] if h is None else _rows_of("h", h, y, y.dtype), *scalars))
+    with _on(x, y, gate, seq_offsets, post_weight, pre_weight, r, h):
+        check(load().mfx_residual_norm(ctypes.byref(a), _stream_handle(x)))
+    return r, h
+
+
+def residual_norm_bwd(x, y, dr, dh, *, gate=None, seq_offsets=None, post_weight=None, pre_weight=None, post_eps=None,
+                      pre_eps=1e-6, alpha=1.0, beta=1.0, weight_offset=0.0, dx=None, dy=None, workspace=None):
+    """(dx, dy, dgate, dpost_weight, dpre_weight) of residual_norm on the same
+    arguments for the gradients dr of r and dh of h, one of them None if there is
+    none (mfx_residual_norm_bwd).  A gate's or weight's gradient has its shape and
+    dtype, None for an absent one.  dx may be dr or x, dy may be dh or y."""
+    torch = _torch()
+    ptrs, dims, strides, scalars = _residual_fields(x, y, gate, seq_offsets, post_weight, pre_weight, post_eps,
+                                                    pre_eps, alpha, beta, weight_offset)
+    H = dims[1]
+    if dx is None:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if dy is None:
+        dy = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    dg, dp, dn = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+                  for t in (gate, post_weight, pre_weight))
+    a = ResidualNormBwdArgs.from_buffer_copy(_RESIDUAL_BWD_PACK(
+        *ptrs, _ptr(dr), _ptr(dh), dx.data_ptr(), dy.data_ptr(), _ptr(dg), _ptr(dp), _ptr(dn), 0, 0, *dims, *strides,
+        H if dr is None else _rows_of("dr", dr, x, x.dtype), H if dh is None else _rows_of("dh", dh, y, y.dtype),
+        _rows_of("dx", dx, x, x.dtype), _rows_of("dy", dy, y, y.dtype), H, *scalars))
+    with _on(x, y, dr, dh, gate, seq_offsets, post_weight, pre_weight, dx, dy, workspace):
+        keep = _workspace(a, "mfx_residual_norm_bwd_workspace_size", workspace, x)  # noqa: F841 (until the launch)
+        check(load().mfx_residual_norm_bwd(ctypes.byref(a), _stream_handle(x)))
+    return dx, dy, dg, dp, dn
 
 
 # ---- GEMM ----------------------------------------------------------------------
