@@ -960,6 +960,98 @@ int mfx_residual_norm_bwd(const mfx_residual_norm_bwd_args* args, void* stream);
 
 size_t mfx_residual_norm_bwd_workspace_size(const mfx_residual_norm_bwd_args* args);
 
+/*
+ * Matrices orthogonalised by Newton-Schulz products: for each of `batch`
+ * matrices G [m, n]
+ *   X = G / (|G|_F + eps)
+ *   steps times:  A = X X^T (of the smaller side),  X = (a I + b A + c A^2) X
+ *   out = scale * X
+ * which with suitable coefficients takes every singular value near 1.  coeffs:
+ * host memory, num_coeffs triples (a, b, c): one for all steps, or one for each.
+ * Coefficients that let the iterates' norm grow past 16 are refused
+ * (MFX_E_UNSUPPORTED), more than 32 steps too.  G of `dtype`, out of
+ * `out_dtype` (f32, bf16, f16), rows and matrices spaced by the strides
+ * (elements), elements contiguous, any alignment; out may be g.  A matrix of
+ * zeros gives zeros (eps > 0), one with an infinity or NaN gives NaN.
+ * terms: f16 terms that the products' operands are held in.  2: error as of
+ * products of fp32 matrices; 1: three times as fast, off by up to 3e-3 of the result's
+ * norm; 0: 1 for bf16 results with both sides 256 or more, else 2.  Sums are fp32, the norm
+ * fp64.
+ * workspace: mfx_newton_schulz_workspace_size() bytes, 256-byte aligned, or NULL for
+ * library scratch.  Deterministic.  No counterpart in the reference.
+ */
+typedef struct {
+  const void* g;
+  void* out;
+  const float* coeffs;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t batch, m, n;
+  int64_t g_batch_stride;
+  int64_t g_row_stride;
+  int64_t out_batch_stride;
+  int64_t out_row_stride;
+  float eps;
+  float scale;
+  int32_t steps;
+  int32_t num_coeffs;
+  int32_t dtype;
+  int32_t out_dtype;
+  int32_t terms;
+  int32_t reserved;
+} mfx_newton_schulz_args;
+
+int mfx_newton_schulz(const mfx_newton_schulz_args* args, void* stream);
+
+size_t mfx_newton_schulz_workspace_size(const mfx_newton_schulz_args* args);
+
+/*
+ * The update of weight matrices w [m, n] by their orthogonalised momentum:
+ *   momentum = mu momentum + (1 - mu) g
+ *   u = nesterov ? mu momentum + (1 - mu) g : momentum     (g without a momentum)
+ *   w = (1 - lr weight_decay) w - lr scale NS(u)
+ * with NS as mfx_newton_schulz (of the unrounded u).  w_out may be w,
+ * momentum_out momentum (updates in place).  g of `dtype`, w of w_dtype, the
+ * momentum (NULL: none) of momentum_dtype, each f32, bf16 or f16.
+ */
+typedef struct {
+  const void* g;
+  const void* w;
+  void* w_out;
+  const void* momentum;
+  void* momentum_out;
+  const float* coeffs;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t batch, m, n;
+  int64_t g_batch_stride;
+  int64_t g_row_stride;
+  int64_t w_batch_stride;
+  int64_t w_row_stride;
+  int64_t w_out_batch_stride;
+  int64_t w_out_row_stride;
+  int64_t momentum_batch_stride;
+  int64_t momentum_row_stride;
+  int64_t momentum_out_batch_stride;
+  int64_t momentum_out_row_stride;
+  float lr;
+  float mu;
+  float weight_decay;
+  float scale;
+  float eps;
+  int32_t nesterov;
+  int32_t steps;
+  int32_t num_coeffs;
+  int32_t dtype;
+  int32_t w_dtype;
+  int32_t momentum_dtype;
+  int32_t terms;
+} mfx_muon_update_args;
+
+int mfx_muon_update(const mfx_muon_update_args* args, void* stream);
+
+size_t mfx_muon_update_workspace_size(const mfx_muon_update_args* args);
+
 /* GEMM with a fused elementwise epilogue: out = epi(inputs) where epi's
  * input `c_input` is the GEMM result C = A B, read at the program's output
  * index (contiguous strides, fp32; its data pointer and gemm->c are

@@ -82,7 +82,7 @@ HIP_FILE_FLAGS = {
 # silently corrupt results.  Their build fails if the compiler spills.
 NO_SPILL_FILES = {"sdpa_flash_bf16_pipe.hip", "sdpa_flash_pipe_wide.hip", "sdpa_bwd_mfma.hip",
                   "sdpa_decode_mfma.hip", "sdpa_decode_mfma_wide.hip", "gemm16.hip", "sdpa_packed_flash16.hip",
-                  "sdpa_packed_bwd16.hip", "linear_xent.hip"}
+                  "sdpa_packed_bwd16.hip", "linear_xent.hip", "newton_schulz.hip"}
 _RESOURCE_REMARK = "-Rpass-analysis=kernel-resource-usage"
 
 

@@ -1,0 +1,814 @@
+// Matrices orthogonalised by Newton-Schulz products, and the weight update
+// built on them (no counterpart in the reference):
+//
+//   X = U / (|U|_F + eps),   `steps` times:  X = (a I + b A + c A^2) X,  A = X X^T
+//
+// A is taken of the smaller side: for a matrix taller than wide A = X^T X and X =
+// X (a I + b A + c A^2), the same products with the operands' roles changed, no
+// transpose stored.  Each step is three products on the matrix cores:
+//
+//   gram     A = X X^T           symmetric
+//   square   Q = a I + b A + c A A   symmetric (A is: both operands are A's rows)
+//   apply    X = Q X   or   X Q
+//
+// of 2 s^2 l, 2 s^3 and 2 s^2 l operations (s, l the sides); gram and square form
+// only the tiles on and below the diagonal and store each twice.
+//
+// Precision.  The products' operands are f16, in one term or in two (a leading
+// one and what it leaves out: 22 bits, three products for one, xent_gemm16.h), all
+// sums fp32.  X, A and Q are stored times powers of two that the host derives from
+// the bound that the coefficients give their norms, so that no entry overflows
+// and the second terms stay clear of the smallest f16.  A singular value that
+// is small beside |U| is raised by up to a^steps (485), and with it what the
+// roundings put there: measured against 64 bits, gradients with a few large
+// directions come out off by 1.5e-3 of their norm in one term, just under a bf16
+// result's own rounding (1.7e-3), and by 2e-6 in two, as products of fp32 matrices
+// do (1.5e-6).  One term is therefore for bf16 results alone.  The norm is summed
+// in 64 bits (squares of small gradients leave the range of fp32).
+//
+// The update takes its momentum on the way in (ns_norm, ns_split) and adds to the
+// weights in the last product's epilogue.
+#include <algorithm>
+#include <cmath>
+
+#include "rowvec.h"
+#include "workspace.h"
+#include "xent_gemm16.h"
+
+namespace mfx {
+namespace ns {
+namespace {
+
+using namespace xent;
+using rowvec::load_run;
+using rowvec::store_run;
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ---- the matrix on its way in ------------------------------------------------------
+
+struct InArgs {
+  const void* g;
+  const void* buf;     // momentum (null: none)
+  void* buf_out;
+  double* norm;        // [B][parts] sums of squares
+  uint16_t* x;         // [B][m][ld] leading terms (f16), the second `lo` elements behind
+  int64_t gs_b, gs_r, bs_b, bs_r, os_b, os_r, lo;
+  int m, n, ld, parts, two;
+  int g_dt, buf_dt;
+  float mu, eps, scale;  // scale: the power of two that X is stored at
+  int nesterov;
+};
+
+__device__ __forceinline__ void load8(const void* p, int dt, int64_t at, int e, int n, float (&out)[8]) {
+  if (dt == MFX_F32) load_run<float, 8>(static_cast<const float*>(p) + at, e, n, 0.f, out);
+  else if (dt == MFX_BF16) load_run<bf16, 8>(static_cast<const bf16*>(p) + at, e, n, 0.f, out);
+  else load_run<_Float16, 8>(static_cast<const _Float16*>(p) + at, e, n, 0.f, out);
+}
+
+// The chunk's U, and in `b` the new momentum.
+__device__ __forceinline__ void take(const InArgs& a, int64_t bz, int row, int e, float (&u)[8], float (&b)[8]) {
+  load8(a.g, a.g_dt, bz * a.gs_b + row * a.gs_r, e, a.n, u);
+  if (!a.buf) return;
+  load8(a.buf, a.buf_dt, bz * a.bs_b + row * a.bs_r, e, a.n, b);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    b[j] = fmaf(a.mu, b[j], (1.f - a.mu) * u[j]);
+    u[j] = a.nesterov ? fmaf(a.mu, b[j], (1.f - a.mu) * u[j]) : b[j];
+  }
+}
+
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
+
+// Sums of squares: workgroup (part, matrix).
+__global__ __launch_bounds__(256) void ns_norm(InArgs a) {
+  __shared__ double lds[4];
+  const uint32_t cpr = (uint32_t)a.ld / 8, units = (uint32_t)a.m * cpr;
+  double s = 0.0;
+  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < units; i += a.parts * 256) {
+    const uint32_t row = i / cpr;
+    float u[8], b[8];
+    take(a, blockIdx.y, (int)row, (int)(i - row * cpr) * 8, u, b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fma((double)u[j], (double)u[j], s);
+  }
+  s = block_sum(s, lds);
+  if (threadIdx.x == 0) a.norm[(int64_t)blockIdx.y * a.parts + blockIdx.x] = s;
+}
+
+// x in one or two f16 terms.
+__device__ __forceinline__ uint16_t lead(float x) { return store_e<1>(x); }
+__device__ __forceinline__ float rest(float x) { return x - (float)static_cast<f16>(x); }
+
+// X = U / (|U| + eps), and the momentum.
+__global__ __launch_bounds__(256) void ns_split(InArgs a) {
+  __shared__ double lds[4];
+  // (At most 256 parts, one a thread; the same order in every workgroup.)
+  const double sum = block_sum((int)threadIdx.x < a.parts ? a.norm[(int64_t)blockIdx.y * a.parts + threadIdx.x] : 0.0, lds);
+  const float f = (float)(a.scale / (sqrt(sum) + (double)a.eps));
+  const uint32_t cpr = (uint32_t)a.ld / 8, units = (uint32_t)a.m * cpr;
+  uint16_t* const x = a.x + (int64_t)blockIdx.y * a.m * a.ld;
+  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < units; i += gridDim.x * 256) {
+    const uint32_t row = i / cpr;
+    const int e = (int)(i - row * cpr) * 8;
+    float u[8], b[8];
+    take(a, blockIdx.y, (int)row, e, u, b);
+    if (a.buf) {
+      const int64_t at = (int64_t)blockIdx.y * a.os_b + row * a.os_r;
+      if (a.buf_dt == MFX_F32) store_run<float, 8>(static_cast<float*>(a.buf_out) + at, e, a.n, b);
+      else if (a.buf_dt == MFX_BF16) store_run<bf16, 8>(static_cast<bf16*>(a.buf_out) + at, e, a.n, b);
+      else store_run<_Float16, 8>(static_cast<_Float16*>(a.buf_out) + at, e, a.n, b);
+    }
+    // (Zeros in the columns past n: 0 times a factor that may be infinite would not be.)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = e + j < a.n ? u[j] * f : 0.f;
+    *reinterpret_cast<uint4*>(x + (int64_t)i * 8) = rowvec::pack16<_Float16>(u);
+    if (!a.two) continue;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = rest(u[j]);
+    *reinterpret_cast<uint4*>(x + a.lo + (int64_t)i * 8) = rowvec::pack16<_Float16>(u);
+  }
+}
+
+// ---- the products ------------------------------------------------------------------
+
+enum Mode { kGram, kSquare, kApply };
+
+// The forms of a product's tiles: square ones, since a symmetric product's
+// tiles are stored transposed too.
+enum Form { kWide, kNarrow, kSlim };
+constexpr int kSide[3] = {256, 128, 64};
+
+template <int SIDE, bool A_KC, bool B_KC, int T>
+struct Cfg : Config<SIDE, SIDE, SIDE == 64 ? 1 : 2, 2, A_KC, B_KC, 1> {
+  static constexpr int TERMS = T;
+  static constexpr bool ROT = false;
+};
+
+struct ProdArgs {
+  GemmShape g;          // of one matrix; tiles_m x tiles_n tiles (symmetric: the lower triangle)
+  int64_t as, bs;       // elements from matrix to matrix of the operands
+  int64_t tiles, all;   // tiles of a matrix and of all
+  int kt;               // k-tiles of a tile
+  int symmetric, two;
+  // Whole tiles first, a workgroup each; then `shares` workgroups share the k-tiles
+  // of the others evenly, each a run of them, and leave partial sums.
+  int64_t whole, shares;
+  float* part;          // [shares + tiles shared][NT * FM * FN * 16]
+  float c1, c2, c3;     // gram, apply: c1 C;  square: c1 C + c2 A + c3 I
+  // Result in f16 terms ...
+  uint16_t* c;          // [rows][ldc]
+  int64_t ldc, cs, lo;
+  // ... or, at the end, the result or the updated weights
+  void* out;            // null: terms
+  const void* w;        // out = keep w + c1 C
+  int64_t os_b, os_r, ws_b, ws_r;
+  int out_dt;
+  float keep;
+};
+
+// Tile t of a matrix.
+__device__ __forceinline__ void tile_of(const ProdArgs& p, int t, int& tm, int& tn) {
+  if (!p.symmetric) {
+    // Bands of 8 tile rows, so that the tiles at work share operand panels.
+    const int band = 8 * p.g.tiles_n, b = t / band, rows = min(8, p.g.tiles_m - b * 8);
+    t -= b * band;
+    tm = b * 8 + t % rows;
+    tn = t / rows;
+    return;
+  }
+  int r = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+  while (r * (r + 1) / 2 > t) --r;
+  while ((r + 1) * (r + 2) / 2 <= t) ++r;
+  tm = r;
+  tn = t - r * (r + 1) / 2;
+}
+
+__device__ __forceinline__ int column(int j, int e, int half) { return j * 32 + (e >> 2) * 8 + half * 4 + (e & 3); }
+
+// Runs of four of a row of any of the three types; `left` of them lie in the row.
+__device__ __forceinline__ f32x4 load4(const void* p, int dt, int64_t at, int left) {
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (dt == MFX_F32) {
+    typedef float run_t __attribute__((ext_vector_type(4), aligned(4)));
+    const float* q = static_cast<const float*>(p) + at;
+    if (left >= 4) {
+      const run_t r = *reinterpret_cast<const run_t*>(q);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = r[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (j < left) v[j] = q[j];
+    }
+  } else {
+    typedef uint32_t run_t __attribute__((ext_vector_type(2), aligned(2)));
+    const uint16_t* q = static_cast<const uint16_t*>(p) + at;
+    uint32_t bits[2] = {0, 0};
+    if (left >= 4) {
+      const run_t r = *reinterpret_cast<const run_t*>(q);
+      bits[0] = r[0];
+      bits[1] = r[1];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (j < left) bits[j >> 1] |= (uint32_t)q[j] << (16 * (j & 1));
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      v[2 * j] = dt == MFX_BF16 ? __uint_as_float(bits[j] << 16) : rowvec::f16_lo(bits[j]);
+      v[2 * j + 1] = dt == MFX_BF16 ? __uint_as_float(bits[j] & 0xffff0000u) : rowvec::f16_hi(bits[j]);
+    }
+  }
+  return v;
+}
+__device__ __forceinline__ void store4(void* p, int dt, int64_t at, int left, const f32x4& v) {
+  if (dt == MFX_F32) {
+    typedef float run_t __attribute__((ext_vector_type(4), aligned(4)));
+    float* q = static_cast<float*>(p) + at;
+    if (left >= 4) {
+      *reinterpret_cast<run_t*>(q) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (j < left) q[j] = v[j];
+    }
+  } else {
+    typedef uint32_t run_t __attribute__((ext_vector_type(2), aligned(2)));
+    uint16_t* q = static_cast<uint16_t*>(p) + at;
+    uint32_t bits[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      bits[j] = dt == MFX_BF16 ? pack2<0>(v[2 * j], v[2 * j + 1]) : pack2<1>(v[2 * j], v[2 * j + 1]);
+    if (left >= 4) {
+      *reinterpret_cast<run_t*>(q) = run_t{bits[0], bits[1]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (j < left) q[j] = (uint16_t)(bits[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
+
+// What becomes of a tile's sums.  A wavefront goes through its block 32 rows at
+// a time, with fences and opaque row numbers between, so that no more than one
+// set of values and addresses is live beside the sums.
+template <class C, Mode MODE>
+__device__ __forceinline__ void finish(const ProdArgs& p, int64_t bz, int tm, int tn, char* smem, Acc<C>& acc) {
+  constexpr int FM = C::FM, FN = C::FN;
+  const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % C::WM, wn = wave / C::WM;
+  const int m0 = tm * C::BM + wm * FM * 32, n0 = tn * C::BN + wn * FN * 32;  // this wavefront's block
+  const int M = p.g.M, N = p.g.N;
+
+  if (MODE == kApply && p.out) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      int l = l32;
+      asm volatile("" : "+v"(l));
+      const int m = m0 + i * 32 + l;
+      if (m < M) {
+        const int64_t wrow = bz * p.ws_b + m * p.ws_r, orow = bz * p.os_b + m * p.os_r;
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int n = n0 + column(j, g * 4, half);
+            if (n >= N) continue;
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[j][i][g * 4 + e] * p.c1;
+            if (p.w) v += load4(p.w, p.out_dt, wrow + n, N - n) * p.keep;
+            store4(p.out, p.out_dt, orow + n, N - n, v);
+          }
+      }
+      fence();
+    }
+    return;
+  }
+
+  // Through LDS (the stages are free), each wavefront its own part: the leading
+  // terms' rows in 16-byte chunks along n, chunk k of row r at slot k ^ (r %
+  // chunks), and of a symmetric product off the diagonal the same transposed, 32
+  // chunks of m a row; then the second terms'.
+  constexpr int BLOCK = 32 * FN * 32;
+  uint16_t* const st = reinterpret_cast<uint16_t*>(smem + wave * (C::SMEM / C::NW));
+  static_assert(4 * BLOCK * 2 <= C::SMEM / C::NW, "a wavefront's four blocks");
+  const int M8 = (M + 7) & ~7, N8 = (N + 7) & ~7;
+  const bool turned = MODE != kApply && tm != tn;
+  uint16_t* const c = p.c + bz * p.cs;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    int l = l32;
+    asm volatile("" : "+v"(l));
+    const int m = m0 + i * 32 + l;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int n = n0 + column(j, g * 4, half);
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[j][i][g * 4 + e] * p.c1;
+        if constexpr (MODE == kSquare) {
+          f32x4 a = {0.f, 0.f, 0.f, 0.f};
+          if (m < M && n < N) {  // (A's rows are padded to whole chunks)
+            const uint16_t* from = static_cast<const uint16_t*>(p.g.a.p) + bz * p.as + (int64_t)m * p.g.a.ld + n;
+            a = load4(from, MFX_F16, 0, 4);
+            if (p.two) a += load4(from, MFX_F16, p.g.a.lo, 4);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(p.c2, a[e], v[e]) + (m == n + e ? p.c3 : 0.f);
+        }
+        uint16_t h[4], r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = m < M && n + e < N ? v[e] : 0.f;  // (zeros in the padding)
+          h[e] = lead(v[e]);
+          r[e] = lead(rest(v[e]));
+        }
+        const int ch = l * (FN * 32) + ((j * 4 + g) ^ (l & (FN * 4 - 1))) * 8 + half * 4;
+        *reinterpret_cast<u16x4*>(st + ch) = u16x4{h[0], h[1], h[2], h[3]};
+        if (p.two) *reinterpret_cast<u16x4*>(st + 2 * BLOCK + ch) = u16x4{r[0], r[1], r[2], r[3]};
+        if (turned) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int row = column(j, g * 4 + e, half);
+            const int at = row * 32 + ((l >> 3) ^ ((row >> 2) & 3)) * 8 + (l & 7);
+            st[BLOCK + at] = h[e];
+            if (p.two) st[3 * BLOCK + at] = r[e];
+          }
+        }
+      }
+    fence();
+    for (int term = 0; term <= p.two; ++term) {
+      uint16_t* const to = c + (term ? p.lo : 0);
+      const uint16_t* const from = st + term * 2 * BLOCK;
+      constexpr int CPR = FN * 4, RPS = 64 / CPR;
+#pragma unroll
+      for (int k = 0; k < 32 / RPS; ++k) {
+        const int r = k * RPS + lane / CPR, ch = lane % CPR, row = m0 + i * 32 + r;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(from + r * (FN * 32) + (ch ^ (r & (CPR - 1))) * 8);
+        if (row < M && n0 + ch * 8 < N8) *reinterpret_cast<u32x4*>(to + (int64_t)row * p.ldc + n0 + ch * 8) = v;
+      }
+      if (turned) {
+#pragma unroll
+        for (int k = 0; k < FN * 2; ++k) {
+          const int r = k * 16 + lane / 4, ch = lane % 4, row = n0 + r, col = m0 + i * 32 + ch * 8;
+          const u32x4 v = *reinterpret_cast<const u32x4*>(from + BLOCK + r * 32 + (ch ^ ((r >> 2) & 3)) * 8);
+          if (row < N && col < M8) *reinterpret_cast<u32x4*>(to + (int64_t)row * p.ldc + col) = v;
+        }
+      }
+    }
+    fence();
+  }
+}
+
+// This workgroup's place among `n`, dealt to the 8 XCDs in turn: each takes a
+// run of neighbours, which share operand panels in its L2.
+__device__ __forceinline__ int64_t dealt(int64_t id, int64_t n) {
+  const int64_t per = n >> 3, rest = n & 7, xcd = id & 7;
+  return (id >> 3) + xcd * per + min(xcd, rest);
+}
+
+template <class C, Mode MODE>
+__global__ __launch_bounds__(C::NT, C::WAVES) void ns_product(ProdArgs p) {
+  __shared__ __attribute__((aligned(16))) char smem[C::SMEM];
+  constexpr int PART = C::NT * C::FM * C::FN * 16;
+  Acc<C> acc;
+  auto sums = [&](int64_t tile, int kt0, int kt1, int& bz, int& tm, int& tn) __attribute__((always_inline)) {
+    bz = (int)(tile / p.tiles);
+    tile_of(p, (int)(tile - (int64_t)bz * p.tiles), tm, tn);
+    GemmShape g = p.g;
+    g.a.p = static_cast<const uint16_t*>(g.a.p) + bz * p.as;
+    g.b.p = static_cast<const uint16_t*>(g.b.p) + bz * p.bs;
+    gemm_tile16<C>(g, tm * C::BM, tn * C::BN, kt0, kt1, reinterpret_cast<bf16*>(smem), acc);
+    __syncthreads();  // the stages are free
+  };
+  int bz, tm, tn;
+  if ((int64_t)blockIdx.x < p.whole) {
+    sums(dealt(blockIdx.x, p.whole), 0, p.kt, bz, tm, tn);
+    finish<C, MODE>(p, bz, tm, tn, smem, acc);
+    return;
+  }
+  const int64_t w = dealt(blockIdx.x - p.whole, p.shares);
+  const int64_t units = (p.all - p.whole) * p.kt;
+  int64_t u = w * units / p.shares;
+  const int64_t end = (w + 1) * units / p.shares;
+  while (u < end) {
+    const int64_t tile = u / p.kt;
+    const int kt0 = (int)(u - tile * p.kt), kt1 = (int)min((int64_t)p.kt, kt0 + (end - u));
+    sums(p.whole + tile, kt0, kt1, bz, tm, tn);
+    // (Slot w + tile: through the units one of them grows at a time.)
+    f32x4* const to = reinterpret_cast<f32x4*>(p.part + (w + tile) * PART) + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          to[((j * C::FM + i) * 4 + q) * C::NT] =
+              f32x4{acc[j][i][q * 4], acc[j][i][q * 4 + 1], acc[j][i][q * 4 + 2], acc[j][i][q * 4 + 3]};
+    u += kt1 - kt0;
+  }
+}
+
+// The shared tiles: their partial sums in order, then what `finish` does.
+template <class C, Mode MODE>
+__global__ __launch_bounds__(C::NT, C::WAVES) void ns_join(ProdArgs p) {
+  __shared__ __attribute__((aligned(16))) char smem[C::SMEM];
+  constexpr int PART = C::NT * C::FM * C::FN * 16;
+  const int64_t tile = dealt(blockIdx.x, p.all - p.whole), units = (p.all - p.whole) * p.kt;
+  // Workgroups whose runs meet the tile's units [tile kt, (tile + 1) kt).
+  const int64_t u0 = tile * p.kt, u1 = u0 + p.kt;
+  int64_t w = u0 * p.shares / units;
+  while ((w + 1) * units / p.shares <= u0) ++w;
+  while (w > 0 && w * units / p.shares > u0) --w;
+  Acc<C> acc;
+#pragma unroll
+  for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
+  for (; w < p.shares && w * units / p.shares < u1; ++w) {
+    if ((w + 1) * units / p.shares <= w * units / p.shares) continue;  // (an empty run)
+    const f32x4* const from = reinterpret_cast<const f32x4*>(p.part + (w + tile) * PART) + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 v = from[((j * C::FM + i) * 4 + q) * C::NT];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][i][q * 4 + e] += v[e];
+        }
+  }
+  int bz, tm, tn;
+  const int64_t t = p.whole + tile;
+  bz = (int)(t / p.tiles);
+  tile_of(p, (int)(t - (int64_t)bz * p.tiles), tm, tn);
+  finish<C, MODE>(p, bz, tm, tn, smem, acc);
+}
+
+// ---- host ------------------------------------------------------------------------
+
+bool float_dtype(int dt) { return dt == MFX_F32 || dt == MFX_BF16 || dt == MFX_F16; }
+
+constexpr int64_t kMaxSide = int64_t(1) << 20;  // rows of a tile are addressed within 31 bits
+constexpr int kMaxSteps = 32;
+
+// How a product's tiles are shared out.
+struct Way {
+  Form form;
+  int64_t tiles, whole, shares;  // tiles of all matrices
+};
+
+// Microseconds of a k-tile with `slots` workgroups on each CU, and once for each
+// round of workgroups.
+struct Cost {
+  int slots;
+  float kt, each;
+};
+constexpr Cost kCost[3] = {{1, 0.85f, 9.f}, {2, 0.57f, 4.f}, {4, 0.42f, 3.f}};
+
+Way choose(int64_t B, int64_t M, int64_t N, int64_t K, bool symmetric, int terms) {
+  const int64_t cus = device_cu_count(), kt = ceil_div(K, kBK16) * terms;
+  Way best{};
+  float least = INFINITY;
+  for (int f = kWide; f <= kSlim; ++f) {
+    const Cost& c = kCost[f];
+    const int64_t side = kSide[f], tm = ceil_div(M, side), tn = ceil_div(N, side);
+    const int64_t tiles = B * (symmetric ? tm * (tm + 1) / 2 : tm * tn), slots = c.slots * cus;
+    const int64_t full = tiles / slots, rest = tiles % slots;
+    auto rounds = [&](float n, int64_t wgs) {
+      // (With fewer than `slots` workgroups on a CU each runs faster.)
+      const float busy = wgs >= slots ? 1.f : 0.25f + 0.75f * (float)ceil_div(wgs, cus) / (float)c.slots;
+      return n * ((float)kt * c.kt * busy) + c.each;
+    };
+    if (!launch_fits(tiles, 256)) continue;
+    float t = (float)full * ((float)kt * c.kt + c.each) + (rest ? rounds(1.f, rest) : 0.f);
+    if (t < least) {
+      least = t;
+      best = Way{(Form)f, tiles, tiles, 0};
+    }
+    // The tiles of the last, partly filled round shared out by their k-tiles, at
+    // least 12 to a workgroup; their sums are written and read again, and there is
+    // a launch more.
+    if (rest) {
+      const int64_t shares = std::min<int64_t>(slots, rest * kt / 12);
+      if (shares <= rest) continue;
+      t = (float)full * ((float)kt * c.kt + c.each) + rounds((float)rest / (float)shares, shares) +
+          6.f + (float)(shares + rest) * (float)(side * side) * 8.f / 4e6f;
+      if (t < least) {
+        least = t;
+        best = Way{(Form)f, tiles, tiles - rest, shares};
+      }
+    }
+  }
+  return best;
+}
+
+size_t part_bytes(const Way& w) {
+  return w.shares ? (size_t)(w.shares + w.tiles - w.whole) * kSide[w.form] * kSide[w.form] * 4 : 0;
+}
+
+struct Plan {
+  int64_t B, m, n, s, l, ld, lds;  // the matrix, its smaller and larger side, rows of X and of A
+  bool wide;
+  int two, steps, parts;
+  Way gram, square, apply;
+  size_t norm_bytes, x_bytes, a_bytes, part, total;
+  float ex[kMaxSteps + 1], ea[kMaxSteps], eq[kMaxSteps];  // the powers of two that X, A, Q are stored at
+};
+
+// The largest power of two that keeps values up to `most` within f16.
+float fit(double most) { return (float)std::exp2(std::floor(std::log2(60000.0 / most))); }
+
+// Bounds of the iterates' norms: X starts at 1 or less; over the spectrum [0, u]
+// of X the polynomials' largest values are at its end or where a derivative is 0.
+int plan_scales(Plan& pl, const float* coeffs, int num) {
+  double u = 1.0;
+  for (int i = 0; i < pl.steps; ++i) {
+    const float* k = coeffs + 3 * (num == 1 ? 0 : i);
+    const double a = k[0], b = k[1], c = k[2];
+    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return fail(MFX_E_INVALID, "coefficients must be finite");
+    u *= 1.01;  // (what rounding adds)
+    const double top = u * u;
+    auto q = [&](double s) { return std::fabs(a + b * s + c * s * s); };
+    double qm = std::max(q(0.0), q(top));
+    if (c != 0.0) {
+      const double s = -b / (2.0 * c);
+      if (s > 0.0 && s < top) qm = std::max(qm, q(s));
+    }
+    double next = std::sqrt(top) * q(top);
+    auto visit = [&](double s) {
+      if (s > 0.0 && s < top) next = std::max(next, std::sqrt(s) * q(s));
+    };
+    // d/dx of x (a + b x^2 + c x^4) is 0 at a + 3 b s + 5 c s^2 = 0.
+    if (c != 0.0) {
+      const double d = 9.0 * b * b - 20.0 * a * c;
+      if (d >= 0.0) {
+        visit((-3.0 * b + std::sqrt(d)) / (10.0 * c));
+        visit((-3.0 * b - std::sqrt(d)) / (10.0 * c));
+      }
+    } else if (b != 0.0) {
+      visit(-a / (3.0 * b));
+    }
+    if (!(qm <= 256.0) || !(next <= 16.0))
+      return fail(MFX_E_UNSUPPORTED, "the coefficients let the iteration grow too large");
+    pl.ex[i] = fit(u);
+    pl.ea[i] = fit(top);
+    pl.eq[i] = fit(std::max(qm, 1.0 / 256.0));
+    u = std::max(next, 1.0 / 16.0);
+  }
+  pl.ex[pl.steps] = 1.f;  // (the result is not stored in terms)
+  return MFX_OK;
+}
+
+int plan_common(Plan& pl, int64_t B, int64_t m, int64_t n, int64_t steps, const float* coeffs, int num_coeffs, float eps,
+                int terms, bool bf16_result) {
+  if (B < 0 || m <= 0 || n <= 0) return fail(MFX_E_INVALID, "batch must be >= 0, m and n positive");
+  if (steps < 1 || !coeffs || (num_coeffs != 1 && num_coeffs != steps))
+    return fail(MFX_E_INVALID, "steps must be >= 1, coefficients for all steps or for each");
+  if (steps > kMaxSteps) return fail(MFX_E_UNSUPPORTED, "more than 32 steps are not supported");
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(MFX_E_INVALID, "eps must be finite and >= 0");
+  if (terms < 0 || terms > 2) return fail(MFX_E_INVALID, "terms must be 0, 1 or 2");
+  if (m > kMaxSide || n > kMaxSide || m * ceil_div(n, 8) > 0x7fffffffLL - 0x1000000 || B > 65535)
+    return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
+  pl.B = B, pl.m = m, pl.n = n;
+  pl.wide = m <= n;
+  pl.s = std::min(m, n), pl.l = std::max(m, n);
+  pl.ld = ceil_div(n, 8) * 8;
+  pl.lds = ceil_div(pl.s, 8) * 8;
+  pl.steps = (int)steps;
+  // One term for bf16 results (their own rounding is larger than its error), and
+  // not for sides whose products are over in no time either way.
+  pl.two = terms == 0 ? !(bf16_result && pl.s >= 256) : terms == 2;
+  if (int rc = plan_scales(pl, coeffs, num_coeffs)) return rc;
+  if (B == 0) return MFX_OK;
+  const int t = pl.two ? 3 : 1;
+  pl.gram = choose(B, pl.s, pl.s, pl.l, true, t);
+  pl.square = choose(B, pl.s, pl.s, pl.s, true, t);
+  pl.apply = choose(B, m, n, pl.s, false, t);
+  if (!pl.gram.tiles || !pl.square.tiles || !pl.apply.tiles)
+    return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
+  if (!launch_fits(B * std::min<int64_t>(2048, ceil_div(m * (pl.ld / 8), 256)), 256))
+    return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
+  // Parts of a matrix's sum of squares: of 1024 chunks or more, at most one a thread of ns_split.
+  pl.parts = (int)std::min<int64_t>(256, ceil_div(m * (pl.ld / 8), 1024));
+  pl.norm_bytes = align256((size_t)B * pl.parts * 8);
+  pl.x_bytes = align256((size_t)B * m * pl.ld * 2 * (1 + pl.two));
+  pl.a_bytes = align256((size_t)B * pl.s * pl.lds * 2 * (1 + pl.two));
+  pl.part = align256(std::max(part_bytes(pl.gram), std::max(part_bytes(pl.square), part_bytes(pl.apply))));
+  pl.total = pl.norm_bytes + 2 * pl.x_bytes + 2 * pl.a_bytes + pl.part;
+  return MFX_OK;
+}
+
+template <class C, Mode MODE>
+int launch(const ProdArgs& p, hipStream_t s) {
+  hipLaunchKernelGGL((ns_product<C, MODE>), dim3((unsigned)(p.whole + p.shares)), dim3(C::NT), 0, s, p);
+  return launch_status("ns_product");
+}
+
+template <int SIDE, Mode MODE>
+int launch_side(const ProdArgs& p, bool a_kc, bool b_kc, hipStream_t s) {
+  int rc;
+  if (!a_kc) {
+    // (Only a tall matrix's gram product reads columns of both.)
+    if constexpr (MODE == kGram)
+      rc = p.two ? launch<Cfg<SIDE, false, false, 3>, MODE>(p, s) : launch<Cfg<SIDE, false, false, 1>, MODE>(p, s);
+    else
+      return fail(MFX_E_INVALID, "no such product");
+  } else if (!b_kc) {
+    if constexpr (MODE == kApply)
+      rc = p.two ? launch<Cfg<SIDE, true, false, 3>, MODE>(p, s) : launch<Cfg<SIDE, true, false, 1>, MODE>(p, s);
+    else
+      return fail(MFX_E_INVALID, "no such product");
+  } else {
+    rc = p.two ? launch<Cfg<SIDE, true, true, 3>, MODE>(p, s) : launch<Cfg<SIDE, true, true, 1>, MODE>(p, s);
+  }
+  if (rc || !p.shares) return rc;
+  typedef Cfg<SIDE, true, true, 1> J;
+  hipLaunchKernelGGL((ns_join<J, MODE>), dim3((unsigned)(p.all - p.whole)), dim3(J::NT), 0, s, p);
+  return launch_status("ns_join");
+}
+
+template <Mode MODE>
+int product(ProdArgs& p, const Way& way, int64_t B, int64_t M, int64_t N, int64_t K, bool a_kc, bool b_kc, float* part,
+            hipStream_t s) {
+  const int side = kSide[way.form];
+  p.g.M = (int)M, p.g.N = (int)N, p.g.K = (int)K;
+  p.g.tiles_m = (int)ceil_div(M, side), p.g.tiles_n = (int)ceil_div(N, side);
+  p.symmetric = MODE != kApply;
+  p.tiles = way.tiles / B, p.all = way.tiles, p.whole = way.whole, p.shares = way.shares;
+  p.kt = (int)ceil_div(K, kBK16) * (p.two ? 3 : 1);
+  p.part = part;
+  if (way.form == kWide) return launch_side<256, MODE>(p, a_kc, b_kc, s);
+  if (way.form == kNarrow) return launch_side<128, MODE>(p, a_kc, b_kc, s);
+  return launch_side<64, MODE>(p, a_kc, b_kc, s);
+}
+
+// Everything behind the checks.  in: g, buf and their strides; last: where the result goes.
+int run(const Plan& pl, InArgs in, const float* coeffs, int num_coeffs, const ProdArgs& last, float scale, char* ws,
+        hipStream_t s) {
+  double* const norm = reinterpret_cast<double*>(ws);
+  uint16_t* x[2];
+  x[0] = reinterpret_cast<uint16_t*>(ws + pl.norm_bytes);
+  x[1] = reinterpret_cast<uint16_t*>(ws + pl.norm_bytes + pl.x_bytes);
+  uint16_t* const a = reinterpret_cast<uint16_t*>(ws + pl.norm_bytes + 2 * pl.x_bytes);
+  uint16_t* const q = reinterpret_cast<uint16_t*>(ws + pl.norm_bytes + 2 * pl.x_bytes + pl.a_bytes);
+  float* const part = reinterpret_cast<float*>(ws + pl.norm_bytes + 2 * pl.x_bytes + 2 * pl.a_bytes);
+  const int64_t xs = pl.m * pl.ld, as = pl.s * pl.lds;
+  in.norm = norm;
+  in.x = x[0];
+  in.lo = pl.B * xs;
+  in.m = (int)pl.m, in.n = (int)pl.n, in.ld = (int)pl.ld, in.parts = pl.parts, in.two = pl.two;
+  in.scale = pl.ex[0];
+  hipLaunchKernelGGL(ns_norm, dim3(pl.parts, (unsigned)pl.B), dim3(256), 0, s, in);
+  if (int rc = launch_status("ns_norm")) return rc;
+  const int64_t chunks = ceil_div(pl.m * (pl.ld / 8), 256);
+  hipLaunchKernelGGL(ns_split, dim3((unsigned)std::min<int64_t>(chunks, 2048), (unsigned)pl.B), dim3(256), 0, s, in);
+  if (int rc = launch_status("ns_split")) return rc;
+  for (int i = 0; i < pl.steps; ++i) {
+    const float* k = coeffs + 3 * (num_coeffs == 1 ? 0 : i);
+    const float ex = pl.ex[i], ea = pl.ea[i], eq = pl.eq[i];
+    const Operand X{x[i & 1], pl.ld, pl.B * xs}, A{a, pl.lds, pl.B * as}, Q{q, pl.lds, pl.B * as};
+    ProdArgs p{};
+    p.two = pl.two;
+    p.g.a = p.g.b = X;
+    p.as = p.bs = xs;
+    p.c = a, p.ldc = pl.lds, p.cs = as, p.lo = pl.B * as;
+    p.c1 = ea / (ex * ex);
+    if (int rc = product<kGram>(p, pl.gram, pl.B, pl.s, pl.s, pl.l, pl.wide, pl.wide, part, s)) return rc;
+    p.g.a = p.g.b = A;
+    p.as = p.bs = as;
+    p.c = q;
+    p.c1 = k[2] * eq / (ea * ea);
+    p.c2 = k[1] * eq / ea;
+    p.c3 = k[0] * eq;
+    if (int rc = product<kSquare>(p, pl.square, pl.B, pl.s, pl.s, pl.s, true, true, part, s)) return rc;
+    if (i + 1 == pl.steps) {
+      p = last;
+      p.two = pl.two;
+      p.c1 = scale / (eq * ex);
+    } else {
+      p.c = x[(i + 1) & 1], p.ldc = pl.ld, p.cs = xs, p.lo = pl.B * xs;
+      p.c1 = pl.ex[i + 1] / (eq * ex);
+    }
+    // Wide: Q's rows by X's columns; tall: X's rows by Q's (Q is symmetric).
+    p.g.a = pl.wide ? Q : X, p.as = pl.wide ? as : xs;
+    p.g.b = pl.wide ? X : Q, p.bs = pl.wide ? xs : as;
+    if (int rc = product<kApply>(p, pl.apply, pl.B, pl.m, pl.n, pl.s, true, !pl.wide, part, s)) return rc;
+  }
+  return MFX_OK;
+}
+
+int bind(const void* p, int64_t row, int64_t batch, const Plan& pl, int dt, const char* what, bool written) {
+  if (!float_dtype(dt)) return fail(MFX_E_UNSUPPORTED, std::string(what) + ": dtype must be f32, bf16 or f16");
+  if (pl.B == 0) return MFX_OK;
+  if (!p) return fail(MFX_E_INVALID, std::string(what) + " must be non-null");
+  if ((uintptr_t)p % dtype_size(dt)) return fail(MFX_E_INVALID, std::string(what) + " must be aligned to its type");
+  if (pl.m > 1 && row < (written ? pl.n : 0)) return fail(MFX_E_INVALID, std::string(what) + ": row stride too small");
+  if (pl.B > 1 && (batch < 0 || (written && batch < (pl.m - 1) * row + pl.n)))
+    return fail(MFX_E_INVALID, std::string(what) + ": matrices must not overlap");
+  return MFX_OK;
+}
+
+int plan_ns(const mfx_newton_schulz_args* a, Plan& pl) {
+  if (!a) return fail(MFX_E_INVALID, "null args");
+  if (int rc = plan_common(pl, a->batch, a->m, a->n, a->steps, a->coeffs, a->num_coeffs, a->eps, a->terms,
+                           a->out_dtype == MFX_BF16))
+    return rc;
+  if (!std::isfinite(a->scale)) return fail(MFX_E_INVALID, "scale must be finite");
+  if (int rc = bind(a->g, a->g_row_stride, a->g_batch_stride, pl, a->dtype, "g", false)) return rc;
+  return bind(a->out, a->out_row_stride, a->out_batch_stride, pl, a->out_dtype, "out", true);
+}
+
+int plan_muon(const mfx_muon_update_args* a, Plan& pl) {
+  if (!a) return fail(MFX_E_INVALID, "null args");
+  if (int rc = plan_common(pl, a->batch, a->m, a->n, a->steps, a->coeffs, a->num_coeffs, a->eps, a->terms,
+                           a->w_dtype == MFX_BF16))
+    return rc;
+  if (!std::isfinite(a->lr) || !std::isfinite(a->scale) || !std::isfinite(a->weight_decay))
+    return fail(MFX_E_INVALID, "lr, scale and weight_decay must be finite");
+  if (!(a->mu >= 0.f && a->mu <= 1.f)) return fail(MFX_E_INVALID, "mu must be within [0, 1]");
+  if (int rc = bind(a->g, a->g_row_stride, a->g_batch_stride, pl, a->dtype, "g", false)) return rc;
+  if (int rc = bind(a->w, a->w_row_stride, a->w_batch_stride, pl, a->w_dtype, "w", false)) return rc;
+  if (int rc = bind(a->w_out, a->w_out_row_stride, a->w_out_batch_stride, pl, a->w_dtype, "w_out", true)) return rc;
+  if ((a->momentum == nullptr) != (a->momentum_out == nullptr))
+    return fail(MFX_E_INVALID, "momentum and momentum_out go together");
+  if (!a->momentum) return MFX_OK;
+  if (int rc = bind(a->momentum, a->momentum_row_stride, a->momentum_batch_stride, pl, a->momentum_dtype, "momentum", false))
+    return rc;
+  return bind(a->momentum_out, a->momentum_out_row_stride, a->momentum_out_batch_stride, pl, a->momentum_dtype,
+              "momentum_out", true);
+}
+
+}  // namespace
+}  // namespace ns
+}  // namespace mfx
+
+extern "C" {
+
+size_t mfx_newton_schulz_workspace_size(const mfx_newton_schulz_args* args) {
+  mfx::ns::Plan pl{};
+  return mfx::ns::plan_ns(args, pl) == MFX_OK ? pl.total : 0;
+}
+
+int mfx_newton_schulz(const mfx_newton_schulz_args* args, void* stream) {
+  using namespace mfx;
+  using namespace mfx::ns;
+  Plan pl{};
+  if (int rc = plan_ns(args, pl)) return rc;
+  const mfx_newton_schulz_args& a = *args;
+  if (a.batch == 0) return MFX_OK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = nullptr;
+  if (int rc = take_workspace(a.workspace, a.workspace_bytes, pl.total, "mfx_newton_schulz_workspace_size", s, &ws))
+    return rc;
+  InArgs in{};
+  in.g = a.g, in.gs_b = a.g_batch_stride, in.gs_r = a.g_row_stride, in.g_dt = a.dtype;
+  in.eps = a.eps;
+  ProdArgs last{};
+  last.out = a.out, last.out_dt = a.out_dtype, last.os_b = a.out_batch_stride, last.os_r = a.out_row_stride;
+  return run(pl, in, a.coeffs, a.num_coeffs, last, a.scale, ws, s);
+}
+
+size_t mfx_muon_update_workspace_size(const mfx_muon_update_args* args) {
+  mfx::ns::Plan pl{};
+  return mfx::ns::plan_muon(args, pl) == MFX_OK ? pl.total : 0;
+}
+
+int mfx_muon_update(const mfx_muon_update_args* args, void* stream) {
+  using namespace mfx;
+  using namespace mfx::ns;
+  Plan pl{};
+  if (int rc = plan_muon(args, pl)) return rc;
+  const mfx_muon_update_args& a = *args;
+  if (a.batch == 0) return MFX_OK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = nullptr;
+  if (int rc = take_workspace(a.workspace, a.workspace_bytes, pl.total, "mfx_muon_update_workspace_size", s, &ws))
+    return rc;
+  InArgs in{};
+  in.g = a.g, in.gs_b = a.g_batch_stride, in.gs_r = a.g_row_stride, in.g_dt = a.dtype;
+  in.buf = a.momentum, in.bs_b = a.momentum_batch_stride, in.bs_r = a.momentum_row_stride, in.buf_dt = a.momentum_dtype;
+  in.buf_out = a.momentum_out, in.os_b = a.momentum_out_batch_stride, in.os_r = a.momentum_out_row_stride;
+  in.eps = a.eps, in.mu = a.mu, in.nesterov = a.nesterov != 0;
+  ProdArgs last{};
+  last.out = a.w_out, last.out_dt = a.w_dtype, last.os_b = a.w_out_batch_stride, last.os_r = a.w_out_row_stride;
+  last.w = a.w, last.ws_b = a.w_batch_stride, last.ws_r = a.w_row_stride;
+  last.keep = 1.f - a.lr * a.weight_decay;
+  return run(pl, in, a.coeffs, a.num_coeffs, last, -a.lr * a.scale, ws, s);
+}
+
+}  // extern "C"

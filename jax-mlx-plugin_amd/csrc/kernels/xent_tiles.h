@@ -1,5 +1,6 @@
-// Shapes shared by the product kernels of the linear cross entropy
-// (xent_gemm16.h, xent_gemm32.h) and their epilogues (linear_xent.hip).
+// Shapes shared by the product kernels of the linear cross entropy and of the
+// Newton-Schulz iteration (xent_gemm16.h, xent_gemm32.h) and their epilogues
+// (linear_xent.hip, newton_schulz.hip).
 #pragma once
 
 #include "sdpa_elem.h"
@@ -12,6 +13,7 @@ constexpr int kBK16 = 32, kBK32 = 32;  // k per tile
 struct Operand {
   const void* p;
   int64_t ld;  // elements from one row (k-contiguous: index; else k) to the next
+  int64_t lo;  // two terms: elements from the leading terms to the second ones
 };
 
 struct GemmShape {
@@ -48,6 +50,10 @@ struct Config {
   static constexpr int WAVES = BM == 256 ? 1 : BM == 128 ? 2 : BM == 64 ? 3 : 4;  // per SIMD
   static constexpr int FM = BM / (32 * WM), FN = BN / (32 * WN);  // blocks of a wavefront
   static constexpr int BK = E == 2 ? kBK32 : kBK16;
+  // Products of terms, one behind the other along k: one, or of operands held
+  // in two terms each the three that matter (xent_gemm16.h).
+  static constexpr int TERMS = 1;
+  static constexpr bool ROT = BM == 64 && A_KC && B_KC;
   // Bytes of a stage, and of all: four in 16 bits; f32: two, in the larger of
   // the two forms' padded rows (xent_gemm32.h).
   static constexpr int STAGE = E == 2 ? 2 * BM * (kBK32 + (BM < 128 ? 8 : 4)) * 4 : (BM + BN) * kBK16 * 2;

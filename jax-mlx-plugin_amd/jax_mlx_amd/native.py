@@ -274,6 +274,31 @@ class ResidualNormBwdArgs(ctypes.Structure):
                 + _RESIDUAL_SCALARS)
 
 
+class NewtonSchulzArgs(ctypes.Structure):
+    """mfx_newton_schulz_args (include/mfx_kernels.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("g", "out", "coeffs", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int64) for n in ("batch", "m", "n", "g_batch_stride", "g_row_stride",
+                                                 "out_batch_stride", "out_row_stride")]
+                + [(n, ctypes.c_float) for n in ("eps", "scale")]
+                + [(n, ctypes.c_int32) for n in ("steps", "num_coeffs", "dtype", "out_dtype", "terms", "reserved")])
+
+
+class MuonUpdateArgs(ctypes.Structure):
+    """mfx_muon_update_args (include/mfx_kernels.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("g", "w", "w_out", "momentum", "momentum_out", "coeffs", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int64) for n in ("batch", "m", "n", "g_batch_stride", "g_row_stride", "w_batch_stride",
+                                                 "w_row_stride", "w_out_batch_stride", "w_out_row_stride",
+                                                 "momentum_batch_stride", "momentum_row_stride",
+                                                 "momentum_out_batch_stride", "momentum_out_row_stride")]
+                + [(n, ctypes.c_float) for n in ("lr", "mu", "weight_decay", "scale", "eps")]
+                + [(n, ctypes.c_int32) for n in ("nesterov", "steps", "num_coeffs", "dtype", "w_dtype",
+                                                 "momentum_dtype", "terms")])
+
+
 MFX_MAX_RANK = 8
 MFX_EW_MAX_INPUTS = 8
 MFX_EW_MAX_INSTRS = 64
@@ -380,7 +405,8 @@ def load(path: str | os.PathLike | None = None, make_default: bool = False) -> c
         getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
         getattr(lib, name).restype = ctypes.c_int
     for name, args in (("mfx_linear_xent", LinearXentArgs), ("mfx_linear_xent_bwd", LinearXentBwdArgs),
-                       ("mfx_embedding_bwd", EmbeddingBwdArgs), ("mfx_residual_norm_bwd", ResidualNormBwdArgs)):
+                       ("mfx_embedding_bwd", EmbeddingBwdArgs), ("mfx_residual_norm_bwd", ResidualNormBwdArgs),
+                       ("mfx_newton_schulz", NewtonSchulzArgs), ("mfx_muon_update", MuonUpdateArgs)):
         getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name + "_workspace_size").argtypes = [ctypes.POINTER(args)]
@@ -1281,6 +1307,93 @@ def residual_norm_bwd(x, y, dr, dh, *, gate=None, seq_offsets=None, post_weight=
         keep = _workspace(a, "mfx_residual_norm_bwd_workspace_size", workspace, x)  # noqa: F841 (until the launch)
         check(load().mfx_residual_norm_bwd(ctypes.byref(a), _stream_handle(x)))
     return dx, dy, dg, dp, dn
+
+
+# ---- orthogonalised updates ------------------------------------------------------
+
+# A quintic whose steps take singular values from 1/500 and up to within 0.7 .. 1.2.
+NEWTON_SCHULZ_COEFFS = (3.4445, -4.7750, 2.0315)
+
+_NS_PACK = struct.Struct("4PN7q2f6i").pack
+_MUON_PACK = struct.Struct("7PN13q5f7i").pack
+
+
+def _matrices(name, t, like=None):
+    """(batch, row) strides of matrices [m, n] or [batch, m, n]."""
+    if t.dim() not in (2, 3) or t.shape[-2] == 0 or t.shape[-1] == 0:
+        raise ValueError(f"{name} must be [m, n] or [batch, m, n]")
+    if like is not None and t.shape != like.shape:
+        raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(t.shape)}")
+    s = t.stride()
+    n = t.shape[-1]
+    if s[-1] != 1 and n > 1:
+        raise ValueError(f"{name}: last dimension must be contiguous")
+    row = s[-2] if t.shape[-2] > 1 else n
+    return s[0] if len(s) == 3 and t.shape[0] > 1 else t.shape[-2] * row, row
+
+
+def _ns_coeffs(coeffs, steps):
+    """(host array, number of triples)."""
+    flat = [float(x) for c in coeffs for x in (c if isinstance(c, (tuple, list)) else (c,))]
+    if len(flat) not in (3, 3 * steps):
+        raise ValueError("coeffs are three numbers, or three for each step")
+    return (ctypes.c_float * len(flat))(*flat), len(flat) // 3
+
+
+def newton_schulz(g, *, steps=5, coeffs=NEWTON_SCHULZ_COEFFS, eps=1e-7, scale=1.0, out_dtype=None, out=None, terms=0,
+                  workspace=None):
+    """scale times the orthogonalised matrix of g [m, n], or of each of [batch,
+    m, n], by `steps` Newton-Schulz steps from g / (|g| + eps)
+    (mfx_newton_schulz), in g's dtype, out_dtype, or that of a given out (which
+    may be g).  coeffs: (a, b, c) of every step, or one triple for each.  terms: 2
+    computes as products of f32 matrices do, 1 three times as fast to within 3e-3;
+    0 takes 1 for bf16 results of sides from 256 on, else 2."""
+    torch = _torch()
+    gs = _matrices("g", g)
+    if out is None:
+        out = torch.empty(g.shape, dtype=out_dtype or g.dtype, device=g.device)
+    cs, num = _ns_coeffs(coeffs, steps)
+    a = NewtonSchulzArgs.from_buffer_copy(_NS_PACK(
+        g.data_ptr(), out.data_ptr(), ctypes.addressof(cs), 0, 0, g.shape[0] if g.dim() == 3 else 1, g.shape[-2],
+        g.shape[-1], *gs, *_matrices("out", out, g), _f32(eps), _f32(scale), steps, num, dtype_code(g.dtype),
+        dtype_code(out.dtype), terms, 0))
+    with _on(g, out, workspace):
+        keep = _workspace(a, "mfx_newton_schulz_workspace_size", workspace, g)  # noqa: F841 (until the launch)
+        check(load().mfx_newton_schulz(ctypes.byref(a), _stream_handle(g)))
+    return out
+
+
+def muon_update(w, g, momentum=None, *, lr, mu=0.95, nesterov=True, weight_decay=0.0, scale=1.0, steps=5,
+                coeffs=NEWTON_SCHULZ_COEFFS, eps=1e-7, terms=0, w_out=None, momentum_out=None, workspace=None):
+    """(w, momentum) after one step (mfx_muon_update), in place unless w_out,
+    momentum_out are given: momentum = mu momentum + (1 - mu) g, u the same once
+    more with nesterov (else the momentum; without one g), and w = (1 - lr
+    weight_decay) w - lr scale newton_schulz(u).  [m, n] or a stack [batch, m, n];
+    w, g and momentum each f32, bf16 or f16."""
+    gs = _matrices("g", g, w)
+    w_out = w if w_out is None else w_out
+    if w_out.dtype != w.dtype:
+        raise ValueError("w_out must have w's dtype")
+    ms = mos = (0, 0)
+    if momentum is None:
+        if momentum_out is not None:
+            raise ValueError("momentum_out needs a momentum")
+    else:
+        momentum_out = momentum if momentum_out is None else momentum_out
+        if momentum_out.dtype != momentum.dtype:
+            raise ValueError("momentum_out must have momentum's dtype")
+        ms, mos = _matrices("momentum", momentum, w), _matrices("momentum_out", momentum_out, w)
+    cs, num = _ns_coeffs(coeffs, steps)
+    a = MuonUpdateArgs.from_buffer_copy(_MUON_PACK(
+        g.data_ptr(), w.data_ptr(), w_out.data_ptr(), _ptr(momentum), _ptr(momentum_out), ctypes.addressof(cs), 0, 0,
+        w.shape[0] if w.dim() == 3 else 1, w.shape[-2], w.shape[-1], *gs, *_matrices("w", w),
+        *_matrices("w_out", w_out, w), *ms, *mos, _f32(lr), _f32(mu), _f32(weight_decay), _f32(scale), _f32(eps),
+        1 if nesterov else 0, steps, num, dtype_code(g.dtype), dtype_code(w.dtype),
+        dtype_code((g if momentum is None else momentum).dtype), terms))
+    with _on(w, g, w_out, momentum, momentum_out, workspace):
+        keep = _workspace(a, "mfx_muon_update_workspace_size", workspace, w)  # noqa: F841 (until the launch)
+        check(load().mfx_muon_update(ctypes.byref(a), _stream_handle(w)))
+    return w_out, momentum_out
 
 
 # ---- GEMM ----------------------------------------------------------------------
