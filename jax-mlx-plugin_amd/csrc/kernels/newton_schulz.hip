@@ -15,7 +15,7 @@
 // only the tiles on and below the diagonal and store each twice.
 //
 // Precision.  The products' operands are f16, in one term or in two (a leading
-// one and what it leaves out: 22 bits, three products for one, xent_gemm16.h), all
+// one and what it leaves out: 22 bits, three products for one, pair_gemm16.h), all
 // sums fp32.  X, A and Q are stored times powers of two that the host derives from
 // the bound that the coefficients give their norms, so that no entry overflows
 // and the second terms stay clear of the smallest f16.  A singular value that
@@ -33,7 +33,7 @@
 
 #include "rowvec.h"
 #include "workspace.h"
-#include "xent_gemm16.h"
+#include "pair_gemm16.h"
 
 namespace mfx {
 namespace ns {
@@ -64,6 +64,12 @@ __device__ __forceinline__ void load8(const void* p, int dt, int64_t at, int e, 
   if (dt == MFX_F32) load_run<float, 8>(static_cast<const float*>(p) + at, e, n, 0.f, out);
   else if (dt == MFX_BF16) load_run<bf16, 8>(static_cast<const bf16*>(p) + at, e, n, 0.f, out);
   else load_run<_Float16, 8>(static_cast<const _Float16*>(p) + at, e, n, 0.f, out);
+}
+
+__device__ __forceinline__ void store8(void* p, int dt, int64_t at, int e, int n, const float (&v)[8]) {
+  if (dt == MFX_F32) store_run<float, 8>(static_cast<float*>(p) + at, e, n, v);
+  else if (dt == MFX_BF16) store_run<bf16, 8>(static_cast<bf16*>(p) + at, e, n, v);
+  else store_run<_Float16, 8>(static_cast<_Float16*>(p) + at, e, n, v);
 }
 
 // The chunk's U, and in `b` the new momentum.
@@ -102,15 +108,15 @@ __global__ __launch_bounds__(256) void ns_norm(InArgs a) {
   if (threadIdx.x == 0) a.norm[(int64_t)blockIdx.y * a.parts + blockIdx.x] = s;
 }
 
-// x in one or two f16 terms.
-__device__ __forceinline__ uint16_t lead(float x) { return store_e<1>(x); }
+// What the leading f16 term of x leaves out.
 __device__ __forceinline__ float rest(float x) { return x - (float)static_cast<f16>(x); }
 
 // X = U / (|U| + eps), and the momentum.
 __global__ __launch_bounds__(256) void ns_split(InArgs a) {
   __shared__ double lds[4];
-  // (At most 256 parts, one a thread; the same order in every workgroup.)
-  const double sum = block_sum((int)threadIdx.x < a.parts ? a.norm[(int64_t)blockIdx.y * a.parts + threadIdx.x] : 0.0, lds);
+  double sum = 0.0;  // (the same order in every workgroup)
+  for (int i = threadIdx.x; i < a.parts; i += 256) sum += a.norm[(int64_t)blockIdx.y * a.parts + i];
+  sum = block_sum(sum, lds);
   const float f = (float)(a.scale / (sqrt(sum) + (double)a.eps));
   const uint32_t cpr = (uint32_t)a.ld / 8, units = (uint32_t)a.m * cpr;
   uint16_t* const x = a.x + (int64_t)blockIdx.y * a.m * a.ld;
@@ -119,12 +125,7 @@ __global__ __launch_bounds__(256) void ns_split(InArgs a) {
     const int e = (int)(i - row * cpr) * 8;
     float u[8], b[8];
     take(a, blockIdx.y, (int)row, e, u, b);
-    if (a.buf) {
-      const int64_t at = (int64_t)blockIdx.y * a.os_b + row * a.os_r;
-      if (a.buf_dt == MFX_F32) store_run<float, 8>(static_cast<float*>(a.buf_out) + at, e, a.n, b);
-      else if (a.buf_dt == MFX_BF16) store_run<bf16, 8>(static_cast<bf16*>(a.buf_out) + at, e, a.n, b);
-      else store_run<_Float16, 8>(static_cast<_Float16*>(a.buf_out) + at, e, a.n, b);
-    }
+    if (a.buf) store8(a.buf_out, a.buf_dt, (int64_t)blockIdx.y * a.os_b + row * a.os_r, e, a.n, b);
     // (Zeros in the columns past n: 0 times a factor that may be infinite would not be.)
 #pragma unroll
     for (int j = 0; j < 8; ++j) u[j] = e + j < a.n ? u[j] * f : 0.f;
@@ -145,10 +146,17 @@ enum Mode { kGram, kSquare, kApply };
 enum Form { kWide, kNarrow, kSlim };
 constexpr int kSide[3] = {256, 128, 64};
 
-template <int SIDE, bool A_KC, bool B_KC, int T>
+// k of a tile: 32 of one term or, of small tiles, whose few products would not
+// cover taking up the next one, of two; else 16 of two.
+constexpr int depth(Form f, bool two) { return two && f != kSlim ? 16 : 32; }
+
+template <int SIDE, bool A_KC, bool B_KC, bool P>
 struct Cfg : Config<SIDE, SIDE, SIDE == 64 ? 1 : 2, 2, A_KC, B_KC, 1> {
-  static constexpr int TERMS = T;
+  static constexpr bool PAIR = P;  // operands in two terms
   static constexpr bool ROT = false;
+  static constexpr int STAGES = 4;
+  static constexpr int BK = depth(SIDE == 64 ? kSlim : kWide, P);
+  static constexpr int SMEM = STAGES * 4 * SIDE * BK * (1 + P);
 };
 
 struct ProdArgs {
@@ -157,10 +165,11 @@ struct ProdArgs {
   int64_t tiles, all;   // tiles of a matrix and of all
   int kt;               // k-tiles of a tile
   int symmetric, two;
-  // Whole tiles first, a workgroup each; then `shares` workgroups share the k-tiles
-  // of the others evenly, each a run of them, and leave partial sums.
-  int64_t whole, shares;
-  float* part;          // [shares + tiles shared][NT * FM * FN * 16]
+  // Whole tiles first, a workgroup each; then of each other tile `splits` ranges of
+  // `per` k-tiles, which leave partial sums.
+  int64_t whole;
+  int splits, per;
+  float* part;          // [splits][tiles split][NT * FM * FN * 16]
   float c1, c2, c3;     // gram, apply: c1 C;  square: c1 C + c2 A + c3 I
   // Result in f16 terms ...
   uint16_t* c;          // [rows][ldc]
@@ -173,200 +182,152 @@ struct ProdArgs {
   float keep;
 };
 
-// Tile t of a matrix.
+// Tile t of a matrix, in bands of 8 tile rows (of 4 where only the lower triangle
+// is there) walked column by column, so that the tiles at work on an XCD share
+// operand panels in its L2.
 __device__ __forceinline__ void tile_of(const ProdArgs& p, int t, int& tm, int& tn) {
   if (!p.symmetric) {
-    // Bands of 8 tile rows, so that the tiles at work share operand panels.
     const int band = 8 * p.g.tiles_n, b = t / band, rows = min(8, p.g.tiles_m - b * 8);
     t -= b * band;
     tm = b * 8 + t % rows;
     tn = t / rows;
     return;
   }
-  int r = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-  while (r * (r + 1) / 2 > t) --r;
-  while ((r + 1) * (r + 2) / 2 <= t) ++r;
-  tm = r;
-  tn = t - r * (r + 1) / 2;
-}
-
-__device__ __forceinline__ int column(int j, int e, int half) { return j * 32 + (e >> 2) * 8 + half * 4 + (e & 3); }
-
-// Runs of four of a row of any of the three types; `left` of them lie in the row.
-__device__ __forceinline__ f32x4 load4(const void* p, int dt, int64_t at, int left) {
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (dt == MFX_F32) {
-    typedef float run_t __attribute__((ext_vector_type(4), aligned(4)));
-    const float* q = static_cast<const float*>(p) + at;
-    if (left >= 4) {
-      const run_t r = *reinterpret_cast<const run_t*>(q);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = r[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 3; ++j)
-        if (j < left) v[j] = q[j];
-    }
-  } else {
-    typedef uint32_t run_t __attribute__((ext_vector_type(2), aligned(2)));
-    const uint16_t* q = static_cast<const uint16_t*>(p) + at;
-    uint32_t bits[2] = {0, 0};
-    if (left >= 4) {
-      const run_t r = *reinterpret_cast<const run_t*>(q);
-      bits[0] = r[0];
-      bits[1] = r[1];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 3; ++j)
-        if (j < left) bits[j >> 1] |= (uint32_t)q[j] << (16 * (j & 1));
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      v[2 * j] = dt == MFX_BF16 ? __uint_as_float(bits[j] << 16) : rowvec::f16_lo(bits[j]);
-      v[2 * j + 1] = dt == MFX_BF16 ? __uint_as_float(bits[j] & 0xffff0000u) : rowvec::f16_hi(bits[j]);
-    }
+  int r0 = 0, rows;
+  for (;; r0 += 4) {
+    rows = min(4, p.g.tiles_m - r0);
+    const int n = rows * r0 + rows * (rows + 1) / 2;
+    if (t < n) break;
+    t -= n;
   }
-  return v;
-}
-__device__ __forceinline__ void store4(void* p, int dt, int64_t at, int left, const f32x4& v) {
-  if (dt == MFX_F32) {
-    typedef float run_t __attribute__((ext_vector_type(4), aligned(4)));
-    float* q = static_cast<float*>(p) + at;
-    if (left >= 4) {
-      *reinterpret_cast<run_t*>(q) = v;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 3; ++j)
-        if (j < left) q[j] = v[j];
-    }
-  } else {
-    typedef uint32_t run_t __attribute__((ext_vector_type(2), aligned(2)));
-    uint16_t* q = static_cast<uint16_t*>(p) + at;
-    uint32_t bits[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      bits[j] = dt == MFX_BF16 ? pack2<0>(v[2 * j], v[2 * j + 1]) : pack2<1>(v[2 * j], v[2 * j + 1]);
-    if (left >= 4) {
-      *reinterpret_cast<run_t*>(q) = run_t{bits[0], bits[1]};
-    } else {
-#pragma unroll
-      for (int j = 0; j < 3; ++j)
-        if (j < left) q[j] = (uint16_t)(bits[j >> 1] >> (16 * (j & 1)));
-    }
-  }
-}
-
-// What becomes of a tile's sums.  A wavefront goes through its block 32 rows at
-// a time, with fences and opaque row numbers between, so that no more than one
-// set of values and addresses is live beside the sums.
-template <class C, Mode MODE>
-__device__ __forceinline__ void finish(const ProdArgs& p, int64_t bz, int tm, int tn, char* smem, Acc<C>& acc) {
-  constexpr int FM = C::FM, FN = C::FN;
-  const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave % C::WM, wn = wave / C::WM;
-  const int m0 = tm * C::BM + wm * FM * 32, n0 = tn * C::BN + wn * FN * 32;  // this wavefront's block
-  const int M = p.g.M, N = p.g.N;
-
-  if (MODE == kApply && p.out) {
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      int l = l32;
-      asm volatile("" : "+v"(l));
-      const int m = m0 + i * 32 + l;
-      if (m < M) {
-        const int64_t wrow = bz * p.ws_b + m * p.ws_r, orow = bz * p.os_b + m * p.os_r;
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int n = n0 + column(j, g * 4, half);
-            if (n >= N) continue;
-            f32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = acc[j][i][g * 4 + e] * p.c1;
-            if (p.w) v += load4(p.w, p.out_dt, wrow + n, N - n) * p.keep;
-            store4(p.out, p.out_dt, orow + n, N - n, v);
-          }
-      }
-      fence();
-    }
+  if (t < rows * r0) {
+    tm = r0 + t % rows;
+    tn = t / rows;
     return;
   }
+  // The band's own triangle.
+  t -= rows * r0;
+  int c = 0;
+  while (t >= rows - c) t -= rows - c++;
+  tm = r0 + c + t;
+  tn = r0 + c;
+}
 
-  // Through LDS (the stages are free), each wavefront its own part: the leading
-  // terms' rows in 16-byte chunks along n, chunk k of row r at slot k ^ (r %
-  // chunks), and of a symmetric product off the diagonal the same transposed, 32
-  // chunks of m a row; then the second terms'.
-  constexpr int BLOCK = 32 * FN * 32;
-  uint16_t* const st = reinterpret_cast<uint16_t*>(smem + wave * (C::SMEM / C::NW));
-  static_assert(4 * BLOCK * 2 <= C::SMEM / C::NW, "a wavefront's four blocks");
-  const int M8 = (M + 7) & ~7, N8 = (N + 7) & ~7;
-  const bool turned = MODE != kApply && tm != tn;
-  uint16_t* const c = p.c + bz * p.cs;
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    int l = l32;
+// What becomes of a block of sums, rows m0 .. + 31 by columns n0 .. + FN * 32 of
+// matrix bz, by one wavefront.  The sums go to LDS (st: FN * 4 KB of the
+// wavefront's own), chunk c (four) of row r at slot c ^ (r % chunks), and from there in
+// runs of eight along a row; of a symmetric product's tile off the diagonal
+// (`turned`) the values go back there and out once more in runs of eight down a
+// column, which are a row's of the other half.
+template <int FN, Mode MODE>
+__device__ __forceinline__ void finish_rows(const ProdArgs& p, int64_t bz, int m0, int n0, bool turned, float* st,
+                                            const f32x16 (&acc)[FN]) {
+  constexpr int W = FN * 32, QUADS = W / 4;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int M = p.g.M, N = p.g.N;
+  {
+    int l = lane & 31;  // (opaque: no address is kept through the products)
     asm volatile("" : "+v"(l));
-    const int m = m0 + i * 32 + l;
+    f32x4* const row = reinterpret_cast<f32x4*>(st + l * W);
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int n = n0 + column(j, g * 4, half);
-        float v[4];
+      for (int g = 0; g < 4; ++g)
+        row[(j * 8 + g * 2 + half) ^ (l & (QUADS - 1))] =
+            f32x4{acc[j][g * 4], acc[j][g * 4 + 1], acc[j][g * 4 + 2], acc[j][g * 4 + 3]};
+  }
+  fence();
+  constexpr int RUNS = FN * 4, RPS = 64 / RUNS;  // of a row; rows at a time
+  uint16_t* const c = p.c + bz * p.cs;
+  // One or two f16 terms of a run.
+  auto put = [&](int64_t at, const float (&v)[8]) __attribute__((always_inline)) {
+    *reinterpret_cast<uint4*>(c + at) = rowvec::pack16<_Float16>(v);
+    if (p.two) {
+      float r[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[j][i][g * 4 + e] * p.c1;
-        if constexpr (MODE == kSquare) {
-          f32x4 a = {0.f, 0.f, 0.f, 0.f};
-          if (m < M && n < N) {  // (A's rows are padded to whole chunks)
-            const uint16_t* from = static_cast<const uint16_t*>(p.g.a.p) + bz * p.as + (int64_t)m * p.g.a.ld + n;
-            a = load4(from, MFX_F16, 0, 4);
-            if (p.two) a += load4(from, MFX_F16, p.g.a.lo, 4);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(p.c2, a[e], v[e]) + (m == n + e ? p.c3 : 0.f);
-        }
-        uint16_t h[4], r[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = m < M && n + e < N ? v[e] : 0.f;  // (zeros in the padding)
-          h[e] = lead(v[e]);
-          r[e] = lead(rest(v[e]));
-        }
-        const int ch = l * (FN * 32) + ((j * 4 + g) ^ (l & (FN * 4 - 1))) * 8 + half * 4;
-        *reinterpret_cast<u16x4*>(st + ch) = u16x4{h[0], h[1], h[2], h[3]};
-        if (p.two) *reinterpret_cast<u16x4*>(st + 2 * BLOCK + ch) = u16x4{r[0], r[1], r[2], r[3]};
-        if (turned) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int row = column(j, g * 4 + e, half);
-            const int at = row * 32 + ((l >> 3) ^ ((row >> 2) & 3)) * 8 + (l & 7);
-            st[BLOCK + at] = h[e];
-            if (p.two) st[3 * BLOCK + at] = r[e];
-          }
-        }
-      }
-    fence();
-    for (int term = 0; term <= p.two; ++term) {
-      uint16_t* const to = c + (term ? p.lo : 0);
-      const uint16_t* const from = st + term * 2 * BLOCK;
-      constexpr int CPR = FN * 4, RPS = 64 / CPR;
-#pragma unroll
-      for (int k = 0; k < 32 / RPS; ++k) {
-        const int r = k * RPS + lane / CPR, ch = lane % CPR, row = m0 + i * 32 + r;
-        const u32x4 v = *reinterpret_cast<const u32x4*>(from + r * (FN * 32) + (ch ^ (r & (CPR - 1))) * 8);
-        if (row < M && n0 + ch * 8 < N8) *reinterpret_cast<u32x4*>(to + (int64_t)row * p.ldc + n0 + ch * 8) = v;
-      }
-      if (turned) {
-#pragma unroll
-        for (int k = 0; k < FN * 2; ++k) {
-          const int r = k * 16 + lane / 4, ch = lane % 4, row = n0 + r, col = m0 + i * 32 + ch * 8;
-          const u32x4 v = *reinterpret_cast<const u32x4*>(from + BLOCK + r * 32 + (ch ^ ((r >> 2) & 3)) * 8);
-          if (row < N && col < M8) *reinterpret_cast<u32x4*>(to + (int64_t)row * p.ldc + col) = v;
-        }
-      }
+      for (int e = 0; e < 8; ++e) r[e] = rest(v[e]);
+      *reinterpret_cast<uint4*>(c + p.lo + at) = rowvec::pack16<_Float16>(r);
     }
+  };
+  // (Unrolled for a square product's reads of A to overlap; the last product's
+  // end, of any type and alignment, stays a loop.)
+  constexpr int UNROLL = MODE == kSquare ? 32 / RPS : 2;
+#pragma unroll UNROLL
+  for (int k = 0; k < 32; k += RPS) {
+    const int r = k + lane / RUNS, run = lane % RUNS, m = m0 + r, n = n0 + run * 8;
+    if (m >= M || n >= N) continue;
+    f32x4* const row = reinterpret_cast<f32x4*>(st + r * W);
+    f32x4 &x = row[(run * 2) ^ (r & (QUADS - 1))], &y = row[(run * 2 + 1) ^ (r & (QUADS - 1))];
+    float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= p.c1;
+    if (MODE == kApply && p.out) {
+      if (p.w) {
+        float w[8];
+        load8(p.w, p.out_dt, bz * p.ws_b + m * p.ws_r, n, N, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(p.keep, w[e], v[e]);
+      }
+      store8(p.out, p.out_dt, bz * p.os_b + m * p.os_r, n, N, v);
+      continue;
+    }
+    if constexpr (MODE == kSquare) {  // a I + b A (A's rows are padded to whole runs)
+      const uint16_t* from = static_cast<const uint16_t*>(p.g.a.p) + bz * p.as + (int64_t)m * p.g.a.ld + n;
+      float a[8];
+      rowvec::unpack16<_Float16>(*reinterpret_cast<const uint4*>(from), a);
+      if (p.two) {
+        float b[8];
+        rowvec::unpack16<_Float16>(*reinterpret_cast<const uint4*>(from + p.g.a.lo), b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] += b[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fmaf(p.c2, a[e], v[e]) + (m == n + e ? p.c3 : 0.f);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = n + e < N ? v[e] : 0.f;  // (zeros in the padding)
+    if (MODE != kApply && turned) {
+      x = f32x4{v[0], v[1], v[2], v[3]};
+      y = f32x4{v[4], v[5], v[6], v[7]};
+    }
+    put((int64_t)m * p.ldc + n, v);
+  }
+  if (MODE == kApply || !turned) return;
+  fence();
+#pragma unroll 2
+  for (int k = 0; k < W; k += 16) {
+    const int r = k + lane / 4, run = lane % 4, n = n0 + r, m = m0 + run * 8;
+    if (n >= N || m >= M) continue;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int row = run * 8 + e;
+      v[e] = st[row * W + ((r >> 2) ^ (row & (QUADS - 1))) * 4 + (r & 3)];
+    }
+    // (Rows past the matrix hold sums of zeros: nothing went over them.)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = m + e < M ? v[e] : 0.f;
+    put((int64_t)n * p.ldc + m, v);
+  }
+}
+
+// What becomes of a tile's sums: a wavefront goes through its block 32 rows at a
+// time, with fences between, so that no more than one set of values and addresses is
+// live beside the sums.
+template <class C, Mode MODE>
+__device__ __forceinline__ void finish(const ProdArgs& p, int64_t bz, int tm, int tn, char* smem, Acc<C>& acc) {
+  constexpr int FM = C::FM, FN = C::FN;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % C::WM, wn = wave / C::WM;
+  static_assert(FN * 4096 <= C::SMEM / C::NW, "a wavefront's part of the stages, which are free");
+  float* const st = reinterpret_cast<float*>(smem + wave * (C::SMEM / C::NW));
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    f32x16 rows[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) rows[j] = acc[j][i];
+    finish_rows<FN, MODE>(p, bz, tm * C::BM + (wm * FM + i) * 32, tn * C::BN + wn * FN * 32, MODE != kApply && tm != tn,
+                          st, rows);
     fence();
   }
 }
@@ -382,81 +343,87 @@ template <class C, Mode MODE>
 __global__ __launch_bounds__(C::NT, C::WAVES) void ns_product(ProdArgs p) {
   __shared__ __attribute__((aligned(16))) char smem[C::SMEM];
   constexpr int PART = C::NT * C::FM * C::FN * 16;
-  Acc<C> acc;
-  auto sums = [&](int64_t tile, int kt0, int kt1, int& bz, int& tm, int& tn) __attribute__((always_inline)) {
-    bz = (int)(tile / p.tiles);
-    tile_of(p, (int)(tile - (int64_t)bz * p.tiles), tm, tn);
-    GemmShape g = p.g;
-    g.a.p = static_cast<const uint16_t*>(g.a.p) + bz * p.as;
-    g.b.p = static_cast<const uint16_t*>(g.b.p) + bz * p.bs;
-    gemm_tile16<C>(g, tm * C::BM, tn * C::BN, kt0, kt1, reinterpret_cast<bf16*>(smem), acc);
-    __syncthreads();  // the stages are free
-  };
-  int bz, tm, tn;
+  int64_t tile, slot = -1;
+  int kt0 = 0, kt1 = p.kt;
   if ((int64_t)blockIdx.x < p.whole) {
-    sums(dealt(blockIdx.x, p.whole), 0, p.kt, bz, tm, tn);
+    tile = dealt(blockIdx.x, p.whole);
+  } else {
+    // (Range by range: workgroups next to each other read the same k of neighbouring
+    // tiles.  Tile by tile each would read a range of its own, 200 us for
+    // 130 where 36 tiles are split into 7.)
+    const int64_t rest = p.all - p.whole;
+    slot = dealt(blockIdx.x - p.whole, rest * p.splits);
+    const int split = (int)(slot / rest);
+    tile = p.whole + (slot - split * rest);
+    kt0 = split * p.per;
+    kt1 = min(kt1, kt0 + p.per);
+  }
+  const int bz = (int)(tile / p.tiles);
+  int tm, tn;
+  tile_of(p, (int)(tile - (int64_t)bz * p.tiles), tm, tn);
+  GemmShape g = p.g;
+  g.a.p = static_cast<const uint16_t*>(g.a.p) + bz * p.as;
+  g.b.p = static_cast<const uint16_t*>(g.b.p) + bz * p.bs;
+  Acc<C> acc;
+  bf16* const stages = reinterpret_cast<bf16*>(smem);
+  if constexpr (C::PAIR && C::BK == 32)
+    gemm_pair16_flat<C>(g, tm * C::BM, tn * C::BN, kt0, kt1, stages, acc);
+  else if constexpr (C::PAIR) gemm_pair16<C>(g, tm * C::BM, tn * C::BN, kt0, kt1, stages, acc);
+  else gemm_tile16<C>(g, tm * C::BM, tn * C::BN, kt0, kt1, stages, acc);
+  __syncthreads();  // the stages are free
+  if (slot < 0) {
     finish<C, MODE>(p, bz, tm, tn, smem, acc);
     return;
   }
-  const int64_t w = dealt(blockIdx.x - p.whole, p.shares);
-  const int64_t units = (p.all - p.whole) * p.kt;
-  int64_t u = w * units / p.shares;
-  const int64_t end = (w + 1) * units / p.shares;
-  while (u < end) {
-    const int64_t tile = u / p.kt;
-    const int kt0 = (int)(u - tile * p.kt), kt1 = (int)min((int64_t)p.kt, kt0 + (end - u));
-    sums(p.whole + tile, kt0, kt1, bz, tm, tn);
-    // (Slot w + tile: through the units one of them grows at a time.)
-    f32x4* const to = reinterpret_cast<f32x4*>(p.part + (w + tile) * PART) + threadIdx.x;
-#pragma unroll
-    for (int j = 0; j < C::FN; ++j)
-#pragma unroll
-      for (int i = 0; i < C::FM; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          to[((j * C::FM + i) * 4 + q) * C::NT] =
-              f32x4{acc[j][i][q * 4], acc[j][i][q * 4 + 1], acc[j][i][q * 4 + 2], acc[j][i][q * 4 + 3]};
-    u += kt1 - kt0;
-  }
-}
-
-// The shared tiles: their partial sums in order, then what `finish` does.
-template <class C, Mode MODE>
-__global__ __launch_bounds__(C::NT, C::WAVES) void ns_join(ProdArgs p) {
-  __shared__ __attribute__((aligned(16))) char smem[C::SMEM];
-  constexpr int PART = C::NT * C::FM * C::FN * 16;
-  const int64_t tile = dealt(blockIdx.x, p.all - p.whole), units = (p.all - p.whole) * p.kt;
-  // Workgroups whose runs meet the tile's units [tile kt, (tile + 1) kt).
-  const int64_t u0 = tile * p.kt, u1 = u0 + p.kt;
-  int64_t w = u0 * p.shares / units;
-  while ((w + 1) * units / p.shares <= u0) ++w;
-  while (w > 0 && w * units / p.shares > u0) --w;
-  Acc<C> acc;
+  uint32_t tid = threadIdx.x;  // (opaque: no address is kept through the products)
+  asm volatile("" : "+v"(tid));
+  f32x4* const to = reinterpret_cast<f32x4*>(p.part + slot * PART) + tid;
 #pragma unroll
   for (int j = 0; j < C::FN; ++j)
 #pragma unroll
     for (int i = 0; i < C::FM; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
-  for (; w < p.shares && w * units / p.shares < u1; ++w) {
-    if ((w + 1) * units / p.shares <= w * units / p.shares) continue;  // (an empty run)
-    const f32x4* const from = reinterpret_cast<const f32x4*>(p.part + (w + tile) * PART) + threadIdx.x;
+      for (int q = 0; q < 4; ++q)
+        to[((j * C::FM + i) * 4 + q) * C::NT] =
+            f32x4{acc[j][i][q * 4], acc[j][i][q * 4 + 1], acc[j][i][q * 4 + 2], acc[j][i][q * 4 + 3]};
+}
+
+// The split tiles: their partial sums in order, then what finish_rows does, each
+// 32 x 32 block by a wavefront of its own (few tiles are split into many
+// ranges: a workgroup a tile took 270 us over 8 tiles of 16).
+constexpr int kJoinWaves = 4;
+template <class C, Mode MODE>
+__global__ __launch_bounds__(kJoinWaves * 64) void ns_join(ProdArgs p) {
+  constexpr int PART = C::NT * C::FM * C::FN * 16, BLOCKS = C::NW * C::FM * C::FN;
+  static_assert(BLOCKS % kJoinWaves == 0, "a workgroup's blocks are of one tile");
+  __shared__ __attribute__((aligned(16))) float st[kJoinWaves][1024];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t id = (int64_t)blockIdx.x * kJoinWaves + wave, tile = id / BLOCKS, rest = p.all - p.whole;
+  const int block = (int)(id - tile * BLOCKS), of = block / (C::FM * C::FN), ij = block % (C::FM * C::FN);
+  const int i = ij % C::FM, j = ij / C::FM, wm = of % C::WM, wn = of / C::WM;
+  const float* const part = p.part + tile * PART + ij * (C::NT * 16) + (of * 64 + lane) * 4;
+  f32x16 acc[1];
 #pragma unroll
-    for (int j = 0; j < C::FN; ++j)
+  for (int e = 0; e < 16; ++e) acc[0][e] = 0.f;
+  constexpr int U = 4;  // partials in flight
+  for (int k = 0; k < p.splits; k += U) {
+    f32x4 v[U][4];
 #pragma unroll
-      for (int i = 0; i < C::FM; ++i)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 v = from[((j * C::FM + i) * 4 + q) * C::NT];
+      for (int q = 0; q < 4; ++q)  // (past the last: the last again, not added)
+        v[u][q] = *reinterpret_cast<const f32x4*>(part + min(k + u, p.splits - 1) * rest * PART + q * (C::NT * 4));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][i][q * 4 + e] += v[e];
-        }
+    for (int u = 0; u < U; ++u)
+      if (k + u < p.splits)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[0][e] += v[u][e / 4][e % 4];
   }
-  int bz, tm, tn;
-  const int64_t t = p.whole + tile;
-  bz = (int)(t / p.tiles);
-  tile_of(p, (int)(t - (int64_t)bz * p.tiles), tm, tn);
-  finish<C, MODE>(p, bz, tm, tn, smem, acc);
+  const int64_t t = p.whole + tile, bz = t / p.tiles;
+  int tm, tn;
+  tile_of(p, (int)(t - bz * p.tiles), tm, tn);
+  finish_rows<1, MODE>(p, bz, tm * C::BM + (wm * C::FM + i) * 32, tn * C::BN + (wn * C::FN + j) * 32,
+                       MODE != kApply && tm != tn, st[wave], acc);
 }
 
 // ---- host ------------------------------------------------------------------------
@@ -469,48 +436,62 @@ constexpr int kMaxSteps = 32;
 // How a product's tiles are shared out.
 struct Way {
   Form form;
-  int64_t tiles, whole, shares;  // tiles of all matrices
+  int64_t tiles, whole;  // of all matrices; those that are not split
+  int splits, per;
 };
 
-// Microseconds of a k-tile with `slots` workgroups on each CU, and once for each
-// round of workgroups.
+// Microseconds of a k-tile with `slots` workgroups on each CU (`alone` of that
+// with none), once for each round of workgroups and more of it for a square
+// product's reads of A, and of a join: once, and by its partial sums at `rate`
+// TB/s.  Fitted to the kernels' times over 13 shapes from [128, 512] to [4096, 4096]
+// and 12 of [512, 2048], each product in every form with 1 to 12 ranges.
 struct Cost {
   int slots;
-  float kt, each;
+  float kt, alone, each, square, join, rate;
 };
-constexpr Cost kCost[3] = {{1, 0.85f, 9.f}, {2, 0.57f, 4.f}, {4, 0.42f, 3.f}};
+constexpr Cost kCost[2][3] = {{{1, 0.818f, 0.73f, 12.4f, 6.5f, 1.7f, 9.9f},
+                               {2, 0.597f, 0.01f, 3.9f, 1.9f, 6.9f, 12.9f},
+                               {4, 0.536f, 0.09f, 3.6f, 1.3f, 7.3f, 60.f}},
+                              {{1, 1.240f, 0.69f, 10.0f, 13.2f, 2.8f, 8.3f},
+                               {2, 0.947f, 0.00f, 1.8f, 4.5f, 8.0f, 8.7f},
+                               {2, 0.578f, 0.18f, 3.4f, 1.9f, 7.6f, 60.f}}};
 
-Way choose(int64_t B, int64_t M, int64_t N, int64_t K, bool symmetric, int terms) {
-  const int64_t cus = device_cu_count(), kt = ceil_div(K, kBK16) * terms;
+// Of `wgs` workgroups of `n` k-tiles each.
+float rounds_us(const Cost& c, int64_t wgs, int64_t n, bool square) {
+  const int64_t cus = device_cu_count(), slots = c.slots * cus, rest = wgs % slots;
+  const float once = c.each + (square ? c.square : 0.f);
+  float t = (float)(wgs / slots) * ((float)n * c.kt + once);
+  if (rest) {
+    const float load = c.slots == 1 ? (float)rest / (float)cus : (float)ceil_div(rest, cus) / (float)c.slots;
+    t += (float)n * c.kt * (c.alone + (1.f - c.alone) * load) + once;
+  }
+  return t;
+}
+
+// The way that takes least by these: every form, its tiles whole or those of the
+// last, partly filled round split along k into ranges of at least 8 k-tiles.
+Way choose(int64_t B, int64_t M, int64_t N, int64_t K, Mode mode, bool two) {
+  const int64_t cus = device_cu_count();
   Way best{};
   float least = INFINITY;
   for (int f = kWide; f <= kSlim; ++f) {
-    const Cost& c = kCost[f];
-    const int64_t side = kSide[f], tm = ceil_div(M, side), tn = ceil_div(N, side);
-    const int64_t tiles = B * (symmetric ? tm * (tm + 1) / 2 : tm * tn), slots = c.slots * cus;
-    const int64_t full = tiles / slots, rest = tiles % slots;
-    auto rounds = [&](float n, int64_t wgs) {
-      // (With fewer than `slots` workgroups on a CU each runs faster.)
-      const float busy = wgs >= slots ? 1.f : 0.25f + 0.75f * (float)ceil_div(wgs, cus) / (float)c.slots;
-      return n * ((float)kt * c.kt * busy) + c.each;
-    };
+    const Cost& c = kCost[two][f];
+    const int64_t side = kSide[f], tm = ceil_div(M, side), tn = ceil_div(N, side), kt = ceil_div(K, depth((Form)f, two));
+    const int64_t tiles = B * (mode != kApply ? tm * (tm + 1) / 2 : tm * tn), rest = tiles % (c.slots * cus);
     if (!launch_fits(tiles, 256)) continue;
-    float t = (float)full * ((float)kt * c.kt + c.each) + (rest ? rounds(1.f, rest) : 0.f);
-    if (t < least) {
-      least = t;
-      best = Way{(Form)f, tiles, tiles, 0};
+    const float whole = rounds_us(c, tiles, kt, mode == kSquare);
+    if (whole < least) {
+      least = whole;
+      best = Way{(Form)f, tiles, tiles, 0, 0};
     }
-    // The tiles of the last, partly filled round shared out by their k-tiles, at
-    // least 12 to a workgroup; their sums are written and read again, and there is
-    // a launch more.
-    if (rest) {
-      const int64_t shares = std::min<int64_t>(slots, rest * kt / 12);
-      if (shares <= rest) continue;
-      t = (float)full * ((float)kt * c.kt + c.each) + rounds((float)rest / (float)shares, shares) +
-          6.f + (float)(shares + rest) * (float)(side * side) * 8.f / 4e6f;
+    for (int64_t n = 2; rest && n <= 64 && n * 8 <= kt; ++n) {
+      const int64_t per = ceil_div(kt, n), wgs = rest * n;
+      if (ceil_div(kt, per) != n || !launch_fits(tiles - rest + wgs, 256)) continue;
+      const float t = rounds_us(c, tiles - rest, kt, mode == kSquare) + rounds_us(c, wgs, per, false) + c.join +
+                      (float)wgs * (float)(side * side) * 8e-6f / c.rate;
       if (t < least) {
         least = t;
-        best = Way{(Form)f, tiles, tiles - rest, shares};
+        best = Way{(Form)f, tiles, tiles - rest, (int)n, (int)per};
       }
     }
   }
@@ -518,7 +499,7 @@ Way choose(int64_t B, int64_t M, int64_t N, int64_t K, bool symmetric, int terms
 }
 
 size_t part_bytes(const Way& w) {
-  return w.shares ? (size_t)(w.shares + w.tiles - w.whole) * kSide[w.form] * kSide[w.form] * 4 : 0;
+  return (size_t)w.splits * (w.tiles - w.whole) * kSide[w.form] * kSide[w.form] * 4;
 }
 
 struct Plan {
@@ -595,16 +576,15 @@ int plan_common(Plan& pl, int64_t B, int64_t m, int64_t n, int64_t steps, const 
   pl.two = terms == 0 ? !(bf16_result && pl.s >= 256) : terms == 2;
   if (int rc = plan_scales(pl, coeffs, num_coeffs)) return rc;
   if (B == 0) return MFX_OK;
-  const int t = pl.two ? 3 : 1;
-  pl.gram = choose(B, pl.s, pl.s, pl.l, true, t);
-  pl.square = choose(B, pl.s, pl.s, pl.s, true, t);
-  pl.apply = choose(B, m, n, pl.s, false, t);
+  pl.gram = choose(B, pl.s, pl.s, pl.l, kGram, pl.two);
+  pl.square = choose(B, pl.s, pl.s, pl.s, kSquare, pl.two);
+  pl.apply = choose(B, m, n, pl.s, kApply, pl.two);
   if (!pl.gram.tiles || !pl.square.tiles || !pl.apply.tiles)
     return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
   if (!launch_fits(B * std::min<int64_t>(2048, ceil_div(m * (pl.ld / 8), 256)), 256))
     return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
-  // Parts of a matrix's sum of squares: of 1024 chunks or more, at most one a thread of ns_split.
-  pl.parts = (int)std::min<int64_t>(256, ceil_div(m * (pl.ld / 8), 1024));
+  // Parts of a matrix's sum of squares: of 512 chunks or more, at most four a thread of ns_split.
+  pl.parts = (int)std::min<int64_t>(1024, ceil_div(m * (pl.ld / 8), 512));
   pl.norm_bytes = align256((size_t)B * pl.parts * 8);
   pl.x_bytes = align256((size_t)B * m * pl.ld * 2 * (1 + pl.two));
   pl.a_bytes = align256((size_t)B * pl.s * pl.lds * 2 * (1 + pl.two));
@@ -615,7 +595,7 @@ int plan_common(Plan& pl, int64_t B, int64_t m, int64_t n, int64_t steps, const 
 
 template <class C, Mode MODE>
 int launch(const ProdArgs& p, hipStream_t s) {
-  hipLaunchKernelGGL((ns_product<C, MODE>), dim3((unsigned)(p.whole + p.shares)), dim3(C::NT), 0, s, p);
+  hipLaunchKernelGGL((ns_product<C, MODE>), dim3((unsigned)(p.whole + p.splits * (p.all - p.whole))), dim3(C::NT), 0, s, p);
   return launch_status("ns_product");
 }
 
@@ -625,20 +605,21 @@ int launch_side(const ProdArgs& p, bool a_kc, bool b_kc, hipStream_t s) {
   if (!a_kc) {
     // (Only a tall matrix's gram product reads columns of both.)
     if constexpr (MODE == kGram)
-      rc = p.two ? launch<Cfg<SIDE, false, false, 3>, MODE>(p, s) : launch<Cfg<SIDE, false, false, 1>, MODE>(p, s);
+      rc = p.two ? launch<Cfg<SIDE, false, false, true>, MODE>(p, s) : launch<Cfg<SIDE, false, false, false>, MODE>(p, s);
     else
       return fail(MFX_E_INVALID, "no such product");
   } else if (!b_kc) {
     if constexpr (MODE == kApply)
-      rc = p.two ? launch<Cfg<SIDE, true, false, 3>, MODE>(p, s) : launch<Cfg<SIDE, true, false, 1>, MODE>(p, s);
+      rc = p.two ? launch<Cfg<SIDE, true, false, true>, MODE>(p, s) : launch<Cfg<SIDE, true, false, false>, MODE>(p, s);
     else
       return fail(MFX_E_INVALID, "no such product");
   } else {
-    rc = p.two ? launch<Cfg<SIDE, true, true, 3>, MODE>(p, s) : launch<Cfg<SIDE, true, true, 1>, MODE>(p, s);
+    rc = p.two ? launch<Cfg<SIDE, true, true, true>, MODE>(p, s) : launch<Cfg<SIDE, true, true, false>, MODE>(p, s);
   }
-  if (rc || !p.shares) return rc;
-  typedef Cfg<SIDE, true, true, 1> J;
-  hipLaunchKernelGGL((ns_join<J, MODE>), dim3((unsigned)(p.all - p.whole)), dim3(J::NT), 0, s, p);
+  if (rc || !p.splits) return rc;
+  typedef Cfg<SIDE, true, true, false> J;
+  const int64_t blocks = (p.all - p.whole) * J::NW * J::FM * J::FN;
+  hipLaunchKernelGGL((ns_join<J, MODE>), dim3((unsigned)(blocks / kJoinWaves)), dim3(kJoinWaves * 64), 0, s, p);
   return launch_status("ns_join");
 }
 
@@ -649,8 +630,9 @@ int product(ProdArgs& p, const Way& way, int64_t B, int64_t M, int64_t N, int64_
   p.g.M = (int)M, p.g.N = (int)N, p.g.K = (int)K;
   p.g.tiles_m = (int)ceil_div(M, side), p.g.tiles_n = (int)ceil_div(N, side);
   p.symmetric = MODE != kApply;
-  p.tiles = way.tiles / B, p.all = way.tiles, p.whole = way.whole, p.shares = way.shares;
-  p.kt = (int)ceil_div(K, kBK16) * (p.two ? 3 : 1);
+  p.tiles = way.tiles / B, p.all = way.tiles, p.whole = way.whole;
+  p.splits = way.splits, p.per = way.per;
+  p.kt = (int)ceil_div(K, depth(way.form, p.two));
   p.part = part;
   if (way.form == kWide) return launch_side<256, MODE>(p, a_kc, b_kc, s);
   if (way.form == kNarrow) return launch_side<128, MODE>(p, a_kc, b_kc, s);

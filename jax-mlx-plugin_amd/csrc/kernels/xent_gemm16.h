@@ -3,10 +3,6 @@
 //
 //   C[m][n] = sum_k A(m, k) B(n, k)        fp32 accumulation
 //
-// or, of operands held as sums of two 16-bit terms each (TERMS = 3), the sum of
-// A_lo B_hi, A_hi B_lo and A_hi B_hi: three walks along k, the small ones first, in
-// one pipeline.  (A_lo B_lo lies below what the two terms of either leave out.)
-//
 // Each operand is stored either k-contiguous, [index][k], or index-contiguous,
 // [k][index]; what happens to a tile's sums is the epilogue's business (a
 // softmax's partial sums, a gradient, a store).  As in gemm16.hip the kernel
@@ -62,8 +58,7 @@ __device__ __forceinline__ int kc_swz(int r) { return (r >> 2) & 3; }
 // KC: [IDX rows][32 k], chunk c of row r at c ^ kc_swz(r).
 // else: [32 k][IDX], chunk c of row r at c ^ tile_swz<IDX>(r).
 // ROT: the tiles of k are walked round from a later one (its number `at`).
-// LO >= 0: k is walked three times, walk LO over the second terms.
-template <bool KC, int IDX, int NW, bool ROT = false, int LO = -1>
+template <bool KC, int IDX, int NW, bool ROT = false>
 struct Tile {
   static constexpr int ELEMS = IDX * kBK16;
   static constexpr int RPI = KC ? 16 : 512 / IDX;  // rows one load instruction covers
@@ -84,10 +79,7 @@ struct Tile {
                         // else: bytes of the last row
   uint32_t voff[NOFF];  // this lane's byte offset in instructions 0 and 1, less the rows between
   int lane_k;           // KC: k of the lane's chunk within a tile
-  int turn;             // ROT, LO: tiles left
-  const bf16* first;    // LO: the leading terms' first tile
-  int64_t lo;           // LO: elements to the second terms
-  int walk;             // LO: the next tile's
+  int turn;             // ROT: tiles left
 #if defined(__HIP_DEVICE_COMPILE__)
   __amdgpu_buffer_rsrc_t rsrc;
 #endif
@@ -106,16 +98,7 @@ struct Tile {
     turn = kt1 - kt0;
     ld2 = (int)o.ld * 2;
     next = KC ? kBK16 : kBK16 * o.ld;
-    if constexpr (LO >= 0) {
-      const int per = (K + kBK16 - 1) / kBK16;
-      walk = kt0 / per;
-      k0 = (kt0 - walk * per) * kBK16;
-      lo = o.lo;
-      first = static_cast<const bf16*>(o.p) + (KC ? (int64_t)idx0 * o.ld : (int64_t)idx0);
-      cur = first + (walk == LO ? lo : 0) + (KC ? (int64_t)k0 : k0 * o.ld);
-    } else {
-      cur = static_cast<const bf16*>(o.p) + (KC ? (int64_t)idx0 * o.ld + k0 : (int64_t)k0 * o.ld + idx0);
-    }
+    cur = static_cast<const bf16*>(o.p) + (KC ? (int64_t)idx0 * o.ld + k0 : (int64_t)k0 * o.ld + idx0);
     last = KC ? (min(left, IDX) - 1) * ld2 + chunks(K) * 2 : chunks(left) * 2;
     constexpr int CPR = KC ? kBK16 / 8 : IDX / 8;  // chunks per row
     const int row = wave * RPI + lane / CPR, slot = lane % CPR;
@@ -129,7 +112,7 @@ struct Tile {
   __device__ __forceinline__ void take() {
 #if defined(__HIP_DEVICE_COMPILE__)
     int extent = KC ? last - k0 * 2 : (min(K - k0, kBK16) - 1) * ld2 + last;
-    if (ROT || LO >= 0 ? turn-- <= 0 : k0 >= k_end) extent = 0;
+    if (ROT ? turn-- <= 0 : k0 >= k_end) extent = 0;
     rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16*>(cur), (short)0, extent, 0x00020000);
     if constexpr (KC) vo = k0 + lane_k < K ? voff[0] : kOOR;
     cur += next;
@@ -139,13 +122,6 @@ struct Tile {
       if (k0 >= k_end) {  // (one range: k from 0)
         cur -= k0;
         k0 = 0;
-      }
-    }
-    if constexpr (LO >= 0) {
-      if (k0 >= K) {
-        k0 = 0;
-        ++walk;
-        cur = first + (walk == LO ? lo : 0);
       }
     }
 #endif
@@ -228,8 +204,7 @@ __device__ __forceinline__ void barrier() {
   fence();
 }
 
-// The sums of tile (m0, n0) over the k-tiles [kt0, kt1) (at least one; TERMS =
-// 3: of the three walks').
+// The sums of tile (m0, n0) over the k-tiles [kt0, kt1) (at least one).
 template <class C>
 __device__ __forceinline__ void gemm_tile16(const GemmShape& g, int m0, int n0, int kt0, int kt1, bf16* smem,
                                             Acc<C>& acc) {
@@ -244,8 +219,8 @@ __device__ __forceinline__ void gemm_tile16(const GemmShape& g, int m0, int n0, 
   // k apart: [33 x 4096] by [65537 x 4096] 151 us from the same k, 142 so; 2%
   // slower where B fits the last cache.
   constexpr bool ROT = C::ROT;
-  using TA = Tile<C::A_KC, C::BM, C::NW, ROT, C::TERMS == 3 ? 0 : -1>;
-  using TB = Tile<C::B_KC, C::BN, C::NW, ROT, C::TERMS == 3 ? 1 : -1>;
+  using TA = Tile<C::A_KC, C::BM, C::NW, ROT>;
+  using TB = Tile<C::B_KC, C::BN, C::NW, ROT>;
   const int at = ROT ? n0 / C::BN % (kt1 - kt0) : 0;
   constexpr int LA = TA::LOADS, NL = LA + TB::LOADS, STAGE = C::STAGE;
   TA ta(g.a, m0, g.M, g.K, kt0, kt1, wave, lane, at);

@@ -1,5 +1,5 @@
 // Shapes shared by the product kernels of the linear cross entropy and of the
-// Newton-Schulz iteration (xent_gemm16.h, xent_gemm32.h) and their epilogues
+// Newton-Schulz iteration (xent_gemm16.h, xent_gemm32.h, pair_gemm16.h) and their epilogues
 // (linear_xent.hip, newton_schulz.hip).
 #pragma once
 
@@ -50,9 +50,6 @@ struct Config {
   static constexpr int WAVES = BM == 256 ? 1 : BM == 128 ? 2 : BM == 64 ? 3 : 4;  // per SIMD
   static constexpr int FM = BM / (32 * WM), FN = BN / (32 * WN);  // blocks of a wavefront
   static constexpr int BK = E == 2 ? kBK32 : kBK16;
-  // Products of terms, one behind the other along k: one, or of operands held
-  // in two terms each the three that matter (xent_gemm16.h).
-  static constexpr int TERMS = 1;
   static constexpr bool ROT = BM == 64 && A_KC && B_KC;
   // Bytes of a stage, and of all: four in 16 bits; f32: two, in the larger of
   // the two forms' padded rows (xent_gemm32.h).

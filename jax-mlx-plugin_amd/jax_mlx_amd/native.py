@@ -459,13 +459,18 @@ def check(rc: int) -> None:
 # a call, an f32 attention of [8, 8, 128, 64] from 12.6 to 10.7.)
 
 _torch_mod = None
+_raw_stream = None
 _DTYPE_CODES: dict = {}
 
 
 def _torch():
-    global _torch_mod
+    global _torch_mod, _raw_stream
     if _torch_mod is None:
         import torch  # noqa: PLC0415
+
+        # (The handle alone, 0.1 us; a Stream object around it costs 2 us a call.)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda index: torch.cuda.current_stream(index).cuda_stream)
 
         _DTYPE_CODES.update({torch.float32: MFX_F32, torch.bfloat16: MFX_BF16, torch.float16: MFX_F16})
         _torch_mod = torch
@@ -481,7 +486,8 @@ def dtype_code(dt) -> int:
 
 
 def _stream_handle(t) -> int:
-    return _torch().cuda.current_stream(t.device).cuda_stream
+    _torch()
+    return _raw_stream(t.get_device())
 
 
 def _require_gpu(*ts) -> None:
@@ -756,7 +762,7 @@ def _on(t, *others):
     if index < 0:
         raise ValueError("tensor must live on the GPU (device memory)")
     for o in others:
-        if o is not None and o.get_device() != index:
+        if o is not None and o is not t and o.get_device() != index:
             raise ValueError(f"tensors on {t.device} and {o.device}: all must live on one GPU")
     if _torch().cuda.current_device() == index:
         return _HERE
@@ -774,6 +780,11 @@ def _fresh(t):
     return _torch().empty_like(t, memory_format=_torch().contiguous_format)
 
 
+def _like(t):
+    """_fresh for a tensor that is mostly contiguous already (half the time then)."""
+    return _torch().empty_like(t) if t.is_contiguous() else _fresh(t)
+
+
 def _workspace(a, query, workspace, like):
     """Sets a.workspace: the caller's, or one from torch's allocator for this
     call (also inside a captured graph, whose pool then owns it)."""
@@ -781,7 +792,7 @@ def _workspace(a, query, workspace, like):
         need = int(getattr(load(), query)(ctypes.byref(a)))
         if not need:
             return None
-        workspace = _torch().empty(need, dtype=_torch().uint8, device=like.device)
+        workspace = like.new_empty(need, dtype=_torch().uint8)
     a.workspace = workspace.data_ptr()
     a.workspace_bytes = workspace.numel() * workspace.element_size()
     return workspace
@@ -1137,13 +1148,19 @@ _EMBED_PACK = struct.Struct("3P5qf3i").pack
 _EMBED_BWD_PACK = struct.Struct("4PN5qf5i").pack
 
 
+def _row_stride(t, H):
+    """Elements from row to row of t [..., H]."""
+    if t.is_contiguous():
+        return H
+    n, _, stride = _rows_view(t)
+    return stride if n > 1 else H  # (one row may carry any)
+
+
 def _token_rows(name, t, ids, H):
     """(dtype code, row stride) of t [..., H], a row for each of ids."""
     if t.shape != (*ids.shape, H):
         raise ValueError(f"{name} must be {(*ids.shape, H)}, got {tuple(t.shape)}")
-    n, _, stride = _rows_view(t)
-    # (One row may carry any stride.)
-    return dtype_code(t.dtype), stride if n > 1 else H
+    return dtype_code(t.dtype), _row_stride(t, H)
 
 
 def _table_rows(name, w):
@@ -1166,11 +1183,10 @@ def embedding(ids, w, *, scale=1.0, out_dtype=None, out=None):
     """out [..., H] = scale * w[ids] (mfx_embedding): ids [...] int32 or int64,
     w [V, H]; an id outside [0, V) gives zeros.  out has w's dtype, out_dtype, or
     its own if given."""
-    torch = _torch()
     icode = _ids_code(ids)
     V, H, code, ws = _table_rows("w", w)
     if out is None:
-        out = torch.empty((*ids.shape, H), dtype=out_dtype or w.dtype, device=w.device)
+        out = w.new_empty((*ids.shape, H), dtype=out_dtype)
     ocode, os_ = _token_rows("out", out, ids, H)
     a = EmbeddingArgs.from_buffer_copy(_EMBED_PACK(w.data_ptr(), ids.data_ptr(), out.data_ptr(), ids.numel(), H, V, ws,
                                                    os_, _f32(scale), code, ocode, icode))
@@ -1184,12 +1200,11 @@ def embedding_bwd(ids, dout, num_rows=None, *, scale=1.0, dw_dtype=None, dw=None
     dout [..., H] of its output (mfx_embedding_bwd), in dout's dtype, dw_dtype, or
     that of a given dw; accumulate adds to a given dw (a table tied to the head:
     linear_xent_bwd's dw)."""
-    torch = _torch()
     icode = _ids_code(ids)
     if dw is None:
         if num_rows is None or accumulate:
             raise ValueError("num_rows, or a dw (to accumulate into), is needed")
-        dw = torch.empty(num_rows, dout.shape[-1], dtype=dw_dtype or dout.dtype, device=dout.device)
+        dw = dout.new_empty((num_rows, dout.shape[-1]), dtype=dw_dtype)
     elif num_rows not in (None, dw.shape[0]):
         raise ValueError(f"dw has {dw.shape[0]} rows, not {num_rows}")
     V, H, wcode, ws = _table_rows("dw", dw)
@@ -1211,17 +1226,16 @@ _RESIDUAL_BWD_PACK = struct.Struct("14PN11q5f5i").pack
 
 def _rows_of(name, t, like, dtype=None):
     """Row stride of t, which has like's shape (and dtype, if given)."""
-    if t.shape != like.shape or (dtype is not None and t.dtype != dtype):
+    if t is not like and (t.shape != like.shape or (dtype is not None and t.dtype != dtype)):
         raise ValueError(f"{name} must be {tuple(like.shape)}{'' if dtype is None else f' of {dtype}'}")
-    n, H, stride = _rows_view(t)
-    return stride if n > 1 else H
+    return _row_stride(t, like.shape[-1])
 
 
 def _residual_fields(x, y, gate, seq_offsets, post_weight, pre_weight, post_eps, pre_eps, alpha, beta, weight_offset):
     """Checked (pointers, dims, strides of x, y and gate, scalars) of both directions."""
     if x.dim() < 2 or x.shape[-1] == 0:
         raise ValueError("x and y are [..., H]")
-    if any(eps is not None and not eps >= 0.0 for eps in (post_eps, pre_eps)):
+    if (post_eps is not None and not post_eps >= 0.0) or (pre_eps is not None and not pre_eps >= 0.0):
         raise ValueError("eps must be >= 0 (None: no norm)")
     xs, ys = _rows_of("x", x, x), _rows_of("y", y, x)
     H = x.shape[-1]
@@ -1266,18 +1280,21 @@ def residual_norm(x, y, *, gate=None, seq_offsets=None, post_weight=None, pre_we
     seq_offsets (int32 [sequences + 1], on the device) [sequences, H]; tokens in no
     sequence keep r = alpha x.  x and r may be f32 beside 16-bit y and h.  r may be
     x, h may be y."""
-    torch = _torch()
     ptrs, dims, strides, scalars = _residual_fields(x, y, gate, seq_offsets, post_weight, pre_weight, post_eps,
                                                     pre_eps, alpha, beta, weight_offset)
+    rs = hs = dims[1]
     if r is None:
-        r = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if h is None and pre_eps is not None:
-        h = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    elif h is not None and pre_eps is None:
-        raise ValueError("h needs its norm (pre_eps)")
-    a = ResidualNormArgs.from_buffer_copy(_RESIDUAL_PACK(
-        *ptrs, r.data_ptr(), _ptr(h), *dims, *strides, _rows_of("r", r, x, x.dtype),
-        dims[1] if h is None else _rows_of("h", h, y, y.dtype), *scalars))
+        r = _like(x)
+    else:
+        rs = _rows_of("r", r, x, x.dtype)
+    if h is not None:
+        if pre_eps is None:
+            raise ValueError("h needs its norm (pre_eps)")
+        hs = _rows_of("h", h, y, y.dtype)
+    elif pre_eps is not None:
+        h = _like(y)
+    a = ResidualNormArgs.from_buffer_copy(_RESIDUAL_PACK(*ptrs, r.data_ptr(), _ptr(h), *dims, *strides, rs, hs,
+                                                         *scalars))
     with _on(x, y, gate, seq_offsets, post_weight, pre_weight, r, h):
         check(load().mfx_residual_norm(ctypes.byref(a), _stream_handle(x)))
     return r, h
@@ -1289,20 +1306,23 @@ def residual_norm_bwd(x, y, dr, dh, *, gate=None, seq_offsets=None, post_weight=
     arguments for the gradients dr of r and dh of h, one of them None if there is
     none (mfx_residual_norm_bwd).  A gate's or weight's gradient has its shape and
     dtype, None for an absent one.  dx may be dr or x, dy may be dh or y."""
-    torch = _torch()
     ptrs, dims, strides, scalars = _residual_fields(x, y, gate, seq_offsets, post_weight, pre_weight, post_eps,
                                                     pre_eps, alpha, beta, weight_offset)
     H = dims[1]
+    dxs = dys = H
     if dx is None:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx = _like(x)
+    else:
+        dxs = _rows_of("dx", dx, x, x.dtype)
     if dy is None:
-        dy = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    dg, dp, dn = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-                  for t in (gate, post_weight, pre_weight))
+        dy = _like(y)
+    else:
+        dys = _rows_of("dy", dy, y, y.dtype)
+    dg, dp, dn = (None if t is None else _like(t) for t in (gate, post_weight, pre_weight))
     a = ResidualNormBwdArgs.from_buffer_copy(_RESIDUAL_BWD_PACK(
         *ptrs, _ptr(dr), _ptr(dh), dx.data_ptr(), dy.data_ptr(), _ptr(dg), _ptr(dp), _ptr(dn), 0, 0, *dims, *strides,
         H if dr is None else _rows_of("dr", dr, x, x.dtype), H if dh is None else _rows_of("dh", dh, y, y.dtype),
-        _rows_of("dx", dx, x, x.dtype), _rows_of("dy", dy, y, y.dtype), H, *scalars))
+        dxs, dys, H, *scalars))
     with _on(x, y, dr, dh, gate, seq_offsets, post_weight, pre_weight, dx, dy, workspace):
         keep = _workspace(a, "mfx_residual_norm_bwd_workspace_size", workspace, x)  # noqa: F841 (until the launch)
         check(load().mfx_residual_norm_bwd(ctypes.byref(a), _stream_handle(x)))
@@ -1348,10 +1368,9 @@ def newton_schulz(g, *, steps=5, coeffs=NEWTON_SCHULZ_COEFFS, eps=1e-7, scale=1.
     may be g).  coeffs: (a, b, c) of every step, or one triple for each.  terms: 2
     computes as products of f32 matrices do, 1 three times as fast to within 3e-3;
     0 takes 1 for bf16 results of sides from 256 on, else 2."""
-    torch = _torch()
     gs = _matrices("g", g)
     if out is None:
-        out = torch.empty(g.shape, dtype=out_dtype or g.dtype, device=g.device)
+        out = g.new_empty(g.shape, dtype=out_dtype)
     cs, num = _ns_coeffs(coeffs, steps)
     a = NewtonSchulzArgs.from_buffer_copy(_NS_PACK(
         g.data_ptr(), out.data_ptr(), ctypes.addressof(cs), 0, 0, g.shape[0] if g.dim() == 3 else 1, g.shape[-2],
