@@ -9,18 +9,21 @@
 //
 // The backward sorts the tokens by id, so that each row of dw is written once,
 // by one owner, without atomics, its tokens added in their order:
-//   embed_index  Each workgroup owns a run of up to 960 rows of the table and
+//   embed_index  Each workgroup owns a run of up to 480 rows of the table and
 //     looks at every id (they are few against the rows of dout, and in the L2
 //     after the first look): a count of the ids below its rows is where its tokens
-//     start in the sorted order, counts of its own rows (by wavefront, each
-//     walking a share of the tokens) give every row's start, and a second look
-//     puts its tokens there in order.  One launch, where a radix sort takes three
-//     for each digit.
-//   embed_rows   A group of lanes owns a piece of a row of dw: sums its
-//     tokens' rows and writes it (zeros for a row without tokens).  A row of
-//     more than kRun tokens (a padding or end token, in the worst case all of
-//     them) is cut at multiples of kRun positions of the sorted order, a group for
-//     each, into fp32 partials;
+//     start in the sorted order, and counts of its own rows (by wavefront, each
+//     walking a share of the tokens and listing those it finds) give every row's
+//     start and every token its place.  One launch, where a radix sort takes
+//     three for each digit.
+//   embed_rows   A group of lanes owns a 16-byte chunk each of a row of dw: sums
+//     its tokens' rows and writes it, zeros if it has none.  What hides the chain
+//     from a row's start over its tokens to their rows is wavefronts, so they are
+//     small: four rows in flight, not eight (63 us for 89 over 16384 tokens of
+//     2048 and 32000 rows), a chunk a lane, not the whole row (51 for 71).  A row of more than kRun
+//     tokens (a padding or end token, in the worst case all of them) is cut at
+//     multiples of kRun positions of the sorted order, a group for each, into fp32
+//     partials;
 //   embed_fold   adds those of a row in order and writes it.
 #include <algorithm>
 #include <cmath>
@@ -34,10 +37,11 @@ namespace {
 
 using namespace rowvec;
 
-constexpr int kRun = 64;          // tokens that one group adds up
+constexpr int kRun = 32;          // tokens that one group adds up
 constexpr int kScanWaves = 16;    // of embed_index
-constexpr int kScanRows = 960;    // table rows of one of its workgroups, at most (60 KB of counts)
-constexpr int kFoldWaves = 8;
+constexpr int kScanRows = 480;    // table rows of one of its workgroups, at most (30 KB of counts)
+constexpr int kScanList = 256;    // tokens that one of its wavefronts can list (32 KB in all)
+constexpr int kFoldWaves = 4;
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -95,15 +99,24 @@ __global__ __launch_bounds__(kBlock) void embed_lookup(LookupArgs a) {
 
 // ---- the order of the tokens -----------------------------------------------------
 
+struct IndexArgs {
+  const void* ids;
+  int32_t* order;
+  int32_t* start;
+  int64_t T, V;
+  int ids64, rows;
+};
+
 // order[]: the tokens with an id in [0, V) by id, those of one id ascending;
 // start[v]: where row v's begin, start[V] their number.
-__global__ __launch_bounds__(kScanWaves * 64) void embed_index(const void* ids, int ids64, int64_t T, int64_t V,
-                                                               int rows, int32_t* order, int32_t* start) {
+__global__ __launch_bounds__(kScanWaves * 64) void embed_index(IndexArgs a) {
   extern __shared__ int32_t count[];  // [wavefront][row]: tokens, then the next one's place
   __shared__ int32_t below_w[kScanWaves], scan_w[kScanWaves];
+  __shared__ int2 list[kScanWaves][kScanList];  // (row, token)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t v0 = (int64_t)blockIdx.x * rows;
-  const int mine = (int)min((int64_t)rows, V - v0);
+  const int64_t T = a.T, V = a.V, v0 = (int64_t)blockIdx.x * a.rows;
+  const int rows = a.rows, mine = (int)min((int64_t)rows, V - v0);
+  const int bits = 32 - __clz((rows - 1) | 1);
   for (int i = tid; i < kScanWaves * rows; i += kScanWaves * 64) count[i] = 0;
   __syncthreads();
 
@@ -112,21 +125,35 @@ __global__ __launch_bounds__(kScanWaves * 64) void embed_index(const void* ids, 
   const int64_t t0 = min(T, wave * per), t1 = min(T, t0 + per);
   int32_t* const own = count + wave * rows;
   constexpr int U = 8;  // looks in flight
+  // look(row or -1, or -2 below, token) for 64 tokens at a time.
+  auto scan = [&](auto look) __attribute__((always_inline)) {
+    for (int64_t t = t0; t < t1; t += 64 * U) {
+      int64_t id[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t k = t + u * 64 + lane;
+        id[u] = k < t1 ? load_id(a.ids, a.ids64, k) : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t r = id[u] - v0;
+        look(id[u] < 0 ? -1 : r < 0 ? -2 : r < mine ? (int)r : -1, (int32_t)(t + u * 64 + lane));
+      }
+    }
+  };
   int32_t below = 0;
-  for (int64_t t = t0; t < t1; t += 64 * U) {
-    int64_t id[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = t + u * 64 + lane;
-      id[u] = at < t1 ? load_id(ids, ids64, at) : -1;
+  int found = 0;  // of this wavefront
+  scan([&](int r, int32_t t) __attribute__((always_inline)) {
+    if (r == -2) ++below;
+    const uint64_t in = __ballot(r >= 0);
+    if (!in) return;
+    if (r >= 0) {
+      atomicAdd(own + r, 1);
+      const int at = found + __popcll(in & ((1ull << lane) - 1));
+      if (at < kScanList) list[wave][at] = make_int2(r, t);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t r = id[u] - v0;
-      if (id[u] >= 0 && r < 0) ++below;
-      else if (id[u] >= 0 && r < mine) atomicAdd(own + r, 1);
-    }
-  }
+    found += __popcll(in);
+  });
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) below += __shfl_xor(below, off, 64);
   if (lane == 0) below_w[wave] = below;
@@ -150,8 +177,8 @@ __global__ __launch_bounds__(kScanWaves * 64) void embed_index(const void* ids, 
     if (w < wave) at += scan_w[w];
   }
   if (tid < mine) {
-    start[v0 + tid] = at;
-    if (v0 + tid == V - 1) start[V] = at + n;
+    a.start[v0 + tid] = at;
+    if (v0 + tid == V - 1) a.start[V] = at + n;
     for (int w = 0; w < kScanWaves; ++w) {
       const int32_t c = count[w * rows + tid];
       count[w * rows + tid] = at;
@@ -160,33 +187,32 @@ __global__ __launch_bounds__(kScanWaves * 64) void embed_index(const void* ids, 
   }
   __syncthreads();
 
-  for (int64_t t = t0; t < t1; t += 64 * U) {
-    int64_t id[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t k = t + u * 64 + lane;
-      id[u] = k < t1 ? load_id(ids, ids64, k) : -1;
+  // The lanes' tokens to their places, all 64 at once: the lanes with a lane's row
+  // are found by the row's bits (one row at a time took 25 us where a workgroup
+  // owned a fifth of 16384 tokens).
+  auto place = [&](int r, int32_t t) __attribute__((always_inline)) {
+    uint64_t same = __ballot(r >= 0);
+    if (!same) return;
+    for (int bit = 0; bit < bits; ++bit) {
+      const uint64_t set = __ballot(r >= 0 && (r >> bit & 1));
+      same &= r >> bit & 1 ? set : ~set;
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t r64 = id[u] - v0;
-      const int r = id[u] >= 0 && r64 >= 0 && r64 < mine ? (int)r64 : -1;
-      // One id of the 64 at a time: its lanes in order.
-      uint64_t left = __ballot(r >= 0);
-      while (left) {
-        const int row = __builtin_amdgcn_readlane(r, __ffsll((unsigned long long)left) - 1);
-        const uint64_t same = __ballot(r == row);
-        const int32_t place = own[row];
-        if (r == row) {
-          const int before = __popcll(same & ((1ull << lane) - 1));
-          order[place + before] = (int32_t)(t + u * 64 + lane);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (lane == 0) own[row] = place + __popcll(same);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        left &= ~same;
-      }
+    if (r >= 0) {
+      const int before = __popcll(same & ((1ull << lane) - 1)), all = __popcll(same);
+      const int32_t to = own[r];
+      a.order[to + before] = t;
+      // (Every lane of the row has read its place: one instruction read them all.)
+      if (before == all - 1) own[r] = to + all;
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
+  if (found <= kScanList) {
+    for (int i = 0; i < found; i += 64) {
+      const int2 x = i + lane < found ? list[wave][i + lane] : make_int2(-1, 0);
+      place(x.x, x.y);
+    }
+  } else {
+    scan(place);
   }
 }
 
@@ -201,37 +227,36 @@ struct SumArgs {
   float* part;       // [2 blocks][part_ld]: of the run at a block's first, and at its last position
   int64_t V, ds, gs, part_ld;
   int64_t blocks;    // of kRun positions (0: no row can have more tokens)
-  int H, segs, ids64, add;
+  int H, segs, ids64, add;  // segs: groups of a row
   float scale;
 };
 
-// Sum of the rows of dout at positions [s, e) of the order.
-template <typename T, int LANES, int NV, int VEC>
-__device__ __forceinline__ void sum_rows(const SumArgs& a, int64_t s, int64_t e, int col, float (&acc)[NV][VEC]) {
-  constexpr int U = NV == 1 ? 8 : 4;  // rows in flight
+// Sum of the rows of dout at n <= kRun positions of the order, from s on; for a
+// group of a wavefront their tokens are in its lanes.
+template <typename T, int LANES, int VEC>
+__device__ __forceinline__ void sum_rows(const SumArgs& a, int64_t s, int n, int32_t tokens, int col,
+                                         float (&acc)[VEC]) {
+  constexpr int U = 4;  // rows in flight
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[i][j] = 0.f;
+  for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
   const T* const dout = static_cast<const T*>(a.dout);
-  for (int64_t p = s; p < e; p += U) {
-    float v[U][NV][VEC];
+  for (int p = 0; p < n; p += U) {
+    float v[U][VEC];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool in = p + u < e;
-      const T* row = dout + (int64_t)(in ? a.order[p + u] : 0) * a.ds;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) load_run<T, VEC>(row, col + i * LANES * VEC, in ? a.H : 0, 0.f, v[u][i]);
+      const bool in = p + u < n;
+      const int32_t t = LANES == 64 ? __builtin_amdgcn_readlane(tokens, (p + u) & 63) : in ? a.order[s + p + u] : 0;
+      load_run<T, VEC>(dout + (int64_t)t * a.ds, col, in ? a.H : 0, 0.f, v[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[i][j] += v[u][i][j];
+      for (int j = 0; j < VEC; ++j) acc[j] += v[u][j];
   }
 }
 
+// (Past the caches: dw is written once and mostly larger than they are; 953 MB of
+// f32 in 200 us for 270.)
 template <typename TO, int VEC>
 __device__ __forceinline__ void write_row(const SumArgs& a, int64_t v, int col, const float (&acc)[VEC]) {
   TO* const row = static_cast<TO*>(a.dw) + v * a.gs;
@@ -244,43 +269,48 @@ __device__ __forceinline__ void write_row(const SumArgs& a, int64_t v, int col, 
 #pragma unroll
     for (int j = 0; j < VEC; ++j) o[j] = acc[j] * a.scale;
   }
-  store_run<TO, VEC>(row, col, a.H, o);
+  store_run<TO, VEC, true>(row, col, a.H, o);
 }
 
-template <typename TI, typename TO, int LANES, int NV>
+template <typename TI, typename TO, int LANES>
 __global__ __launch_bounds__(kBlock) void embed_rows(SumArgs a) {
   constexpr int VEC = kVec<TI, TO>;
+  static_assert(kRun <= 64, "one load holds a run's tokens");
   const uint32_t g = group_id<LANES>(), which = g / (uint32_t)a.segs;
   int64_t task = which;
-  const int col = (int)(g - which * a.segs) * (LANES * NV * VEC) + (int)(threadIdx.x % LANES) * VEC;
-  float acc[NV][VEC];
+  const int lane = threadIdx.x % LANES;
+  const int col = (int)(g - which * a.segs) * (LANES * VEC) + lane * VEC;
+  float acc[VEC];
+  int64_t s, e;
   // The blocks of long runs first: they take longest.
-  if (task < 2 * a.blocks) {
+  const bool block = task < 2 * a.blocks;
+  if (block) {
     const int64_t n = a.start[a.V], p0 = (task >> 1) * kRun, p1 = min(p0 + kRun, n);
     if (p0 >= n) return;
-    const int64_t first = load_id(a.ids, a.ids64, a.order[p0]), last = load_id(a.ids, a.ids64, a.order[p1 - 1]);
-    if ((task & 1) && first == last) return;
-    const int64_t v = task & 1 ? last : first;
-    const int64_t s = a.start[v], e = a.start[v + 1];
+    const int64_t head = load_id(a.ids, a.ids64, a.order[p0]), tail = load_id(a.ids, a.ids64, a.order[p1 - 1]);
+    if ((task & 1) && head == tail) return;
+    const int64_t v = task & 1 ? tail : head;
+    s = a.start[v], e = a.start[v + 1];
     if (e - s <= kRun) return;
-    sum_rows<TI, LANES, NV, VEC>(a, max(s, p0), min(e, p1), col, acc);
-    float* const to = a.part + task * a.part_ld;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < VEC; j += 4)
-        if (col + i * LANES * VEC + j < a.H)  // (part_ld is H rounded up to whole chunks)
-          *reinterpret_cast<f32x4*>(to + col + i * LANES * VEC + j) =
-              f32x4{acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]};
+    s = max(s, p0), e = min(e, p1);
+  } else {
+    task -= 2 * a.blocks;
+    if (task >= a.V) return;
+    s = a.start[task], e = a.start[task + 1];
+    if (e - s > kRun || (a.add && s == e)) return;
+  }
+  const int n = (int)(e - s);
+  const int32_t tokens = LANES == 64 && lane < n ? a.order[s + lane] : 0;
+  sum_rows<TI, LANES, VEC>(a, s, n, tokens, col, acc);
+  if (!block) {
+    write_row<TO, VEC>(a, task, col, acc);
     return;
   }
-  task -= 2 * a.blocks;
-  if (task >= a.V) return;
-  const int64_t s = a.start[task], e = a.start[task + 1];
-  if (e - s > kRun || (a.add && s == e)) return;
-  sum_rows<TI, LANES, NV, VEC>(a, s, e, col, acc);
+  float* const to = a.part + task * a.part_ld + col;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) write_row<TO, VEC>(a, task, col + i * LANES * VEC, acc[i]);
+  for (int j = 0; j < VEC; j += 4)
+    if (col + j < a.H)  // (part_ld is H rounded up to whole chunks)
+      *reinterpret_cast<f32x4*>(to + j) = f32x4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]};
 }
 
 // Workgroup (block, segment): the long run that starts in the block, if any.
@@ -303,7 +333,7 @@ __global__ __launch_bounds__(kFoldWaves * 64) void embed_fold(SumArgs a) {
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
   if (col < a.H) {
-    constexpr int U = 4;
+    constexpr int U = 8;
     for (int64_t q = q0; q < q1; q += U) {
       f32x4 x[U][2];
 #pragma unroll
@@ -405,7 +435,7 @@ int plan_fwd(const mfx_embedding_args* a, FwdPlan& pl) {
 }
 
 struct BwdPlan {
-  Split sp;
+  int lanes, segs;
   int64_t blocks, grid, fold, part_ld;
   int rows;
   int64_t scans;
@@ -419,11 +449,13 @@ int plan_bwd(const mfx_embedding_bwd_args* a, BwdPlan& pl) {
     if (int rc = check_ids(a->ids, a->ids_dtype)) return rc;
     if (int rc = check_rows(a->dout, a->dout_stride, a->T, a->H, a->dtype, "dout", false)) return rc;
   }
-  pl.sp = split(a->V, a->H, vec_of(a->dtype, a->dw_dtype), 2);
+  const int vec = vec_of(a->dtype, a->dw_dtype);
+  pl.lanes = a->H <= 16 * vec ? 16 : 64;
+  pl.segs = (int)ceil_div(a->H, pl.lanes * vec);
   pl.blocks = a->T > kRun ? ceil_div(a->T, kRun) : 0;
-  pl.grid = ceil_div((2 * pl.blocks + a->V) * pl.sp.segs, kBlock / pl.sp.lanes);
+  pl.grid = ceil_div((2 * pl.blocks + a->V) * pl.segs, kBlock / pl.lanes);
   pl.fold = pl.blocks * ceil_div(a->H, 512);
-  // A workgroup of the index for each CU, of at most 960 rows (a thread each).
+  // A workgroup of the index for each CU, of at most 480 rows (a thread each).
   pl.rows = (int)std::min<int64_t>(kScanRows, ceil_div(a->V, device_cu_count()));
   pl.scans = ceil_div(a->V, pl.rows);
   if (!launch_fits(pl.grid, kBlock) || !launch_fits(pl.fold, kFoldWaves * 64) ||
@@ -449,9 +481,8 @@ void launch_lookup(const LookupArgs& p, const FwdPlan& pl, hipStream_t s) {
 template <typename TI, typename TO>
 void launch_rows(const SumArgs& p, const BwdPlan& pl, hipStream_t s) {
   const dim3 grid((unsigned)pl.grid), block(kBlock);
-  if (pl.sp.lanes == 16) hipLaunchKernelGGL((embed_rows<TI, TO, 16, 1>), grid, block, 0, s, p);
-  else if (pl.sp.nv == 1) hipLaunchKernelGGL((embed_rows<TI, TO, 64, 1>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((embed_rows<TI, TO, 64, 2>), grid, block, 0, s, p);
+  if (pl.lanes == 16) hipLaunchKernelGGL((embed_rows<TI, TO, 16>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((embed_rows<TI, TO, 64>), grid, block, 0, s, p);
 }
 
 // f(TI{}, TO{}) for a pair of element types.
@@ -507,11 +538,11 @@ int mfx_embedding_bwd(const mfx_embedding_bwd_args* args, void* stream) {
   int32_t* const order = reinterpret_cast<int32_t*>(ws);
   int32_t* const start = reinterpret_cast<int32_t*>(ws + pl.order_bytes);
   const int ids64 = a.ids_dtype == MFX_I64;
-  hipLaunchKernelGGL(embed_index, dim3((unsigned)pl.scans), dim3(kScanWaves * 64), (size_t)kScanWaves * pl.rows * 4, s,
-                     a.ids, ids64, a.T, a.V, pl.rows, order, start);
+  const IndexArgs x{a.ids, order, start, a.T, a.V, ids64, pl.rows};
+  hipLaunchKernelGGL(embed_index, dim3((unsigned)pl.scans), dim3(kScanWaves * 64), (size_t)kScanWaves * pl.rows * 4, s, x);
   if (int rc = launch_status("embed_index")) return rc;
   const SumArgs p{a.dout, a.ids, a.dw, order, start, reinterpret_cast<float*>(ws + pl.order_bytes + pl.start_bytes),
-                  a.V, a.dout_stride, a.dw_stride, pl.part_ld, pl.blocks, (int)a.H, pl.sp.segs, ids64,
+                  a.V, a.dout_stride, a.dw_stride, pl.part_ld, pl.blocks, (int)a.H, pl.segs, ids64,
                   a.accumulate != 0, a.scale};
   with_types(a.dtype, a.dw_dtype, [&](auto ti, auto to) { launch_rows<decltype(ti), decltype(to)>(p, pl, s); });
   if (int rc = launch_status("embed_rows")) return rc;

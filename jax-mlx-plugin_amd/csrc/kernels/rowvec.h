@@ -166,18 +166,22 @@ __device__ __forceinline__ void load_run(const T* row, int e, int n, float fill,
   }
 }
 
-template <typename T, int VEC>
+// NT: past the caches.
+template <typename T, int VEC, bool NT = false>
 __device__ __forceinline__ void store_run(T* row, int e, int n, const float (&v)[VEC]) {
   if (e + VEC <= n) {
     if constexpr (sizeof(T) == 4) {
       typedef float run_t __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
       for (int c = 0; c < VEC; c += 4)
-        *reinterpret_cast<run_t*>(row + e + c) = run_t{v[c], v[c + 1], v[c + 2], v[c + 3]};
+        if constexpr (NT)
+          __builtin_nontemporal_store(run_t{v[c], v[c + 1], v[c + 2], v[c + 3]}, reinterpret_cast<run_t*>(row + e + c));
+        else *reinterpret_cast<run_t*>(row + e + c) = run_t{v[c], v[c + 1], v[c + 2], v[c + 3]};
     } else {
       typedef uint32_t run_t __attribute__((ext_vector_type(4), aligned(2)));
       const typename Vec16<T>::type w = pack16<T>(v);
-      *reinterpret_cast<run_t*>(row + e) = run_t{w.x, w.y, w.z, w.w};
+      if constexpr (NT) __builtin_nontemporal_store(run_t{w.x, w.y, w.z, w.w}, reinterpret_cast<run_t*>(row + e));
+      else *reinterpret_cast<run_t*>(row + e) = run_t{w.x, w.y, w.z, w.w};
     }
   } else {
 #pragma unroll

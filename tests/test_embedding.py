@@ -102,14 +102,15 @@ def test_lookup_and_gradient(cuda, nat, case):
     assert torch.equal(got[none], before[none])  # rows without tokens, bit for bit
 
 
-RUNS = [[1], [64], [65], [64, 64], [63, 66, 1], [1, 64, 65], [200], [129, 0, 3, 128], [5] * 30 + [500], [0, 0, 64, 0]]
+RUNS = [[1], [32], [33], [32, 32], [31, 34, 1], [1, 32, 33], [64], [65], [64, 64], [63, 66, 1], [1, 64, 65], [200],
+        [129, 0, 3, 128], [5] * 30 + [500], [0, 0, 64, 0], [0, 32, 0, 33, 0]]
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("order", ["sorted", "mixed"])
 @pytest.mark.parametrize("runs", RUNS, ids=str)
 def test_runs_about_a_pieces_length(cuda, nat, runs, order):
-    """Rows of 0, 1, 64, 65 .. tokens that start anywhere in a piece, against exact sums of small integers."""
+    """Rows of 0, 1, 32, 33 .. tokens that start anywhere in a piece, against exact sums of small integers."""
     torch = cuda
     V, H = len(runs) + 1, 520
     ids = np.repeat(np.arange(len(runs)), runs)
