@@ -50,248 +50,415 @@ struct Args {
   float alpha, beta, o, post_eps, pre_eps;
 };
 
-// VEC values of a row of any of the three types, chosen at run time (uniform).
-__device__ __forceinline__ void load_any(const void* p, int dt, int64_t at, int e, int n, float (&out)[VEC]) {
-  if (dt == MFX_F32) load_run<float, VEC>(static_cast<const float*>(p) + at, e, n, 0.f, out);
-  else if (dt == MFX_BF16) load_run<bf16, VEC>(static_cast<const bf16*>(p) + at, e, n, 0.f, out);
-  else load_run<_Float16, VEC>(static_cast<const _Float16*>(p) + at, e, n, 0.f, out);
-}
-__device__ __forceinline__ void store_any(void* p, int dt, int64_t at, int e, int n, const float (&v)[VEC]) {
-  if (dt == MFX_F32) store_run<float, VEC>(static_cast<float*>(p) + at, e, n, v);
-  else if (dt == MFX_BF16) store_run<bf16, VEC>(static_cast<bf16*>(p) + at, e, n, v);
-  else store_run<_Float16, VEC>(static_cast<_Float16*>(p) + at, e, n, v);
+// A lane's VEC elements of a row as they come, so that loads stay in flight: no
+// branch and no use between one load and the next (a load of a row's whole chunks
+// beside one of its last elements, each unpacked on the spot, waited for every tensor
+// of a row in turn: 155 us for 8192 rows of 4096 backward).  A lane past the row's
+// end reads its last VEC elements again.  Of a row that is not whole chunks (not
+// EASY) its last lane does so too and shifts what it needs down, zeros behind it.
+template <typename T, bool EASY>
+struct Raw {
+  static constexpr int N = VEC * sizeof(T) / 4;
+  uint32_t w[N];
+  __device__ __forceinline__ void load(const void* p, int64_t at, int e, int n) {
+    if (EASY || n >= VEC) {
+      typedef uint32_t run_t __attribute__((ext_vector_type(4), aligned(2)));
+      const T* from = static_cast<const T*>(p) + at + min(e, n - VEC);
+#pragma unroll
+      for (int c = 0; c < N / 4; ++c) {
+        const run_t r = reinterpret_cast<const run_t*>(from)[c];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[c * 4 + j] = r[j];
+      }
+    } else {  // a row shorter than a chunk, the same for all lanes
+#pragma unroll
+      for (int j = 0; j < N; ++j) w[j] = 0;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (e == 0 && j < n) {
+          if constexpr (sizeof(T) == 4) w[j] = static_cast<const uint32_t*>(p)[at + j];
+          else w[j / 2] |= (uint32_t)static_cast<const uint16_t*>(p)[at + j] << (16 * (j & 1));
+        }
+    }
+  }
+  // Elements of the row from e on (EASY: any where e lies past its end).
+  __device__ __forceinline__ void get(int e, int n, float (&out)[VEC]) const {
+    uint32_t x[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = w[j];
+    if (!EASY && n >= VEC) {
+      const int s = max(0, min(VEC, e + VEC - n));  // elements to shift down by
+      const int words = sizeof(T) == 4 ? s : s >> 1;
+#pragma unroll
+      for (int step = 1; step <= N; step *= 2)
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = words & step ? (j + step < N ? x[j + step] : 0u) : x[j];
+      if constexpr (sizeof(T) == 2)
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = s & 1 ? x[j] >> 16 | (j + 1 < N ? x[j + 1] << 16 : 0u) : x[j];
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) out[j] = __uint_as_float(x[j]);
+    } else {
+      unpack16<T>(make_uint4(x[0], x[1], x[2], x[3]), out);
+    }
+  }
+};
+
+// The same of a tensor of any of the three types, chosen at run time (uniform).
+template <bool EASY>
+struct RawAny {
+  Raw<float, EASY> f;  // (of a 16-bit tensor the first half)
+  __device__ __forceinline__ void load(const void* p, int dt, int64_t at, int e, int n) {
+    if (dt == MFX_F32) return f.load(p, at, e, n);
+    Raw<bf16, EASY> h;
+    h.load(p, at, e, n);
+#pragma unroll
+    for (int j = 0; j < h.N; ++j) f.w[j] = h.w[j];
+  }
+  template <typename T>
+  __device__ __forceinline__ void get16(int e, int n, float (&out)[VEC]) const {
+    Raw<T, EASY> h;
+#pragma unroll
+    for (int j = 0; j < h.N; ++j) h.w[j] = f.w[j];
+    h.get(e, n, out);
+  }
+  __device__ __forceinline__ void get(int dt, int e, int n, float (&out)[VEC]) const {
+    if (dt == MFX_F32) f.get(e, n, out);
+    else if (dt == MFX_BF16) get16<bf16>(e, n, out);
+    else get16<_Float16>(e, n, out);
+  }
+};
+
+// A chunk's elements of a row; EASY rows have no last, partial one.
+template <typename T, bool EASY>
+__device__ __forceinline__ void store_chunk(void* p, int64_t at, int e, int n, const float (&v)[VEC]) {
+  T* const row = static_cast<T*>(p) + at;
+  if constexpr (EASY) {
+    if (e < n) store_run<T, VEC>(row, e, e + VEC, v);
+  } else {
+    store_run<T, VEC>(row, e, n, v);
+  }
 }
 
-// The last sequence that starts at or before token t, 0 if none does.
+template <bool EASY>
+__device__ __forceinline__ void store_any(void* p, int dt, int64_t at, int e, int n, const float (&v)[VEC]) {
+  if (dt == MFX_F32) store_chunk<float, EASY>(p, at, e, n, v);
+  else if (dt == MFX_BF16) store_chunk<bf16, EASY>(p, at, e, n, v);
+  else store_chunk<_Float16, EASY>(p, at, e, n, v);
+}
+
+// The last sequence that starts at or before token t, 0 if none does: 64 offsets at
+// a time, a lane each.  All lanes of a wavefront look for tokens of their own group.
 __device__ __forceinline__ int64_t find_seq(const int32_t* off, int64_t S, int64_t t) {
-  int64_t lo = 0, hi = S;  // off[lo] <= t or lo = 0; off[hi] > t or hi = S
-  while (hi - lo > 1) {
-    const int64_t m = (lo + hi) >> 1;
-    if (off[m] <= t) lo = m;
-    else hi = m;
+  int64_t lo = 0, n = S;  // among the n from lo on
+  while (n > 1) {
+    const int64_t step = (n + 63) / 64;
+    const int64_t i = lo + (threadIdx.x & 63) * step;
+    const uint64_t at = __ballot(i < lo + n && off[min(i, S)] <= t);
+    // (Offsets ascend: the lanes that say so are the first ones.)
+    const int hits = (int)__popcll(at), last = hits > 0 ? hits - 1 : 0;
+    n = min(step, n - last * step);
+    lo += last * step;
   }
   return lo;
 }
 
+// What a gate's rows are shared by: kNone no gate, kShared one row, or one a
+// sequence, kToken one a token, kAny any of them, decided at run time.
+enum Kind { kNone, kShared, kToken, kAny };
+
 template <int LANES>
 struct Group {
-  static constexpr int THREADS = LANES > kBlock ? LANES : kBlock;
+  static constexpr int THREADS = LANES > 64 ? LANES : kBlock;
   static constexpr int RPB = THREADS / LANES;  // groups of a workgroup
 };
 
-// A row's gate in registers: whether the row takes part of y at all, and, for
-// a sequence's gate, which sequence's is loaded.
-template <int LANES, int NV>
-struct Gate {
-  float g[NV][VEC];
-  int64_t seq = -1, loaded = -1;
-  __device__ __forceinline__ void load(const Args& a, int64_t row, int lane) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      load_any(a.gate, a.gate_dt, row * a.gs, (i * LANES + lane) * VEC, a.H, g[i]);
+#define FOR_CHUNKS _Pragma("unroll") for (int i = 0; i < NV; ++i)
+#define FOR_ELEMS FOR_CHUNKS _Pragma("unroll") for (int j = 0; j < VEC; ++j)
+
+// A lane's chunks of a row: elements (i * LANES + lane) * VEC and on.
+template <int LANES_, int NV_, bool EASY_>
+struct Place {
+  static constexpr int LANES = LANES_, NV = NV_;
+  static constexpr bool EASY = EASY_;
+  int lane, n;
+  bool in[NV];  // any of the chunk lies in the row
+  __device__ __forceinline__ Place(int H) : lane(threadIdx.x % LANES), n(H) {
+    FOR_CHUNKS in[i] = e(i) < n;
   }
-  __device__ __forceinline__ void begin(const Args& a, int64_t t, int lane) {
-    if (a.mode == MFX_GATE_FEATURE) load(a, 0, lane);
-    if (a.mode == MFX_GATE_NONE) {
+  __device__ __forceinline__ int e(int i) const { return (i * LANES + lane) * VEC; }
+  template <typename T>
+  __device__ __forceinline__ void load(Raw<T, EASY> (&r)[NV], const void* p, int64_t at) const {
+    FOR_CHUNKS r[i].load(p, at, e(i), n);
+  }
+  template <typename T>
+  __device__ __forceinline__ void get(const Raw<T, EASY> (&r)[NV], float (&out)[NV][VEC]) const {
+    FOR_CHUNKS r[i].get(e(i), n, out[i]);
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(void* p, int64_t at, const float (&v)[NV][VEC]) const {
+    FOR_CHUNKS store_chunk<T, EASY>(p, at, e(i), n, v[i]);
+  }
+  // Sum over the row of f(i, j, so far) (lanes past its end add nothing).
+  template <class F>
+  __device__ __forceinline__ float sum(F f) const {
+    float s = 0.f;
+    FOR_CHUNKS {
+      float c = 0.f;
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) g[i][j] = 1.f;
+      for (int j = 0; j < VEC; ++j) c = f(i, j, c);
+      s += in[i] ? c : 0.f;
     }
-    if (a.mode == MFX_GATE_SEQUENCE && a.S > 0) seq = find_seq(a.off, a.S, t);
-  }
-  // Row t's gate; false: the row is in no sequence.
-  __device__ __forceinline__ bool row(const Args& a, int64_t t, int lane) {
-    if (a.mode == MFX_GATE_TOKEN) load(a, t, lane);
-    if (a.mode != MFX_GATE_SEQUENCE) return true;
-    if (a.S <= 0) return false;
-    while (seq + 1 < a.S && a.off[seq + 1] <= t) ++seq;
-    if (t < a.off[seq] || t >= a.off[seq + 1]) return false;
-    if (seq != loaded) load(a, seq, lane);
-    loaded = seq;
-    return true;
+    return s;
   }
 };
 
-template <int LANES, int NV>
-__device__ __forceinline__ void load_weight(const Args& a, const void* w, int lane, float (&out)[NV][VEC]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (w) {
-      load_any(w, a.param_dt, 0, (i * LANES + lane) * VEC, a.H, out[i]);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) out[i][j] += a.o;
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) out[i][j] = 1.f;
+template <class P>
+__device__ __forceinline__ void load_weight(const Args& a, const P& at, const void* w, float (&out)[P::NV][VEC]) {
+  constexpr int NV = P::NV;
+  FOR_ELEMS out[i][j] = 1.f;
+  if (!w) return;
+  FOR_CHUNKS {
+    RawAny<P::EASY> r;
+    r.load(w, a.param_dt, 0, at.e(i), at.n);
+    r.get(a.param_dt, at.e(i), at.n, out[i]);
+  }
+  FOR_ELEMS out[i][j] += a.o;
+}
+
+// The gate of a group's rows: the one row of all, or the row's sequence's (whose
+// row is loaded when it changes) or its own.
+template <class P, Kind KIND>
+struct Gate {
+  static constexpr int NV = P::NV;
+  float g[NV][VEC];
+  RawAny<P::EASY> next[NV];  // of a gate by token: the next row's
+  int64_t seq = -1;
+  int32_t first = 0, end = 0;  // its tokens
+  __device__ __forceinline__ bool token(const Args& a) const {
+    return KIND == kToken || (KIND == kAny && a.mode == MFX_GATE_TOKEN);
+  }
+  __device__ __forceinline__ bool sequence(const Args& a) const {
+    return (KIND == kShared || KIND == kAny) && a.mode == MFX_GATE_SEQUENCE;
+  }
+  __device__ __forceinline__ void take(const Args& a, const P& at) {
+    FOR_CHUNKS next[i].get(a.gate_dt, at.e(i), at.n, g[i]);
+  }
+  __device__ __forceinline__ void fetch(const Args& a, const P& at, int64_t row) {
+    FOR_CHUNKS next[i].load(a.gate, a.gate_dt, row * a.gs, at.e(i), at.n);
+  }
+  __device__ __forceinline__ void turn(const Args& a, const P& at) {
+    first = a.off[seq];
+    end = a.off[seq + 1];
+    fetch(a, at, seq);
+    take(a, at);
+  }
+  __device__ __forceinline__ void begin(const Args& a, const P& at, int64_t t) {
+    FOR_ELEMS g[i][j] = 1.f;
+    if (token(a)) {
+      fetch(a, at, t);
+    } else if (sequence(a)) {
+      if (a.S <= 0) return;
+      seq = find_seq(a.off, a.S, t);
+      turn(a, at);
+    } else if (KIND == kShared || a.mode == MFX_GATE_FEATURE) {
+      fetch(a, at, 0);
+      take(a, at);
     }
   }
-}
+  // Row t's gate, and the fetch of row `after`'s; false: the row is in no sequence.
+  __device__ __forceinline__ bool row(const Args& a, const P& at, int64_t t, int64_t after) {
+    if (token(a)) {
+      take(a, at);
+      fetch(a, at, after);
+    }
+    if (!sequence(a)) return true;
+    if (a.S <= 0) return false;
+    if (t >= end && seq + 1 < a.S && a.off[seq + 1] <= t) {
+      do ++seq;
+      while (seq + 1 < a.S && a.off[seq + 1] <= t);
+      turn(a, at);
+    }
+    return t >= first && t < end;
+  }
+};
 
-template <typename T, int LANES, int NV>
-__device__ __forceinline__ void load_row(const void* p, int64_t at, int lane, int n, float (&out)[NV][VEC]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    load_run<T, VEC>(static_cast<const T*>(p) + at, (i * LANES + lane) * VEC, n, 0.f, out[i]);
-}
-template <typename T, int LANES, int NV>
-__device__ __forceinline__ void store_row(void* p, int64_t at, int lane, int n, const float (&v)[NV][VEC]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i) store_run<T, VEC>(static_cast<T*>(p) + at, (i * LANES + lane) * VEC, n, v[i]);
-}
-
-#define FOR_ELEMS                  \
-  _Pragma("unroll") for (int i = 0; i < NV; ++i) _Pragma("unroll") for (int j = 0; j < VEC; ++j)
-
-template <typename TX, typename TY, int LANES, int NV>
-__global__ __launch_bounds__(Group<LANES>::THREADS) void residual_fwd(Args a) {
-  constexpr int RPB = Group<LANES>::RPB;
+template <typename TX, typename TY, class P, Kind KIND>
+__global__ __launch_bounds__(Group<P::LANES>::THREADS) void residual_fwd(Args a) {
+  constexpr int LANES = P::LANES, NV = P::NV, RPB = Group<LANES>::RPB;
+  constexpr bool GATED = KIND != kNone;
   __shared__ float lds[Group<LANES>::THREADS / 64];
-  const int lane = threadIdx.x % LANES;
+  const P at(a.H);
   const int64_t grp = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES;
   const int64_t t0 = grp * a.per, t1 = min(a.T, t0 + a.per);
   if (t0 >= t1) return;  // (a whole group; groups of more than a wavefront are workgroups)
   const float inv_n = 1.f / (float)a.H;
   const bool post = a.post_eps >= 0.f, pre = a.pre_eps >= 0.f;
+  Raw<TX, P::EASY> xr[NV];
+  Raw<TY, P::EASY> yr[NV];
+  at.load(yr, a.y, t0 * a.ys);
+  at.load(xr, a.x, t0 * a.xs);
   float wp[NV][VEC], wn[NV][VEC];
-  if (post) load_weight<LANES, NV>(a, a.wp, lane, wp);
-  if (pre) load_weight<LANES, NV>(a, a.wn, lane, wn);
-  Gate<LANES, NV> gate;
-  gate.begin(a, t0, lane);
+  load_weight(a, at, a.wp, wp);
+  load_weight(a, at, a.wn, wn);
+  Gate<P, KIND> gate;
+  if (GATED) gate.begin(a, at, t0);
   for (int64_t t = t0; t < t1; ++t) {
     float x[NV][VEC], y[NV][VEC];
-    load_row<TX, LANES, NV>(a.x, t * a.xs, lane, a.H, x);
-    const bool in = gate.row(a, t, lane);
-    load_row<TY, LANES, NV>(a.y, t * a.ys, lane, in ? a.H : 0, y);
+    at.get(yr, y);
+    at.get(xr, x);
+    const int64_t next = min(t + 1, t1 - 1);
+    if (t + 1 < t1) {
+      at.load(yr, a.y, next * a.ys);
+      at.load(xr, a.x, next * a.xs);
+    }
+    const bool in = !GATED || gate.row(a, at, t, next);
     float f = a.beta;
     if (post) {
-      float q = 0.f;
-      FOR_ELEMS q = fmaf(y[i][j], y[i][j], q);
-      const float inv = rsqrtf(row_reduce<LANES, false>(q, lds) * inv_n + a.post_eps);
-      f = in ? f * inv : 0.f;
+      const float q = at.sum([&](int i, int j, float s) { return fmaf(y[i][j], y[i][j], s); });
+      f *= rsqrtf(row_reduce<LANES, false>(q, lds) * inv_n + a.post_eps);
       FOR_ELEMS y[i][j] *= wp[i][j];
     }
-    float q = 0.f;
     FOR_ELEMS {
-      const float part = in ? f * gate.g[i][j] * y[i][j] : 0.f;
-      x[i][j] = fmaf(a.alpha, x[i][j], part);
-      q = fmaf(x[i][j], x[i][j], q);
+      if (GATED) x[i][j] = fmaf(a.alpha, x[i][j], in ? f * gate.g[i][j] * y[i][j] : 0.f);
+      else x[i][j] = fmaf(a.alpha, x[i][j], f * y[i][j]);
     }
-    store_row<TX, LANES, NV>(a.r, t * a.rs, lane, a.H, x);
+    at.template store<TX>(a.r, t * a.rs, x);
     if (!pre) continue;
+    const float q = at.sum([&](int i, int j, float s) { return fmaf(x[i][j], x[i][j], s); });
     const float inv = rsqrtf(row_reduce<LANES, false>(q, lds) * inv_n + a.pre_eps);
     FOR_ELEMS x[i][j] *= inv * wn[i][j];
-    store_row<TY, LANES, NV>(a.h, t * a.hs, lane, a.H, x);
+    at.template store<TY>(a.h, t * a.hs, x);
   }
 }
 
 // Adds the groups' sums of a workgroup and writes its partial row k.
-template <int LANES, int NV>
-__device__ __forceinline__ void write_partial(const Args& a, int k, int lane, int grp, float* fold,
-                                              float (&v)[NV][VEC]) {
-  constexpr int RPB = Group<LANES>::RPB, W = LANES * NV * VEC;
+template <class P>
+__device__ __forceinline__ void write_partial(const Args& a, const P& at, int k, int grp, float* fold,
+                                              float (&v)[P::NV][VEC]) {
+  constexpr int NV = P::NV, RPB = Group<P::LANES>::RPB, W = P::LANES * NV * VEC;
   if (k < 0) return;
   if constexpr (RPB > 1) {
     __syncthreads();
-    FOR_ELEMS fold[grp * W + (i * LANES + lane) * VEC + j] = v[i][j];
+    FOR_ELEMS fold[grp * W + at.e(i) + j] = v[i][j];
     __syncthreads();
     if (grp != 0) return;
 #pragma unroll
-    for (int b = 1; b < RPB; ++b) FOR_ELEMS v[i][j] += fold[b * W + (i * LANES + lane) * VEC + j];
+    for (int b = 1; b < RPB; ++b) FOR_ELEMS v[i][j] += fold[b * W + at.e(i) + j];
   }
-  store_row<float, LANES, NV>(a.part + ((int64_t)blockIdx.x * a.nsum + k) * a.ld, 0, lane, a.H, v);
+  at.template store<float>(a.part + ((int64_t)blockIdx.x * a.nsum + k) * a.ld, 0, v);
 }
 
-template <typename TX, typename TY, int LANES, int NV>
-__global__ __launch_bounds__(Group<LANES>::THREADS) void residual_bwd(Args a) {
-  constexpr int RPB = Group<LANES>::RPB;
+template <typename TX, typename TY, class P, Kind KIND>
+__global__ __launch_bounds__(Group<P::LANES>::THREADS) void residual_bwd(Args a) {
+  constexpr int LANES = P::LANES, NV = P::NV, RPB = Group<LANES>::RPB;
+  constexpr bool GATED = KIND != kNone;
   __shared__ float lds[2 * Group<LANES>::THREADS / 64];
   __shared__ float fold[RPB > 1 ? RPB * LANES * NV * VEC : 1];
-  const int lane = threadIdx.x % LANES, in_wg = threadIdx.x / LANES;
+  const P at(a.H);
+  const int in_wg = threadIdx.x / LANES;
   const int64_t grp = (int64_t)blockIdx.x * RPB + in_wg;
   const int64_t t0 = min(a.T, grp * a.per), t1 = min(a.T, t0 + a.per);
   const float inv_n = 1.f / (float)a.H;
   const bool post = a.post_eps >= 0.f, pre = a.pre_eps >= 0.f;
-  float wp[NV][VEC], wn[NV][VEC], sp[NV][VEC], sn[NV][VEC], sg[NV][VEC];
+  float sp[NV][VEC], sn[NV][VEC], sg[NV][VEC];
   FOR_ELEMS sp[i][j] = sn[i][j] = sg[i][j] = 0.f;
-  load_weight<LANES, NV>(a, a.wp, lane, wp);
-  load_weight<LANES, NV>(a, a.wn, lane, wn);
-  Gate<LANES, NV> gate;
-  if (t0 < t1) gate.begin(a, t0, lane);
-  int64_t cur = -1;  // the sequence whose gate's gradient is in sg
-  auto flush = [&]() {
-    if (cur >= 0) store_row<float, LANES, NV>(a.slots + (grp + cur) * a.ld, 0, lane, a.H, sg);
-    FOR_ELEMS sg[i][j] = 0.f;
-  };
-  for (int64_t t = t0; t < t1; ++t) {
-    float x[NV][VEC], y[NV][VEC], d[NV][VEC], u[NV][VEC];
-    load_row<TX, LANES, NV>(a.x, t * a.xs, lane, a.H, x);
-    load_row<TX, LANES, NV>(a.dr, t * a.drs, lane, a.dr ? a.H : 0, d);
-    load_row<TY, LANES, NV>(a.dh, t * a.dhs, lane, a.dh ? a.H : 0, u);
-    const bool in = gate.row(a, t, lane);
-    load_row<TY, LANES, NV>(a.y, t * a.ys, lane, in ? a.H : 0, y);
-    float iy = 1.f;
-    if (post) {
-      float q = 0.f;
-      FOR_ELEMS q = fmaf(y[i][j], y[i][j], q);
-      iy = rsqrtf(row_reduce<LANES, false>(q, lds) * inv_n + a.post_eps);
-      FOR_ELEMS y[i][j] = in ? y[i][j] * iy : 0.f;  // yh
-    }
-    if (pre) {
-      float q = 0.f, m = 0.f;
-      FOR_ELEMS {
-        const float part = in ? a.beta * gate.g[i][j] * (y[i][j] * wp[i][j]) : 0.f;
-        x[i][j] = fmaf(a.alpha, x[i][j], part);  // r
-        q = fmaf(x[i][j], x[i][j], q);
-        m = fmaf(u[i][j] * wn[i][j], x[i][j], m);
-      }
-      row_reduce_sum2<LANES>(q, m, lds);
-      const float ir = rsqrtf(q * inv_n + a.pre_eps);
-      const float mr = m * ir * inv_n;
-      FOR_ELEMS {
-        const float rh = x[i][j] * ir;
-        sn[i][j] = fmaf(u[i][j], rh, sn[i][j]);
-        d[i][j] = fmaf(ir, u[i][j] * wn[i][j] - rh * mr, d[i][j]);
-      }
-    }
-    // x: dx, u: dy
-    FOR_ELEMS x[i][j] = a.alpha * d[i][j];
-    store_row<TX, LANES, NV>(a.dx, t * a.dxs, lane, a.H, x);
-    if (a.mode == MFX_GATE_SEQUENCE && a.slots && in && gate.seq != cur) {
-      flush();
-      cur = gate.seq;
-    }
-    float m = 0.f;
-    FOR_ELEMS {
-      const float bd = in ? a.beta * d[i][j] : 0.f;
-      const float z = y[i][j] * wp[i][j];
-      const float dz = in ? bd * gate.g[i][j] : 0.f;
-      if (a.mode == MFX_GATE_TOKEN) x[i][j] = bd * z;
-      else sg[i][j] = fmaf(bd, z, sg[i][j]);
-      u[i][j] = dz;
+  if (t0 < t1) {
+    Raw<TX, P::EASY> xr[NV], dr[NV];
+    Raw<TY, P::EASY> yr[NV], ur[NV];
+    // (Without a gradient: x or y in its place, not used.)
+    const void* const dh = a.dh ? a.dh : a.y;
+    const void* const up = a.dr ? a.dr : a.x;
+    const int64_t us = a.dh ? a.dhs : a.ys, ds = a.dr ? a.drs : a.xs;
+    auto fetch = [&](int64_t t) __attribute__((always_inline)) {
+      at.load(yr, a.y, t * a.ys);
+      at.load(xr, a.x, t * a.xs);
+      at.load(ur, dh, t * us);
+      at.load(dr, up, t * ds);
+    };
+    fetch(t0);
+    float wp[NV][VEC], wn[NV][VEC];
+    load_weight(a, at, a.wp, wp);
+    load_weight(a, at, a.wn, wn);
+    Gate<P, KIND> gate;
+    if (GATED) gate.begin(a, at, t0);
+    int64_t cur = -1;  // the sequence whose gate's gradient is in sg
+    auto flush = [&]() {
+      if (cur >= 0) at.template store<float>(a.slots + (grp + cur) * a.ld, 0, sg);
+      FOR_ELEMS sg[i][j] = 0.f;
+    };
+    for (int64_t t = t0; t < t1; ++t) {
+      float x[NV][VEC], y[NV][VEC], d[NV][VEC], u[NV][VEC];
+      at.get(yr, y);
+      at.get(xr, x);
+      at.get(ur, u);
+      at.get(dr, d);
+      if (!a.dh) FOR_ELEMS u[i][j] = 0.f;
+      if (!a.dr) FOR_ELEMS d[i][j] = 0.f;
+      if (t + 1 < t1) fetch(t + 1);
+      const bool in = !GATED || gate.row(a, at, t, min(t + 1, t1 - 1));
+      float iy = 1.f;
       if (post) {
-        sp[i][j] = fmaf(dz, y[i][j], sp[i][j]);
-        u[i][j] = dz * wp[i][j];
-        m = fmaf(u[i][j], y[i][j], m);
+        const float q = at.sum([&](int i, int j, float s) { return fmaf(y[i][j], y[i][j], s); });
+        iy = rsqrtf(row_reduce<LANES, false>(q, lds) * inv_n + a.post_eps);
+        FOR_ELEMS y[i][j] *= iy;  // yh
       }
+      if (GATED && !in) FOR_ELEMS y[i][j] = 0.f;
+      if (pre) {
+        FOR_ELEMS {
+          const float z = y[i][j] * wp[i][j];
+          x[i][j] = fmaf(a.alpha, x[i][j], a.beta * (GATED ? (in ? gate.g[i][j] * z : 0.f) : z));  // r
+        }
+        float q = at.sum([&](int i, int j, float s) { return fmaf(x[i][j], x[i][j], s); });
+        float m = at.sum([&](int i, int j, float s) { return fmaf(u[i][j] * wn[i][j], x[i][j], s); });
+        row_reduce_sum2<LANES>(q, m, lds);
+        const float ir = rsqrtf(q * inv_n + a.pre_eps);
+        const float mr = m * ir * inv_n;
+        FOR_ELEMS {
+          const float rh = x[i][j] * ir;
+          sn[i][j] = fmaf(u[i][j], rh, sn[i][j]);
+          d[i][j] = fmaf(ir, u[i][j] * wn[i][j] - rh * mr, d[i][j]);
+        }
+      }
+      FOR_ELEMS x[i][j] = a.alpha * d[i][j];
+      at.template store<TX>(a.dx, t * a.dxs, x);
+      // u: dz, then dy
+      FOR_ELEMS u[i][j] = a.beta * d[i][j];
+      if constexpr (GATED) {
+        if (gate.sequence(a) && a.slots && in && gate.seq != cur) {
+          flush();
+          cur = gate.seq;
+        }
+        if (!in) FOR_ELEMS u[i][j] = 0.f;
+        if (gate.token(a)) {
+          FOR_ELEMS x[i][j] = u[i][j] * (y[i][j] * wp[i][j]);
+          if (a.dgate) FOR_CHUNKS store_any<P::EASY>(a.dgate, a.gate_dt, t * a.dgs, at.e(i), at.n, x[i]);
+        } else {
+          FOR_ELEMS sg[i][j] = fmaf(u[i][j], y[i][j] * wp[i][j], sg[i][j]);
+        }
+        if (in) FOR_ELEMS u[i][j] *= gate.g[i][j];
+      }
+      if (post) {
+        FOR_ELEMS {
+          sp[i][j] = fmaf(u[i][j], y[i][j], sp[i][j]);
+          u[i][j] *= wp[i][j];
+        }
+        const float m = at.sum([&](int i, int j, float s) { return fmaf(u[i][j], y[i][j], s); });
+        const float my = row_reduce<LANES, false>(m, lds) * inv_n;
+        FOR_ELEMS u[i][j] = GATED && !in ? 0.f : iy * (u[i][j] - y[i][j] * my);
+      }
+      at.template store<TY>(a.dy, t * a.dys, u);
     }
-    if (a.mode == MFX_GATE_TOKEN && a.dgate) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        store_any(a.dgate, a.gate_dt, t * a.dgs, (i * LANES + lane) * VEC, a.H, x[i]);
-    }
-    if (post) {
-      const float my = row_reduce<LANES, false>(m, lds) * inv_n;
-      FOR_ELEMS u[i][j] = in ? iy * (u[i][j] - y[i][j] * my) : 0.f;
-    }
-    store_row<TY, LANES, NV>(a.dy, t * a.dys, lane, a.H, u);
+    if (GATED && gate.sequence(a) && a.slots) flush();
   }
-  if (a.mode == MFX_GATE_SEQUENCE && a.slots) flush();
-  write_partial<LANES, NV>(a, a.at_wp, lane, in_wg, fold, sp);
-  write_partial<LANES, NV>(a, a.at_wn, lane, in_wg, fold, sn);
-  write_partial<LANES, NV>(a, a.at_g, lane, in_wg, fold, sg);
+  write_partial(a, at, a.at_wp, in_wg, fold, sp);
+  write_partial(a, at, a.at_wn, in_wg, fold, sn);
+  if (KIND == kShared || KIND == kAny) write_partial(a, at, a.at_g, in_wg, fold, sg);
 }
 #undef FOR_ELEMS
+#undef FOR_CHUNKS
 
 // ---- the sums over partial rows ----------------------------------------------------
 
@@ -367,20 +534,23 @@ __global__ __launch_bounds__(WAVES * 64) void residual_gates(Args a) {
 bool float_dtype(int dt) { return dt == MFX_F32 || dt == MFX_BF16 || dt == MFX_F16; }
 
 constexpr int64_t kMaxH = 32768;
+constexpr int kGF = 16, kGB = 8;
 
-// Lanes that own a row and their chunks: few lanes leave memory requests in
-// flight to few rows, many make the sums over a row dearer.
+// Lanes that own a row and their chunks.  Rows of whole chunks take a chunk a lane
+// while a workgroup can hold them; others, a path of its own, make do with fewer
+// shapes.
 struct Shape {
   int lanes, nv;
+  bool easy;
 };
 Shape shape_of(int64_t H) {
-  if (H <= 64 * VEC) return {64, 1};
-  if (H <= 128 * VEC) return {64, 2};
-  if (H <= 256 * VEC) return {256, 1};
-  if (H <= 512 * VEC) return {256, 2};
-  if (H <= 1024 * VEC) return {512, 2};
-  if (H <= 2048 * VEC) return {1024, 2};
-  return {1024, 4};
+  const bool easy = H % VEC == 0;
+  const int64_t chunks = ceil_div(H, VEC);
+  for (int lanes : {64, 128, 256, 512, 1024}) {
+    if (!easy && (lanes == 128 || lanes == 512)) continue;
+    if (chunks <= lanes) return {lanes, 1, easy};
+  }
+  return {1024, chunks <= 2048 && easy ? 2 : 4, easy};
 }
 
 struct Plan {
@@ -400,11 +570,13 @@ int bind(const void* p, int64_t stride, int64_t T, int64_t H, int dt, const char
   return MFX_OK;
 }
 
-// What both directions share; groups: as many as `most` of them.
+int64_t groups_of(int64_t H, bool bwd);
+
+// What both directions share.
 int plan_common(Plan& pl, int64_t T, int64_t H, int64_t S, float alpha, float beta, float o, float post_eps, float pre_eps,
                 int res_dtype, int dtype, int param_dtype, int mode, int gate_dtype, const void* x, int64_t xs,
                 const void* y, int64_t ys, const void* gate, int64_t gs, const int32_t* off, const void* wp,
-                const void* wn, int64_t most) {
+                const void* wn, bool bwd) {
   Args& a = pl.a;
   if (T < 0 || H <= 0 || S < 0) return fail(MFX_E_INVALID, "T and num_seqs must be >= 0, H positive");
   if (!float_dtype(res_dtype) || !float_dtype(dtype)) return fail(MFX_E_UNSUPPORTED, "dtypes must be f32, bf16 or f16");
@@ -444,50 +616,69 @@ int plan_common(Plan& pl, int64_t T, int64_t H, int64_t S, float alpha, float be
   pl.res_dtype = res_dtype;
   pl.dtype = dtype;
   if (T == 0) return MFX_OK;
-  a.per = ceil_div(T, most);
-  const int rpb = pl.sh.lanes < kBlock ? kBlock / pl.sh.lanes : 1;
+  a.per = ceil_div(T, groups_of(H, bwd));
+  const int rpb = pl.sh.lanes <= 64 ? kBlock / pl.sh.lanes : 1;
   pl.groups = ceil_div(T, a.per);
   pl.wgs = ceil_div(pl.groups, rpb);
   return MFX_OK;
 }
 
-// f(TX{}, TY{}, lanes, chunks) for the plan's types and shape.
-template <int L, int N>
+// f(TX{}, TY{}, a Place, a Kind) for the plan's types and shape.
+template <int L, int N, bool E>
 struct Sized {
-  static constexpr int lanes = L, nv = N;
+  typedef Place<L, N, E> P;
 };
+template <Kind K>
+using KindOf = std::integral_constant<Kind, K>;
 template <class F, typename TX, typename TY>
-void with_shape(const Shape& s, TX x, TY y, F f) {
-  if (s.lanes == 64 && s.nv == 1) f(x, y, Sized<64, 1>{});
-  else if (s.lanes == 64) f(x, y, Sized<64, 2>{});
-  else if (s.lanes == 256 && s.nv == 1) f(x, y, Sized<256, 1>{});
-  else if (s.lanes == 256) f(x, y, Sized<256, 2>{});
-  else if (s.lanes == 512) f(x, y, Sized<512, 2>{});
-  else if (s.nv == 2) f(x, y, Sized<1024, 2>{});
-  else f(x, y, Sized<1024, 4>{});
+void with_shape(const Plan& pl, TX x, TY y, F f) {
+  const Shape& s = pl.sh;
+  if (!s.easy) {
+    const KindOf<kAny> k;
+    if (s.lanes == 64) f(x, y, Sized<64, 1, false>{}, k);
+    else if (s.lanes == 256) f(x, y, Sized<256, 1, false>{}, k);
+    else if (s.nv == 1) f(x, y, Sized<1024, 1, false>{}, k);
+    else f(x, y, Sized<1024, 4, false>{}, k);
+    return;
+  }
+  if (s.lanes == 1024 && s.nv > 1) {
+    const KindOf<kAny> k;
+    if (s.nv == 2) f(x, y, Sized<1024, 2, true>{}, k);
+    else f(x, y, Sized<1024, 4, true>{}, k);
+    return;
+  }
+  auto kind = [&](auto k) {
+    if (s.lanes == 64) f(x, y, Sized<64, 1, true>{}, k);
+    else if (s.lanes == 128) f(x, y, Sized<128, 1, true>{}, k);
+    else if (s.lanes == 256) f(x, y, Sized<256, 1, true>{}, k);
+    else if (s.lanes == 512) f(x, y, Sized<512, 1, true>{}, k);
+    else f(x, y, Sized<1024, 1, true>{}, k);
+  };
+  if (pl.a.mode == MFX_GATE_NONE) kind(KindOf<kNone>{});
+  else if (pl.a.mode == MFX_GATE_TOKEN) kind(KindOf<kToken>{});
+  else kind(KindOf<kShared>{});
 }
 template <class F>
 void with_kernel(const Plan& pl, F f) {
-  if (pl.dtype == MFX_F32) with_shape(pl.sh, float{}, float{}, f);
-  else if (pl.dtype == MFX_BF16 && pl.res_dtype == MFX_F32) with_shape(pl.sh, float{}, bf16{}, f);
-  else if (pl.dtype == MFX_BF16) with_shape(pl.sh, bf16{}, bf16{}, f);
-  else if (pl.res_dtype == MFX_F32) with_shape(pl.sh, float{}, _Float16{}, f);
-  else with_shape(pl.sh, _Float16{}, _Float16{}, f);
+  if (pl.dtype == MFX_F32) with_shape(pl, float{}, float{}, f);
+  else if (pl.dtype == MFX_BF16 && pl.res_dtype == MFX_F32) with_shape(pl, float{}, bf16{}, f);
+  else if (pl.dtype == MFX_BF16) with_shape(pl, bf16{}, bf16{}, f);
+  else if (pl.res_dtype == MFX_F32) with_shape(pl, float{}, _Float16{}, f);
+  else with_shape(pl, _Float16{}, _Float16{}, f);
 }
 
-// Groups: what fills the device's wavefront slots (forward) or half of them
-// (backward: each workgroup's partial rows cost traffic).
+// Groups: 16 wavefronts a CU (forward) or 8 (backward, where each workgroup's
+// partial rows cost traffic), and a workgroup a CU at least.
 int64_t groups_of(int64_t H, bool bwd) {
-  const Shape s = shape_of(H);
-  return (int64_t)device_cu_count() * (bwd ? 16 : 32) * 64 / s.lanes;
+  const int lanes = shape_of(H).lanes;
+  return (int64_t)device_cu_count() * std::max(1, (bwd ? kGB : kGF) * 64 / lanes);
 }
 
 int plan_fwd(const mfx_residual_norm_args* p, Plan& pl) {
   if (!p) return fail(MFX_E_INVALID, "null args");
-  const int64_t most = p->H > 0 && p->H <= kMaxH ? groups_of(p->H, false) : 1;
   if (int rc = plan_common(pl, p->T, p->H, p->num_seqs, p->alpha, p->beta, p->weight_offset, p->post_eps, p->pre_eps,
                            p->res_dtype, p->dtype, p->param_dtype, p->gate_mode, p->gate_dtype, p->x, p->x_stride, p->y,
-                           p->y_stride, p->gate, p->gate_stride, p->seq_offsets, p->post_weight, p->pre_weight, most))
+                           p->y_stride, p->gate, p->gate_stride, p->seq_offsets, p->post_weight, p->pre_weight, false))
     return rc;
   if (p->T == 0) return MFX_OK;
   if (int rc = bind(p->r, p->r_stride, p->T, p->H, p->res_dtype, "r", true)) return rc;
@@ -499,10 +690,9 @@ int plan_fwd(const mfx_residual_norm_args* p, Plan& pl) {
 
 int plan_bwd(const mfx_residual_norm_bwd_args* p, Plan& pl) {
   if (!p) return fail(MFX_E_INVALID, "null args");
-  const int64_t most = p->H > 0 && p->H <= kMaxH ? groups_of(p->H, true) : 1;
   if (int rc = plan_common(pl, p->T, p->H, p->num_seqs, p->alpha, p->beta, p->weight_offset, p->post_eps, p->pre_eps,
                            p->res_dtype, p->dtype, p->param_dtype, p->gate_mode, p->gate_dtype, p->x, p->x_stride, p->y,
-                           p->y_stride, p->gate, p->gate_stride, p->seq_offsets, p->post_weight, p->pre_weight, most))
+                           p->y_stride, p->gate, p->gate_stride, p->seq_offsets, p->post_weight, p->pre_weight, true))
     return rc;
   Args& a = pl.a;
   if (p->T > 0 && !p->dr && !p->dh) return fail(MFX_E_INVALID, "dr or dh must be non-null");  // (empty: no address)
@@ -562,10 +752,10 @@ int mfx_residual_norm(const mfx_residual_norm_args* args, void* stream) {
   Plan pl;
   if (int rc = plan_fwd(args, pl)) return rc;
   if (args->T == 0) return MFX_OK;
-  with_kernel(pl, [&](auto tx, auto ty, auto sz) {
-    typedef decltype(sz) Z;
-    hipLaunchKernelGGL((residual_fwd<decltype(tx), decltype(ty), Z::lanes, Z::nv>), dim3((unsigned)pl.wgs),
-                       dim3(Group<Z::lanes>::THREADS), 0, static_cast<hipStream_t>(stream), pl.a);
+  with_kernel(pl, [&](auto tx, auto ty, auto sz, auto k) {
+    typedef typename decltype(sz)::P P;
+    hipLaunchKernelGGL((residual_fwd<decltype(tx), decltype(ty), P, decltype(k)::value>), dim3((unsigned)pl.wgs),
+                       dim3(Group<P::LANES>::THREADS), 0, static_cast<hipStream_t>(stream), pl.a);
   });
   return launch_status("residual_fwd");
 }
@@ -589,10 +779,10 @@ int mfx_residual_norm_bwd(const mfx_residual_norm_bwd_args* args, void* stream) 
   a.part = reinterpret_cast<float*>(ws);
   a.slots = pl.slot_bytes ? reinterpret_cast<float*>(ws + pl.part_bytes) : nullptr;
   if (a.T > 0) {
-    with_kernel(pl, [&](auto tx, auto ty, auto sz) {
-      typedef decltype(sz) Z;
-      hipLaunchKernelGGL((residual_bwd<decltype(tx), decltype(ty), Z::lanes, Z::nv>), dim3((unsigned)pl.wgs),
-                         dim3(Group<Z::lanes>::THREADS), 0, s, a);
+    with_kernel(pl, [&](auto tx, auto ty, auto sz, auto k) {
+      typedef typename decltype(sz)::P P;
+      hipLaunchKernelGGL((residual_bwd<decltype(tx), decltype(ty), P, decltype(k)::value>), dim3((unsigned)pl.wgs),
+                         dim3(Group<P::LANES>::THREADS), 0, s, a);
     });
     if (int rc = launch_status("residual_bwd")) return rc;
   }
