@@ -825,12 +825,13 @@ int mfx_embedding(const mfx_embedding_args* args, void* stream);
  *   dw[v] = (accumulate ? dw[v] : 0) + scale * sum over t with ids[t] = v of dout[t]
  * dout [T, H] of `dtype`, dw [V, H] of `dw_dtype` (any of the three types
  * each).  The tokens are sorted by id: every row is written once, its tokens
- * added in fp32 in their order, or in pieces of 32 sorted positions where there are
- * more (deterministic, no atomics on memory).  accumulate: rows without tokens are
+ * added in fp32 in their order, or in pieces where there are more than 32
+ * (deterministic, no atomics on memory).  accumulate: rows without tokens are
  * left alone, the others rounded once (a head tied to the table: pass
  * mfx_linear_xent_bwd's dw).  dw must not share memory with dout or ids.
  * workspace: mfx_embedding_bwd_workspace_size() bytes, 256-byte aligned (4
- * bytes a token and a row, H / 4 bytes a token), or NULL for library scratch.
+ * bytes a token and a row, H / 4 bytes a token; none for few tokens and a small
+ * table), or NULL for library scratch.
  */
 typedef struct {
   const void* dout;

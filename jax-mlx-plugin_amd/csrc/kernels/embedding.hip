@@ -25,6 +25,11 @@
 //     multiples of kRun positions of the sorted order, a group for each, into fp32
 //     partials;
 //   embed_fold   adds those of a row in order and writes it.
+//
+// Of few tokens and a small table the launches are most of the time: there
+// embed_few does it all in one.  A workgroup owns a few rows of the table, or a part
+// of their columns, looks at every id, a thread each, puts the tokens of its rows in
+// order by counting, and its wavefronts sum and write the rows' pieces.
 #include <algorithm>
 #include <cmath>
 
@@ -42,6 +47,15 @@ constexpr int kScanWaves = 16;    // of embed_index
 constexpr int kScanRows = 480;    // table rows of one of its workgroups, at most (30 KB of counts)
 constexpr int kScanList = 256;    // tokens that one of its wavefronts can list (32 KB in all)
 constexpr int kFoldWaves = 4;
+// embed_few: its tokens, a thread each; the table rows of one of its workgroups, at
+// most; and the elements of dout and bytes of dw up to which it is taken.  Against the
+// three launches, us: 257 x 512 tokens in 1000 rows 8.6 to 15.7, 64 x 4096 in 500 rows
+// 7.9 to 11.9, 512 x 512 in 1000 rows 12.8 to 15.9; past the limits 257 x 4096 in 500
+// rows 25 to 17, 64 x 512 in 32000 rows 16.4 to 14.9 (bf16, replayed from a graph).
+constexpr int kFewTokens = 512;
+constexpr int kFewRows = 512;
+constexpr int64_t kFewElems = 1 << 18;
+constexpr int64_t kFewBytes = 4 << 20;
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -368,6 +382,100 @@ __global__ __launch_bounds__(kFoldWaves * 64) void embed_fold(SumArgs a) {
   }
 }
 
+// ---- few tokens in one launch --------------------------------------------------------
+
+template <typename TI, typename TO>
+__global__ __launch_bounds__(kFewTokens) void embed_few(SumArgs a, int tokens, int rows) {
+  constexpr int VEC = kVec<TI, TO>, WAVES = kFewTokens / 64;
+  __shared__ int found[kFewTokens];      // the rows of this workgroup's tokens, in the tokens' order
+  __shared__ int16_t order[kFewTokens];  // the tokens by row
+  __shared__ int count[kFewRows], start[kFewRows + 1], in_wave[WAVES];
+  __shared__ float sums[WAVES][64 * VEC];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t v0 = (int64_t)blockIdx.x * rows;
+  const int mine = (int)min((int64_t)rows, a.V - v0);
+  const int seg0 = (int)((int64_t)a.segs * blockIdx.y / gridDim.y);
+  const int segs = (int)((int64_t)a.segs * (blockIdx.y + 1) / gridDim.y) - seg0;
+  const int64_t id = tid < tokens ? load_id(a.ids, a.ids64, tid) : -1;
+  const bool in = id >= v0 && id < v0 + mine;
+  const uint64_t hits = __ballot(in);
+  if (lane == 0) in_wave[wave] = (int)__popcll(hits);
+  if (tid < rows) count[tid] = 0;
+  __syncthreads();
+  int at = (int)__popcll(hits & ((1ull << lane) - 1));
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w)
+    if (w < wave) at += in_wave[w];
+  const int r = in ? (int)(id - v0) : 0;
+  if (in) {
+    found[at] = r;
+    atomicAdd(count + r, 1);
+  }
+  __syncthreads();
+  if (tid <= mine) {
+    int s = 0;
+    for (int k = 0; k < tid; ++k) s += count[k];
+    start[tid] = s;
+  }
+  __syncthreads();
+  if (in) {
+    int place = start[r];
+    for (int k = 0; k < at; ++k) place += found[k] == r;
+    order[place] = (int16_t)tid;
+  }
+  __syncthreads();
+
+  const TI* const dout = static_cast<const TI*>(a.dout);
+  // Sum of the tokens [s, e) of the order.
+  auto sum = [&](int s, int e, int col, float (&acc)[VEC]) __attribute__((always_inline)) {
+    constexpr int U = 8;  // rows in flight
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    for (int p = s; p < e; p += U) {
+      float v[U][VEC];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool one = p + u < e;
+        const int t = one ? __builtin_amdgcn_readfirstlane(order[p + u]) : 0;
+        load_run<TI, VEC>(dout + (int64_t)t * a.ds, col, one ? a.H : 0, 0.f, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] += v[u][j];
+    }
+  };
+  float acc[VEC];
+  // A wavefront to each piece of a row of few tokens ...
+  for (int task = wave; task < mine * segs; task += WAVES) {
+    const int row = task / segs, col = (seg0 + task - row * segs) * (64 * VEC) + lane * VEC;
+    const int s = start[row], e = start[row + 1];
+    if (e - s > kRun || (a.add && s == e)) continue;
+    sum(s, e, col, acc);
+    write_row<TO, VEC>(a, v0 + row, col, acc);
+  }
+  // ... and all of them a share of the tokens of a row of more.
+  for (int row = 0; row < mine; ++row) {
+    const int s = start[row], n = start[row + 1] - s;
+    if (n <= kRun) continue;
+    for (int seg = 0; seg < segs; ++seg) {
+      const int col = (seg0 + seg) * (64 * VEC) + lane * VEC;
+      sum(s + n * wave / WAVES, s + n * (wave + 1) / WAVES, col, acc);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) sums[wave][lane * VEC + j] = acc[j];
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) acc[j] += sums[w][lane * VEC + j];
+        write_row<TO, VEC>(a, v0 + row, col, acc);
+      }
+      __syncthreads();
+    }
+  }
+}
+
 // ---- host ------------------------------------------------------------------------
 
 bool float_dtype(int dt) { return dt == MFX_F32 || dt == MFX_BF16 || dt == MFX_F16; }
@@ -435,6 +543,7 @@ int plan_fwd(const mfx_embedding_args* a, FwdPlan& pl) {
 }
 
 struct BwdPlan {
+  bool few;  // embed_few: `scans` by `grid` workgroups of `rows` rows and a part of the columns, no workspace
   int lanes, segs;
   int64_t blocks, grid, fold, part_ld;
   int rows;
@@ -450,6 +559,17 @@ int plan_bwd(const mfx_embedding_bwd_args* a, BwdPlan& pl) {
     if (int rc = check_rows(a->dout, a->dout_stride, a->T, a->H, a->dtype, "dout", false)) return rc;
   }
   const int vec = vec_of(a->dtype, a->dw_dtype);
+  pl.few = a->T <= kFewTokens && a->T * a->H <= kFewElems &&
+           a->V * a->H * dtype_size(a->dw_dtype) <= kFewBytes;
+  if (pl.few) {
+    // Two workgroups a CU at most.
+    pl.segs = (int)ceil_div(a->H, 64 * vec);
+    pl.rows = (int)std::min<int64_t>(kFewRows, ceil_div(a->V, 2 * device_cu_count()));
+    pl.scans = ceil_div(a->V, pl.rows);
+    pl.grid = std::min<int64_t>(pl.segs, std::max<int64_t>(1, 2 * device_cu_count() / pl.scans));
+    pl.order_bytes = pl.start_bytes = pl.part_bytes = pl.total = 0;
+    return MFX_OK;
+  }
   pl.lanes = a->H <= 16 * vec ? 16 : 64;
   pl.segs = (int)ceil_div(a->H, pl.lanes * vec);
   pl.blocks = a->T > kRun ? ceil_div(a->T, kRun) : 0;
@@ -479,7 +599,12 @@ void launch_lookup(const LookupArgs& p, const FwdPlan& pl, hipStream_t s) {
 }
 
 template <typename TI, typename TO>
-void launch_rows(const SumArgs& p, const BwdPlan& pl, hipStream_t s) {
+void launch_rows(const SumArgs& p, const BwdPlan& pl, int64_t T, hipStream_t s) {
+  if (pl.few) {
+    hipLaunchKernelGGL((embed_few<TI, TO>), dim3((unsigned)pl.scans, (unsigned)pl.grid),
+                       dim3(kFewTokens), 0, s, p, (int)T, pl.rows);
+    return;
+  }
   const dim3 grid((unsigned)pl.grid), block(kBlock);
   if (pl.lanes == 16) hipLaunchKernelGGL((embed_rows<TI, TO, 16>), grid, block, 0, s, p);
   else hipLaunchKernelGGL((embed_rows<TI, TO, 64>), grid, block, 0, s, p);
@@ -538,15 +663,18 @@ int mfx_embedding_bwd(const mfx_embedding_bwd_args* args, void* stream) {
   int32_t* const order = reinterpret_cast<int32_t*>(ws);
   int32_t* const start = reinterpret_cast<int32_t*>(ws + pl.order_bytes);
   const int ids64 = a.ids_dtype == MFX_I64;
-  const IndexArgs x{a.ids, order, start, a.T, a.V, ids64, pl.rows};
-  hipLaunchKernelGGL(embed_index, dim3((unsigned)pl.scans), dim3(kScanWaves * 64), (size_t)kScanWaves * pl.rows * 4, s, x);
-  if (int rc = launch_status("embed_index")) return rc;
+  if (!pl.few) {
+    const IndexArgs x{a.ids, order, start, a.T, a.V, ids64, pl.rows};
+    hipLaunchKernelGGL(embed_index, dim3((unsigned)pl.scans), dim3(kScanWaves * 64), (size_t)kScanWaves * pl.rows * 4, s,
+                       x);
+    if (int rc = launch_status("embed_index")) return rc;
+  }
   const SumArgs p{a.dout, a.ids, a.dw, order, start, reinterpret_cast<float*>(ws + pl.order_bytes + pl.start_bytes),
                   a.V, a.dout_stride, a.dw_stride, pl.part_ld, pl.blocks, (int)a.H, pl.segs, ids64,
                   a.accumulate != 0, a.scale};
-  with_types(a.dtype, a.dw_dtype, [&](auto ti, auto to) { launch_rows<decltype(ti), decltype(to)>(p, pl, s); });
-  if (int rc = launch_status("embed_rows")) return rc;
-  if (!pl.blocks) return MFX_OK;
+  with_types(a.dtype, a.dw_dtype, [&](auto ti, auto to) { launch_rows<decltype(ti), decltype(to)>(p, pl, a.T, s); });
+  if (int rc = launch_status(pl.few ? "embed_few" : "embed_rows")) return rc;
+  if (pl.few || !pl.blocks) return MFX_OK;
   const dim3 grid((unsigned)pl.fold), block(kFoldWaves * 64);
   if (a.dw_dtype == MFX_F32) hipLaunchKernelGGL((embed_fold<float>), grid, block, 0, s, p);
   else if (a.dw_dtype == MFX_BF16) hipLaunchKernelGGL((embed_fold<bf16>), grid, block, 0, s, p);

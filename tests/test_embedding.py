@@ -58,6 +58,11 @@ CASES = [
     (129, 7, 3, "f16", "f32", "i64", 1.0),
     (1, 2049, 1, "f32", "f32", "i64", 2.0),
     (65, 1, 70, "bf16", "bf16", "i64", 1.0),
+    (512, 24, 40000, "bf16", "bf16", "i32", 1.0),  # the most tokens of the gradient's one launch
+    (513, 33, 50, "bf16", "f32", "i32", -3.0),
+    (600, 7, 3, "f16", "f32", "i64", 1.0),
+    (64, 1024, 2000, "bf16", "f32", "i64", 1.0),   # a table too large for it
+    (500, 8200, 2, "f32", "f32", "i64", 1.0),      # and few rows, their columns split
     (2500, 640, 1100, "f16", "f16", "i64", 1.0),   # more rows than a workgroup of the index takes at V / CUs
 ]
 IDS = [f"T{c[0]}-H{c[1]}-V{c[2]}-{c[3]}-{c[4]}" for c in CASES]
@@ -251,8 +256,8 @@ def test_refusals(nat):
             assert call(**bad) == UNSUPPORTED, bad
     assert fwd(T=2 ** 27, H=4096, w_stride=4096, out_stride=4096) == UNSUPPORTED and b"too large" in lib.mfx_last_error()
     assert bwd(V=2 ** 27, H=4096, dout_stride=4096, dw_stride=4096) == UNSUPPORTED and b"too large" in lib.mfx_last_error()
-    assert bwd(workspace=0x400000, workspace_bytes=16) == WORKSPACE
-    assert bwd(workspace=0x400010, workspace_bytes=1 << 20) == INVALID
+    assert bwd(T=3000, workspace=0x400000, workspace_bytes=16) == WORKSPACE
+    assert bwd(T=3000, workspace=0x400010, workspace_bytes=1 << 20) == INVALID
     assert fwd(T=0, w=0, ids=0, out=0) == 0
 
 
