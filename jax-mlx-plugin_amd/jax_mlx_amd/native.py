@@ -625,7 +625,7 @@ def _mask_fields(mask):
 
 def _f32(x):
     """x as a C float holds it (past the range: an infinity, which packing refuses to make)."""
-    return ctypes.c_float(x).value
+    return x if -1e38 < x < 1e38 else ctypes.c_float(x).value
 
 
 def sdpa_args(q, k, v, out, *, scale=None, causal=False, mask=None, layout="bhtd",
@@ -1233,13 +1233,20 @@ def _rows_of(name, t, like, dtype=None):
 
 def _residual_fields(x, y, gate, seq_offsets, post_weight, pre_weight, post_eps, pre_eps, alpha, beta, weight_offset):
     """Checked (pointers, dims, strides of x, y and gate, scalars) of both directions."""
-    if x.dim() < 2 or x.shape[-1] == 0:
+    shape = x.shape
+    H = shape[-1] if len(shape) >= 2 else 0
+    if H == 0:
         raise ValueError("x and y are [..., H]")
-    if (post_eps is not None and not post_eps >= 0.0) or (pre_eps is not None and not pre_eps >= 0.0):
+    if post_eps is None:
+        post_eps = -1.0
+    elif not post_eps >= 0.0:
         raise ValueError("eps must be >= 0 (None: no norm)")
-    xs, ys = _rows_of("x", x, x), _rows_of("y", y, x)
-    H = x.shape[-1]
-    T = x.numel() // H
+    if pre_eps is None:
+        pre_eps = -1.0
+    elif not pre_eps >= 0.0:
+        raise ValueError("eps must be >= 0 (None: no norm)")
+    if y.shape != shape:
+        raise ValueError(f"y must be {tuple(shape)}")
     pd = None
     for w in (post_weight, pre_weight):
         if w is not None:
@@ -1247,26 +1254,29 @@ def _residual_fields(x, y, gate, seq_offsets, post_weight, pre_weight, post_eps,
                 raise ValueError("weights must be contiguous [H] vectors of one dtype")
             pd = w.dtype
     mode, S, gs, off = MFX_GATE_NONE, 0, H, 0
-    if seq_offsets is not None:
-        if gate is None:
-            raise ValueError("seq_offsets belong to a gate")
-        if seq_offsets.dtype != _torch().int32 or seq_offsets.dim() != 1 or not seq_offsets.is_contiguous():
-            raise TypeError("seq_offsets must be a contiguous int32 vector")
-        S = seq_offsets.numel() - 1
-        if S < 0 or gate.shape != (S, H) or gate.stride(1) != 1:
-            raise ValueError("a gate by sequence is [sequences, H], seq_offsets one entry more")
-        mode, gs, off = MFX_GATE_SEQUENCE, gate.stride(0) if S > 1 else H, seq_offsets.data_ptr()
-    elif gate is not None and gate.dim() == 1:
-        if gate.shape != (H,) or not gate.is_contiguous():
-            raise ValueError("a gate for all rows is a contiguous [H] vector")
-        mode = MFX_GATE_FEATURE
-    elif gate is not None:
-        mode, gs = MFX_GATE_TOKEN, _rows_of("a gate by token", gate, x)
     code = dtype_code(y.dtype)
-    return ((x.data_ptr(), y.data_ptr(), _ptr(gate), off, _ptr(post_weight), _ptr(pre_weight)), (T, H, S),
-            (xs, ys, gs), (_f32(alpha), _f32(beta), _f32(weight_offset), -1.0 if post_eps is None else _f32(post_eps),
-                           -1.0 if pre_eps is None else _f32(pre_eps), dtype_code(x.dtype), code,
-                           code if pd is None else dtype_code(pd), mode, code if gate is None else dtype_code(gate.dtype)))
+    gcode = code
+    if gate is not None:
+        gcode = dtype_code(gate.dtype)
+        if seq_offsets is not None:
+            if seq_offsets.dtype != _torch().int32 or seq_offsets.dim() != 1 or not seq_offsets.is_contiguous():
+                raise TypeError("seq_offsets must be a contiguous int32 vector")
+            S = seq_offsets.numel() - 1
+            if S < 0 or gate.shape != (S, H) or gate.stride(1) != 1:
+                raise ValueError("a gate by sequence is [sequences, H], seq_offsets one entry more")
+            mode, gs, off = MFX_GATE_SEQUENCE, gate.stride(0) if S > 1 else H, seq_offsets.data_ptr()
+        elif gate.dim() == 1:
+            if gate.shape != (H,) or not gate.is_contiguous():
+                raise ValueError("a gate for all rows is a contiguous [H] vector")
+            mode = MFX_GATE_FEATURE
+        else:
+            mode, gs = MFX_GATE_TOKEN, _rows_of("a gate by token", gate, x)
+    elif seq_offsets is not None:
+        raise ValueError("seq_offsets belong to a gate")
+    return ((x.data_ptr(), y.data_ptr(), _ptr(gate), off, _ptr(post_weight), _ptr(pre_weight)),
+            (x.numel() // H, H, S), (_row_stride(x, H), _row_stride(y, H), gs),
+            (_f32(alpha), _f32(beta), _f32(weight_offset), _f32(post_eps), _f32(pre_eps), dtype_code(x.dtype), code,
+             code if pd is None else dtype_code(pd), mode, gcode))
 
 
 def residual_norm(x, y, *, gate=None, seq_offsets=None, post_weight=None, pre_weight=None, post_eps=None,
