@@ -14,6 +14,16 @@
 // of 2 s^2 l, 2 s^3 and 2 s^2 l operations (s, l the sides); gram and square form
 // only the tiles on and below the diagonal and store each twice.
 //
+// Where X is long (3 small products take less than gram and apply) two steps are
+// taken at once: A of the second is Q A Q, since Q is a polynomial in A, and X is
+// multiplied by Q' Q, so gram and apply run every other step:
+//
+//   T = Q A,  A' = T Q,  Q' = a I + b A' + c A' A',  P = Q' Q,  X = P X
+//
+// all of them symmetric.  Their entries are off by as much as before (1.7e-6 to
+// 2.1e-6 in fp32, 4e-6 with a few large directions), but in one f16 term by up to
+// three times, so it is for two terms.
+//
 // Precision.  The products' operands are f16, in one term or in two (a leading
 // one and what it leaves out: 22 bits, three products for one, pair_gemm16.h), all
 // sums fp32.  X, A and Q are stored times powers of two that the host derives from
@@ -438,6 +448,7 @@ struct Way {
   Form form;
   int64_t tiles, whole;  // of all matrices; those that are not split
   int splits, per;
+  float us;
 };
 
 // Microseconds of a k-tile with `slots` workgroups on each CU (`alone` of that
@@ -482,7 +493,7 @@ Way choose(int64_t B, int64_t M, int64_t N, int64_t K, Mode mode, bool two) {
     const float whole = rounds_us(c, tiles, kt, mode == kSquare);
     if (whole < least) {
       least = whole;
-      best = Way{(Form)f, tiles, tiles, 0, 0};
+      best = Way{(Form)f, tiles, tiles, 0, 0, whole};
     }
     for (int64_t n = 2; rest && n <= 64 && n * 8 <= kt; ++n) {
       const int64_t per = ceil_div(kt, n), wgs = rest * n;
@@ -491,7 +502,7 @@ Way choose(int64_t B, int64_t M, int64_t N, int64_t K, Mode mode, bool two) {
                       (float)wgs * (float)(side * side) * 8e-6f / c.rate;
       if (t < least) {
         least = t;
-        best = Way{(Form)f, tiles, tiles - rest, (int)n, (int)per};
+        best = Way{(Form)f, tiles, tiles - rest, (int)n, (int)per, t};
       }
     }
   }
@@ -506,9 +517,11 @@ struct Plan {
   int64_t B, m, n, s, l, ld, lds;  // the matrix, its smaller and larger side, rows of X and of A
   bool wide;
   int two, steps, parts;
-  Way gram, square, apply;
+  bool paired;
+  Way gram, square, apply, small;  // small: of two matrices of the smaller side
   size_t norm_bytes, x_bytes, a_bytes, part, total;
-  float ex[kMaxSteps + 1], ea[kMaxSteps], eq[kMaxSteps];  // the powers of two that X, A, Q are stored at
+  // The powers of two that X, A, Q are stored at, and of two steps taken together Q A and Q' Q.
+  float ex[kMaxSteps + 1], ea[kMaxSteps], eq[kMaxSteps], et[kMaxSteps], ep[kMaxSteps];
 };
 
 // The largest power of two that keeps values up to `most` within f16.
@@ -517,7 +530,7 @@ float fit(double most) { return (float)std::exp2(std::floor(std::log2(60000.0 / 
 // Bounds of the iterates' norms: X starts at 1 or less; over the spectrum [0, u]
 // of X the polynomials' largest values are at its end or where a derivative is 0.
 int plan_scales(Plan& pl, const float* coeffs, int num) {
-  double u = 1.0;
+  double u = 1.0, before = 1.0;
   for (int i = 0; i < pl.steps; ++i) {
     const float* k = coeffs + 3 * (num == 1 ? 0 : i);
     const double a = k[0], b = k[1], c = k[2];
@@ -548,7 +561,11 @@ int plan_scales(Plan& pl, const float* coeffs, int num) {
       return fail(MFX_E_UNSUPPORTED, "the coefficients let the iteration grow too large");
     pl.ex[i] = fit(u);
     pl.ea[i] = fit(top);
-    pl.eq[i] = fit(std::max(qm, 1.0 / 256.0));
+    qm = std::max(qm, 1.0 / 256.0);
+    pl.eq[i] = fit(qm);
+    pl.et[i] = fit(1.02 * qm * top);
+    if (i) pl.ep[i - 1] = fit(1.02 * before * qm);
+    before = qm;
     u = std::max(next, 1.0 / 16.0);
   }
   pl.ex[pl.steps] = 1.f;  // (the result is not stored in terms)
@@ -581,6 +598,10 @@ int plan_common(Plan& pl, int64_t B, int64_t m, int64_t n, int64_t steps, const 
   pl.apply = choose(B, m, n, pl.s, kApply, pl.two);
   if (!pl.gram.tiles || !pl.square.tiles || !pl.apply.tiles)
     return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
+  if (pl.two) {
+    pl.small = choose(B, pl.s, pl.s, pl.s, kGram, true);
+    pl.paired = pl.steps > 1 && pl.small.tiles && 3.f * pl.small.us < pl.gram.us + pl.apply.us;
+  }
   if (!launch_fits(B * std::min<int64_t>(2048, ceil_div(m * (pl.ld / 8), 256)), 256))
     return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
   // Parts of a matrix's sum of squares: of 512 chunks or more, at most four a thread of ns_split.
@@ -588,8 +609,9 @@ int plan_common(Plan& pl, int64_t B, int64_t m, int64_t n, int64_t steps, const 
   pl.norm_bytes = align256((size_t)B * pl.parts * 8);
   pl.x_bytes = align256((size_t)B * m * pl.ld * 2 * (1 + pl.two));
   pl.a_bytes = align256((size_t)B * pl.s * pl.lds * 2 * (1 + pl.two));
-  pl.part = align256(std::max(part_bytes(pl.gram), std::max(part_bytes(pl.square), part_bytes(pl.apply))));
-  pl.total = pl.norm_bytes + 2 * pl.x_bytes + 2 * pl.a_bytes + pl.part;
+  pl.part = align256(std::max(std::max(part_bytes(pl.gram), part_bytes(pl.square)),
+                              std::max(part_bytes(pl.apply), pl.paired ? part_bytes(pl.small) : 0)));
+  pl.total = pl.norm_bytes + 2 * pl.x_bytes + (2 + pl.paired) * pl.a_bytes + pl.part;
   return MFX_OK;
 }
 
@@ -648,7 +670,8 @@ int run(const Plan& pl, InArgs in, const float* coeffs, int num_coeffs, const Pr
   x[1] = reinterpret_cast<uint16_t*>(ws + pl.norm_bytes + pl.x_bytes);
   uint16_t* const a = reinterpret_cast<uint16_t*>(ws + pl.norm_bytes + 2 * pl.x_bytes);
   uint16_t* const q = reinterpret_cast<uint16_t*>(ws + pl.norm_bytes + 2 * pl.x_bytes + pl.a_bytes);
-  float* const part = reinterpret_cast<float*>(ws + pl.norm_bytes + 2 * pl.x_bytes + 2 * pl.a_bytes);
+  uint16_t* const t = reinterpret_cast<uint16_t*>(ws + pl.norm_bytes + 2 * pl.x_bytes + 2 * pl.a_bytes);
+  float* const part = reinterpret_cast<float*>(ws + pl.total - pl.part);
   const int64_t xs = pl.m * pl.ld, as = pl.s * pl.lds;
   in.norm = norm;
   in.x = x[0];
@@ -660,33 +683,64 @@ int run(const Plan& pl, InArgs in, const float* coeffs, int num_coeffs, const Pr
   const int64_t chunks = ceil_div(pl.m * (pl.ld / 8), 256);
   hipLaunchKernelGGL(ns_split, dim3((unsigned)std::min<int64_t>(chunks, 2048), (unsigned)pl.B), dim3(256), 0, s, in);
   if (int rc = launch_status("ns_split")) return rc;
-  for (int i = 0; i < pl.steps; ++i) {
+  auto of = [&](uint16_t* p) { return Operand{p, pl.lds, pl.B * as}; };
+  // to = factor left right, of matrices of the smaller side
+  auto small = [&](uint16_t* to, uint16_t* left, uint16_t* right, float factor) {
+    ProdArgs p{};
+    p.two = pl.two;
+    p.g.a = of(left), p.g.b = of(right);
+    p.as = p.bs = as;
+    p.c = to, p.ldc = pl.lds, p.cs = as, p.lo = pl.B * as;
+    p.c1 = factor;
+    return product<kGram>(p, pl.small, pl.B, pl.s, pl.s, pl.s, true, true, part, s);
+  };
+  // to = step i's Q of A
+  auto square = [&](uint16_t* to, uint16_t* from, int i) {
     const float* k = coeffs + 3 * (num_coeffs == 1 ? 0 : i);
-    const float ex = pl.ex[i], ea = pl.ea[i], eq = pl.eq[i];
-    const Operand X{x[i & 1], pl.ld, pl.B * xs}, A{a, pl.lds, pl.B * as}, Q{q, pl.lds, pl.B * as};
+    const float ea = pl.ea[i], eq = pl.eq[i];
+    ProdArgs p{};
+    p.two = pl.two;
+    p.g.a = p.g.b = of(from);
+    p.as = p.bs = as;
+    p.c = to, p.ldc = pl.lds, p.cs = as, p.lo = pl.B * as;
+    p.c1 = k[2] * eq / (ea * ea);
+    p.c2 = k[1] * eq / ea;
+    p.c3 = k[0] * eq;
+    return product<kSquare>(p, pl.square, pl.B, pl.s, pl.s, pl.s, true, true, part, s);
+  };
+  for (int i = 0, turn = 0; i < pl.steps; turn ^= 1) {
+    const Operand X{x[turn], pl.ld, pl.B * xs};
     ProdArgs p{};
     p.two = pl.two;
     p.g.a = p.g.b = X;
     p.as = p.bs = xs;
     p.c = a, p.ldc = pl.lds, p.cs = as, p.lo = pl.B * as;
-    p.c1 = ea / (ex * ex);
+    p.c1 = pl.ea[i] / (pl.ex[i] * pl.ex[i]);
     if (int rc = product<kGram>(p, pl.gram, pl.B, pl.s, pl.s, pl.l, pl.wide, pl.wide, part, s)) return rc;
-    p.g.a = p.g.b = A;
-    p.as = p.bs = as;
-    p.c = q;
-    p.c1 = k[2] * eq / (ea * ea);
-    p.c2 = k[1] * eq / ea;
-    p.c3 = k[0] * eq;
-    if (int rc = product<kSquare>(p, pl.square, pl.B, pl.s, pl.s, pl.s, true, true, part, s)) return rc;
-    if (i + 1 == pl.steps) {
+    if (int rc = square(q, a, i)) return rc;
+    const float ex = pl.ex[i];
+    float by = pl.eq[i];  // what the factor of X is stored at, and where it is
+    uint16_t* f = q;
+    if (pl.paired && i + 1 < pl.steps) {
+      const float eq = pl.eq[i], et = pl.et[i];
+      if (int rc = small(t, q, a, et / (eq * pl.ea[i]))) return rc;
+      if (int rc = small(a, t, q, pl.ea[i + 1] / (et * eq))) return rc;
+      if (int rc = square(t, a, i + 1)) return rc;
+      by = pl.ep[i];
+      f = a;
+      if (int rc = small(a, t, q, by / (pl.eq[i + 1] * eq))) return rc;
+      ++i;
+    }
+    if (++i == pl.steps) {
       p = last;
       p.two = pl.two;
-      p.c1 = scale / (eq * ex);
+      p.c1 = scale / (by * ex);
     } else {
-      p.c = x[(i + 1) & 1], p.ldc = pl.ld, p.cs = xs, p.lo = pl.B * xs;
-      p.c1 = pl.ex[i + 1] / (eq * ex);
+      p.c = x[turn ^ 1], p.ldc = pl.ld, p.cs = xs, p.lo = pl.B * xs;
+      p.c1 = pl.ex[i] / (by * ex);
     }
     // Wide: Q's rows by X's columns; tall: X's rows by Q's (Q is symmetric).
+    const Operand Q = of(f);
     p.g.a = pl.wide ? Q : X, p.as = pl.wide ? as : xs;
     p.g.b = pl.wide ? X : Q, p.bs = pl.wide ? xs : as;
     if (int rc = product<kApply>(p, pl.apply, pl.B, pl.m, pl.n, pl.s, true, !pl.wide, part, s)) return rc;

@@ -105,6 +105,18 @@ def test_newton_schulz(cuda, nat, case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("steps", [1, 2, 3, 6])
+@pytest.mark.parametrize("shape", [(1, 264, 8200), (1, 8193, 250), (3, 72, 4000)], ids=str)
+def test_steps_of_long_matrices(cuda, nat, shape, steps):
+    """Two steps at once, and the odd one behind them, each step with its own coefficients."""
+    torch = cuda
+    g = gradient(torch, *shape, "f32", seed=3)
+    coeffs = [QUINTIC, (3.25, -4.5, 1.875), QUINTIC, (3.0, -4.0, 1.75), (1.875, -1.25, 0.375), (1.5, -0.5, 0.0)][:steps]
+    out = nat.newton_schulz(g, steps=steps, coeffs=coeffs)
+    near(out, iterate(torch, g, steps, coeffs), TOL[2], "f32")
+
+
+@pytest.mark.gpu
 def test_takes_singular_values_to_one(cuda, nat):
     """The cubic (1.5, -0.5, 0) repeated converges to U V^T of the singular value decomposition; its
     coefficients are exact and a small value s grows by 1.5 a step, at least 0.01 of |G| here: 24 steps."""
