@@ -153,8 +153,11 @@ enum Mode { kGram, kSquare, kApply };
 
 // The forms of a product's tiles: square ones, since a symmetric product's
 // tiles are stored transposed too.
-enum Form { kWide, kNarrow, kSlim };
-constexpr int kSide[3] = {256, 128, 64};
+// kMid is for one term and operands along k: of a symmetric product of 4096 a side
+// 256 x 256 are 136 tiles, which leave half the CUs without one, 192 x 192 are 253, 81
+// and 87 us (gram, square) for 89 and 100, or 94 and 97 in 128 x 128.
+enum Form { kWide, kNarrow, kSlim, kMid };
+constexpr int kForms = 4, kSide[kForms] = {256, 128, 64, 192};
 
 // k of a tile: 32 of one term or, of small tiles, whose few products would not
 // cover taking up the next one, of two; else 16 of two.
@@ -164,6 +167,7 @@ template <int SIDE, bool A_KC, bool B_KC, bool P>
 struct Cfg : Config<SIDE, SIDE, SIDE == 64 ? 1 : 2, 2, A_KC, B_KC, 1> {
   static constexpr bool PAIR = P;  // operands in two terms
   static constexpr bool ROT = false;
+  static constexpr int WAVES = SIDE == 256 || SIDE == 192 ? 1 : SIDE == 128 ? 2 : 3;  // per SIMD
   static constexpr int STAGES = 4;
   static constexpr int BK = depth(SIDE == 64 ? kSlim : kWide, P);
   static constexpr int SMEM = STAGES * 4 * SIDE * BK * (1 + P);
@@ -225,14 +229,14 @@ __device__ __forceinline__ void tile_of(const ProdArgs& p, int t, int& tm, int& 
 
 // What becomes of a block of sums, rows m0 .. + 31 by columns n0 .. + FN * 32 of
 // matrix bz, by one wavefront.  The sums go to LDS (st: FN * 4 KB of the
-// wavefront's own), chunk c (four) of row r at slot c ^ (r % chunks), and from there in
+// wavefront's own), chunk c (four) of row r at slot c ^ (r % chunks) (of 24 chunks: % 8), and from there in
 // runs of eight along a row; of a symmetric product's tile off the diagonal
 // (`turned`) the values go back there and out once more in runs of eight down a
 // column, which are a row's of the other half.
 template <int FN, Mode MODE>
 __device__ __forceinline__ void finish_rows(const ProdArgs& p, int64_t bz, int m0, int n0, bool turned, float* st,
                                             const f32x16 (&acc)[FN]) {
-  constexpr int W = FN * 32, QUADS = W / 4;
+  constexpr int W = FN * 32, QUADS = W / 4, TURN = QUADS & (QUADS - 1) ? 7 : QUADS - 1;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int M = p.g.M, N = p.g.N;
   {
@@ -243,11 +247,11 @@ __device__ __forceinline__ void finish_rows(const ProdArgs& p, int64_t bz, int m
     for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        row[(j * 8 + g * 2 + half) ^ (l & (QUADS - 1))] =
+        row[(j * 8 + g * 2 + half) ^ (l & TURN)] =
             f32x4{acc[j][g * 4], acc[j][g * 4 + 1], acc[j][g * 4 + 2], acc[j][g * 4 + 3]};
   }
   fence();
-  constexpr int RUNS = FN * 4, RPS = 64 / RUNS;  // of a row; rows at a time
+  constexpr int RUNS = FN * 4, STEPS = RUNS / 2;  // of a row; steps of 64 runs
   uint16_t* const c = p.c + bz * p.cs;
   // One or two f16 terms of a run.
   auto put = [&](int64_t at, const float (&v)[8]) __attribute__((always_inline)) {
@@ -261,13 +265,13 @@ __device__ __forceinline__ void finish_rows(const ProdArgs& p, int64_t bz, int m
   };
   // (Unrolled for a square product's reads of A to overlap; the last product's
   // end, of any type and alignment, stays a loop.)
-  constexpr int UNROLL = MODE == kSquare ? 32 / RPS : 2;
+  constexpr int UNROLL = MODE == kSquare ? STEPS : 2;
 #pragma unroll UNROLL
-  for (int k = 0; k < 32; k += RPS) {
-    const int r = k + lane / RUNS, run = lane % RUNS, m = m0 + r, n = n0 + run * 8;
+  for (int k = 0; k < STEPS; ++k) {
+    const int at = k * 64 + lane, r = at / RUNS, run = at % RUNS, m = m0 + r, n = n0 + run * 8;
     if (m >= M || n >= N) continue;
     f32x4* const row = reinterpret_cast<f32x4*>(st + r * W);
-    f32x4 &x = row[(run * 2) ^ (r & (QUADS - 1))], &y = row[(run * 2 + 1) ^ (r & (QUADS - 1))];
+    f32x4 &x = row[(run * 2) ^ (r & TURN)], &y = row[(run * 2 + 1) ^ (r & TURN)];
     float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] *= p.c1;
@@ -312,7 +316,7 @@ __device__ __forceinline__ void finish_rows(const ProdArgs& p, int64_t bz, int m
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int row = run * 8 + e;
-      v[e] = st[row * W + ((r >> 2) ^ (row & (QUADS - 1))) * 4 + (r & 3)];
+      v[e] = st[row * W + ((r >> 2) ^ (row & TURN)) * 4 + (r & 3)];
     }
     // (Rows past the matrix hold sums of zeros: nothing went over them.)
 #pragma unroll
@@ -460,9 +464,10 @@ struct Cost {
   int slots;
   float kt, alone, each, square, join, rate;
 };
-constexpr Cost kCost[2][3] = {{{1, 0.818f, 0.73f, 12.4f, 6.5f, 1.7f, 9.9f},
+constexpr Cost kCost[2][kForms] = {{{1, 0.818f, 0.73f, 12.4f, 6.5f, 1.7f, 9.9f},
                                {2, 0.597f, 0.01f, 3.9f, 1.9f, 6.9f, 12.9f},
-                               {4, 0.536f, 0.09f, 3.6f, 1.3f, 7.3f, 60.f}},
+                               {4, 0.536f, 0.09f, 3.6f, 1.3f, 7.3f, 60.f},
+                               {1, 0.639f, 0.71f, 5.9f, 5.9f, 8.3f, 26.f}},
                               {{1, 1.240f, 0.69f, 10.0f, 13.2f, 2.8f, 8.3f},
                                {2, 0.947f, 0.00f, 1.8f, 4.5f, 8.0f, 8.7f},
                                {2, 0.578f, 0.18f, 3.4f, 1.9f, 7.6f, 60.f}}};
@@ -481,11 +486,13 @@ float rounds_us(const Cost& c, int64_t wgs, int64_t n, bool square) {
 
 // The way that takes least by these: every form, its tiles whole or those of the
 // last, partly filled round split along k into ranges of at least 8 k-tiles.
-Way choose(int64_t B, int64_t M, int64_t N, int64_t K, Mode mode, bool two) {
+// along: both operands are rows along k.
+Way choose(int64_t B, int64_t M, int64_t N, int64_t K, Mode mode, bool two, bool along) {
   const int64_t cus = device_cu_count();
   Way best{};
   float least = INFINITY;
-  for (int f = kWide; f <= kSlim; ++f) {
+  for (int f = kWide; f < kForms; ++f) {
+    if (f == kMid && (two || !along)) continue;
     const Cost& c = kCost[two][f];
     const int64_t side = kSide[f], tm = ceil_div(M, side), tn = ceil_div(N, side), kt = ceil_div(K, depth((Form)f, two));
     const int64_t tiles = B * (mode != kApply ? tm * (tm + 1) / 2 : tm * tn), rest = tiles % (c.slots * cus);
@@ -593,13 +600,13 @@ int plan_common(Plan& pl, int64_t B, int64_t m, int64_t n, int64_t steps, const 
   pl.two = terms == 0 ? !(bf16_result && pl.s >= 256) : terms == 2;
   if (int rc = plan_scales(pl, coeffs, num_coeffs)) return rc;
   if (B == 0) return MFX_OK;
-  pl.gram = choose(B, pl.s, pl.s, pl.l, kGram, pl.two);
-  pl.square = choose(B, pl.s, pl.s, pl.s, kSquare, pl.two);
-  pl.apply = choose(B, m, n, pl.s, kApply, pl.two);
+  pl.gram = choose(B, pl.s, pl.s, pl.l, kGram, pl.two, pl.wide);
+  pl.square = choose(B, pl.s, pl.s, pl.s, kSquare, pl.two, true);
+  pl.apply = choose(B, m, n, pl.s, kApply, pl.two, false);
   if (!pl.gram.tiles || !pl.square.tiles || !pl.apply.tiles)
     return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
   if (pl.two) {
-    pl.small = choose(B, pl.s, pl.s, pl.s, kGram, true);
+    pl.small = choose(B, pl.s, pl.s, pl.s, kGram, true, true);
     pl.paired = pl.steps > 1 && pl.small.tiles && 3.f * pl.small.us < pl.gram.us + pl.apply.us;
   }
   if (!launch_fits(B * std::min<int64_t>(2048, ceil_div(m * (pl.ld / 8), 256)), 256))
@@ -624,7 +631,9 @@ int launch(const ProdArgs& p, hipStream_t s) {
 template <int SIDE, Mode MODE>
 int launch_side(const ProdArgs& p, bool a_kc, bool b_kc, hipStream_t s) {
   int rc;
-  if (!a_kc) {
+  if constexpr (SIDE == kSide[kMid]) {
+    rc = launch<Cfg<SIDE, true, true, false>, MODE>(p, s);
+  } else if (!a_kc) {
     // (Only a tall matrix's gram product reads columns of both.)
     if constexpr (MODE == kGram)
       rc = p.two ? launch<Cfg<SIDE, false, false, true>, MODE>(p, s) : launch<Cfg<SIDE, false, false, false>, MODE>(p, s);
@@ -658,6 +667,8 @@ int product(ProdArgs& p, const Way& way, int64_t B, int64_t M, int64_t N, int64_
   p.part = part;
   if (way.form == kWide) return launch_side<256, MODE>(p, a_kc, b_kc, s);
   if (way.form == kNarrow) return launch_side<128, MODE>(p, a_kc, b_kc, s);
+  if constexpr (MODE != kApply)
+    if (way.form == kMid) return launch_side<192, MODE>(p, a_kc, b_kc, s);
   return launch_side<64, MODE>(p, a_kc, b_kc, s);
 }
 

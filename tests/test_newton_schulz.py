@@ -105,6 +105,14 @@ def test_newton_schulz(cuda, nat, case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 4001, 4090), (1, 3490, 3400)], ids=str)
+def test_large_sides(cuda, nat, shape):
+    torch = cuda
+    g = gradient(torch, *shape, "bf16", seed=4)
+    near(nat.newton_schulz(g, steps=2, terms=1), iterate(torch, g, 2), TOL[1], "bf16")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("steps", [1, 2, 3, 6])
 @pytest.mark.parametrize("shape", [(1, 264, 8200), (1, 8193, 250), (3, 72, 4000)], ids=str)
 def test_steps_of_long_matrices(cuda, nat, shape, steps):
