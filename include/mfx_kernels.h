@@ -917,7 +917,7 @@ int mfx_residual_norm(const mfx_residual_norm_args* args, void* stream);
  * rows that share them.  Rows in no sequence get dy = 0.  dx may be dr or x, dy may
  * be dh or y.  Nothing is kept from the forward; deterministic, no atomics.
  * workspace: mfx_residual_norm_bwd_workspace_size() bytes, 256-byte aligned
- * (fp32 rows of H: up to 16 a compute unit for each weight's gradient, as many
+ * (fp32 rows of H: up to 8 a compute unit for each weight's gradient, as many
  * and one for each sequence for a gate by sequence), or NULL for library scratch.
  */
 typedef struct {

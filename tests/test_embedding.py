@@ -113,11 +113,13 @@ RUNS = [[1], [32], [33], [32, 32], [31, 34, 1], [1, 32, 33], [64], [65], [64, 64
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("order", ["sorted", "mixed"])
+@pytest.mark.parametrize("rest", [1, 2100], ids=["small", "large"])
 @pytest.mark.parametrize("runs", RUNS, ids=str)
-def test_runs_about_a_pieces_length(cuda, nat, runs, order):
-    """Rows of 0, 1, 32, 33 .. tokens that start anywhere in a piece, against exact sums of small integers."""
+def test_runs_about_a_pieces_length(cuda, nat, runs, rest, order):
+    """Rows of 0, 1, 32, 33 .. tokens that start anywhere in a piece, against exact sums of small integers,
+    in a small table (one launch) and one of more than 4 MB."""
     torch = cuda
-    V, H = len(runs) + 1, 520
+    V, H = len(runs) + rest, 520
     ids = np.repeat(np.arange(len(runs)), runs)
     if order == "mixed":
         np.random.default_rng(1).shuffle(ids)
@@ -139,11 +141,12 @@ def test_every_token_the_same(cuda, nat):
 
 
 @pytest.mark.gpu
-def test_strided_rows_and_what_lies_between(cuda, nat):
+@pytest.mark.parametrize("V", [90, 4000])
+def test_strided_rows_and_what_lies_between(cuda, nat, V):
     """Rows of wider tensors at any alignment: the columns between stay."""
     torch = cuda
     rng = np.random.default_rng(3)
-    T, H, V = 200, 515, 90
+    T, H = 200, 515
     wide = torch.from_numpy(rng.standard_normal((V, H + 9))).to(torch.bfloat16).cuda()
     w = wide[:, 3:3 + H]
     ids = torch.from_numpy(rng.integers(0, V, (4, T // 4))).cuda()
