@@ -153,23 +153,25 @@ enum Mode { kGram, kSquare, kApply };
 
 // The forms of a product's tiles: square ones, since a symmetric product's
 // tiles are stored transposed too.
-// kMid is for one term and operands along k: of a symmetric product of 4096 a side
-// 256 x 256 are 136 tiles, which leave half the CUs without one, 192 x 192 are 253, 81
-// and 87 us (gram, square) for 89 and 100, or 94 and 97 in 128 x 128.
+// kMid is for operands along k.  In one term it is for symmetric products of about 4096 a
+// side, 253 tiles of 192 x 192 where 136 of 256 x 256 leave half the CUs without one: 81
+// and 87 us (gram, square) for 89 and 100, or 94 and 97 in 128 x 128.  In two terms the
+// products of 32 k with their reads from LDS fit in registers, those of 256 x 256 do
+// not: 187 and 202 us for 258 and 264 (4096 a side), 42 and 45 for 52 and 55 (2048).
 enum Form { kWide, kNarrow, kSlim, kMid };
 constexpr int kForms = 4, kSide[kForms] = {256, 128, 64, 192};
 
-// k of a tile: 32 of one term or, of small tiles, whose few products would not
-// cover taking up the next one, of two; else 16 of two.
-constexpr int depth(Form f, bool two) { return two && f != kSlim ? 16 : 32; }
+// k of a tile: 32, but of two terms in the two larger of the first forms 16 (their
+// stages, and the fragments of more, would not fit).
+constexpr int depth(Form f, bool two) { return two && f < kSlim ? 16 : 32; }
 
 template <int SIDE, bool A_KC, bool B_KC, bool P>
 struct Cfg : Config<SIDE, SIDE, SIDE == 64 ? 1 : 2, 2, A_KC, B_KC, 1> {
   static constexpr bool PAIR = P;  // operands in two terms
   static constexpr bool ROT = false;
   static constexpr int WAVES = SIDE == 256 || SIDE == 192 ? 1 : SIDE == 128 ? 2 : 3;  // per SIMD
-  static constexpr int STAGES = 4;
-  static constexpr int BK = depth(SIDE == 64 ? kSlim : kWide, P);
+  static constexpr int BK = depth(SIDE == 64 ? kSlim : SIDE == 192 ? kMid : kWide, P);
+  static constexpr int STAGES = SIDE == 192 && P ? 2 : 4;  // (its 54 products of a tile cover taking up the next)
   static constexpr int SMEM = STAGES * 4 * SIDE * BK * (1 + P);
 };
 
@@ -470,7 +472,8 @@ constexpr Cost kCost[2][kForms] = {{{1, 0.818f, 0.73f, 12.4f, 6.5f, 1.7f, 9.9f},
                                {1, 0.639f, 0.71f, 5.9f, 5.9f, 8.3f, 26.f}},
                               {{1, 1.240f, 0.69f, 10.0f, 13.2f, 2.8f, 8.3f},
                                {2, 0.947f, 0.00f, 1.8f, 4.5f, 8.0f, 8.7f},
-                               {2, 0.578f, 0.18f, 3.4f, 1.9f, 7.6f, 60.f}}};
+                               {2, 0.578f, 0.18f, 3.4f, 1.9f, 7.6f, 60.f},
+                              {1, 1.494f, 0.74f, 7.4f, 9.1f, 4.6f, 12.9f}}};
 
 // Of `wgs` workgroups of `n` k-tiles each.
 float rounds_us(const Cost& c, int64_t wgs, int64_t n, bool square) {
@@ -492,7 +495,7 @@ Way choose(int64_t B, int64_t M, int64_t N, int64_t K, Mode mode, bool two, bool
   Way best{};
   float least = INFINITY;
   for (int f = kWide; f < kForms; ++f) {
-    if (f == kMid && (two || !along)) continue;
+    if (f == kMid && !along) continue;
     const Cost& c = kCost[two][f];
     const int64_t side = kSide[f], tm = ceil_div(M, side), tn = ceil_div(N, side), kt = ceil_div(K, depth((Form)f, two));
     const int64_t tiles = B * (mode != kApply ? tm * (tm + 1) / 2 : tm * tn), rest = tiles % (c.slots * cus);
@@ -602,7 +605,7 @@ int plan_common(Plan& pl, int64_t B, int64_t m, int64_t n, int64_t steps, const 
   if (B == 0) return MFX_OK;
   pl.gram = choose(B, pl.s, pl.s, pl.l, kGram, pl.two, pl.wide);
   pl.square = choose(B, pl.s, pl.s, pl.s, kSquare, pl.two, true);
-  pl.apply = choose(B, m, n, pl.s, kApply, pl.two, false);
+  pl.apply = choose(B, m, n, pl.s, kApply, pl.two, !pl.wide);
   if (!pl.gram.tiles || !pl.square.tiles || !pl.apply.tiles)
     return fail(MFX_E_UNSUPPORTED, "problem too large for one launch");
   if (pl.two) {
@@ -632,7 +635,8 @@ template <int SIDE, Mode MODE>
 int launch_side(const ProdArgs& p, bool a_kc, bool b_kc, hipStream_t s) {
   int rc;
   if constexpr (SIDE == kSide[kMid]) {
-    rc = launch<Cfg<SIDE, true, true, false>, MODE>(p, s);
+    if (!a_kc || !b_kc) return fail(MFX_E_INVALID, "no such product");
+    rc = p.two ? launch<Cfg<SIDE, true, true, true>, MODE>(p, s) : launch<Cfg<SIDE, true, true, false>, MODE>(p, s);
   } else if (!a_kc) {
     // (Only a tall matrix's gram product reads columns of both.)
     if constexpr (MODE == kGram)
@@ -667,8 +671,7 @@ int product(ProdArgs& p, const Way& way, int64_t B, int64_t M, int64_t N, int64_
   p.part = part;
   if (way.form == kWide) return launch_side<256, MODE>(p, a_kc, b_kc, s);
   if (way.form == kNarrow) return launch_side<128, MODE>(p, a_kc, b_kc, s);
-  if constexpr (MODE != kApply)
-    if (way.form == kMid) return launch_side<192, MODE>(p, a_kc, b_kc, s);
+  if (way.form == kMid) return launch_side<192, MODE>(p, a_kc, b_kc, s);
   return launch_side<64, MODE>(p, a_kc, b_kc, s);
 }
 

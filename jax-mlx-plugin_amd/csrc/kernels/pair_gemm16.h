@@ -285,7 +285,9 @@ __device__ __forceinline__ void gemm_pair16(const GemmShape& g, int m0, int n0, 
   wait_loads<0>();  // (those out of range: the stages are the caller's now)
 }
 
-// The same over tiles of 32 k, for blocks of few products.
+// The same over tiles of 32 k, all of whose fragments are in registers before its products
+// start and the next tile's are read beside them: for 64 x 64 blocks, of few products, and 96 x 96 of
+// a wavefront, whose 54 cover taking up the next tile from two stages.
 template <class C>
 __device__ __forceinline__ void gemm_pair16_flat(const GemmShape& g, int m0, int n0, int kt0, int kt1, bf16* smem,
                                                  Acc<C>& acc) {
