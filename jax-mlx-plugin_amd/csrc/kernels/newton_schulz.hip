@@ -38,10 +38,10 @@
 //
 // What bounds it.  Large products: what the L2s deliver to LDS, 8 to 10 TB/s in
 // tiles of 192 and 256 (4096 a side: 81 us gram, 87 square, 122 to 126 apply in one term, up to
-// 1.1 PFLOP/s; a library product of that size 1.25).  Two terms of 2048 a side 33 us and
+// 1.1 PFLOP/s; a library product of that size 1.25).  Two terms of 2048 a side 33 to 36 us and
 // a join of 9 to 12.  Small ones: 512 a side 9 to 11 us, half of it a start and an end.
 // Together, five steps: 512 x 512 in two terms 158 us, 12 of 2048 x 512 in one 258, the update of
-// 2048 x 8200 in f32 1.59 ms, of 4096 x 4096 in bf16 1.53 ms.
+// 2048 x 8200 in f32 1.58 ms, of 4096 x 4096 in bf16 1.53 ms.
 //
 // The update takes its momentum on the way in (ns_norm, ns_split) and adds to the
 // weights in the last product's epilogue.
