@@ -103,6 +103,9 @@ CASES = [
     (300, 1536, "bf16", "bf16", "bf16", "feature", "bf16", None, 1e-6, 1e-6, 1.0, 1.0, 1.0),  # rows of 192,
     (40, 2560, "f16", "f32", "f16", "token", "f16", None, 1e-6, 1e-6, 1.0, 1.0, 0.0),         # 384
     (50, 5120, "bf16", "bf16", "f32", "seq", "bf16", [20, 0, 28], 1e-6, 1e-6, 1.0, 0.5, 0.0),  # and 768 lanes
+    (600, 8192, "bf16", "f32", "bf16", "feature", "bf16", None, 1e-6, 1e-6, 1.0, 1.0, 0.0),  # two chunks a lane
+    (30, 4001, "f16", "f16", "f16", "seq", "f16", [11, 0, 17], 1e-6, 1e-6, 1.0, 1.0, 0.0),    # odd rows of 512
+    (300, 5003, "bf16", "bf16", "bf16", "token", "bf16", None, 1e-6, 1e-6, 1.0, 1.0, 0.0),    # and 768 lanes
     (64, 700, "f32", "f32", None, None, "f32", None, None, None, 2.0, 1.0, 0.0),         # the sum alone
     (2500, 640, "bf16", "bf16", "bf16", "seq", "bf16", [1] * 700 + [1500], None, 1e-6, 1.0, 1.0, 0.0),
 ]
