@@ -540,12 +540,11 @@ bool float_dtype(int dt) { return dt == MFX_F32 || dt == MFX_BF16 || dt == MFX_F
 
 constexpr int64_t kMaxH = 32768;
 
-// Lanes that own a row and their chunks.  Rows of whole chunks take a chunk a lane, of
-// lanes that leave few idle, while the lanes have registers for the backward (its 4096
-// rows of 5120 take 58 us in 768 lanes for 70 in 1024; of 8192 with a gate 126 us in 512 lanes of
-// two chunks for 156, of 6144 89 for 184); others, a path of its own whose shifts take
-// registers, make do with fewer shapes, of a chunk a lane while there are lanes (5001: 371
-// us in 512 lanes of two for 233 in 1024).
+// Lanes that own a row and their chunks: a chunk a lane, of lanes that leave few
+// idle, while the lanes have registers for the backward (its 4096 rows of 5120 take 58 us
+// in 768 lanes for 70 in 1024; of 8192 with a gate 126 us in 512 lanes of two chunks for 156, of
+// 6144 89 for 184).  Rows that are not whole chunks, whose shifts take registers too, have a
+// chunk a lane while there are lanes (5001: 109 us in 768, 234 in 1024, 371 in 512 of two).
 struct Shape {
   int lanes, nv;
   bool easy;
@@ -554,7 +553,6 @@ Shape shape_of(int64_t H) {
   const bool easy = H % VEC == 0;
   const int64_t chunks = ceil_div(H, VEC);
   for (int lanes : {64, 128, 192, 256, 384, 512, 768}) {
-    if (!easy && (lanes == 128 || lanes == 192 || lanes == 384)) continue;
     if (chunks <= lanes) return {lanes, 1, easy};
   }
   if (chunks <= 1024) return easy ? Shape{512, 2, true} : Shape{1024, 1, false};
@@ -644,7 +642,10 @@ void with_shape(const Plan& pl, TX x, TY y, F f) {
   if (!s.easy) {
     const KindOf<kAny> k;
     if (s.lanes == 64) f(x, y, Sized<64, 1, false>{}, k);
+    else if (s.lanes == 128) f(x, y, Sized<128, 1, false>{}, k);
+    else if (s.lanes == 192) f(x, y, Sized<192, 1, false>{}, k);
     else if (s.lanes == 256) f(x, y, Sized<256, 1, false>{}, k);
+    else if (s.lanes == 384) f(x, y, Sized<384, 1, false>{}, k);
     else if (s.lanes == 512) f(x, y, Sized<512, 1, false>{}, k);
     else if (s.lanes == 768) f(x, y, Sized<768, 1, false>{}, k);
     else if (s.nv == 1) f(x, y, Sized<1024, 1, false>{}, k);

@@ -106,6 +106,9 @@ CASES = [
     (600, 8192, "bf16", "f32", "bf16", "feature", "bf16", None, 1e-6, 1e-6, 1.0, 1.0, 0.0),  # two chunks a lane
     (30, 4001, "f16", "f16", "f16", "seq", "f16", [11, 0, 17], 1e-6, 1e-6, 1.0, 1.0, 0.0),    # odd rows of 512
     (300, 5003, "bf16", "bf16", "bf16", "token", "bf16", None, 1e-6, 1e-6, 1.0, 1.0, 0.0),    # and 768 lanes
+    (700, 1001, "bf16", "f32", "bf16", "feature", "bf16", None, 1e-6, 1e-6, 1.0, 1.0, 1.0),   # of 128,
+    (21, 1500, "f32", "f32", "f32", "token", "f32", None, 1e-6, 1e-6, 1.0, 1.0, 0.0),         # 192
+    (400, 2999, "f16", "f16", "f16", "seq", "f16", [1, 398], None, 1e-6, 1.0, 1.0, 0.0),      # and 384
     (64, 700, "f32", "f32", None, None, "f32", None, None, None, 2.0, 1.0, 0.0),         # the sum alone
     (2500, 640, "bf16", "bf16", "bf16", "seq", "bf16", [1] * 700 + [1500], None, 1e-6, 1.0, 1.0, 0.0),
 ]
