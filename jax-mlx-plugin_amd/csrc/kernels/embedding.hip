@@ -416,10 +416,13 @@ __global__ __launch_bounds__(kFewTokens) void embed_few(SumArgs a, int tokens, i
     atomicAdd(count + r, 1);
   }
   __syncthreads();
-  if (tid <= mine) {
+  static_assert(kFewRows <= kFewTokens, "a thread for each row");
+  if (tid < mine) {
     int s = 0;
     for (int k = 0; k < tid; ++k) s += count[k];
     start[tid] = s;
+    // (The last row's end too: a workgroup of kFewRows rows has no thread behind its last.)
+    if (tid == mine - 1) start[mine] = s + count[tid];
   }
   __syncthreads();
   if (in) {

@@ -165,6 +165,33 @@ def test_strided_rows_and_what_lies_between(cuda, nat, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("tokens", [64, 512])
+@pytest.mark.parametrize("V,H,name", [(262144, 4, "f32"), (262144, 8, "bf16"), (300001, 6, "f16"), (261632, 3, "bf16"),
+                                      (2097152, 1, "f16"), (32768, 32, "f32")])
+def test_one_launch_over_the_longest_tables(cuda, nat, V, H, name, tokens, accumulate):
+    """Tables of narrow rows of up to 4 MB: a workgroup's rows are as many as its threads.  Tokens in the rows
+    about the workgroups' ends and the table's, a run of them longer than a piece; exact sums of small integers."""
+    torch = cuda
+    rng = np.random.default_rng(4)
+    edges = [r + d for r in (0, 512, 1024, 131072, V // 512 * 512, V) for d in (-2, -1, 0, 1)]
+    edges = np.array([r for r in edges if 0 <= r < V])
+    ids = rng.choice(edges, tokens)
+    ids[:40] = V - 1
+    ids[40:44] = 511
+    ids[44:46] = -1, V
+    dout = rng.integers(-1, 2, (tokens, H))
+    dw = torch.full((V, H), 3.0, device="cuda", dtype=dt(torch, name))
+    nat.embedding_bwd(torch.from_numpy(ids).cuda(), torch.from_numpy(dout).to(dw.dtype).cuda(), dw=dw,
+                      accumulate=accumulate)
+    want = np.full((V, H), 3.0 if accumulate else 0.0)
+    keep = (ids >= 0) & (ids < V)
+    np.add.at(want, ids[keep], dout[keep])
+    assert abs(want).max() <= 256  # exact in every type
+    assert np.array_equal(host(dw), want)
+
+
+@pytest.mark.gpu
 def test_no_tokens(cuda, nat):
     torch = cuda
     ids = torch.empty(0, dtype=torch.int64, device="cuda")
