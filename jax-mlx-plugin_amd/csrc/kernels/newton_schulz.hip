@@ -134,7 +134,8 @@ __global__ __launch_bounds__(256) void ns_split(InArgs a) {
   double sum = 0.0;  // (the same order in every workgroup)
   for (int i = threadIdx.x; i < a.parts; i += 256) sum += a.norm[(int64_t)blockIdx.y * a.parts + i];
   sum = block_sum(sum, lds);
-  const float f = (float)(a.scale / (sqrt(sum) + (double)a.eps));
+  // (In 64 bits: the factor of matrices smaller than 1e-34 is past fp32's range.)
+  const double f = (double)a.scale / (sqrt(sum) + (double)a.eps);
   const uint32_t cpr = (uint32_t)a.ld / 8, units = (uint32_t)a.m * cpr;
   uint16_t* const x = a.x + (int64_t)blockIdx.y * a.m * a.ld;
   for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < units; i += gridDim.x * 256) {
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(256) void ns_split(InArgs a) {
     if (a.buf) store8(a.buf_out, a.buf_dt, (int64_t)blockIdx.y * a.os_b + row * a.os_r, e, a.n, b);
     // (Zeros in the columns past n: 0 times a factor that may be infinite would not be.)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] = e + j < a.n ? u[j] * f : 0.f;
+    for (int j = 0; j < 8; ++j) u[j] = e + j < a.n ? (float)((double)u[j] * f) : 0.f;
     *reinterpret_cast<uint4*>(x + (int64_t)i * 8) = rowvec::pack16<_Float16>(u);
     if (!a.two) continue;
 #pragma unroll

@@ -170,6 +170,31 @@ def test_zeros_rank_and_values_that_are_not_finite(cuda, nat):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-42, 1e-37, 1e-34, 1e36, 1e37])
+@pytest.mark.parametrize("shape", [(1, 80, 120), (2, 300, 70)], ids=str)
+def test_sizes_at_the_ends_of_fp32(cuda, nat, shape, size):
+    """Entries down to the smallest (of few bits: the reference takes them as they are) and up to the largest."""
+    torch = cuda
+    g = gradient(torch, *shape, "f32", size=size)
+    assert torch.isfinite(g).all() and g.any()
+    near(nat.newton_schulz(g, eps=0.0), iterate(torch, g, eps=0.0), TOL[2], "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eps", [1e-7, 1.2e-38, 2e-45])
+def test_zeros_with_any_eps(cuda, nat, eps):
+    """Zeros give zeros however small eps is, and weights that only decay."""
+    torch = cuda
+    z = torch.zeros(2, 70, 200, device="cuda")
+    assert not nat.newton_schulz(z, eps=eps).any()  # (a NaN counts)
+    for terms in (1, 2):
+        assert not nat.newton_schulz(z.bfloat16().mT.contiguous(), eps=eps, terms=terms).any()
+    w = torch.randn(2, 70, 200, device="cuda", generator=torch.Generator("cuda").manual_seed(8))
+    got, _ = nat.muon_update(w, z, z.clone(), lr=0.5, weight_decay=0.5, eps=eps, w_out=torch.empty_like(w))
+    assert torch.equal(got, 0.75 * w)
+
+
+@pytest.mark.gpu
 def test_strided_and_in_place(cuda, nat):
     """Matrices inside wider ones at any alignment; out over g: the same bits."""
     torch = cuda
