@@ -974,10 +974,11 @@ size_t mfx_residual_norm_bwd_workspace_size(const mfx_residual_norm_bwd_args* ar
  * `out_dtype` (f32, bf16, f16), rows and matrices spaced by the strides
  * (elements), elements contiguous, any alignment; out may be g.  A matrix of
  * zeros gives zeros (eps > 0), one with an infinity or NaN gives NaN.
- * terms: f16 terms that the products' operands are held in.  2: error as of
- * products of fp32 matrices; 1: three times as fast, off by up to 3e-3 of the result's
- * norm; 0: 1 for bf16 results with both sides 256 or more, else 2.  Sums are fp32, the norm
- * fp64.
+ * terms: f16 terms that the products' operands are held in.  2 (0: the same):
+ * error as of products of fp32 matrices, whatever the matrix.  1: in 0.4 to 0.7 of the
+ * time, to 11 bits: what lies far below a matrix's largest directions is raised with
+ * their rounding in it, 1.5e-3 of the result's norm for directions of like size, 2e-2 and
+ * more where a few are a hundred times the rest.  Sums are fp32, the norm fp64.
  * workspace: mfx_newton_schulz_workspace_size() bytes, 256-byte aligned, or NULL for
  * library scratch.  Deterministic.  No counterpart in the reference.
  */

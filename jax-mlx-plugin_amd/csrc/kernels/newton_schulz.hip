@@ -30,10 +30,12 @@
 // the bound that the coefficients give their norms, so that no entry overflows
 // and the second terms stay clear of the smallest f16.  A singular value that
 // is small beside |U| is raised by up to a^steps (485), and with it what the
-// roundings put there: measured against 64 bits, gradients with a few large
-// directions come out off by 1.5e-3 of their norm in one term, just under a bf16
-// result's own rounding (1.7e-3), and by 2e-6 in two, as products of fp32 matrices
-// do (1.5e-6).  One term is therefore for bf16 results alone.  The norm is summed
+// roundings put there.  Measured against 64 bits, 512 x 512 whose entries are one
+// direction and noise of 1, 1/100 and 1/300 of its size: off by 1.5e-6, 1.7e-5 and
+// 4.5e-5 of the result's norm in two terms, products of fp32 matrices by 2.2e-6, 2.4e-5 and
+// 6.7e-5; in one term by 1.3e-3, 2.1e-2 and 5.8e-2, more than any result's own rounding
+// (bf16 1.7e-3).  So two terms are the rule, whatever the types, and one term is for
+// callers who ask for it and know their gradients.  The norm is summed
 // in 64 bits (squares of small gradients leave the range of fp32).
 //
 // What bounds it.  Large products: what the L2s deliver to LDS, 8 to 10 TB/s in
@@ -591,7 +593,7 @@ int plan_scales(Plan& pl, const float* coeffs, int num) {
 }
 
 int plan_common(Plan& pl, int64_t B, int64_t m, int64_t n, int64_t steps, const float* coeffs, int num_coeffs, float eps,
-                int terms, bool bf16_result) {
+                int terms) {
   if (B < 0 || m <= 0 || n <= 0) return fail(MFX_E_INVALID, "batch must be >= 0, m and n positive");
   if (steps < 1 || !coeffs || (num_coeffs != 1 && num_coeffs != steps))
     return fail(MFX_E_INVALID, "steps must be >= 1, coefficients for all steps or for each");
@@ -606,9 +608,7 @@ int plan_common(Plan& pl, int64_t B, int64_t m, int64_t n, int64_t steps, const 
   pl.ld = ceil_div(n, 8) * 8;
   pl.lds = ceil_div(pl.s, 8) * 8;
   pl.steps = (int)steps;
-  // One term for bf16 results (their own rounding is larger than its error), and
-  // not for sides whose products are over in no time either way.
-  pl.two = terms == 0 ? !(bf16_result && pl.s >= 256) : terms == 2;
+  pl.two = terms != 1;
   if (int rc = plan_scales(pl, coeffs, num_coeffs)) return rc;
   if (B == 0) return MFX_OK;
   pl.gram = choose(B, pl.s, pl.s, pl.l, kGram, pl.two, pl.wide);
@@ -783,8 +783,7 @@ int bind(const void* p, int64_t row, int64_t batch, const Plan& pl, int dt, cons
 
 int plan_ns(const mfx_newton_schulz_args* a, Plan& pl) {
   if (!a) return fail(MFX_E_INVALID, "null args");
-  if (int rc = plan_common(pl, a->batch, a->m, a->n, a->steps, a->coeffs, a->num_coeffs, a->eps, a->terms,
-                           a->out_dtype == MFX_BF16))
+  if (int rc = plan_common(pl, a->batch, a->m, a->n, a->steps, a->coeffs, a->num_coeffs, a->eps, a->terms))
     return rc;
   if (!std::isfinite(a->scale)) return fail(MFX_E_INVALID, "scale must be finite");
   if (int rc = bind(a->g, a->g_row_stride, a->g_batch_stride, pl, a->dtype, "g", false)) return rc;
@@ -793,8 +792,7 @@ int plan_ns(const mfx_newton_schulz_args* a, Plan& pl) {
 
 int plan_muon(const mfx_muon_update_args* a, Plan& pl) {
   if (!a) return fail(MFX_E_INVALID, "null args");
-  if (int rc = plan_common(pl, a->batch, a->m, a->n, a->steps, a->coeffs, a->num_coeffs, a->eps, a->terms,
-                           a->w_dtype == MFX_BF16))
+  if (int rc = plan_common(pl, a->batch, a->m, a->n, a->steps, a->coeffs, a->num_coeffs, a->eps, a->terms))
     return rc;
   if (!std::isfinite(a->lr) || !std::isfinite(a->scale) || !std::isfinite(a->weight_decay))
     return fail(MFX_E_INVALID, "lr, scale and weight_decay must be finite");

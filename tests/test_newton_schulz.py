@@ -67,6 +67,21 @@ def gradient(torch, B, m, n, name, seed=0, low=2.0, size=1e-3):
     return (x * size).to(dt(torch, name))
 
 
+def f32_error(torch, u, ref, steps=5, coeffs=QUINTIC, eps=1e-7):
+    """Of the definition in plain f32 products on the GPU, of the norm (the largest of the matrices')."""
+    u = u.double()
+    x = (u / (u.flatten(1).norm(dim=1)[:, None, None] + eps)).float()
+    wide = x.shape[1] <= x.shape[2]
+    for i in range(steps):
+        a, b, c = coeffs[i] if isinstance(coeffs[0], tuple) else coeffs
+        t = x.mT.contiguous()
+        s = torch.bmm(x, t) if wide else torch.bmm(t, x)
+        q = b * s + c * torch.bmm(s, s)
+        x = a * x + (torch.bmm(q, x) if wide else torch.bmm(x, q))
+    off = (x.double().cpu() - ref).flatten(1).norm(dim=1) / ref.flatten(1).norm(dim=1)
+    return float(off.max())
+
+
 CASES = [
     # B, m, n, in, out, terms
     (1, 1, 1, "f32", "f32", 0),
@@ -192,6 +207,29 @@ def test_zeros_with_any_eps(cuda, nat, eps):
     w = torch.randn(2, 70, 200, device="cuda", generator=torch.Generator("cuda").manual_seed(8))
     got, _ = nat.muon_update(w, z, z.clone(), lr=0.5, weight_decay=0.5, eps=eps, w_out=torch.empty_like(w))
     assert torch.equal(got, 0.75 * w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ratio", [100.0, 300.0])
+@pytest.mark.parametrize("shape", [(1, 512, 512), (2, 300, 1000), (1, 2048, 264)], ids=str)
+def test_one_direction_far_above_the_rest(cuda, nat, shape, ratio):
+    """What the iteration raises by a^steps is what the operands' roundings leave of the rest, so a bf16
+    result too needs products of f32.  Held to eight times the error of plain f32 products on the same
+    matrix: an operand in two terms keeps 22 bits, four times f32's step, and the product of the second terms
+    is left out, once more."""
+    torch = cuda
+    B, m, n = shape
+    g = torch.Generator("cuda").manual_seed(6)
+    mk = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    x = (mk(B, m, 1) * mk(B, 1, n) + mk(B, m, n) / ratio).bfloat16()
+    ref = iterate(torch, x)
+    tol = 8 * f32_error(torch, x, ref)
+    near(nat.newton_schulz(x), ref, tol, "bf16")
+    near(nat.newton_schulz(x, out_dtype=torch.float32), ref, tol, "f32")
+    w, _ = nat.muon_update(torch.zeros_like(x), x, lr=-1.0)
+    near(w, ref, tol, "bf16")
+    f16 = x.half()
+    near(nat.newton_schulz(f16), iterate(torch, f16), tol, "f16")
 
 
 @pytest.mark.gpu
