@@ -188,6 +188,30 @@ def test_forward_and_backward(cuda, nat, case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,lanes,dtype,res,kind,post,pre", [
+    (200, 64, "bf16", "f32", "seq", True, True), (512, 64, "f16", "f16", "token", True, True),
+    (512, 64, "f32", "f32", "seq", False, True), (333, 64, "bf16", "bf16", "token", True, False),
+    (1024, 128, "bf16", "bf16", "token", False, True), (1537, 256, "f16", "f16", "seq", True, True),
+    (2048, 256, "bf16", "f32", "token", True, True), (2048, 256, "bf16", "bf16", None, True, True),
+    (4096, 512, "bf16", "bf16", "token", True, True), (4096, 512, "f16", "f32", "feature", True, True),
+    (5120, 768, "bf16", "bf16", "seq", True, True), (5120, 768, "bf16", "bf16", "token", True, True)], ids=str)
+def test_several_rows_of_a_group(cuda, nat, H, lanes, dtype, res, kind, post, pre):
+    """Four rows a group in the forward and more in the backward, whose rows, gates and sums pass from one to the
+    next: a group of `lanes` lanes, 16 wavefronts a CU and a workgroup a CU at least.  Sequences of all lengths begin
+    and end inside groups, between them tokens in none."""
+    torch = cuda
+    T = 3 * torch.cuda.get_device_properties(0).multi_processor_count * max(1, 16 * 64 // lanes) + 1
+    lens = None
+    if kind == "seq":
+        rng = np.random.default_rng(5)
+        lens = [0, 1, 2, 3, 4, 5, 0, 0, 9]
+        while sum(lens) < T - 40:
+            lens.append(int(min(T - 11 - sum(lens), np.exp(rng.uniform(0, np.log(T / 4))))))
+    case = (T, H, dtype, res, dtype, kind, dtype, lens, 1e-6 if post else None, 1e-6 if pre else None, 1.0, 0.5, 1.0)
+    check(torch, nat, case, make(torch, case, first=5))
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences(cuda, nat):
     """Central differences of the forward in f32 along random directions: steps of 2^-7 leave an error of
     second order (under 1e-3 here) beside 2^-24 of the sums over 2^-7."""
