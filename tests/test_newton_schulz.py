@@ -233,6 +233,42 @@ def test_one_direction_far_above_the_rest(cuda, nat, shape, ratio):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("low", [2.0, 0.0])
+@pytest.mark.parametrize("shape", [(1, 65, 63), (1, 250, 1000), (1, 1000, 520), (3, 2048, 512), (1, 600, 5000), (1, 5001, 258),
+                                   (1, 1543, 1537), (1, 1100, 1301), (1, 2047, 4099), (1, 3500, 3333)], ids=str)
+def test_two_terms_block_by_block(cuda, nat, shape, low):
+    """No part of a result is worse than the rest: each block of 32 x 32 is held to eight times what plain f32
+    products make of the matrix (four times f32's step in an operand, and the product left out once more), of
+    the block's share of it or of its own norm, whichever is more."""
+    torch = cuda
+    B, m, n = shape
+    g = gradient(torch, B, m, n, "f32", seed=11, low=low)
+    ref = iterate(torch, g)
+    tol = 8 * f32_error(torch, g, ref)
+    off = nat.newton_schulz(g).double().cpu() - ref
+    pad = (0, -n % 32, 0, -m % 32)
+
+    def blocks(v):
+        v = torch.nn.functional.pad(v, pad)
+        return v.reshape(B, v.shape[1] // 32, 32, v.shape[2] // 32, 32).square().sum((2, 4)).sqrt()
+
+    share = ref.flatten(1).norm(dim=1)[:, None, None] * 32 / (m * n) ** 0.5
+    assert ((off.flatten(1).norm(dim=1) <= tol * ref.flatten(1).norm(dim=1))).all()
+    assert (blocks(off) <= tol * torch.maximum(blocks(ref), share)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 300, 301), (1, 1000, 520), (1, 5001, 258), (1, 258, 4999), (1, 1543, 1537), (12, 520, 264),
+                                   (1, 65, 63)], ids=str)
+def test_one_term_where_asked_for(cuda, nat, shape):
+    torch = cuda
+    g = gradient(torch, *shape, "bf16", seed=9)
+    near(nat.newton_schulz(g, terms=1), iterate(torch, g), TOL[1], "bf16")
+    w, _ = nat.muon_update(torch.zeros_like(g), g, lr=-1.0, terms=1)
+    assert torch.equal(w, nat.newton_schulz(g, terms=1))
+
+
+@pytest.mark.gpu
 def test_strided_and_in_place(cuda, nat):
     """Matrices inside wider ones at any alignment; out over g: the same bits."""
     torch = cuda
