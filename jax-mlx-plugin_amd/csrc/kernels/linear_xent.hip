@@ -38,6 +38,7 @@
 #include <cmath>
 #include <string>
 
+#include "workspace.h"
 #include "xent_gemm16.h"
 #include "xent_gemm32.h"
 
@@ -447,7 +448,6 @@ namespace {
 constexpr size_t kPieceBytes = 512u << 20;      // of d at a time
 constexpr int64_t kMaxStride = int64_t(1) << 21;  // a tile's 256 rows are addressed within 31 bits
 
-size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Workgroups of 256 for `n` threads' work; the kernel's threads go on in
@@ -732,18 +732,6 @@ int check_bwd(const mfx_linear_xent_bwd_args* a) {
   if (int rc = check_matrix(a->w, a->w_stride, a->H, size, "w")) return rc;
   if (a->dh) return check_matrix(a->dh, a->dh_stride, a->H, size, "dh");
   return MFX_OK;
-}
-
-// The caller's workspace or the library's scratch for the stream.
-int take_workspace(void* given, size_t given_bytes, size_t need, const char* query, hipStream_t s, char** out) {
-  if (given) {
-    if (given_bytes < need) return fail(MFX_E_WORKSPACE, std::string("workspace smaller than ") + query + "()");
-    if ((uintptr_t)given % 256) return fail(MFX_E_INVALID, "workspace must be 256-byte aligned");
-    *out = static_cast<char*>(given);
-    return MFX_OK;
-  }
-  *out = static_cast<char*>(device_scratch(need, s));
-  return *out ? MFX_OK : MFX_E_HIP;
 }
 
 // dw of no rows.
