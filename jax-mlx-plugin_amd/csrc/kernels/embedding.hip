@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kBlock) void embed_lookup(LookupArgs a) {
   float v[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    // (An id outside the table reads nothing: V may be 0.)
+    // (An id outside the table reads nothing.)
     load_run<TI, VEC>(src, col + i * LANES * VEC, valid ? a.H : 0, 0.f, v[i]);
   }
 #pragma unroll

@@ -330,7 +330,7 @@ __device__ __forceinline__ void finish_rows(const ProdArgs& p, int64_t bz, int m
       const int row = run * 8 + e;
       v[e] = st[row * W + ((r >> 2) ^ (row & TURN)) * 4 + (r & 3)];
     }
-    // (Rows past the matrix hold sums of zeros: nothing went over them.)
+    // (Nothing went over rows past the matrix, which hold sums of what lies there.)
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = m + e < M ? v[e] : 0.f;
     put((int64_t)n * p.ldc + m, v);

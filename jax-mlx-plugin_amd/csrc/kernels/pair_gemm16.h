@@ -11,8 +11,8 @@
 // block, where three walks along k would take 48 and 24.
 //
 // Schedule of 128 x 128 and 64 x 64 blocks.  Four LDS stages, loaded three tiles ahead.  Step 0 multiplies A_lo by
-// B_hi and reads A_hi, step 1 A_hi by B_hi and reads B_lo, and the next tile's
-// loads but two go out between the products of both; step 2 multiplies A_hi by B_lo,
+// B_hi and reads A_hi, step 1 A_hi by B_hi and reads B_lo, and the loads of the
+// tile three ahead go out between the products of both; step 2 multiplies A_hi by B_lo,
 // and at its slot B0 the next tile has landed for everyone (the one barrier of a
 // tile) and its A_lo and B_hi are read.
 #pragma once
