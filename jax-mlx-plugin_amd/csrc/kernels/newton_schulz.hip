@@ -38,12 +38,12 @@
 // callers who ask for it and know their gradients.  The norm is summed
 // in 64 bits (squares of small gradients leave the range of fp32).
 //
-// What bounds it.  Large products: what the L2s deliver to LDS, 8 to 10 TB/s in
-// tiles of 192 and 256 (4096 a side: 81 us gram, 87 square, 122 to 126 apply in one term, up to
-// 1.1 PFLOP/s; a library product of that size 1.25).  Two terms of 2048 a side 33 to 36 us and
-// a join of 9 to 12.  Small ones: 512 a side 9 to 11 us, half of it a start and an end.
-// Together, five steps: 512 x 512 in two terms 158 us, 12 of 2048 x 512 in one 258, the update of
-// 2048 x 8200 in f32 1.58 ms, of 4096 x 4096 in bf16 1.53 ms.
+// What bounds it.  Large products: what the L2s deliver to LDS, 7 to 8 TB/s in
+// tiles of 192 and 256 (4096 a side: 199 us gram, 211 square, 327 apply, whose three
+// products of f16 run at a library product's 1.26 PFLOP/s; in one term 87, 92 and 122).  2048 a
+// side 36 to 38 us and a join of 10 to 12.  Small ones: 512 a side 9 to 12 us, half of it a start and an end.
+// Together, five steps: 512 x 512 158 us, 12 of 2048 x 512 in bf16 429 to 447, the update of
+// 2048 x 8200 in f32 1.57 to 1.64 ms, of 4096 x 4096 in bf16 3.70 to 3.74.
 //
 // The update takes its momentum on the way in (ns_norm, ns_split) and adds to the
 // weights in the last product's epilogue.
@@ -165,7 +165,7 @@ enum Mode { kGram, kSquare, kApply };
 // tiles are stored transposed too.
 // kMid is for operands along k.  In one term it is for symmetric products of about 4096 a
 // side, 253 tiles of 192 x 192 where 136 of 256 x 256 leave half the CUs without one: 81
-// and 87 us (gram, square) for 89 and 100, or 94 and 97 in 128 x 128.  In two terms the
+// and 87 us (gram, square; by themselves, over and over) for 89 and 100, or 94 and 97 in 128 x 128.  In two terms the
 // products of 32 k with their reads from LDS fit in registers, those of 256 x 256 do
 // not: 187 and 202 us for 258 and 264 (4096 a side), 42 and 45 for 52 and 55 (2048).
 enum Form { kWide, kNarrow, kSlim, kMid };

@@ -22,10 +22,12 @@
 // workgroup (of a sequence in the group's run for a sequence's gate), which
 // residual_params / residual_gates add up in order: no atomics.
 //
-// Measured: 8192 rows of 4096 in bf16 forward 42 us (6.3 TB/s), backward with the
-// stream in f32 and both norms 120 us and 5 for the weights (5.1 TB/s, a copy's rate); 4099 of
+// Measured: 8192 rows of 4096 in bf16 forward 46 us (5.9 TB/s, with the call), backward with the
+// stream in f32 and both norms 123 us and 5 for the weights (5.0 TB/s, a copy's rate); 4099 of
 // 2048 with a gate backward 25 and 4.  Rows of up to 1536 with a gate and both norms wait for
-// their three sums: 8192 of 1536 backward 44 us (3.4 TB/s).  64 rows of 4096 take 4 us.
+// their three sums: 8192 of 1536 backward 54 us with the call (2.8 TB/s).  64 rows of 4096 take 4 us.
+// Rows of over 8192 (and, by less, gated and odd ones of over 4096) spill registers in the
+// backward: 2048 of 16384 528 us (0.8 TB/s).
 #include <algorithm>
 #include <cmath>
 
